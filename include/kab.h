@@ -483,6 +483,94 @@ int kab_kv_decode_workspace(const KabKvDecodeParams* params, int* splits, size_t
 int kab_kv_decode_fp8(const KabKvDecodeParams* params, void* workspace, size_t workspace_bytes,
                       void* stream);
 
+/* ------------------------------------------------------------------ decode with FP4 weights */
+
+/* out[m, n] = tensor_scale[n or 0] * sum_k x[m, k] * e2m1(codes[n, k]) * scales[n, k / block]
+ * (+ bias[n]): a weight-only FP4 linear for a few tokens, the activations as they are. codes
+ * [n, k / 2] (low nibble = even k, 8-byte aligned rows), scales e4m3 per 16 (KAB_NVFP4) or e8m0
+ * per 32 (KAB_MXFP4), [n, k / block] row-major or, with `swizzle`, in the 128 x 4 blocked layout
+ * the GEMMs read. x [m, k] of `dtype` (row stride ldx elements, 16-byte aligned rows), bias of
+ * `bias_dtype` or NULL, out [m, ldo] of `dtype`. Products are exact, sums fp32. The workspace
+ * (kab_gemv_fp4_workspace; `bytes` may be 0) holds fp32 partial sums and, in its first
+ * `zero_bytes`, counters: zero those once when it is allocated; every launch leaves them at zero.
+ * It serves one stream at a time and one shape: another shape's counters may lie elsewhere. */
+int kab_gemv_fp4_workspace(int64_t m, int64_t n, int64_t k, int fmt, int dtype, size_t* bytes,
+                           size_t* zero_bytes);
+int kab_gemv_fp4(const void* x, int dtype, int64_t ldx, const uint8_t* codes, const uint8_t* scales,
+                 int swizzle, int fmt, const float* tensor_scale, int scale_per_row, int64_t m,
+                 int64_t n, int64_t k, const void* bias, int bias_dtype, void* out, int64_t ldo,
+                 void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------ paged FP8 KV cache */
+
+/* A pool of pages of `page_tokens` (16, 32, 64 or 128) cached tokens each, K and V in e4m3 with
+ * one fp32 scale per (page, KV head): value = code * scale. Code strides in bytes (multiples of
+ * 16, unit last stride), scale and mass strides in elements. `mass` [num_pages, heads_kv,
+ * page_tokens] (unit last stride) is the attention weight every cached token has received, or
+ * NULL. Token t of sequence b stands in slot t % page_tokens of page
+ * page_table[b * table_stride + t / page_tokens]; only the pages of the first lengths[b] tokens
+ * are read. A page number outside the pool is skipped and a length past max_pages * page_tokens
+ * is cut, each raising the bounds bit of kab_device_status. */
+typedef struct KabKvPages {
+  uint8_t* k_pages;
+  uint8_t* v_pages;
+  float* k_scale;
+  float* v_scale;
+  float* mass;
+  int64_t k_stride_page, k_stride_head, k_stride_token;
+  int64_t v_stride_page, v_stride_head, v_stride_token;
+  int64_t ks_stride_page, ks_stride_head, vs_stride_page, vs_stride_head;
+  int64_t mass_stride_page, mass_stride_head;
+  int64_t num_pages, heads_kv, page_tokens, head_dim;
+  const int32_t* page_table;
+  int64_t table_stride, max_pages, batch;
+  const int32_t* lengths;
+} KabKvPages;
+
+/* Writes the first counts[b] (NULL: all) of `new_tokens` tokens of k and v [batch, heads_kv,
+ * new_tokens, head_dim] (element strides, multiples of 8, 16-byte aligned rows) after the
+ * lengths[b] tokens of sequence b. A page's scale is the smallest power of two s >= 2^-126 with
+ * |value| <= 448 s for every finite value appended to it, or its old scale where that is larger;
+ * when it grows, the codes that the page holds already are rewritten as e4m3(code * old / s).
+ * Infinities become the largest code, NaN stays NaN. The new slots' mass becomes 0.
+ * lengths_out[b] = lengths[b] + counts[b]; it may be `lengths` itself. */
+int kab_kv_pages_append(const KabKvPages* cache, const void* k, const void* v, int dtype,
+                        int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_t,
+                        int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_t,
+                        int64_t new_tokens, const int32_t* counts, int32_t* lengths_out, void* stream);
+
+/* Attention of q [batch, heads_q, q_len, head_dim] (element strides, unit last) over the cache:
+ * softmax(q K^T * sm_scale) V, grouped-query heads, into out [batch, heads_q, q_len, head_dim]
+ * of q's dtype, contiguous. With `causal` the queries are the newest q_len tokens: query i sees
+ * the first lengths[b] - q_len + 1 + i; otherwise every query sees all. A query that sees
+ * nothing gives zeros. With `use_mass`, every cached token's weight, summed over the query heads
+ * of its KV head and the query tokens, is added to its mass. head_dim 64 or 128. The workspace:
+ * as for kab_gemv_fp4. */
+typedef struct KabKvPagesAttention {
+  KabKvPages cache;
+  const void* q;
+  int q_dtype;
+  int causal;
+  int use_mass;
+  float sm_scale;
+  int64_t q_stride_b, q_stride_h, q_stride_t;
+  int64_t heads_q, q_len;
+  void* out;
+} KabKvPagesAttention;
+int kab_kv_pages_attention_workspace(const KabKvPagesAttention* params, size_t* bytes, size_t* zero_bytes);
+int kab_kv_pages_attention(const KabKvPagesAttention* params, void* workspace, size_t workspace_bytes,
+                           void* stream);
+
+/* Keeps min(lengths[b], budget) tokens of every (sequence, KV head): the first `sinks`, the last
+ * `recent` and, between them, those of the largest mass (equal masses: the first; NaN counts as
+ * the largest), in their order, and copies their codes, scales and masses into the pages
+ * out_table[b * out_stride + i / page_tokens] of the same pool, which no sequence may use. Each
+ * written page's scale is the smallest power of two that holds its values (as in the append).
+ * kept [batch, heads_kv, budget]: the kept token numbers, -1 past the last; lengths_out [batch].
+ * sinks + recent <= budget. */
+int kab_kv_pages_evict(const KabKvPages* cache, const int32_t* out_table, int64_t out_stride, int64_t budget,
+                       int64_t recent, int64_t sinks, int32_t* kept, int32_t* lengths_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -23,7 +23,8 @@ ROOT = HERE.parent
 CSRC = HERE / "csrc"
 BUILD = HERE / "_build"
 OUT = HERE / "kernel_agent_b200" / "_native" / "libkab.so"
-SOURCES = ["kab_core.cu", "kab_quant.cu", "kab_compare.cu", "kab_gemm.cu", "kab_attention.cu"]
+SOURCES = ["kab_core.cu", "kab_quant.cu", "kab_compare.cu", "kab_gemm.cu", "kab_attention.cu", "kab_pages.cu",
+           "kab_gemv.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ARCH + [
     "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",

@@ -72,7 +72,8 @@ int kab_device_check(int device) {
 int kab_device_status(unsigned* bits, int clear, void* stream) {
   KAB_REQUIRE(bits != nullptr, "bits is null");
   const cudaStream_t s = kab::as_stream(stream);
-  unsigned v = kab::gemm_device_status(clear != 0, s) | kab::attention_device_status(clear != 0, s);
+  unsigned v = kab::gemm_device_status(clear != 0, s) | kab::attention_device_status(clear != 0, s) |
+               kab::pages_device_status(clear != 0, s);
   const cudaError_t e = cudaStreamSynchronize(s);
   if (e != cudaSuccess) return kab::fail(KAB_ECUDA, "device status: %s", cudaGetErrorString(e));
   *bits = v;

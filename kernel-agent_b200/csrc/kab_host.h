@@ -32,6 +32,7 @@ inline bool valid_dtype(int dtype) {
 // Per-translation-unit device status readers (each TU with waiting kernels owns a word).
 unsigned gemm_device_status(bool clear, cudaStream_t stream);
 unsigned attention_device_status(bool clear, cudaStream_t stream);
+unsigned pages_device_status(bool clear, cudaStream_t stream);
 
 }  // namespace kab
 

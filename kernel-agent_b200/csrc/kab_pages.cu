@@ -1,0 +1,247 @@
+// extern "C" entry points of the paged FP8 KV cache (kv_pages.cuh, attention_pages.cuh): the
+// append, the attention over the pages and the eviction, and this translation unit's device
+// status word.
+#include <algorithm>
+
+#include "kab_host.h"
+
+namespace kab {
+__device__ unsigned g_pages_status = 0;
+}  // namespace kab
+
+#include "attention_pages.cuh"
+#include "kv_pages.cuh"
+
+namespace kab {
+
+unsigned pages_device_status(bool clear, cudaStream_t stream) {
+  unsigned v = 0;
+  cudaMemcpyFromSymbolAsync(&v, g_pages_status, sizeof v, 0, cudaMemcpyDeviceToHost, stream);
+  cudaStreamSynchronize(stream);
+  if (clear) {
+    const unsigned zero = 0;
+    cudaMemcpyToSymbolAsync(g_pages_status, &zero, sizeof zero, 0, cudaMemcpyHostToDevice, stream);
+  }
+  return v;
+}
+
+namespace {
+
+// The device address of the status word of the current device (looked up once per device).
+unsigned* status_word() {
+  static unsigned* at[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+  if (at[dev] == nullptr) {
+    void* p = nullptr;
+    if (cudaGetSymbolAddress(&p, g_pages_status) != cudaSuccess) return nullptr;
+    at[dev] = static_cast<unsigned*>(p);
+  }
+  return at[dev];
+}
+
+int pool_check(const KabKvPages* c, PagePool* p) {
+  KAB_REQUIRE(c != nullptr, "null parameters");
+  KAB_REQUIRE(c->head_dim == 64 || c->head_dim == 128, "head_dim %lld: the paged cache takes 64 or 128",
+              (long long)c->head_dim);
+  KAB_REQUIRE(c->page_tokens == 16 || c->page_tokens == 32 || c->page_tokens == 64 || c->page_tokens == 128,
+              "page_tokens %lld: 16, 32, 64 or 128", (long long)c->page_tokens);
+  KAB_REQUIRE(c->batch >= 0 && c->heads_kv > 0 && c->num_pages >= 0 && c->max_pages >= 0, "bad shape");
+  KAB_REQUIRE(c->batch < 65536 && c->heads_kv < 65536, "at most 65535 sequences and KV heads");
+  KAB_REQUIRE(c->num_pages < (int64_t(1) << 31) && c->max_pages * c->page_tokens < (int64_t(1) << 30),
+              "the page table or the pool is too large");
+  if (c->batch == 0) return KAB_OK;
+  KAB_REQUIRE(c->lengths != nullptr, "null lengths");
+  KAB_REQUIRE(c->num_pages == 0 || (c->k_pages && c->v_pages && c->k_scale && c->v_scale), "null pages");
+  KAB_REQUIRE(c->max_pages == 0 || (c->page_table != nullptr && c->num_pages > 0), "null page table or empty pool");
+  KAB_REQUIRE(aligned(c->k_pages, 16) && aligned(c->v_pages, 16), "the pages must be 16-byte aligned");
+  KAB_REQUIRE(c->k_stride_page % 16 == 0 && c->k_stride_head % 16 == 0 && c->k_stride_token % 16 == 0 &&
+                  c->v_stride_page % 16 == 0 && c->v_stride_head % 16 == 0 && c->v_stride_token % 16 == 0,
+              "page strides must be multiples of 16 bytes");
+  *p = PagePool{};
+  p->codes[0] = c->k_pages;
+  p->codes[1] = c->v_pages;
+  p->scale[0] = c->k_scale;
+  p->scale[1] = c->v_scale;
+  p->mass = c->mass;
+  p->sp[0] = c->k_stride_page, p->sh[0] = c->k_stride_head, p->st[0] = c->k_stride_token;
+  p->sp[1] = c->v_stride_page, p->sh[1] = c->v_stride_head, p->st[1] = c->v_stride_token;
+  p->ssp[0] = c->ks_stride_page, p->ssh[0] = c->ks_stride_head;
+  p->ssp[1] = c->vs_stride_page, p->ssh[1] = c->vs_stride_head;
+  p->msp = c->mass_stride_page, p->msh = c->mass_stride_head;
+  p->table = c->page_table;
+  p->table_stride = c->table_stride;
+  p->lengths = c->lengths;
+  p->num_pages = static_cast<int>(c->num_pages);
+  p->heads = static_cast<int>(c->heads_kv);
+  p->page_shift = c->page_tokens == 16 ? 4 : c->page_tokens == 32 ? 5 : c->page_tokens == 64 ? 6 : 7;
+  p->max_pages = static_cast<int>(c->max_pages);
+  p->batch = static_cast<int>(c->batch);
+  return KAB_OK;
+}
+
+template <int T>
+void launch_append(const AppendArgs& a, dim3 grid, int ch, unsigned* status, cudaStream_t s) {
+  if (ch <= 1) append_pages_kernel<T, 1><<<grid, 256, 0, s>>>(a, status);
+  else if (ch <= 2) append_pages_kernel<T, 2><<<grid, 256, 0, s>>>(a, status);
+  else if (ch <= 4) append_pages_kernel<T, 4><<<grid, 256, 0, s>>>(a, status);
+  else append_pages_kernel<T, 8><<<grid, 256, 0, s>>>(a, status);
+}
+
+int attention_check(const KabKvPagesAttention* p, PagesAttnArgs* g) {
+  KAB_REQUIRE(p != nullptr, "null parameters");
+  if (int e = pool_check(&p->cache, &g->pool)) return e;
+  KAB_REQUIRE(valid_dtype(p->q_dtype), "unknown dtype %d", p->q_dtype);
+  KAB_REQUIRE(p->heads_q >= 0 && p->q_len >= 0, "negative shape");
+  KAB_REQUIRE(p->heads_q % p->cache.heads_kv == 0, "heads_q %lld is not a multiple of heads_kv %lld",
+              (long long)p->heads_q, (long long)p->cache.heads_kv);
+  KAB_REQUIRE(p->heads_q * p->q_len < (int64_t(1) << 20), "too many query rows per sequence");
+  KAB_REQUIRE(!p->use_mass || p->cache.mass != nullptr || p->cache.num_pages == 0, "use_mass without a mass");
+  g->q = p->q;
+  g->qb = p->q_stride_b;
+  g->qh = p->q_stride_h;
+  g->qt = p->q_stride_t;
+  g->out = p->out;
+  g->scale_log2 = p->sm_scale * 1.4426950408889634f;
+  g->heads_q = static_cast<int>(p->heads_q);
+  g->q_len = static_cast<int>(p->q_len);
+  g->causal = p->causal != 0;
+  return KAB_OK;
+}
+
+size_t attention_workspace(const KabKvPagesAttention* p) {
+  return p->use_mass ? static_cast<size_t>(p->cache.batch * p->heads_q * p->q_len) * 8 : 0;
+}
+
+template <int T, int D>
+int launch_attention(const PagesAttnArgs& g, bool mass, unsigned* status, cudaStream_t s) {
+  pages_attention_kernel<T, D><<<dim3(g.heads_q * g.q_len, g.pool.batch), 128, 0, s>>>(g, status);
+  if (mass) {
+    const int tokens = g.pool.max_pages << g.pool.page_shift;
+    pages_mass_kernel<T, D><<<dim3(std::max(1, std::min(tokens / 4, 256)), g.pool.heads, g.pool.batch), 128, 0, s>>>(
+        g, status);
+  }
+  return check_launch("kab_kv_pages_attention");
+}
+
+}  // namespace
+}  // namespace kab
+
+using namespace kab;
+
+extern "C" {
+
+int kab_kv_pages_append(const KabKvPages* cache, const void* k, const void* v, int dtype, int64_t k_stride_b,
+                        int64_t k_stride_h, int64_t k_stride_t, int64_t v_stride_b, int64_t v_stride_h,
+                        int64_t v_stride_t, int64_t new_tokens, const int32_t* counts, int32_t* lengths_out,
+                        void* stream) {
+  AppendArgs a{};
+  if (int e = pool_check(cache, &a.pool)) return e;
+  KAB_REQUIRE(valid_dtype(dtype), "unknown dtype %d", dtype);
+  KAB_REQUIRE(new_tokens >= 0 && new_tokens < (int64_t(1) << 30), "bad number of new tokens");
+  if (cache->batch == 0) return KAB_OK;
+  KAB_REQUIRE(lengths_out != nullptr, "null lengths_out");
+  KAB_REQUIRE(new_tokens == 0 || (k != nullptr && v != nullptr), "null pointer");
+  KAB_REQUIRE(aligned(k, 16) && aligned(v, 16) && k_stride_b % 8 == 0 && k_stride_h % 8 == 0 && k_stride_t % 8 == 0 &&
+                  v_stride_b % 8 == 0 && v_stride_h % 8 == 0 && v_stride_t % 8 == 0,
+              "k and v must be 16-byte aligned and their strides multiples of 8 elements");
+  unsigned* status = status_word();
+  KAB_REQUIRE(status != nullptr, "no device status word");
+  const cudaStream_t s = as_stream(stream);
+  const int P = static_cast<int>(cache->page_tokens);
+  a.x[0] = k, a.x[1] = v;
+  a.xb[0] = k_stride_b, a.xh[0] = k_stride_h, a.xt[0] = k_stride_t;
+  a.xb[1] = v_stride_b, a.xh[1] = v_stride_h, a.xt[1] = v_stride_t;
+  a.counts = counts;
+  const bool in_place = lengths_out == cache->lengths;
+  a.lengths_out = in_place ? nullptr : lengths_out;
+  a.new_tokens = static_cast<int>(new_tokens);
+  // a first page with one free slot, then whole pages
+  a.touched = new_tokens == 0 ? 1 : static_cast<int>((new_tokens + P - 2) / P + 1);
+  a.d_shift = cache->head_dim == 64 ? 3 : 4;
+  KAB_REQUIRE(cache->batch * a.touched < (int64_t(1) << 31), "too many pages");
+  if (new_tokens > 0 || !in_place) {
+    const int rows = static_cast<int>(std::min<int64_t>(new_tokens, P));
+    const int ch = (rows * (1 << a.d_shift) + 255) / 256;
+    const dim3 grid(static_cast<unsigned>(cache->batch * a.touched), static_cast<unsigned>(cache->heads_kv), 2);
+    if (dtype == KAB_BF16) launch_append<kBF16>(a, grid, ch, status, s);
+    else if (dtype == KAB_F16) launch_append<kF16>(a, grid, ch, status, s);
+    else launch_append<kF32>(a, grid, ch, status, s);
+    if (int e = check_launch("kab_kv_pages_append")) return e;
+  }
+  if (in_place && new_tokens > 0) {
+    advance_lengths_kernel<<<(a.pool.batch + 255) / 256, 256, 0, s>>>(
+        cache->lengths, counts, a.new_tokens, a.pool.max_pages << a.pool.page_shift, a.pool.batch, lengths_out);
+    return check_launch("kab_kv_pages_append lengths");
+  }
+  return KAB_OK;
+}
+
+int kab_kv_pages_attention_workspace(const KabKvPagesAttention* params, size_t* bytes, size_t* zero_bytes) {
+  PagesAttnArgs g{};
+  if (int e = attention_check(params, &g)) return e;
+  KAB_REQUIRE(bytes != nullptr && zero_bytes != nullptr, "null pointer");
+  *bytes = attention_workspace(params);
+  *zero_bytes = 0;
+  return KAB_OK;
+}
+
+int kab_kv_pages_attention(const KabKvPagesAttention* params, void* workspace, size_t workspace_bytes, void* stream) {
+  PagesAttnArgs g{};
+  if (int e = attention_check(params, &g)) return e;
+  if (params->cache.batch == 0 || params->heads_q == 0 || params->q_len == 0) return KAB_OK;
+  KAB_REQUIRE(params->q != nullptr && params->out != nullptr, "null pointer");
+  const size_t need = attention_workspace(params);
+  KAB_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && aligned(workspace, 256)),
+              "the workspace needs %zu bytes, 256-byte aligned (kab_kv_pages_attention_workspace)", need);
+  unsigned* status = status_word();
+  KAB_REQUIRE(status != nullptr, "no device status word");
+  if (params->use_mass) g.ml = static_cast<float*>(workspace);
+  const cudaStream_t s = as_stream(stream);
+  const bool mass = params->use_mass && params->cache.max_pages > 0;
+#define KAB_PAGES_D(TT)                                                              \
+  return params->cache.head_dim == 128 ? launch_attention<TT, 128>(g, mass, status, s) \
+                                       : launch_attention<TT, 64>(g, mass, status, s)
+  if (params->q_dtype == KAB_BF16) KAB_PAGES_D(kBF16);
+  if (params->q_dtype == KAB_F16) KAB_PAGES_D(kF16);
+  KAB_PAGES_D(kF32);
+#undef KAB_PAGES_D
+}
+
+int kab_kv_pages_evict(const KabKvPages* cache, const int32_t* out_table, int64_t out_stride, int64_t budget,
+                       int64_t recent, int64_t sinks, int32_t* kept, int32_t* lengths_out, void* stream) {
+  EvictArgs a{};
+  if (int e = pool_check(cache, &a.pool)) return e;
+  KAB_REQUIRE(budget >= 1 && recent >= 0 && sinks >= 0 && sinks + recent <= budget,
+              "budget %lld must be at least 1 and hold the %lld first and %lld last tokens", (long long)budget,
+              (long long)sinks, (long long)recent);
+  KAB_REQUIRE(budget < (int64_t(1) << 30), "the budget is too large");
+  if (cache->batch == 0) return KAB_OK;
+  KAB_REQUIRE(out_table && kept && lengths_out, "null pointer");
+  KAB_REQUIRE(cache->mass != nullptr || cache->num_pages == 0, "an eviction needs the tokens' mass");
+  unsigned* status = status_word();
+  KAB_REQUIRE(status != nullptr, "no device status word");
+  a.out_table = out_table;
+  a.out_stride = out_stride;
+  a.kept = kept;
+  a.lengths_out = lengths_out;
+  a.budget = static_cast<int>(budget);
+  a.recent = static_cast<int>(recent);
+  a.sinks = static_cast<int>(sinks);
+  const cudaStream_t s = as_stream(stream);
+  const unsigned heads = static_cast<unsigned>(cache->heads_kv), batch = static_cast<unsigned>(cache->batch);
+  evict_select_kernel<<<dim3(heads, batch), 1024, 0, s>>>(a, status);
+  if (int e = check_launch("kab_kv_pages_evict select")) return e;
+  const int64_t P = cache->page_tokens;
+  const int64_t pages = std::min((budget + P - 1) / P, std::max<int64_t>(cache->max_pages, 1));
+  const dim3 grid(static_cast<unsigned>(pages), heads, batch);
+  const int half = cache->head_dim == 64 ? 2 : 3;
+  const int ch = static_cast<int>((P << half) / 128);
+  if (ch <= 1) evict_move_kernel<1><<<grid, 128, 0, s>>>(a, half, status);
+  else if (ch <= 2) evict_move_kernel<2><<<grid, 128, 0, s>>>(a, half, status);
+  else if (ch <= 4) evict_move_kernel<4><<<grid, 128, 0, s>>>(a, half, status);
+  else evict_move_kernel<8><<<grid, 128, 0, s>>>(a, half, status);
+  return check_launch("kab_kv_pages_evict move");
+}
+
+}  // extern "C"

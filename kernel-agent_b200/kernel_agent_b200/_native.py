@@ -92,6 +92,30 @@ class KabKvDecodeParams(ctypes.Structure):
     ]
 
 
+class KabKvPages(ctypes.Structure):
+    _fields_ = [
+        ("k_pages", c_void_p), ("v_pages", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+        ("mass", c_void_p),
+        ("k_stride_page", c_int64), ("k_stride_head", c_int64), ("k_stride_token", c_int64),
+        ("v_stride_page", c_int64), ("v_stride_head", c_int64), ("v_stride_token", c_int64),
+        ("ks_stride_page", c_int64), ("ks_stride_head", c_int64),
+        ("vs_stride_page", c_int64), ("vs_stride_head", c_int64),
+        ("mass_stride_page", c_int64), ("mass_stride_head", c_int64),
+        ("num_pages", c_int64), ("heads_kv", c_int64), ("page_tokens", c_int64), ("head_dim", c_int64),
+        ("page_table", c_void_p), ("table_stride", c_int64), ("max_pages", c_int64), ("batch", c_int64),
+        ("lengths", c_void_p),
+    ]
+
+
+class KabKvPagesAttention(ctypes.Structure):
+    _fields_ = [
+        ("cache", KabKvPages),
+        ("q", c_void_p), ("q_dtype", c_int), ("causal", c_int), ("use_mass", c_int), ("sm_scale", c_float),
+        ("q_stride_b", c_int64), ("q_stride_h", c_int64), ("q_stride_t", c_int64),
+        ("heads_q", c_int64), ("q_len", c_int64), ("out", c_void_p),
+    ]
+
+
 # name -> argument types (the return type is int unless listed in _RESTYPES)
 _SIGNATURES: dict[str, list] = {
     "kab_last_error": [],
@@ -151,6 +175,15 @@ _SIGNATURES: dict[str, list] = {
                          c_void_p, c_int64, c_int64, c_void_p],
     "kab_kv_decode_workspace": [POINTER(KabKvDecodeParams), POINTER(c_int), POINTER(c_size_t)],
     "kab_kv_decode_fp8": [POINTER(KabKvDecodeParams), c_void_p, c_size_t, c_void_p],
+    "kab_gemv_fp4_workspace": [c_int64, c_int64, c_int64, c_int, c_int, POINTER(c_size_t), POINTER(c_size_t)],
+    "kab_gemv_fp4": [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_int64, c_int64,
+                     c_int64, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_size_t, c_void_p],
+    "kab_kv_pages_append": [POINTER(KabKvPages), c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64,
+                            c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p],
+    "kab_kv_pages_attention_workspace": [POINTER(KabKvPagesAttention), POINTER(c_size_t), POINTER(c_size_t)],
+    "kab_kv_pages_attention": [POINTER(KabKvPagesAttention), c_void_p, c_size_t, c_void_p],
+    "kab_kv_pages_evict": [POINTER(KabKvPages), c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p,
+                           c_void_p],
     "kab_mxfp8_saturation": [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p],
     "kab_fp4_scale_check": [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int, c_void_p,
                             c_void_p],

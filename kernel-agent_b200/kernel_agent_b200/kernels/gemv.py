@@ -1,0 +1,90 @@
+"""Weight-only FP4 linear for the few tokens of a decode step.
+
+:func:`fp4_w4a16_linear` multiplies activations as they are (no quantisation of ``x``) with a
+weight that :func:`kernel_agent_b200.kernels.quant.quantize_fp4` made, in the layout that
+:func:`~kernel_agent_b200.kernels.quant.fp4_w4a4_linear` reads: one copy of a weight serves the
+prompt (W4A4 on the tensor cores' FP4 rate) and the single tokens, where only the weight's bytes
+count. The reference's decode example for such weights is
+``src/kernel_agent/agent/examples/cuda_fp4_gemv.py``.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from .. import _native as nat
+from . import quant as q
+from ._workspace import workspace
+from .gemm import _bias
+
+_FORMATS = {"nvfp4": (nat.KAB_NVFP4, 16), "mxfp4": (nat.KAB_MXFP4, 32)}
+_PLANS: dict[tuple, tuple[int, int]] = {}
+
+
+def _plan(m: int, n: int, k: int, fmt: int, dtype: int, device: int | None) -> tuple[int, int]:
+    """Workspace bytes of a shape, and how many of them start at zero (asked once)."""
+    key = (m, n, k, fmt, dtype, device)
+    plan = _PLANS.get(key)
+    if plan is None:
+        nbytes, zero = ctypes.c_size_t(0), ctypes.c_size_t(0)
+        nat.call("kab_gemv_fp4_workspace", m, n, k, fmt, dtype, ctypes.byref(nbytes), ctypes.byref(zero))
+        plan = _PLANS[key] = (int(nbytes.value), int(zero.value))
+    return plan
+
+
+def fp4_w4a16_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, tensor_scale: torch.Tensor | float,
+                     bias: torch.Tensor | None = None, *, fmt: str = "nvfp4") -> torch.Tensor:
+    """``x @ Wᵀ (+ bias)`` with ``W = e2m1(codes) * scales * tensor_scale``: exact products of
+    ``x`` (bf16, fp16 or fp32) and the weight's values, fp32 sums, ``acc * tensor_scale (+
+    bias)`` in fp32 and one rounding to ``x``'s dtype.
+
+    ``x [..., K]``; ``codes [N, K / 2]`` (packed e2m1, low nibble first); ``scales [N, K /
+    block]`` (e4m3 per 16 for ``fmt="nvfp4"``, e8m0 per 32 for ``"mxfp4"``) or the same already
+    swizzled (flat, 128 x 4 blocks); ``tensor_scale`` one value or one per row of the weight.
+    Made for up to about 32 rows of ``x``, where the weight's bytes bound it; more rows work, the
+    weight being read again for every 8."""
+    if fmt not in _FORMATS:
+        raise ValueError(f"unknown FP4 format {fmt!r} (one of {', '.join(_FORMATS)})")
+    code, block = _FORMATS[fmt]
+    nat.require_cuda(x, codes, scales, bias)
+    if x.dim() < 1 or codes.dim() != 2:
+        raise ValueError(f"expected x [..., K] and codes [N, K / 2]; got {tuple(x.shape)}, {tuple(codes.shape)}")
+    n, k = codes.shape[0], x.shape[-1]
+    if k % block:
+        raise ValueError(f"the last dimension {k} is not a multiple of the {fmt} block ({block})")
+    if codes.shape[1] * 2 != k or codes.element_size() != 1:
+        raise ValueError(f"codes {tuple(codes.shape)} {codes.dtype} do not fit x {tuple(x.shape)}: expected "
+                         f"[N, {k // 2}] bytes")
+    if scales.element_size() != 1:
+        raise ValueError(f"scales must be one byte each (e4m3 or e8m0), got {scales.dtype}")
+    cols = k // block
+    swizzle = scales.dim() == 1
+    if swizzle and scales.numel() != -(-n // 128) * 128 * (-(-cols // 4)) * 4:
+        raise ValueError(f"swizzled scales have {scales.numel()} bytes, expected "
+                         f"{-(-n // 128) * 128 * (-(-cols // 4)) * 4}")
+    if not swizzle and tuple(scales.shape) != (n, cols):
+        raise ValueError(f"expected scales [{n}, {cols}], got {tuple(scales.shape)}")
+    x2 = q._rows(q._input(x))
+    m = x2.shape[0]
+    c, s = codes.contiguous(), scales.contiguous()
+    if c.data_ptr() % 8:
+        c = c.clone()
+    ts = tensor_scale
+    if not isinstance(ts, torch.Tensor) or ts.dtype != torch.float32 or not ts.is_cuda or not ts.is_contiguous():
+        ts = torch.as_tensor(ts, dtype=torch.float32, device=x.device).contiguous()
+    if ts.numel() not in (1, n):
+        raise ValueError(f"tensor_scale has {ts.numel()} values, expected 1 or {n}")
+    b, bias_code = (None, nat.KAB_F32) if bias is None else _bias(bias, n, x.device)
+    out = torch.empty(m, n, dtype=x2.dtype, device=x.device)
+    if m and n:
+        dtype = nat.dtype_code(x2)
+        with torch.cuda.device(x.device):
+            stream = nat.stream_of(x2)
+            nbytes, zero = _plan(m, n, k, code, dtype, x.device.index)
+            ws = workspace(f"gemv {m} {n} {k} {code} {dtype}", x.device, stream, nbytes, zero) if nbytes else None
+            nat.call("kab_gemv_fp4", x2.data_ptr(), dtype, x2.stride(0) if m > 1 else max(k, 8), c.data_ptr(),
+                     s.data_ptr(), int(swizzle), code, ts.data_ptr(), int(ts.numel() > 1), m, n, k, nat.ptr(b),
+                     bias_code, out.data_ptr(), n, nat.ptr(ws), nbytes, stream)
+    return q._linear_out(out, x, n)

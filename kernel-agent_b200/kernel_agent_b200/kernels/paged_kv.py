@@ -1,0 +1,234 @@
+"""A paged FP8 KV cache with one scale per (page, KV head): append, attention, eviction.
+
+Where :mod:`kernel_agent_b200.kernels.kv_quant` holds one contiguous cache per batch with a scale
+per (token, head), this cache is a pool of pages that sequences of any lengths share through a
+page table, and the scales shrink to one per page and head. A page's scale is a power of two, so
+a page that grows past it, or tokens that move to another page, keep their values (but for codes
+that become subnormal).
+
+* :func:`append_kv_pages`: quantise new tokens into their slots (prompts and single tokens).
+* :func:`paged_kv_attention`: attention of the newest tokens over the pages; optionally adds the
+  weight that every cached token received to its ``mass``.
+* :func:`evict_kv_pages`: keep the first, the newest and the heaviest tokens, in other pages.
+* :class:`PagedFp8KVCache`: the pool, its page table and its free pages.
+
+K and V pages are ``[num_pages, kv_heads, page_tokens, head_dim]`` e4m3 (views with other strides
+are fine, the last one 1), their scales ``[num_pages, kv_heads]`` fp32, ``mass [num_pages,
+kv_heads, page_tokens]`` fp32; ``page_table [batch, max_pages]`` and ``lengths [batch]`` int32, on
+the device. The kernels check page numbers and lengths themselves: a bad one is skipped and raises
+bit 2 of :func:`kernel_agent_b200._native.device_status`.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from .. import _native as nat
+from ._workspace import workspace
+
+_E4M3 = torch.float8_e4m3fn
+PAGE_TOKENS = (16, 32, 64, 128)
+HEAD_DIMS = (64, 128)
+_TEMPLATES: dict[tuple, tuple] = {}
+
+
+def _pool_fields(p, k_pages, k_scale, v_pages, v_scale, mass, page_table, lengths) -> None:
+    """Checks the cache's tensors and fills everything of ``p`` but the pointers."""
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
+        raise ValueError(f"pages must be [num_pages, kv_heads, page_tokens, head_dim]; got K {tuple(k_pages.shape)}, "
+                         f"V {tuple(v_pages.shape)}")
+    if k_pages.dtype != _E4M3 or v_pages.dtype != _E4M3:
+        raise ValueError("the pages must be float8_e4m3fn")
+    pages, heads, page, dim = k_pages.shape
+    if page not in PAGE_TOKENS:
+        raise ValueError(f"page_tokens {page}: one of {', '.join(map(str, PAGE_TOKENS))}")
+    if dim not in HEAD_DIMS:
+        raise ValueError(f"head_dim {dim}: the paged cache takes 64 or 128")
+    for name, t, shape in (("k_scale", k_scale, (pages, heads)), ("v_scale", v_scale, (pages, heads)),
+                           ("mass", mass, (pages, heads, page))):
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != shape):
+            raise ValueError(f"{name} must be float32 {list(shape)}; got {t.dtype} {tuple(t.shape)}")
+    if mass is not None and mass.stride(2) != 1:
+        raise ValueError("mass needs a unit last stride")
+    if k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
+        raise ValueError("the pages need a unit last stride")
+    if page_table.dtype != torch.int32 or page_table.dim() != 2:
+        raise ValueError(f"page_table must be int32 [batch, max_pages]; got {page_table.dtype} "
+                         f"{tuple(page_table.shape)}")
+    if page_table.shape[1] > 1 and page_table.stride(1) != 1:
+        raise ValueError("page_table needs a unit last stride")
+    batch = page_table.shape[0]
+    if lengths.dtype != torch.int32 or tuple(lengths.shape) != (batch,) or not lengths.is_contiguous():
+        raise ValueError(f"lengths must be int32 [{batch}], contiguous; got {lengths.dtype} {tuple(lengths.shape)}")
+    p.k_stride_page, p.k_stride_head, p.k_stride_token = k_pages.stride()[:3]
+    p.v_stride_page, p.v_stride_head, p.v_stride_token = v_pages.stride()[:3]
+    p.ks_stride_page, p.ks_stride_head = k_scale.stride()
+    p.vs_stride_page, p.vs_stride_head = v_scale.stride()
+    if mass is not None:
+        p.mass_stride_page, p.mass_stride_head = mass.stride()[:2]
+    p.num_pages, p.heads_kv, p.page_tokens, p.head_dim = pages, heads, page, dim
+    p.table_stride, p.max_pages, p.batch = page_table.stride(0), page_table.shape[1], batch
+
+
+def _layout(t: torch.Tensor | None) -> tuple | None:
+    return None if t is None else (t.shape, t.stride(), t.dtype)
+
+
+def _cache_key(*tensors) -> tuple:
+    return tuple(_layout(t) for t in tensors)
+
+
+def _pointers(p, k_pages, k_scale, v_pages, v_scale, mass, page_table, lengths) -> None:
+    p.k_pages, p.k_scale = k_pages.data_ptr(), k_scale.data_ptr()
+    p.v_pages, p.v_scale = v_pages.data_ptr(), v_scale.data_ptr()
+    if mass is not None:
+        p.mass = mass.data_ptr()
+    p.page_table, p.lengths = page_table.data_ptr(), lengths.data_ptr()
+
+
+def _pool(cache: tuple) -> "nat.KabKvPages":
+    """The parameters of a cache; the checks run once per layout."""
+    key = ("pool", *_cache_key(*cache))
+    made = _TEMPLATES.get(key)
+    if made is None:
+        p = nat.KabKvPages()
+        _pool_fields(p, *cache)
+        made = _TEMPLATES[key] = (bytes(p),)
+    p = nat.KabKvPages.from_buffer_copy(made[0])
+    _pointers(p, *cache)
+    return p
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """Rows that the kernels can load 16 bytes at a time."""
+    st = t.stride()
+    if st[3] != 1 or st[0] % 8 or st[1] % 8 or st[2] % 8 or t.data_ptr() % 16:
+        return t.contiguous()
+    return t
+
+
+def append_kv_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, k_scale: torch.Tensor,
+                    v_pages: torch.Tensor, v_scale: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+                    counts: torch.Tensor | None = None, mass: torch.Tensor | None = None,
+                    out_lengths: torch.Tensor | None = None) -> torch.Tensor:
+    """Write the first ``counts[b]`` (default: all) tokens of ``k``, ``v [batch, kv_heads, new,
+    head_dim]`` (bf16, fp16 or fp32) after the ``lengths[b]`` cached tokens of each sequence, into
+    the pages that ``page_table`` gives them; returns the new lengths (``out_lengths`` if given,
+    which may be ``lengths`` itself).
+
+    A page's scale is the smallest power of two ``s >= 2**-126`` with ``|x| <= 448 s`` for every
+    finite value appended to it; codes are ``e4m3(x / s)``, to nearest even. Appending to a page
+    that would need a larger scale rewrites the page's codes as ``e4m3(code * old / s)``. An
+    infinity becomes the largest code of its sign, NaN stays NaN. ``mass`` of the new slots
+    becomes 0."""
+    nat.require_cuda(k, v, k_pages, k_scale, v_pages, v_scale, page_table, lengths, counts, mass, out_lengths)
+    p = _pool((k_pages, k_scale, v_pages, v_scale, mass, page_table, lengths))
+    if k.dim() != 4 or v.shape != k.shape or k.shape[0] != p.batch or k.shape[1] != p.heads_kv \
+            or k.shape[3] != p.head_dim:
+        raise ValueError(f"expected k and v [{p.batch}, {p.heads_kv}, new, {p.head_dim}]; got {tuple(k.shape)}, "
+                         f"{tuple(v.shape)}")
+    if k.dtype != v.dtype or k.dtype not in nat.DTYPES:
+        raise ValueError(f"k and v must both be float32, bfloat16 or float16; got {k.dtype}, {v.dtype}")
+    for name, t in (("counts", counts), ("out_lengths", out_lengths)):
+        if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (p.batch,) or not t.is_contiguous()):
+            raise ValueError(f"{name} must be int32 [{p.batch}], contiguous; got {t.dtype} {tuple(t.shape)}")
+    k, v = _rows16(k.detach()), _rows16(v.detach())
+    out = torch.empty_like(lengths) if out_lengths is None else out_lengths
+    with torch.cuda.device(k.device):
+        nat.call("kab_kv_pages_append", ctypes.byref(p), k.data_ptr(), v.data_ptr(), nat.DTYPES[k.dtype],
+                 *k.stride()[:3], *v.stride()[:3], k.shape[2], nat.ptr(counts), out.data_ptr(), nat.stream_of(k))
+    return out
+
+
+def paged_kv_attention(q: torch.Tensor, k_pages: torch.Tensor, k_scale: torch.Tensor, v_pages: torch.Tensor,
+                       v_scale: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+                       scale: float | None = None, causal: bool = True, mass: torch.Tensor | None = None,
+                       out: torch.Tensor | None = None) -> torch.Tensor:
+    """softmax(Q Kᵀ · scale) V over the pages, in ``q``'s dtype: ``q [B, Hq, D]`` (one query token
+    per sequence) or ``[B, Hq, Lq, D]`` (bf16, fp16 or fp32; Hq a multiple of the cache's KV
+    heads), ``scale`` default ``D ** -0.5``.
+
+    With ``causal`` the queries are the newest ``Lq`` cached tokens: query i sees the first
+    ``lengths[b] - Lq + 1 + i`` tokens; without it every query sees every token. A query that sees
+    nothing gives zeros. With ``mass``, the weight of every cached token, summed over the query
+    heads of its KV head and the query tokens, is added to its entry. Made for the few rows (query
+    heads per KV head x query tokens) of a decode step: each 16 rows read the cache once more.
+    Results do not depend on the other sequences' lengths but in the last bits (the cache is cut
+    into equal parts for the GPU, whose softmax sums are merged), and are the same for the same
+    inputs."""
+    if q.dim() not in (3, 4):
+        raise ValueError(f"q must be [B, Hq, D] or [B, Hq, Lq, D]; got {tuple(q.shape)}")
+    nat.require_cuda(q, k_pages, k_scale, v_pages, v_scale, page_table, lengths, mass, out)
+    if q.dtype not in nat.DTYPES:
+        raise ValueError(f"unsupported dtype {q.dtype} (float32, bfloat16 or float16)")
+    q4 = q.detach() if q.dim() == 4 else q.detach().unsqueeze(2)
+    if q4.stride(3) != 1:
+        q4 = q4.contiguous()
+    cache = (k_pages, k_scale, v_pages, v_scale, mass, page_table, lengths)
+    key = ("attention", q4.shape, q4.stride(), q4.dtype, q4.device.index, scale, bool(causal), *_cache_key(*cache))
+    made = _TEMPLATES.get(key)
+    if made is None:
+        t = nat.KabKvPagesAttention()
+        _pool_fields(t.cache, *cache)
+        b, hq, lq, d = q4.shape
+        if b != t.cache.batch or d != t.cache.head_dim or hq % t.cache.heads_kv:
+            raise ValueError(f"q {tuple(q.shape)} does not fit the cache: {t.cache.batch} sequences, "
+                             f"{t.cache.heads_kv} KV heads, head_dim {t.cache.head_dim}")
+        t.q_dtype, t.causal, t.use_mass = nat.DTYPES[q4.dtype], int(bool(causal)), int(mass is not None)
+        t.sm_scale = float(d ** -0.5 if scale is None else scale)
+        t.q_stride_b, t.q_stride_h, t.q_stride_t = q4.stride()[:3]
+        t.heads_q, t.q_len = hq, lq
+        _pointers(t.cache, *cache)
+        nbytes, zero = ctypes.c_size_t(0), ctypes.c_size_t(0)
+        with torch.cuda.device(q4.device):
+            nat.call("kab_kv_pages_attention_workspace", ctypes.byref(t), ctypes.byref(nbytes), ctypes.byref(zero))
+        made = _TEMPLATES[key] = (bytes(t), int(nbytes.value), int(zero.value))
+    template, nbytes, zero = made
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError(f"out must be {q.dtype} {list(q.shape)}, contiguous; got {out.dtype} {tuple(out.shape)}")
+    p = nat.KabKvPagesAttention.from_buffer_copy(template)
+    _pointers(p.cache, *cache)
+    p.q, p.out = q4.data_ptr(), out.data_ptr()
+    with torch.cuda.device(q4.device):
+        stream = nat.stream_of(q4)
+        ws = workspace(f"pages attention {zero}", q4.device, stream, nbytes, zero) if nbytes else None
+        nat.call("kab_kv_pages_attention", ctypes.byref(p), nat.ptr(ws), nbytes, stream)
+    return out
+
+
+def evict_kv_pages(k_pages: torch.Tensor, k_scale: torch.Tensor, v_pages: torch.Tensor, v_scale: torch.Tensor,
+                   mass: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, out_page_table: torch.Tensor,
+                   *, budget: int, recent: int = 0, sinks: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
+    """Keep ``min(lengths[b], budget)`` tokens of every (sequence, KV head) and copy them, in their
+    order, into the pages of ``out_page_table [batch, >= ceil(budget / page_tokens)]``: pages of the
+    same pool that no sequence uses (the old ones are free afterwards). Kept are the first
+    ``sinks`` tokens, the last ``recent`` and, of the others, those of the largest ``mass`` (equal
+    masses: the first; NaN counts as the largest). Codes move to the smallest power-of-two scale
+    that holds the page's new tokens; masses move along.
+
+    Returns ``(kept [batch, kv_heads, budget] int32, lengths [batch] int32)``: the kept token
+    numbers (-1 past the last) and the new lengths."""
+    budget, recent, sinks = int(budget), int(recent), int(sinks)
+    if mass is None:
+        raise ValueError("an eviction needs the tokens' mass")
+    nat.require_cuda(k_pages, k_scale, v_pages, v_scale, mass, page_table, lengths, out_page_table)
+    p = _pool((k_pages, k_scale, v_pages, v_scale, mass, page_table, lengths))
+    if budget < 1 or recent < 0 or sinks < 0 or sinks + recent > budget:
+        raise ValueError(f"budget {budget} must be at least 1 and hold the {sinks} first and {recent} last tokens")
+    need = min(-(-budget // p.page_tokens), max(p.max_pages, 1))
+    if out_page_table.dtype != torch.int32 or out_page_table.dim() != 2 or out_page_table.shape[0] != p.batch \
+            or out_page_table.shape[1] < need or (out_page_table.shape[1] > 1 and out_page_table.stride(1) != 1):
+        raise ValueError(f"out_page_table must be int32 [{p.batch}, >= {need}] with a unit last stride; got "
+                         f"{out_page_table.dtype} {tuple(out_page_table.shape)}")
+    if out_page_table.data_ptr() == page_table.data_ptr() and page_table.numel():
+        raise ValueError("out_page_table must name other pages than page_table")
+    kept = torch.empty(p.batch, p.heads_kv, budget, dtype=torch.int32, device=mass.device)
+    out = torch.empty_like(lengths)
+    with torch.cuda.device(mass.device):
+        nat.call("kab_kv_pages_evict", ctypes.byref(p), out_page_table.data_ptr(), out_page_table.stride(0), budget,
+                 recent, sinks, kept.data_ptr(), out.data_ptr(), nat.stream_of(mass))
+    return kept, out
