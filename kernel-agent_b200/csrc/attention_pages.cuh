@@ -1,6 +1,29 @@
 // Attention of a few query tokens over the paged FP8 cache (kv_pages.cuh):
 // softmax(q K^T * scale) V per query row, K = code * page scale, and the weight that every cached
 // token receives added to its mass.
+//
+// The cache is read once and that bounds it: 2 D bytes per token and KV head against
+// 4 D * rows operations, far below the tensor cores' rate for the few rows (query heads of one KV
+// head x query tokens) of a decode step. So the products run on mma.sync.m16n8k16 (f16 in, fp32
+// accumulators), 16 rows at a time: e4m3 -> f16 is one exact conversion per two codes, and the
+// instruction's fragments let the codes go from shared memory to the tensor core without leaving
+// the warp. What has to be fast is the stream: every warp keeps its own ring of 16-token slabs of
+// K and V in flight with cp.async and never waits for another warp inside a segment.
+//
+//  * Work is cut into equal parts whatever the lengths: the slabs of all (sequence, KV head, 16
+//    rows) items stand in one line, and each block takes a contiguous part of it. A block's first
+//    and last item may be shared with its neighbours: their partial results (maximum, sum,
+//    output) go to two slots of the block's own, and the block that finishes an item last merges
+//    them in order, so the same inputs give the same bits.
+//  * Queries enter as f16, each row in units of a power of two that puts its largest value in
+//    [2^14, 2^15): bf16 and f16 values keep all their bits down to 2^-29 of the row's largest;
+//    fp32 ones are split into two f16 terms (22 bits) and the product is taken twice.
+//  * The running maximum is that of t = s + log2(V scale), s the score in log2 units: the weight
+//    that multiplies the V codes is w = 2^(s - m) * V scale <= 2^15 with m = max t - 15, so w fits
+//    f16 with 11 bits down to 2^-29 of the largest and the page's scale costs one multiplication.
+//    Sums use 2^(s - m) itself, in fp32. (Adding every slab's product to the output with its own
+//    scale instead would cost 64 more multiply-adds per lane and slab.) log2(V scale) is cut at
+//    -80, which keeps the sums finite; values below 2^-80 * 448 round to zero beside it.
 #pragma once
 
 #include "kv_pages.cuh"
@@ -14,7 +37,12 @@ struct PagesAttnArgs {
   void* out;
   float scale_log2;  // sm_scale * log2(e)
   int heads_q, q_len, causal;
-  float* ml;  // [batch, heads_q, q_len, 2]: each row's maximum (log2 units) and sum
+  int rows, row_tiles;   // rows of one KV head (query heads x query tokens), tiles of 16 of them
+  unsigned* counters;    // [batch, heads, row_tiles]
+  float* partial;        // [grid, 2 slots, 16 rows, D + 2]: output, maximum, sum
+  float* scores;         // [batch, heads, rows, capacity] in log2 units, or NULL
+  float* ml;             // [batch, heads, rows, 2]: reference and reciprocal sum, with scores
+  int64_t capacity;      // max_pages * page_tokens
 };
 
 template <int T>
@@ -24,96 +52,558 @@ __device__ __forceinline__ void store_elem(void* base, int64_t i, float v) {
   else static_cast<__half*>(base)[i] = __float2half_rn(v);
 }
 
-// One block per (query head, query token, sequence): each warp takes every fourth token, its
-// lanes share the head dimension, and carries the running maximum, sum and output of its tokens.
+// ------------------------------------------------------------------ instructions
+
+// Two e4m3 codes (low half of `pair`, low byte first) as f16.
+__device__ __forceinline__ uint32_t e4m3x2_f16(uint32_t pair) {
+  uint32_t r;
+  asm("{\n .reg .b16 lo, hi;\n mov.b32 {lo, hi}, %1;\n cvt.rn.f16x2.e4m3x2 %0, lo;\n}" : "=r"(r) : "r"(pair));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3x2_f16_high(uint32_t pair) {
+  uint32_t r;
+  asm("{\n .reg .b16 lo, hi;\n mov.b32 {lo, hi}, %1;\n cvt.rn.f16x2.e4m3x2 %0, hi;\n}" : "=r"(r) : "r"(pair));
+  return r;
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t f16x2_of(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 f16x2_values(uint32_t v) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 16 bytes to shared memory without waiting; `bytes` 0 writes zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// ------------------------------------------------------------------ layout
+
+template <int D, bool SPLIT>
+struct PagesLayout {
+  static constexpr int kWarps = 8, kThreads = 256, kStages = 3, kSlab = 16;
+  static constexpr int kSlabBytes = kSlab * D;              // K or V of one slab
+  static constexpr int kStageBytes = 2 * kSlabBytes;
+  static constexpr int kQBytes = D / 16 * 32 * 16 * (SPLIT ? 2 : 1);
+  static constexpr int kRing = kWarps * kStages * kStageBytes;
+  static constexpr int kScales = kWarps * kStages * 2 * 4;
+  static constexpr int kSmem = kQBytes + kRing + kScales + 256;
+  static_assert(kRing >= kWarps * 16 * (D + 2) * 4, "the merge reuses the ring");
+};
+
+// Byte offset of 16-byte chunk `chunk` of token `row` in a slab: the chunks are permuted so that
+// both readers touch all 32 banks: K (8 consecutive tokens x 4 lanes' chunks) and V (every second
+// token x neighbouring chunks).
+template <int D>
+__device__ __forceinline__ uint32_t slab_offset(int row, int chunk) {
+  if constexpr (D == 128) return row * 128 + ((chunk ^ (row & 7)) << 4);
+  else return (row >> 1) * 128 + (((((row & 1) << 2) | chunk) ^ (((row >> 1) & 3) << 1)) << 4);
+}
+
+constexpr float kNoScore = -3.3e38f;  // below every finite score
+constexpr float kWeightBits = 15.0f;  // the largest weight is 2^15 in f16
+constexpr float kLeastLogScale = -80.0f;
+
+// ------------------------------------------------------------------ the kernel
+
+// Where a position of the line of slabs lies: sequence, head, row tile, and the item's first slab.
+struct PagesItem {
+  int b, h, tile, length, slabs;
+  int64_t first;
+};
+
 template <int T, int D>
-__global__ void __launch_bounds__(128) pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
-  constexpr int E = D / 32;
+__global__ void __launch_bounds__(256, 2) pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
+  constexpr bool SPLIT = T == kF32;
+  using L = PagesLayout<D, SPLIT>;
+  constexpr int ST = L::kStages, TILES = D / 8, CHUNKS = D / 16, COPIES = D / 32;
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint4* q_frag = reinterpret_cast<uint4*>(smem);
+  uint8_t* ring = smem + L::kQBytes;
+  float* sc_all = reinterpret_cast<float*>(ring + L::kRing);
+  float* q_unit = sc_all + L::kWarps * ST * 2;                     // [16] units of the query rows
+  int* shared_i = reinterpret_cast<int*>(q_unit + 16);             // [8..] broadcast words
+  int64_t* shared_l = reinterpret_cast<int64_t*>(shared_i + 12);
+  float* merge_o = reinterpret_cast<float*>(ring);                 // [8][16][D]
+  float* merge_ml = merge_o + L::kWarps * 16 * D;                  // [8][16][2]
+
   const PagePool& p = a.pool;
-  const int hq = blockIdx.x / a.q_len, qi = blockIdx.x % a.q_len, b = blockIdx.y;
-  const int h = hq / (a.heads_q / p.heads), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int P = 1 << p.page_shift;
-  const int n = page_length(p, b, status);
-  const int seen = a.causal ? max(0, n - a.q_len + 1 + qi) : n;
-  float q[E], o[E] = {};
-#pragma unroll
-  for (int e = 0; e < E; ++e) q[e] = load_elem<T>(a.q, b * a.qb + hq * a.qh + qi * a.qt + lane * E + e) * a.scale_log2;
-  float m = -INFINITY, l = 0.0f;
-  for (int t = warp; t < seen; t += 4) {
-    const int page = page_of(p, b, t >> p.page_shift, status);
-    if (page < 0) continue;
-    const uint8_t* k = p.codes[0] + page * p.sp[0] + h * p.sh[0] + (t & (P - 1)) * p.st[0] + lane * E;
-    const uint8_t* v = p.codes[1] + page * p.sp[1] + h * p.sh[1] + (t & (P - 1)) * p.st[1] + lane * E;
-    float s = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) s = fmaf(q[e], e4m3_value_hw(k[e]), s);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    s *= p.scale[0][page * p.ssp[0] + h * p.ssh[0]];
-    const float top = fmaxf(m, s), old = m == -INFINITY ? 0.0f : exp2f(m - top), w = exp2f(s - top);
-    const float vs = w * p.scale[1][page * p.ssp[1] + h * p.ssh[1]];
-    l = l * old + w;
-    m = top;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = o[e] * old + vs * e4m3_value_hw(v[e]);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int P = 1 << p.page_shift, group = a.heads_q / p.heads, per_seq = p.heads * a.row_tiles;
+  const int cap = p.max_pages << p.page_shift;
+
+  // ---- this block's part of the line
+  auto slabs_of = [&](int b) -> int64_t {
+    const int n = min(max(__ldg(p.lengths + b), 0), cap);
+    return max((n + 15) >> 4, 1);  // an empty sequence is one empty slab: its output is written too
+  };
+  const int chunk = (p.batch + 255) / 256;
+  int64_t mine = 0;
+  for (int i = 0; i < chunk; ++i) {
+    const int b = tid * chunk + i;
+    if (b < p.batch) mine += slabs_of(b) * per_seq;
   }
-  __shared__ float sm[4], sl[4], so[4][D];
-  if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
-  }
+  int64_t upto = mine;
 #pragma unroll
-  for (int e = 0; e < E; ++e) so[warp][lane * E + e] = o[e];
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += y;
+  }
+  int64_t* warp_sum = reinterpret_cast<int64_t*>(ring);
+  if (lane == 31) warp_sum[warp] = upto;
   __syncthreads();
-  const float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  float total = 0.0f, w[4];
+  int64_t total = 0, before = upto - mine;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    w[i] = sm[i] == -INFINITY ? 0.0f : exp2f(sm[i] - top);
-    total += w[i] * sl[i];
+  for (int w = 0; w < 8; ++w) {
+    if (w < warp) before += warp_sum[w];
+    total += warp_sum[w];
   }
-  const int64_t row = (static_cast<int64_t>(b) * a.heads_q + hq) * a.q_len + qi;
-  if (threadIdx.x < D) {
-    float acc = 0.0f;
+  const int64_t grid = min(static_cast<int64_t>(gridDim.x), total);
+  if (blockIdx.x >= grid) return;
+  const int64_t lo = total * blockIdx.x / grid, hi = total * (blockIdx.x + 1) / grid;
+  if (lo >= before && lo < before + mine) {  // one thread: the sequence that `lo` lies in
+    int64_t at = before;
+    int b = tid * chunk;
+    while (lo >= at + slabs_of(b) * per_seq) at += slabs_of(b++) * per_seq;
+    shared_i[0] = b;
+    shared_l[0] = at;
+  }
+  __syncthreads();
+  PagesItem it;
+  it.b = shared_i[0];
+  {
+    const int64_t at = shared_l[0], n = slabs_of(it.b);
+    const int i = static_cast<int>((lo - at) / n);
+    it.h = i / a.row_tiles;
+    it.tile = i % a.row_tiles;
+    it.first = at + i * n;
+  }
+
+  uint8_t* my_ring = ring + warp * ST * L::kStageBytes;
+  const uint32_t my_ring_s = static_cast<uint32_t>(__cvta_generic_to_shared(my_ring));
+  float* my_sc = sc_all + warp * ST * 2;
+  const uint32_t my_sc_s = static_cast<uint32_t>(__cvta_generic_to_shared(my_sc));
+
+  for (int64_t pos = lo; pos < hi;) {
+    it.length = page_length(p, it.b, status);
+    it.slabs = static_cast<int>(slabs_of(it.b));
+    const int s0 = static_cast<int>(pos - it.first);
+    const int s1 = static_cast<int>(min(static_cast<int64_t>(it.slabs), hi - it.first));
+    const int n = it.length;
+    const int rows = min(16, a.rows - it.tile * 16);
+    const int seen_by_all = a.causal ? max(0, n - a.q_len + 1) : n;
+
+    // ---- the queries, as fragments
+    {
+      const int r = tid >> 4, part = tid & 15, rr = it.tile * 16 + r;
+      constexpr int E = D / 16;
+      float v[E];
+      uint32_t top = 0;
+      if (r < rows) {
+        const int hq = it.h * group + rr / a.q_len, qi = rr % a.q_len;
+        const int64_t base = it.b * a.qb + hq * a.qh + qi * a.qt + part * E;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc += w[i] * so[i][threadIdx.x];
-    store_elem<T>(a.out, row * D + threadIdx.x, seen > 0 ? acc / total : 0.0f);
-  }
-  if (a.ml != nullptr && threadIdx.x == 0) {
-    a.ml[2 * row] = top;
-    a.ml[2 * row + 1] = total;
+        for (int e = 0; e < E; ++e) v[e] = load_elem<T>(a.q, base + e);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = 0.0f;
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      // 2^(14 - e): the largest value lands in [2^14, 2^15); rows of zeros, infinities or NaN as they are
+      const int e = static_cast<int>(top >> 23) - 127;
+      const bool plain = top == 0 || top >= 0x7F800000u;
+      const float up = plain ? 1.0f : e >= 0 ? __uint_as_float((127u + 14u - min(e, 127)) << 23)
+                                             : __uint_as_float((127u + min(14 - max(e, -100), 127)) << 23);
+      __syncthreads();  // the previous item's readers of q_frag, q_unit and the merge are done
+      if (part == 0) q_unit[r] = 1.0f / up;
+      // dims of (step j, lane t): chunk * 16 + 4 i + {0, 1} in a0 / a1, {2, 3} in a2 / a3
+#pragma unroll
+      for (int e2 = 0; e2 < E; e2 += 2) {
+        const int d = part * E + e2, c = d >> 4, i = (d & 15) >> 2, pair = (d >> 1) & 1;
+        const int tt = D == 128 ? c >> 1 : c, j = (D == 128 ? (c & 1) * 4 : 0) + i;
+        const float x0 = v[e2] * up, x1 = v[e2 + 1] * up;
+        uint32_t* slot = reinterpret_cast<uint32_t*>(&q_frag[j * 32 + (r & 7) * 4 + tt]) + 2 * pair + (r >> 3);
+        const uint32_t hi2 = f16x2_of(x0, x1);
+        *slot = hi2;
+        if constexpr (SPLIT) {
+          const float2 h = f16x2_values(hi2);
+          slot[D / 16 * 32 * 4] = plain ? 0u : f16x2_of(x0 - h.x, x1 - h.y);
+        }
+      }
+      __syncthreads();
+    }
+    const float unit0 = q_unit[g] * a.scale_log2, unit1 = q_unit[g + 8] * a.scale_log2;
+    int seen0 = n, seen1 = n;
+    if (a.causal) {
+      seen0 = max(0, n - a.q_len + 1 + (it.tile * 16 + g) % a.q_len);
+      seen1 = max(0, n - a.q_len + 1 + (it.tile * 16 + g + 8) % a.q_len);
+    }
+
+    float o[TILES][4], m0 = kNoScore, m1 = kNoScore, l0 = 0.0f, l1 = 0.0f;
+#pragma unroll
+    for (int j = 0; j < TILES; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+
+    const uint8_t* kbase = p.codes[0] + it.h * p.sh[0];
+    const uint8_t* vbase = p.codes[1] + it.h * p.sh[1];
+    const int32_t* table = p.table + it.b * p.table_stride;
+    uint32_t valid = 0;  // bit s: stage s holds a page of the pool
+
+    auto page_at = [&](int slab) -> int {
+      if (slab >= s1 || slab * 16 >= n) return -1;
+      const int page = __ldg(table + ((slab * 16) >> p.page_shift));
+      if (page >= 0 && page < p.num_pages) return page;
+      if (lane == 0) atomicOr(status, kDevBounds);
+      return -1;
+    };
+    auto issue = [&](int slab, int page, int stage) {
+      if (page >= 0) {
+        const int tok0 = slab * 16, slot = tok0 & (P - 1);
+        const uint8_t* ks = kbase + page * p.sp[0] + slot * p.st[0];
+        const uint8_t* vs = vbase + page * p.sp[1] + slot * p.st[1];
+        const uint32_t dst = my_ring_s + stage * L::kStageBytes;
+#pragma unroll
+        for (int i = 0; i < COPIES; ++i) {
+          const int c = lane + 32 * i, row = c / CHUNKS, ch = c % CHUNKS;
+          const uint32_t off = slab_offset<D>(row, ch);
+          copy16(dst + off, ks + row * p.st[0] + ch * 16, tok0 + row < n ? 16 : 0);
+          // V of tokens that not every row sees is added apart, so that a NaN there stays with the
+          // rows that see it
+          copy16(dst + L::kSlabBytes + off, vs + row * p.st[1] + ch * 16, tok0 + row < seen_by_all ? 16 : 0);
+        }
+        if (lane < 2) copy4(my_sc_s + (stage * 2 + lane) * 4, p.scale[lane] + page * p.ssp[lane] + it.h * p.ssh[lane]);
+        valid |= 1u << stage;
+      } else {
+        valid &= ~(1u << stage);
+      }
+      copies_commit();
+    };
+
+    const int first = s0 + warp;
+#pragma unroll
+    for (int i = 0; i < ST - 1; ++i) issue(first + 8 * i, page_at(first + 8 * i), i);
+    int next_page = page_at(first + 8 * (ST - 1));
+    int stage = 0;
+    for (int slab = first; slab < s1; slab += 8) {
+      copies_wait<ST - 2>();
+      __syncwarp();
+      const int ahead = slab + 8 * (ST - 1);
+      issue(ahead, next_page, stage == 0 ? ST - 1 : stage - 1);
+      next_page = page_at(ahead + 8);
+      if ((valid >> stage) & 1u) {
+        const uint8_t* kb = my_ring + stage * L::kStageBytes;
+        const uint8_t* vb = kb + L::kSlabBytes;
+        const float ksc = my_sc[stage * 2], vsc = my_sc[stage * 2 + 1];
+        float s[2][4] = {};
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h) {
+          const int ch = D == 128 ? 2 * t + h : t;
+          const uint4 k0 = *reinterpret_cast<const uint4*>(kb + slab_offset<D>(g, ch));
+          const uint4 k1 = *reinterpret_cast<const uint4*>(kb + slab_offset<D>(g + 8, ch));
+          const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint4 af = q_frag[(h * 4 + i) * 32 + lane];
+            const uint32_t aq[4] = {af.x, af.y, af.z, af.w};
+            const uint32_t b00 = e4m3x2_f16(w0[i]), b01 = e4m3x2_f16_high(w0[i]);
+            const uint32_t b10 = e4m3x2_f16(w1[i]), b11 = e4m3x2_f16_high(w1[i]);
+            mma_f16(s[0], aq, b00, b01);
+            mma_f16(s[1], aq, b10, b11);
+            if constexpr (SPLIT) {
+              const uint4 lf = q_frag[D / 16 * 32 + (h * 4 + i) * 32 + lane];
+              const uint32_t al[4] = {lf.x, lf.y, lf.z, lf.w};
+              mma_f16(s[0], al, b00, b01);
+              mma_f16(s[1], al, b10, b11);
+            }
+          }
+        }
+        const int tok = slab * 16 + 2 * t;
+        const float c0 = unit0 * ksc, c1 = unit1 * ksc;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          s[i][0] *= c0;
+          s[i][1] *= c0;
+          s[i][2] *= c1;
+          s[i][3] *= c1;
+        }
+        if (slab * 16 + 16 > seen_by_all) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              if (tok + 8 * i + e >= seen0) s[i][e] = -INFINITY;
+              if (tok + 8 * i + e >= seen1) s[i][2 + e] = -INFINITY;
+            }
+          }
+        }
+        if (a.scores != nullptr) {
+          const int64_t base = ((static_cast<int64_t>(it.b) * p.heads + it.h) * a.rows + it.tile * 16) * a.capacity + tok;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (g < rows) *reinterpret_cast<float2*>(a.scores + base + g * a.capacity + 8 * i) = make_float2(s[i][0], s[i][1]);
+            if (g + 8 < rows)
+              *reinterpret_cast<float2*>(a.scores + base + (g + 8) * a.capacity + 8 * i) = make_float2(s[i][2], s[i][3]);
+          }
+        }
+        const float size = fabsf(vsc), lv = size > 0.0f ? fmaxf(__log2f(size), kLeastLogScale) : kLeastLogScale;
+        float t0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+        float t1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+        t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 1));
+        t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 1));
+        t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 2)) + (lv - kWeightBits);
+        t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 2)) + (lv - kWeightBits);
+        if (__any_sync(0xffffffffu, t0 > m0 || t1 > m1)) {
+          const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
+          const float f0 = exp2_approx(m0 - n0), f1 = exp2_approx(m1 - n1);
+          m0 = n0;
+          m1 = n1;
+          l0 *= f0;
+          l1 *= f1;
+#pragma unroll
+          for (int j = 0; j < TILES; ++j) {
+            o[j][0] *= f0;
+            o[j][1] *= f0;
+            o[j][2] *= f1;
+            o[j][3] *= f1;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          s[i][0] = exp2_approx(s[i][0] - m0);
+          s[i][1] = exp2_approx(s[i][1] - m0);
+          s[i][2] = exp2_approx(s[i][2] - m1);
+          s[i][3] = exp2_approx(s[i][3] - m1);
+        }
+        l0 += (s[0][0] + s[0][1]) + (s[1][0] + s[1][1]);
+        l1 += (s[0][2] + s[0][3]) + (s[1][2] + s[1][3]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[i][e] *= vsc;
+        }
+        const uint32_t pa[4] = {f16x2_of(s[0][0], s[0][1]), f16x2_of(s[0][2], s[0][3]), f16x2_of(s[1][0], s[1][1]),
+                                f16x2_of(s[1][2], s[1][3])};
+        uint32_t pl[4];
+        if constexpr (SPLIT) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 h = f16x2_values(pa[i]);
+            const float x0 = s[i >> 1][(i & 1) * 2], x1 = s[i >> 1][(i & 1) * 2 + 1];
+            pl[i] = f16x2_of(x0 - h.x, x1 - h.y);
+          }
+        }
+        // V codes of tokens 2t, 2t + 1 (b0) and 2t + 8, 2t + 9 (b1); column g of tile j is dim
+        // g * D / 8 + j, so a lane's bytes of a token are consecutive
+        constexpr int W = D / 32;  // 4-byte words per lane and token
+        uint32_t r0[W], r1[W], r2[W], r3[W];
+        auto take = [&](int row, uint32_t(&r)[W]) {
+          if constexpr (D == 128) {
+            const uint4 x = *reinterpret_cast<const uint4*>(vb + slab_offset<D>(row, g));
+            r[0] = x.x, r[1] = x.y, r[2] = x.z, r[3] = x.w;
+          } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(vb + slab_offset<D>(row, g >> 1) + (g & 1) * 8);
+            r[0] = x.x, r[1] = x.y;
+          }
+        };
+        take(2 * t, r0);
+        take(2 * t + 1, r1);
+        take(2 * t + 8, r2);
+        take(2 * t + 9, r3);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const uint32_t x0 = __byte_perm(r0[w], r1[w], 0x5140), x1 = __byte_perm(r0[w], r1[w], 0x7362);
+          const uint32_t y0 = __byte_perm(r2[w], r3[w], 0x5140), y1 = __byte_perm(r2[w], r3[w], 0x7362);
+          const uint32_t bx[4] = {e4m3x2_f16(x0), e4m3x2_f16_high(x0), e4m3x2_f16(x1), e4m3x2_f16_high(x1)};
+          const uint32_t by[4] = {e4m3x2_f16(y0), e4m3x2_f16_high(y0), e4m3x2_f16(y1), e4m3x2_f16_high(y1)};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            mma_f16(o[4 * w + i], pa, bx[i], by[i]);
+            if constexpr (SPLIT) mma_f16(o[4 * w + i], pl, bx[i], by[i]);
+          }
+        }
+        // the tokens that only some rows see (fewer than q_len of them)
+        for (int x = max(seen_by_all, slab * 16); x < min(n, slab * 16 + 16); ++x) {
+          const int k = x - slab * 16, from = (g << 2) | ((k & 7) >> 1);
+          const float e0 = k & 1 ? (k < 8 ? s[0][1] : s[1][1]) : (k < 8 ? s[0][0] : s[1][0]);
+          const float e1 = k & 1 ? (k < 8 ? s[0][3] : s[1][3]) : (k < 8 ? s[0][2] : s[1][2]);
+          const float w0 = __shfl_sync(0xffffffffu, e0, from), w1 = __shfl_sync(0xffffffffu, e1, from);
+          const int page = __ldg(table + (x >> p.page_shift));
+          const uint8_t* v = vbase + page * p.sp[1] + (x & (P - 1)) * p.st[1];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {  // columns 2t and 2t + 1 of every tile
+#pragma unroll
+            for (int j = 0; j < TILES; ++j) {
+              const float value = e4m3_value_hw(__ldg(v + (2 * t + c) * (D / 8) + j));
+              if (x < seen0) o[j][c] = fmaf(w0, value, o[j][c]);
+              if (x < seen1) o[j][2 + c] = fmaf(w1, value, o[j][2 + c]);
+            }
+          }
+        }
+      }
+      stage = stage == ST - 1 ? 0 : stage + 1;
+    }
+    copies_wait<0>();
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+
+    // ---- the warps' parts of this block's share of the item
+    __syncthreads();  // the ring is free
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+      for (int j = 0; j < TILES; j += 4) {
+        const int d = (2 * t + c) * (D / 8) + j;
+        *reinterpret_cast<float4*>(&merge_o[(warp * 16 + g) * D + d]) =
+            make_float4(o[j][c], o[j + 1][c], o[j + 2][c], o[j + 3][c]);
+        *reinterpret_cast<float4*>(&merge_o[(warp * 16 + g + 8) * D + d]) =
+            make_float4(o[j][2 + c], o[j + 1][2 + c], o[j + 2][2 + c], o[j + 3][2 + c]);
+      }
+    }
+    if (t == 0) {
+      merge_ml[(warp * 16 + g) * 2] = m0;
+      merge_ml[(warp * 16 + g) * 2 + 1] = l0;
+      merge_ml[(warp * 16 + g + 8) * 2] = m1;
+      merge_ml[(warp * 16 + g + 8) * 2 + 1] = l1;
+    }
+    __syncthreads();
+    const bool whole = s0 == 0 && s1 == it.slabs;
+    const int64_t item = (static_cast<int64_t>(it.b) * p.heads + it.h) * a.row_tiles + it.tile;
+    const int64_t row_base = (static_cast<int64_t>(it.b) * p.heads + it.h) * a.rows + it.tile * 16;
+    auto finish = [&](int r, int d, float4 acc, float ref, float sum) {
+      const int rr = it.tile * 16 + r, qi = rr % a.q_len;
+      const int seen = a.causal ? max(0, n - a.q_len + 1 + qi) : n;
+      const float inv = seen > 0 ? 1.0f / sum : 0.0f;
+      const int64_t at = (row_base + r) * D + d;
+      store_elem<T>(a.out, at, acc.x * inv);
+      store_elem<T>(a.out, at + 1, acc.y * inv);
+      store_elem<T>(a.out, at + 2, acc.z * inv);
+      store_elem<T>(a.out, at + 3, acc.w * inv);
+      if (d == 0 && a.ml != nullptr) {
+        a.ml[2 * (row_base + r)] = ref;
+        a.ml[2 * (row_base + r) + 1] = inv;
+      }
+    };
+    float* my_part = a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (it.first <= lo ? 0 : 1)) * 16 * (D + 2);
+    for (int i = tid; i < rows * (D / 4); i += 256) {
+      const int r = i / (D / 4), d = i % (D / 4) * 4;
+      float ref = kNoScore, sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) ref = fmaxf(ref, merge_ml[(w * 16 + r) * 2]);
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        const float f = exp2_approx(merge_ml[(w * 16 + r) * 2] - ref);
+        sum = fmaf(f, merge_ml[(w * 16 + r) * 2 + 1], sum);
+        const float4 x = *reinterpret_cast<const float4*>(&merge_o[(w * 16 + r) * D + d]);
+        acc.x = fmaf(f, x.x, acc.x);
+        acc.y = fmaf(f, x.y, acc.y);
+        acc.z = fmaf(f, x.z, acc.z);
+        acc.w = fmaf(f, x.w, acc.w);
+      }
+      if (whole) {
+        finish(r, d, acc, ref, sum);
+      } else {
+        __stcg(reinterpret_cast<float4*>(my_part + r * D + d), acc);
+        if (d == 0) __stcg(reinterpret_cast<float2*>(my_part + 16 * D + 2 * r), make_float2(ref, sum));
+      }
+    }
+    if (!whole) {
+      // ---- the block that brings an item's last part merges all of them, in their order
+      const int64_t end = it.first + it.slabs;
+      const int c0 = static_cast<int>(((it.first + 1) * grid + total - 1) / total - 1);
+      const int c1 = static_cast<int>((end * grid + total - 1) / total - 1);
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        const unsigned done = atomicAdd(a.counters + item, 1u);
+        shared_i[1] = done == static_cast<unsigned>(c1 - c0);
+        if (shared_i[1]) a.counters[item] = 0;
+      }
+      __syncthreads();
+      if (shared_i[1]) {
+        __threadfence();
+        auto part_of = [&](int c) -> const float* {
+          const int64_t begin = total * c / grid;
+          return a.partial + (static_cast<int64_t>(c) * 2 + (it.first <= begin ? 0 : 1)) * 16 * (D + 2);
+        };
+        for (int i = tid; i < rows * (D / 4); i += 256) {
+          const int r = i / (D / 4), d = i % (D / 4) * 4;
+          float ref = kNoScore, sum = 0.0f;
+          float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          for (int c = c0; c <= c1; ++c) ref = fmaxf(ref, __ldcg(part_of(c) + 16 * D + 2 * r));
+#pragma unroll 4
+          for (int c = c0; c <= c1; ++c) {
+            const float* part = part_of(c);
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(part + 16 * D + 2 * r));
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(part + r * D + d));
+            const float f = exp2_approx(ml.x - ref);
+            sum = fmaf(f, ml.y, sum);
+            acc.x = fmaf(f, x.x, acc.x);
+            acc.y = fmaf(f, x.y, acc.y);
+            acc.z = fmaf(f, x.z, acc.z);
+            acc.w = fmaf(f, x.w, acc.w);
+          }
+          finish(r, d, acc, ref, sum);
+        }
+      }
+    }
+    // ---- the next item
+    pos = it.first + s1;
+    it.first += it.slabs;
+    if (++it.tile == a.row_tiles) {
+      it.tile = 0;
+      if (++it.h == p.heads) {
+        it.h = 0;
+        ++it.b;
+      }
+    }
   }
 }
 
-// One warp per (token, KV head): the weights of its query rows, recomputed and summed in order.
-template <int T, int D>
-__global__ void __launch_bounds__(128) pages_mass_kernel(PagesAttnArgs a, unsigned* status) {
-  constexpr int E = D / 32;
+// The mass of every cached token: its weights, from the stored scores and the rows' final
+// reference and sum, added in the order of the rows. One thread per token and KV head.
+__global__ void __launch_bounds__(256) pages_mass_kernel(PagesAttnArgs a) {
   const PagePool& p = a.pool;
-  const int h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31;
-  const int P = 1 << p.page_shift, group = a.heads_q / p.heads;
-  const int n = page_length(p, b, status);
-  for (int t = blockIdx.x * 4 + (threadIdx.x >> 5); t < n; t += gridDim.x * 4) {
-    const int page = page_of(p, b, t >> p.page_shift, status);
-    if (page < 0) continue;
-    const uint8_t* k = p.codes[0] + page * p.sp[0] + h * p.sh[0] + (t & (P - 1)) * p.st[0] + lane * E;
-    const float ks = p.scale[0][page * p.ssp[0] + h * p.ssh[0]];
-    float received = 0.0f;
-    for (int r = 0; r < group * a.q_len; ++r) {
-      const int hq = h * group + r / a.q_len, qi = r % a.q_len;
-      if (a.causal && t >= n - a.q_len + 1 + qi) continue;
-      float s = 0.0f;
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        s = fmaf(load_elem<T>(a.q, b * a.qb + hq * a.qh + qi * a.qt + lane * E + e) * a.scale_log2,
-                 e4m3_value_hw(k[e]), s);
-#pragma unroll
-      for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-      const float* ml = a.ml + 2 * ((static_cast<int64_t>(b) * a.heads_q + hq) * a.q_len + qi);
-      received += exp2f(s * ks - ml[0]) / ml[1];
-    }
-    if (lane == 0) p.mass[page * p.msp + h * p.msh + (t & (P - 1))] += received;
+  const int h = blockIdx.y, b = blockIdx.z;
+  const int n = min(max(__ldg(p.lengths + b), 0), p.max_pages << p.page_shift);
+  const int x = blockIdx.x * 256 + threadIdx.x;
+  if (x >= n) return;
+  const int page = __ldg(p.table + b * p.table_stride + (x >> p.page_shift));
+  if (page < 0 || page >= p.num_pages) return;  // reported by the attention
+  const int64_t row0 = (static_cast<int64_t>(b) * p.heads + h) * a.rows;
+  const float* s = a.scores + row0 * a.capacity + x;
+  const float2* ml = reinterpret_cast<const float2*>(a.ml) + row0;
+  float received = 0.0f;
+#pragma unroll 4
+  for (int r = 0; r < a.rows; ++r) {
+    const float2 f = __ldg(ml + r);
+    received += exp2_approx(__ldg(s + r * a.capacity) - f.x) * f.y;
   }
+  p.mass[page * p.msp + h * p.msh + (x & ((1 << p.page_shift) - 1))] += received;
 }
 
 }  // namespace kab

@@ -106,22 +106,67 @@ int attention_check(const KabKvPagesAttention* p, PagesAttnArgs* g) {
   g->heads_q = static_cast<int>(p->heads_q);
   g->q_len = static_cast<int>(p->q_len);
   g->causal = p->causal != 0;
+  g->rows = static_cast<int>(p->heads_q / p->cache.heads_kv * p->q_len);
+  g->row_tiles = (g->rows + 15) / 16;
+  g->capacity = p->cache.max_pages * p->cache.page_tokens;
   return KAB_OK;
 }
 
-size_t attention_workspace(const KabKvPagesAttention* p) {
-  return p->use_mass ? static_cast<size_t>(p->cache.batch * p->heads_q * p->q_len) * 8 : 0;
+// The launch's workspace: counters (zero between launches), the blocks' partial results and, with
+// mass, the scores and the rows' references.
+struct AttentionPlan {
+  int grid = 0;
+  size_t counters = 0, partial = 0, ml = 0, scores = 0;
+  size_t bytes() const { return counters + partial + ml + scores; }
+};
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+// Opts the kernel instance into its shared memory and returns the blocks of it that fit on the
+// GPU at once (asked once per device), or -1.
+template <int T, int D>
+int attention_blocks() {
+  using L = PagesLayout<D, T == kF32>;
+  static int blocks[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
+  if (blocks[dev] == 0) {
+    auto kern = pages_attention_kernel<T, D>;
+    int n = 0;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, L::kThreads, L::kSmem) != cudaSuccess || n < 1)
+      return -1;
+    blocks[dev] = n * sm_count();
+  }
+  return blocks[dev];
+}
+int attention_blocks(int dtype, int64_t d) {
+  if (dtype == KAB_BF16) return d == 128 ? attention_blocks<kBF16, 128>() : attention_blocks<kBF16, 64>();
+  if (dtype == KAB_F16) return d == 128 ? attention_blocks<kF16, 128>() : attention_blocks<kF16, 64>();
+  return d == 128 ? attention_blocks<kF32, 128>() : attention_blocks<kF32, 64>();
+}
+
+int attention_plan(const KabKvPagesAttention* p, const PagesAttnArgs& g, AttentionPlan* plan) {
+  plan->grid = attention_blocks(p->q_dtype, p->cache.head_dim);
+  if (plan->grid < 0) return fail(KAB_ECUDA, "cannot configure the paged attention kernel");
+  const size_t items = static_cast<size_t>(p->cache.batch * p->cache.heads_kv);
+  plan->counters = round256(items * g.row_tiles * 4);
+  plan->partial = round256(static_cast<size_t>(plan->grid) * 2 * 16 * (p->cache.head_dim + 2) * 4);
+  if (p->use_mass) {
+    plan->ml = round256(items * g.rows * 8);
+    plan->scores = round256(items * g.rows * static_cast<size_t>(g.capacity) * 4);
+  }
+  return KAB_OK;
 }
 
 template <int T, int D>
-int launch_attention(const PagesAttnArgs& g, bool mass, unsigned* status, cudaStream_t s) {
-  pages_attention_kernel<T, D><<<dim3(g.heads_q * g.q_len, g.pool.batch), 128, 0, s>>>(g, status);
-  if (mass) {
-    const int tokens = g.pool.max_pages << g.pool.page_shift;
-    pages_mass_kernel<T, D><<<dim3(std::max(1, std::min(tokens / 4, 256)), g.pool.heads, g.pool.batch), 128, 0, s>>>(
-        g, status);
-  }
-  return check_launch("kab_kv_pages_attention");
+int launch_attention(const PagesAttnArgs& g, int grid, unsigned* status, cudaStream_t s) {
+  using L = PagesLayout<D, T == kF32>;
+  pages_attention_kernel<T, D><<<grid, L::kThreads, L::kSmem, s>>>(g, status);
+  if (int e = check_launch("kab_kv_pages_attention")) return e;
+  if (g.scores == nullptr || g.capacity == 0) return KAB_OK;
+  const dim3 blocks(static_cast<unsigned>((g.capacity + 255) / 256), g.pool.heads, g.pool.batch);
+  pages_mass_kernel<<<blocks, 256, 0, s>>>(g);
+  return check_launch("kab_kv_pages_attention mass");
 }
 
 }  // namespace
@@ -181,8 +226,11 @@ int kab_kv_pages_attention_workspace(const KabKvPagesAttention* params, size_t* 
   PagesAttnArgs g{};
   if (int e = attention_check(params, &g)) return e;
   KAB_REQUIRE(bytes != nullptr && zero_bytes != nullptr, "null pointer");
-  *bytes = attention_workspace(params);
-  *zero_bytes = 0;
+  AttentionPlan plan;
+  if (params->cache.batch > 0 && g.rows > 0)
+    if (int e = attention_plan(params, g, &plan)) return e;
+  *bytes = plan.bytes();
+  *zero_bytes = plan.counters;
   return KAB_OK;
 }
 
@@ -191,17 +239,23 @@ int kab_kv_pages_attention(const KabKvPagesAttention* params, void* workspace, s
   if (int e = attention_check(params, &g)) return e;
   if (params->cache.batch == 0 || params->heads_q == 0 || params->q_len == 0) return KAB_OK;
   KAB_REQUIRE(params->q != nullptr && params->out != nullptr, "null pointer");
-  const size_t need = attention_workspace(params);
-  KAB_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && aligned(workspace, 256)),
-              "the workspace needs %zu bytes, 256-byte aligned (kab_kv_pages_attention_workspace)", need);
+  AttentionPlan plan;
+  if (int e = attention_plan(params, g, &plan)) return e;
+  KAB_REQUIRE(workspace != nullptr && workspace_bytes >= plan.bytes() && aligned(workspace, 256),
+              "the workspace needs %zu bytes, 256-byte aligned (kab_kv_pages_attention_workspace)", plan.bytes());
   unsigned* status = status_word();
   KAB_REQUIRE(status != nullptr, "no device status word");
-  if (params->use_mass) g.ml = static_cast<float*>(workspace);
+  uint8_t* w = static_cast<uint8_t*>(workspace);
+  g.counters = reinterpret_cast<unsigned*>(w);
+  g.partial = reinterpret_cast<float*>(w + plan.counters);
+  if (params->use_mass) {
+    g.ml = reinterpret_cast<float*>(w + plan.counters + plan.partial);
+    g.scores = reinterpret_cast<float*>(w + plan.counters + plan.partial + plan.ml);
+  }
   const cudaStream_t s = as_stream(stream);
-  const bool mass = params->use_mass && params->cache.max_pages > 0;
 #define KAB_PAGES_D(TT)                                                              \
-  return params->cache.head_dim == 128 ? launch_attention<TT, 128>(g, mass, status, s) \
-                                       : launch_attention<TT, 64>(g, mass, status, s)
+  return params->cache.head_dim == 128 ? launch_attention<TT, 128>(g, plan.grid, status, s) \
+                                       : launch_attention<TT, 64>(g, plan.grid, status, s)
   if (params->q_dtype == KAB_BF16) KAB_PAGES_D(kBF16);
   if (params->q_dtype == KAB_F16) KAB_PAGES_D(kF16);
   KAB_PAGES_D(kF32);
