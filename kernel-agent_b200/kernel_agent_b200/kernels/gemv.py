@@ -16,7 +16,7 @@ import torch
 
 from .. import _native as nat
 from . import quant as q
-from ._workspace import workspace
+from ._launch import device_of, guard, stream_of, workspace
 from .gemm import _bias
 
 _FORMATS = {"nvfp4": (nat.KAB_NVFP4, 16), "mxfp4": (nat.KAB_MXFP4, 32)}
@@ -48,13 +48,14 @@ def fp4_w4a16_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     if fmt not in _FORMATS:
         raise ValueError(f"unknown FP4 format {fmt!r} (one of {', '.join(_FORMATS)})")
     code, block = _FORMATS[fmt]
-    nat.require_cuda(x, codes, scales, bias)
+    device = device_of(x, codes, scales, bias)
     if x.dim() < 1 or codes.dim() != 2:
         raise ValueError(f"expected x [..., K] and codes [N, K / 2]; got {tuple(x.shape)}, {tuple(codes.shape)}")
-    n, k = codes.shape[0], x.shape[-1]
+    n, half = codes.shape
+    k = x.shape[-1]
     if k % block:
         raise ValueError(f"the last dimension {k} is not a multiple of the {fmt} block ({block})")
-    if codes.shape[1] * 2 != k or codes.element_size() != 1:
+    if half * 2 != k or codes.element_size() != 1:
         raise ValueError(f"codes {tuple(codes.shape)} {codes.dtype} do not fit x {tuple(x.shape)}: expected "
                          f"[N, {k // 2}] bytes")
     if scales.element_size() != 1:
@@ -64,27 +65,33 @@ def fp4_w4a16_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     if swizzle and scales.numel() != -(-n // 128) * 128 * (-(-cols // 4)) * 4:
         raise ValueError(f"swizzled scales have {scales.numel()} bytes, expected "
                          f"{-(-n // 128) * 128 * (-(-cols // 4)) * 4}")
-    if not swizzle and tuple(scales.shape) != (n, cols):
+    if not swizzle and scales.shape != (n, cols):
         raise ValueError(f"expected scales [{n}, {cols}], got {tuple(scales.shape)}")
-    x2 = q._rows(q._input(x))
+    x2 = x if x.dim() == 2 else x.reshape(-1, k)
+    if x2.dtype not in nat.DTYPES:
+        x2 = x2.float()
+    if x2.stride(1) != 1 or x2.stride(0) % 8 or x2.data_ptr() % 16:
+        x2 = x2.contiguous()
     m = x2.shape[0]
     c, s = codes.contiguous(), scales.contiguous()
     if c.data_ptr() % 8:
         c = c.clone()
     ts = tensor_scale
-    if not isinstance(ts, torch.Tensor) or ts.dtype != torch.float32 or not ts.is_cuda or not ts.is_contiguous():
+    if not isinstance(ts, torch.Tensor) or ts.dtype != torch.float32 or ts.get_device() != device \
+            or not ts.is_contiguous():
         ts = torch.as_tensor(ts, dtype=torch.float32, device=x.device).contiguous()
-    if ts.numel() not in (1, n):
+    per_row = ts.numel() > 1
+    if ts.numel() != (n if per_row else 1):
         raise ValueError(f"tensor_scale has {ts.numel()} values, expected 1 or {n}")
     b, bias_code = (None, nat.KAB_F32) if bias is None else _bias(bias, n, x.device)
-    out = torch.empty(m, n, dtype=x2.dtype, device=x.device)
+    out = torch.empty((m, n), dtype=x2.dtype, device=x.device)
     if m and n:
-        dtype = nat.dtype_code(x2)
-        with torch.cuda.device(x.device):
-            stream = nat.stream_of(x2)
-            nbytes, zero = _plan(m, n, k, code, dtype, x.device.index)
-            ws = workspace(f"gemv {m} {n} {k} {code} {dtype}", x.device, stream, nbytes, zero) if nbytes else None
+        dtype = nat.DTYPES[x2.dtype]
+        with guard(device):
+            stream = stream_of(device)
+            nbytes, zero = _plan(m, n, k, code, dtype, device)
+            ws = workspace(("gemv", m, n, k, code, dtype), device, stream, nbytes, zero) if nbytes else None
             nat.call("kab_gemv_fp4", x2.data_ptr(), dtype, x2.stride(0) if m > 1 else max(k, 8), c.data_ptr(),
-                     s.data_ptr(), int(swizzle), code, ts.data_ptr(), int(ts.numel() > 1), m, n, k, nat.ptr(b),
-                     bias_code, out.data_ptr(), n, nat.ptr(ws), nbytes, stream)
-    return q._linear_out(out, x, n)
+                     s.data_ptr(), swizzle, code, ts.data_ptr(), per_row, m, n, k, None if b is None else b.data_ptr(),
+                     bias_code, out.data_ptr(), n, None if ws is None else ws.data_ptr(), nbytes, stream)
+    return out if out.dtype == x.dtype and x.dim() == 2 else q._linear_out(out, x, n)

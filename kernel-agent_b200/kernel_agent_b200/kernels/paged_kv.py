@@ -26,7 +26,7 @@ import ctypes
 import torch
 
 from .. import _native as nat
-from ._workspace import workspace
+from ._launch import device_of, guard, stream_of, workspace
 
 _E4M3 = torch.float8_e4m3fn
 PAGE_TOKENS = (16, 32, 64, 128)
@@ -72,12 +72,12 @@ def _pool_fields(p, k_pages, k_scale, v_pages, v_scale, mass, page_table, length
     p.table_stride, p.max_pages, p.batch = page_table.stride(0), page_table.shape[1], batch
 
 
-def _layout(t: torch.Tensor | None) -> tuple | None:
-    return None if t is None else (t.shape, t.stride(), t.dtype)
-
-
-def _cache_key(*tensors) -> tuple:
-    return tuple(_layout(t) for t in tensors)
+def _layout(k_pages, k_scale, v_pages, v_scale, mass, page_table, lengths) -> tuple:
+    """Everything of a cache's tensors that the checks and the parameters go by, but the pointers."""
+    return (k_pages.shape, k_pages.stride(), k_pages.dtype, k_scale.shape, k_scale.stride(), k_scale.dtype,
+            v_pages.shape, v_pages.stride(), v_pages.dtype, v_scale.shape, v_scale.stride(), v_scale.dtype,
+            page_table.shape, page_table.stride(), page_table.dtype, lengths.shape, lengths.stride(), lengths.dtype,
+            None if mass is None else (mass.shape, mass.stride(), mass.dtype))
 
 
 def _pointers(p, k_pages, k_scale, v_pages, v_scale, mass, page_table, lengths) -> None:
@@ -90,7 +90,7 @@ def _pointers(p, k_pages, k_scale, v_pages, v_scale, mass, page_table, lengths) 
 
 def _pool(cache: tuple) -> "nat.KabKvPages":
     """The parameters of a cache; the checks run once per layout."""
-    key = ("pool", *_cache_key(*cache))
+    key = _layout(*cache)
     made = _TEMPLATES.get(key)
     if made is None:
         p = nat.KabKvPages()
@@ -123,7 +123,7 @@ def append_kv_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, k_s
     that would need a larger scale rewrites the page's codes as ``e4m3(code * old / s)``. An
     infinity becomes the largest code of its sign, NaN stays NaN. ``mass`` of the new slots
     becomes 0."""
-    nat.require_cuda(k, v, k_pages, k_scale, v_pages, v_scale, page_table, lengths, counts, mass, out_lengths)
+    device = device_of(k, v, k_pages, k_scale, v_pages, v_scale, page_table, lengths, counts, mass, out_lengths)
     p = _pool((k_pages, k_scale, v_pages, v_scale, mass, page_table, lengths))
     if k.dim() != 4 or v.shape != k.shape or k.shape[0] != p.batch or k.shape[1] != p.heads_kv \
             or k.shape[3] != p.head_dim:
@@ -134,11 +134,11 @@ def append_kv_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, k_s
     for name, t in (("counts", counts), ("out_lengths", out_lengths)):
         if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (p.batch,) or not t.is_contiguous()):
             raise ValueError(f"{name} must be int32 [{p.batch}], contiguous; got {t.dtype} {tuple(t.shape)}")
-    k, v = _rows16(k.detach()), _rows16(v.detach())
+    k, v = _rows16(k), _rows16(v)
     out = torch.empty_like(lengths) if out_lengths is None else out_lengths
-    with torch.cuda.device(k.device):
+    with guard(device):
         nat.call("kab_kv_pages_append", ctypes.byref(p), k.data_ptr(), v.data_ptr(), nat.DTYPES[k.dtype],
-                 *k.stride()[:3], *v.stride()[:3], k.shape[2], nat.ptr(counts), out.data_ptr(), nat.stream_of(k))
+                 *k.stride()[:3], *v.stride()[:3], k.shape[2], nat.ptr(counts), out.data_ptr(), stream_of(device))
     return out
 
 
@@ -160,14 +160,14 @@ def paged_kv_attention(q: torch.Tensor, k_pages: torch.Tensor, k_scale: torch.Te
     inputs."""
     if q.dim() not in (3, 4):
         raise ValueError(f"q must be [B, Hq, D] or [B, Hq, Lq, D]; got {tuple(q.shape)}")
-    nat.require_cuda(q, k_pages, k_scale, v_pages, v_scale, page_table, lengths, mass, out)
+    device = device_of(q, k_pages, k_scale, v_pages, v_scale, page_table, lengths, mass, out)
     if q.dtype not in nat.DTYPES:
         raise ValueError(f"unsupported dtype {q.dtype} (float32, bfloat16 or float16)")
-    q4 = q.detach() if q.dim() == 4 else q.detach().unsqueeze(2)
+    q4 = q if q.dim() == 4 else q.unsqueeze(2)
     if q4.stride(3) != 1:
         q4 = q4.contiguous()
     cache = (k_pages, k_scale, v_pages, v_scale, mass, page_table, lengths)
-    key = ("attention", q4.shape, q4.stride(), q4.dtype, q4.device.index, scale, bool(causal), *_cache_key(*cache))
+    key = ("attention", q4.shape, q4.stride(), q4.dtype, device, scale, bool(causal), _layout(*cache))
     made = _TEMPLATES.get(key)
     if made is None:
         t = nat.KabKvPagesAttention()
@@ -182,7 +182,7 @@ def paged_kv_attention(q: torch.Tensor, k_pages: torch.Tensor, k_scale: torch.Te
         t.heads_q, t.q_len = hq, lq
         _pointers(t.cache, *cache)
         nbytes, zero = ctypes.c_size_t(0), ctypes.c_size_t(0)
-        with torch.cuda.device(q4.device):
+        with guard(device):
             nat.call("kab_kv_pages_attention_workspace", ctypes.byref(t), ctypes.byref(nbytes), ctypes.byref(zero))
         made = _TEMPLATES[key] = (bytes(t), int(nbytes.value), int(zero.value))
     template, nbytes, zero = made
@@ -193,9 +193,9 @@ def paged_kv_attention(q: torch.Tensor, k_pages: torch.Tensor, k_scale: torch.Te
     p = nat.KabKvPagesAttention.from_buffer_copy(template)
     _pointers(p.cache, *cache)
     p.q, p.out = q4.data_ptr(), out.data_ptr()
-    with torch.cuda.device(q4.device):
-        stream = nat.stream_of(q4)
-        ws = workspace(f"pages attention {zero}", q4.device, stream, nbytes, zero) if nbytes else None
+    with guard(device):
+        stream = stream_of(device)
+        ws = workspace("pages attention", device, stream, nbytes, zero) if nbytes else None
         nat.call("kab_kv_pages_attention", ctypes.byref(p), nat.ptr(ws), nbytes, stream)
     return out
 
@@ -215,7 +215,7 @@ def evict_kv_pages(k_pages: torch.Tensor, k_scale: torch.Tensor, v_pages: torch.
     budget, recent, sinks = int(budget), int(recent), int(sinks)
     if mass is None:
         raise ValueError("an eviction needs the tokens' mass")
-    nat.require_cuda(k_pages, k_scale, v_pages, v_scale, mass, page_table, lengths, out_page_table)
+    device = device_of(k_pages, k_scale, v_pages, v_scale, mass, page_table, lengths, out_page_table)
     p = _pool((k_pages, k_scale, v_pages, v_scale, mass, page_table, lengths))
     if budget < 1 or recent < 0 or sinks < 0 or sinks + recent > budget:
         raise ValueError(f"budget {budget} must be at least 1 and hold the {sinks} first and {recent} last tokens")
@@ -228,7 +228,7 @@ def evict_kv_pages(k_pages: torch.Tensor, k_scale: torch.Tensor, v_pages: torch.
         raise ValueError("out_page_table must name other pages than page_table")
     kept = torch.empty(p.batch, p.heads_kv, budget, dtype=torch.int32, device=mass.device)
     out = torch.empty_like(lengths)
-    with torch.cuda.device(mass.device):
+    with guard(device):
         nat.call("kab_kv_pages_evict", ctypes.byref(p), out_page_table.data_ptr(), out_page_table.stride(0), budget,
-                 recent, sinks, kept.data_ptr(), out.data_ptr(), nat.stream_of(mass))
+                 recent, sinks, kept.data_ptr(), out.data_ptr(), stream_of(device))
     return kept, out
