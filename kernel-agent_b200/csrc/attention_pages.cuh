@@ -13,8 +13,8 @@
 //  * Work is cut into equal parts whatever the lengths: the slabs of all (sequence, KV head, 16
 //    rows) items stand in one line, and each block takes a contiguous part of it. A block's first
 //    and last item may be shared with its neighbours: their partial results (maximum, sum,
-//    output) go to two slots of the block's own, and the block that finishes an item last merges
-//    them in order, so the same inputs give the same bits.
+//    output) go to two slots of the block's own, and a second small launch merges them in an
+//    order of their own, so the same inputs give the same bits.
 //  * Queries enter as f16, each row in units of a power of two that puts its largest value in
 //    [2^14, 2^15): bf16 and f16 values keep all their bits down to 2^-29 of the row's largest;
 //    fp32 ones are split into two f16 terms (22 bits) and the product is taken twice.
@@ -30,6 +30,11 @@
 
 namespace kab {
 
+// An item that several blocks share: which one, and the last of the blocks (-1: none begins here).
+struct PagesCut {
+  int b, h, tile, last, slot;
+};
+
 struct PagesAttnArgs {
   PagePool pool;
   const void* q;
@@ -38,8 +43,8 @@ struct PagesAttnArgs {
   float scale_log2;  // sm_scale * log2(e)
   int heads_q, q_len, causal;
   int rows, row_tiles;   // rows of one KV head (query heads x query tokens), tiles of 16 of them
-  unsigned* counters;    // [batch, heads, row_tiles]
   float* partial;        // [grid, 2 slots, 16 rows, D + 2]: output, maximum, sum
+  PagesCut* cuts;        // [grid]: the item that begins in a block and goes on in the next ones
   float* scores;         // [batch, heads, rows, capacity] in log2 units, or NULL
   float* ml;             // [batch, heads, rows, 2]: reference and reciprocal sum, with scores
   int64_t capacity;      // max_pages * page_tokens
@@ -101,14 +106,18 @@ __device__ __forceinline__ void copies_wait() {
 
 template <int D, bool SPLIT>
 struct PagesLayout {
-  static constexpr int kWarps = 8, kThreads = 256, kStages = 3, kSlab = 16;
+  static constexpr int kWarps = 4, kThreads = kWarps * 32, kStages = 3, kSlab = 16;
+  static constexpr int kBlocks = 16 / kWarps;  // per SM: 16 warps of 128 registers
   static constexpr int kSlabBytes = kSlab * D;              // K or V of one slab
   static constexpr int kStageBytes = 2 * kSlabBytes;
   static constexpr int kQBytes = D / 16 * 32 * 16 * (SPLIT ? 2 : 1);
   static constexpr int kRing = kWarps * kStages * kStageBytes;
   static constexpr int kScales = kWarps * kStages * 2 * 4;
   static constexpr int kSmem = kQBytes + kRing + kScales + 256;
-  static_assert(kRing >= kWarps * 16 * (D + 2) * 4, "the merge reuses the ring");
+  // a row of the warps' outputs in the merge: 4 floats of padding per 32 and a pitch that shifts
+  // the next row by 16 (8) banks, so that the fragments' float4 stores touch all banks
+  static constexpr int kPitch = D + D / 32 * 4;
+  static_assert(kRing >= kWarps * 16 * (kPitch + 2) * 4, "the merge reuses the ring");
 };
 
 // Byte offset of 16-byte chunk `chunk` of token `row` in a slab: the chunks are permuted so that
@@ -120,6 +129,7 @@ __device__ __forceinline__ uint32_t slab_offset(int row, int chunk) {
   else return (row >> 1) * 128 + (((((row & 1) << 2) | chunk) ^ (((row >> 1) & 3) << 1)) << 4);
 }
 
+constexpr int kItemCost = 6;  // an item's queries, merge and output cost about as much as six slabs
 constexpr float kNoScore = -3.3e38f;  // below every finite score
 constexpr float kWeightBits = 15.0f;  // the largest weight is 2^15 in f16
 constexpr float kLeastLogScale = -80.0f;
@@ -132,11 +142,34 @@ struct PagesItem {
   int64_t first;
 };
 
+// Four output elements of row r (of a KV head's rows) from their weighted sum and the row's sum.
 template <int T, int D>
-__global__ void __launch_bounds__(256, 2) pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
+__device__ __forceinline__ void pages_finish(const PagesAttnArgs& a, int b, int h, int r, int d, int n, float4 acc,
+                                             float ref, float sum) {
+  const int seen = a.causal ? max(0, n - a.q_len + 1 + r % a.q_len) : n;
+  const float inv = seen > 0 ? 1.0f / sum : 0.0f;  // a row that sees nothing gives zeros
+  const int64_t row = (static_cast<int64_t>(b) * a.pool.heads + h) * a.rows + r, at = row * D + d;
+  if constexpr (T == kF32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) =
+        make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+  } else {
+    store_elem<T>(a.out, at, acc.x * inv);
+    store_elem<T>(a.out, at + 1, acc.y * inv);
+    store_elem<T>(a.out, at + 2, acc.z * inv);
+    store_elem<T>(a.out, at + 3, acc.w * inv);
+  }
+  if (d == 0 && a.ml != nullptr) {
+    a.ml[2 * row] = ref;
+    a.ml[2 * row + 1] = inv;
+  }
+}
+
+template <int T, int D>
+__global__ void __launch_bounds__(PagesLayout<D, T == kF32>::kThreads, PagesLayout<D, T == kF32>::kBlocks)
+pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
   constexpr bool SPLIT = T == kF32;
   using L = PagesLayout<D, SPLIT>;
-  constexpr int ST = L::kStages, TILES = D / 8, CHUNKS = D / 16, COPIES = D / 32;
+  constexpr int ST = L::kStages, NW = L::kWarps, NT = L::kThreads, TILES = D / 8, CHUNKS = D / 16, COPIES = D / 32;
   extern __shared__ __align__(128) uint8_t smem[];
   uint4* q_frag = reinterpret_cast<uint4*>(smem);
   uint8_t* ring = smem + L::kQBytes;
@@ -144,24 +177,27 @@ __global__ void __launch_bounds__(256, 2) pages_attention_kernel(PagesAttnArgs a
   float* q_unit = sc_all + L::kWarps * ST * 2;                     // [16] units of the query rows
   int* shared_i = reinterpret_cast<int*>(q_unit + 16);             // [8..] broadcast words
   int64_t* shared_l = reinterpret_cast<int64_t*>(shared_i + 12);
-  float* merge_o = reinterpret_cast<float*>(ring);                 // [8][16][D]
-  float* merge_ml = merge_o + L::kWarps * 16 * D;                  // [8][16][2]
+  constexpr int PITCH = L::kPitch;
+  float* merge_o = reinterpret_cast<float*>(ring);                 // [8][16][PITCH]
+  float* merge_ml = merge_o + L::kWarps * 16 * PITCH;              // [8][16][2]
 
   const PagePool& p = a.pool;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int P = 1 << p.page_shift, group = a.heads_q / p.heads, per_seq = p.heads * a.row_tiles;
   const int cap = p.max_pages << p.page_shift;
 
+  // the merge may be set up while this kernel runs: it waits for its end by itself
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // ---- this block's part of the line
-  auto slabs_of = [&](int b) -> int64_t {
+  auto units_of = [&](int b) -> int64_t {
     const int n = min(max(__ldg(p.lengths + b), 0), cap);
-    return max((n + 15) >> 4, 1);  // an empty sequence is one empty slab: its output is written too
+    return max((n + 15) >> 4, 1) + kItemCost;  // an empty sequence is one empty slab: its output is written too
   };
-  const int chunk = (p.batch + 255) / 256;
+  const int chunk = (p.batch + NT - 1) / NT;
   int64_t mine = 0;
   for (int i = 0; i < chunk; ++i) {
     const int b = tid * chunk + i;
-    if (b < p.batch) mine += slabs_of(b) * per_seq;
+    if (b < p.batch) mine += units_of(b) * per_seq;
   }
   int64_t upto = mine;
 #pragma unroll
@@ -174,17 +210,20 @@ __global__ void __launch_bounds__(256, 2) pages_attention_kernel(PagesAttnArgs a
   __syncthreads();
   int64_t total = 0, before = upto - mine;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) {
+  for (int w = 0; w < NW; ++w) {
     if (w < warp) before += warp_sum[w];
     total += warp_sum[w];
   }
   const int64_t grid = min(static_cast<int64_t>(gridDim.x), total);
-  if (blockIdx.x >= grid) return;
+  if (blockIdx.x >= grid) {
+    if (tid == 0) a.cuts[blockIdx.x].last = -1;
+    return;
+  }
   const int64_t lo = total * blockIdx.x / grid, hi = total * (blockIdx.x + 1) / grid;
   if (lo >= before && lo < before + mine) {  // one thread: the sequence that `lo` lies in
     int64_t at = before;
     int b = tid * chunk;
-    while (lo >= at + slabs_of(b) * per_seq) at += slabs_of(b++) * per_seq;
+    while (lo >= at + units_of(b) * per_seq) at += units_of(b++) * per_seq;
     shared_i[0] = b;
     shared_l[0] = at;
   }
@@ -192,7 +231,7 @@ __global__ void __launch_bounds__(256, 2) pages_attention_kernel(PagesAttnArgs a
   PagesItem it;
   it.b = shared_i[0];
   {
-    const int64_t at = shared_l[0], n = slabs_of(it.b);
+    const int64_t at = shared_l[0], n = units_of(it.b);
     const int i = static_cast<int>((lo - at) / n);
     it.h = i / a.row_tiles;
     it.tile = i % a.row_tiles;
@@ -204,19 +243,89 @@ __global__ void __launch_bounds__(256, 2) pages_attention_kernel(PagesAttnArgs a
   float* my_sc = sc_all + warp * ST * 2;
   const uint32_t my_sc_s = static_cast<uint32_t>(__cvta_generic_to_shared(my_sc));
 
+  // this lane's share of a slab's copies: chunk lane % CHUNKS of every STEP-th token
+  constexpr int STEP = 32 / CHUNKS;
+  const int k_tok = static_cast<int>(p.st[0]), v_tok = static_cast<int>(p.st[1]);
+  const int k_page = static_cast<int>(p.sp[0]), v_page = static_cast<int>(p.sp[1]);
+  const int k_lane = lane / CHUNKS * k_tok + lane % CHUNKS * 16, v_lane = lane / CHUNKS * v_tok + lane % CHUNKS * 16;
+  const int sc_page = static_cast<int>(lane & 1 ? p.ssp[1] : p.ssp[0]);
+  const uint32_t lane_off = slab_offset<D>(lane / CHUNKS, lane % CHUNKS);
+  // slab_offset of the share's i-th token: for D = 128 the tokens are 4 apart, which flips bit 2 of the chunk
+  auto share_off = [&](int i) -> uint32_t { return (D == 128 && (i & 1) ? lane_off ^ 64u : lane_off) + i * 512; };
+
+  PagesCut cut{0, 0, 0, -1, 0};
   for (int64_t pos = lo; pos < hi;) {
     it.length = page_length(p, it.b, status);
-    it.slabs = static_cast<int>(slabs_of(it.b));
-    const int s0 = static_cast<int>(pos - it.first);
-    const int s1 = static_cast<int>(min(static_cast<int64_t>(it.slabs), hi - it.first));
+    const int64_t end = it.first + units_of(it.b);
+    it.slabs = static_cast<int>(end - it.first) - kItemCost;
+    // the item's first kItemCost units stand for what an item costs beside its slabs
+    const int s0 = max(0, static_cast<int>(pos - it.first) - kItemCost);
+    const int s1 = static_cast<int>(min(end, hi) - it.first) - kItemCost;
+    pos = end;
     const int n = it.length;
     const int rows = min(16, a.rows - it.tile * 16);
     const int seen_by_all = a.causal ? max(0, n - a.q_len + 1) : n;
 
+    if (s1 > 0) {
+    // tokens that row g (half 0) or g + 8 (half 1) of the tile sees
+    auto seen_of = [&](int half) -> int {
+      return a.causal ? max(0, n - a.q_len + 1 + (it.tile * 16 + g + 8 * half) % a.q_len) : n;
+    };
+
+    const uint8_t* kbase = p.codes[0] + it.h * p.sh[0];
+    const uint8_t* vbase = p.codes[1] + it.h * p.sh[1];
+    const int32_t* table = p.table + it.b * p.table_stride;
+    // lane 0 fetches K's scales, lane 1 V's
+    const float* sc_base = lane & 1 ? p.scale[1] + it.h * p.ssh[1] : p.scale[0] + it.h * p.ssh[0];
+    uint32_t valid = 0;  // bit s: stage s holds a page of the pool
+
+    auto page_at = [&](int slab) -> int {
+      if (slab >= s1 || slab * 16 >= n) return -1;
+      const int page = __ldg(table + (slab >> (p.page_shift - 4)));
+      if (static_cast<unsigned>(page) < static_cast<unsigned>(p.num_pages)) return page;
+      if (lane == 0) atomicOr(status, kDevBounds);
+      return -1;
+    };
+    auto issue = [&](int slab, int page, int stage) {
+      if (page >= 0) {
+        const int slot = (slab << 4) & (P - 1);
+        const uint8_t* ks = kbase + static_cast<int64_t>(page) * k_page + (slot * k_tok + k_lane);
+        const uint8_t* vs = vbase + static_cast<int64_t>(page) * v_page + (slot * v_tok + v_lane);
+        const uint32_t dst = my_ring_s + stage * L::kStageBytes;
+        if (slab * 16 + 16 <= seen_by_all) {
+#pragma unroll
+          for (int i = 0; i < COPIES; ++i) {
+            copy16(dst + share_off(i), ks + i * STEP * k_tok, 16);
+            copy16(dst + share_off(i) + L::kSlabBytes, vs + i * STEP * v_tok, 16);
+          }
+        } else {
+          // zeros past the sequence's end; V of tokens that not every row sees is added apart, so
+          // that a NaN there stays with the rows that see it
+#pragma unroll
+          for (int i = 0; i < COPIES; ++i) {
+            const int tok = slab * 16 + lane / CHUNKS + i * STEP;
+            copy16(dst + share_off(i), ks + i * STEP * k_tok, tok < n ? 16 : 0);
+            copy16(dst + share_off(i) + L::kSlabBytes, vs + i * STEP * v_tok, tok < seen_by_all ? 16 : 0);
+          }
+        }
+        if (lane < 2) copy4(my_sc_s + (stage * 2 + lane) * 4, sc_base + static_cast<int64_t>(page) * sc_page);
+        valid |= 1u << stage;
+      } else {
+        valid &= ~(1u << stage);
+      }
+      copies_commit();
+    };
+
+    __syncthreads();  // the previous item's readers of the ring, q_frag and q_unit are done
+    const int first = s0 + warp;
+#pragma unroll
+    for (int i = 0; i < ST - 1; ++i) issue(first + NW * i, page_at(first + NW * i), i);
+    int next_page = page_at(first + NW * (ST - 1));
+
     // ---- the queries, as fragments
     {
-      const int r = tid >> 4, part = tid & 15, rr = it.tile * 16 + r;
-      constexpr int E = D / 16;
+      constexpr int PARTS = NT / 16, E = D / PARTS;
+      const int r = tid / PARTS, part = tid % PARTS, rr = it.tile * 16 + r;
       float v[E];
       uint32_t top = 0;
       if (r < rows) {
@@ -231,13 +340,12 @@ __global__ void __launch_bounds__(256, 2) pages_attention_kernel(PagesAttnArgs a
 #pragma unroll
       for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      for (int o = PARTS / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
       // 2^(14 - e): the largest value lands in [2^14, 2^15); rows of zeros, infinities or NaN as they are
       const int e = static_cast<int>(top >> 23) - 127;
       const bool plain = top == 0 || top >= 0x7F800000u;
       const float up = plain ? 1.0f : e >= 0 ? __uint_as_float((127u + 14u - min(e, 127)) << 23)
                                              : __uint_as_float((127u + min(14 - max(e, -100), 127)) << 23);
-      __syncthreads();  // the previous item's readers of q_frag, q_unit and the merge are done
       if (part == 0) q_unit[r] = 1.0f / up;
       // dims of (step j, lane t): chunk * 16 + 4 i + {0, 1} in a0 / a1, {2, 3} in a2 / a3
 #pragma unroll
@@ -256,62 +364,17 @@ __global__ void __launch_bounds__(256, 2) pages_attention_kernel(PagesAttnArgs a
       __syncthreads();
     }
     const float unit0 = q_unit[g] * a.scale_log2, unit1 = q_unit[g + 8] * a.scale_log2;
-    int seen0 = n, seen1 = n;
-    if (a.causal) {
-      seen0 = max(0, n - a.q_len + 1 + (it.tile * 16 + g) % a.q_len);
-      seen1 = max(0, n - a.q_len + 1 + (it.tile * 16 + g + 8) % a.q_len);
-    }
-
     float o[TILES][4], m0 = kNoScore, m1 = kNoScore, l0 = 0.0f, l1 = 0.0f;
 #pragma unroll
     for (int j = 0; j < TILES; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
 
-    const uint8_t* kbase = p.codes[0] + it.h * p.sh[0];
-    const uint8_t* vbase = p.codes[1] + it.h * p.sh[1];
-    const int32_t* table = p.table + it.b * p.table_stride;
-    uint32_t valid = 0;  // bit s: stage s holds a page of the pool
-
-    auto page_at = [&](int slab) -> int {
-      if (slab >= s1 || slab * 16 >= n) return -1;
-      const int page = __ldg(table + ((slab * 16) >> p.page_shift));
-      if (page >= 0 && page < p.num_pages) return page;
-      if (lane == 0) atomicOr(status, kDevBounds);
-      return -1;
-    };
-    auto issue = [&](int slab, int page, int stage) {
-      if (page >= 0) {
-        const int tok0 = slab * 16, slot = tok0 & (P - 1);
-        const uint8_t* ks = kbase + page * p.sp[0] + slot * p.st[0];
-        const uint8_t* vs = vbase + page * p.sp[1] + slot * p.st[1];
-        const uint32_t dst = my_ring_s + stage * L::kStageBytes;
-#pragma unroll
-        for (int i = 0; i < COPIES; ++i) {
-          const int c = lane + 32 * i, row = c / CHUNKS, ch = c % CHUNKS;
-          const uint32_t off = slab_offset<D>(row, ch);
-          copy16(dst + off, ks + row * p.st[0] + ch * 16, tok0 + row < n ? 16 : 0);
-          // V of tokens that not every row sees is added apart, so that a NaN there stays with the
-          // rows that see it
-          copy16(dst + L::kSlabBytes + off, vs + row * p.st[1] + ch * 16, tok0 + row < seen_by_all ? 16 : 0);
-        }
-        if (lane < 2) copy4(my_sc_s + (stage * 2 + lane) * 4, p.scale[lane] + page * p.ssp[lane] + it.h * p.ssh[lane]);
-        valid |= 1u << stage;
-      } else {
-        valid &= ~(1u << stage);
-      }
-      copies_commit();
-    };
-
-    const int first = s0 + warp;
-#pragma unroll
-    for (int i = 0; i < ST - 1; ++i) issue(first + 8 * i, page_at(first + 8 * i), i);
-    int next_page = page_at(first + 8 * (ST - 1));
     int stage = 0;
-    for (int slab = first; slab < s1; slab += 8) {
+    for (int slab = first; slab < s1; slab += NW) {
       copies_wait<ST - 2>();
       __syncwarp();
-      const int ahead = slab + 8 * (ST - 1);
+      const int ahead = slab + NW * (ST - 1);
       issue(ahead, next_page, stage == 0 ? ST - 1 : stage - 1);
-      next_page = page_at(ahead + 8);
+      next_page = page_at(ahead + NW);
       if ((valid >> stage) & 1u) {
         const uint8_t* kb = my_ring + stage * L::kStageBytes;
         const uint8_t* vb = kb + L::kSlabBytes;
@@ -349,6 +412,7 @@ __global__ void __launch_bounds__(256, 2) pages_attention_kernel(PagesAttnArgs a
           s[i][3] *= c1;
         }
         if (slab * 16 + 16 > seen_by_all) {
+          const int seen0 = seen_of(0), seen1 = seen_of(1);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
 #pragma unroll
@@ -456,8 +520,8 @@ __global__ void __launch_bounds__(256, 2) pages_attention_kernel(PagesAttnArgs a
 #pragma unroll
             for (int j = 0; j < TILES; ++j) {
               const float value = e4m3_value_hw(__ldg(v + (2 * t + c) * (D / 8) + j));
-              if (x < seen0) o[j][c] = fmaf(w0, value, o[j][c]);
-              if (x < seen1) o[j][2 + c] = fmaf(w1, value, o[j][2 + c]);
+              if (x < seen_of(0)) o[j][c] = fmaf(w0, value, o[j][c]);
+              if (x < seen_of(1)) o[j][2 + c] = fmaf(w1, value, o[j][2 + c]);
             }
           }
         }
@@ -473,14 +537,16 @@ __global__ void __launch_bounds__(256, 2) pages_attention_kernel(PagesAttnArgs a
     // ---- the warps' parts of this block's share of the item
     __syncthreads();  // the ring is free
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int half = 0; half < 2; ++half) {
+      if (g + 8 * half >= rows) break;
 #pragma unroll
-      for (int j = 0; j < TILES; j += 4) {
-        const int d = (2 * t + c) * (D / 8) + j;
-        *reinterpret_cast<float4*>(&merge_o[(warp * 16 + g) * D + d]) =
-            make_float4(o[j][c], o[j + 1][c], o[j + 2][c], o[j + 3][c]);
-        *reinterpret_cast<float4*>(&merge_o[(warp * 16 + g + 8) * D + d]) =
-            make_float4(o[j][2 + c], o[j + 1][2 + c], o[j + 2][2 + c], o[j + 3][2 + c]);
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int j = 0; j < TILES; j += 4) {
+          const int d = (2 * t + c) * (D / 8) + j, e = 2 * half + c;
+          *reinterpret_cast<float4*>(&merge_o[(warp * 16 + g + 8 * half) * PITCH + d + d / 32 * 4]) =
+              make_float4(o[j][e], o[j + 1][e], o[j + 2][e], o[j + 3][e]);
+        }
       }
     }
     if (t == 0) {
@@ -491,89 +557,37 @@ __global__ void __launch_bounds__(256, 2) pages_attention_kernel(PagesAttnArgs a
     }
     __syncthreads();
     const bool whole = s0 == 0 && s1 == it.slabs;
-    const int64_t item = (static_cast<int64_t>(it.b) * p.heads + it.h) * a.row_tiles + it.tile;
-    const int64_t row_base = (static_cast<int64_t>(it.b) * p.heads + it.h) * a.rows + it.tile * 16;
-    auto finish = [&](int r, int d, float4 acc, float ref, float sum) {
-      const int rr = it.tile * 16 + r, qi = rr % a.q_len;
-      const int seen = a.causal ? max(0, n - a.q_len + 1 + qi) : n;
-      const float inv = seen > 0 ? 1.0f / sum : 0.0f;
-      const int64_t at = (row_base + r) * D + d;
-      store_elem<T>(a.out, at, acc.x * inv);
-      store_elem<T>(a.out, at + 1, acc.y * inv);
-      store_elem<T>(a.out, at + 2, acc.z * inv);
-      store_elem<T>(a.out, at + 3, acc.w * inv);
-      if (d == 0 && a.ml != nullptr) {
-        a.ml[2 * (row_base + r)] = ref;
-        a.ml[2 * (row_base + r) + 1] = inv;
-      }
-    };
     float* my_part = a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (it.first <= lo ? 0 : 1)) * 16 * (D + 2);
-    for (int i = tid; i < rows * (D / 4); i += 256) {
+    for (int i = tid; i < rows * (D / 4); i += NT) {
       const int r = i / (D / 4), d = i % (D / 4) * 4;
       float ref = kNoScore, sum = 0.0f;
 #pragma unroll
-      for (int w = 0; w < 8; ++w) ref = fmaxf(ref, merge_ml[(w * 16 + r) * 2]);
+      for (int w = 0; w < NW; ++w) ref = fmaxf(ref, merge_ml[(w * 16 + r) * 2]);
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-      for (int w = 0; w < 8; ++w) {
+      for (int w = 0; w < NW; ++w) {
         const float f = exp2_approx(merge_ml[(w * 16 + r) * 2] - ref);
         sum = fmaf(f, merge_ml[(w * 16 + r) * 2 + 1], sum);
-        const float4 x = *reinterpret_cast<const float4*>(&merge_o[(w * 16 + r) * D + d]);
+        const float4 x = *reinterpret_cast<const float4*>(&merge_o[(w * 16 + r) * PITCH + d + d / 32 * 4]);
         acc.x = fmaf(f, x.x, acc.x);
         acc.y = fmaf(f, x.y, acc.y);
         acc.z = fmaf(f, x.z, acc.z);
         acc.w = fmaf(f, x.w, acc.w);
       }
       if (whole) {
-        finish(r, d, acc, ref, sum);
+        pages_finish<T, D>(a, it.b, it.h, it.tile * 16 + r, d, n, acc, ref, sum);
       } else {
         __stcg(reinterpret_cast<float4*>(my_part + r * D + d), acc);
         if (d == 0) __stcg(reinterpret_cast<float2*>(my_part + 16 * D + 2 * r), make_float2(ref, sum));
       }
     }
-    if (!whole) {
-      // ---- the block that brings an item's last part merges all of them, in their order
-      const int64_t end = it.first + it.slabs;
-      const int c0 = static_cast<int>(((it.first + 1) * grid + total - 1) / total - 1);
-      const int c1 = static_cast<int>((end * grid + total - 1) / total - 1);
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) {
-        const unsigned done = atomicAdd(a.counters + item, 1u);
-        shared_i[1] = done == static_cast<unsigned>(c1 - c0);
-        if (shared_i[1]) a.counters[item] = 0;
-      }
-      __syncthreads();
-      if (shared_i[1]) {
-        __threadfence();
-        auto part_of = [&](int c) -> const float* {
-          const int64_t begin = total * c / grid;
-          return a.partial + (static_cast<int64_t>(c) * 2 + (it.first <= begin ? 0 : 1)) * 16 * (D + 2);
-        };
-        for (int i = tid; i < rows * (D / 4); i += 256) {
-          const int r = i / (D / 4), d = i % (D / 4) * 4;
-          float ref = kNoScore, sum = 0.0f;
-          float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          for (int c = c0; c <= c1; ++c) ref = fmaxf(ref, __ldcg(part_of(c) + 16 * D + 2 * r));
-#pragma unroll 4
-          for (int c = c0; c <= c1; ++c) {
-            const float* part = part_of(c);
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(part + 16 * D + 2 * r));
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(part + r * D + d));
-            const float f = exp2_approx(ml.x - ref);
-            sum = fmaf(f, ml.y, sum);
-            acc.x = fmaf(f, x.x, acc.x);
-            acc.y = fmaf(f, x.y, acc.y);
-            acc.z = fmaf(f, x.z, acc.z);
-            acc.w = fmaf(f, x.w, acc.w);
-          }
-          finish(r, d, acc, ref, sum);
-        }
-      }
+    if (s0 == 0 && !whole) {
+      // the merge goes from this block to the one that holds the item's last unit
+      cut = PagesCut{it.b, it.h, it.tile, static_cast<int>((end * grid + total - 1) / total - 1), it.first <= lo ? 0 : 1};
+    }
     }
     // ---- the next item
-    pos = it.first + s1;
-    it.first += it.slabs;
+    it.first = end;
     if (++it.tile == a.row_tiles) {
       it.tile = 0;
       if (++it.h == p.heads) {
@@ -582,11 +596,68 @@ __global__ void __launch_bounds__(256, 2) pages_attention_kernel(PagesAttnArgs a
       }
     }
   }
+  if (tid == 0) a.cuts[blockIdx.x] = cut;
+}
+
+// The items that several blocks share: four warps per row add the blocks' outputs, each with its
+// weight, in an order that depends on nothing but their number. A block per cut and four rows.
+template <int T, int D>
+__global__ void __launch_bounds__(512) pages_merge_kernel(PagesAttnArgs a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const PagesCut cut = a.cuts[blockIdx.x];
+  if (cut.last < 0) return;
+  constexpr int LANES = D / 4, SIDES = 32 / LANES, SHARES = 4 * SIDES;  // lanes per part, parts side by side
+  __shared__ float4 sums[4][SHARES][LANES];
+  const int lane = threadIdx.x & 31, group = threadIdx.x >> 7, share = (threadIdx.x >> 5 & 3) * SIDES + lane / LANES;
+  const int row = blockIdx.y * 4 + group, r = cut.tile * 16 + row, parts = cut.last - static_cast<int>(blockIdx.x) + 1;
+  const bool live = row < 16 && r < a.rows;
+  auto part_of = [&](int i) -> const float* {
+    const int64_t slot = i == 0 ? 2 * static_cast<int64_t>(blockIdx.x) + cut.slot : 2 * (static_cast<int64_t>(blockIdx.x) + i);
+    return a.partial + slot * 16 * (D + 2);
+  };
+  float ref = kNoScore, sum = 0.0f;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (live) {
+    for (int i = lane; i < parts; i += 32) ref = fmaxf(ref, __ldg(part_of(i) + 16 * D + 2 * row));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, o));
+    for (int i = lane; i < parts; i += 32) {
+      const float2 ml = __ldg(reinterpret_cast<const float2*>(part_of(i) + 16 * D + 2 * row));
+      sum = fmaf(exp2_approx(ml.x - ref), ml.y, sum);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const int d = lane % LANES * 4;
+#pragma unroll 8
+    for (int i = share; i < parts; i += SHARES) {
+      const float* part = part_of(i);
+      const float f = exp2_approx(__ldg(part + 16 * D + 2 * row) - ref);
+      const float4 x = __ldg(reinterpret_cast<const float4*>(part + row * D + d));
+      acc.x = fmaf(f, x.x, acc.x);
+      acc.y = fmaf(f, x.y, acc.y);
+      acc.z = fmaf(f, x.z, acc.z);
+      acc.w = fmaf(f, x.w, acc.w);
+    }
+    sums[group][share][lane % LANES] = acc;
+  }
+  __syncthreads();
+  if (!live || share != 0) return;
+#pragma unroll
+  for (int s = 1; s < SHARES; ++s) {
+    const float4 x = sums[group][s][lane];
+    acc.x += x.x;
+    acc.y += x.y;
+    acc.z += x.z;
+    acc.w += x.w;
+  }
+  const int n = min(max(__ldg(a.pool.lengths + cut.b), 0), a.pool.max_pages << a.pool.page_shift);
+  pages_finish<T, D>(a, cut.b, cut.h, r, lane * 4, n, acc, ref, sum);
 }
 
 // The mass of every cached token: its weights, from the stored scores and the rows' final
 // reference and sum, added in the order of the rows. One thread per token and KV head.
 __global__ void __launch_bounds__(256) pages_mass_kernel(PagesAttnArgs a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const PagePool& p = a.pool;
   const int h = blockIdx.y, b = blockIdx.z;
   const int n = min(max(__ldg(p.lengths + b), 0), p.max_pages << p.page_shift);

@@ -58,6 +58,12 @@ int pool_check(const KabKvPages* c, PagePool* p) {
   KAB_REQUIRE(c->k_stride_page % 16 == 0 && c->k_stride_head % 16 == 0 && c->k_stride_token % 16 == 0 &&
                   c->v_stride_page % 16 == 0 && c->v_stride_head % 16 == 0 && c->v_stride_token % 16 == 0,
               "page strides must be multiples of 16 bytes");
+  const int64_t wide = int64_t(1) << 31;
+  KAB_REQUIRE(c->k_stride_page < wide && c->v_stride_page < wide && c->ks_stride_page < wide &&
+                  c->vs_stride_page < wide && c->k_stride_token * c->page_tokens < wide &&
+                  c->v_stride_token * c->page_tokens < wide && c->k_stride_page >= 0 && c->v_stride_page >= 0 &&
+                  c->k_stride_token >= 0 && c->v_stride_token >= 0 && c->ks_stride_page >= 0 && c->vs_stride_page >= 0,
+              "page strides and a page's tokens must span less than 2^31 bytes");
   *p = PagePool{};
   p->codes[0] = c->k_pages;
   p->codes[1] = c->v_pages;
@@ -112,12 +118,12 @@ int attention_check(const KabKvPagesAttention* p, PagesAttnArgs* g) {
   return KAB_OK;
 }
 
-// The launch's workspace: counters (zero between launches), the blocks' partial results and, with
-// mass, the scores and the rows' references.
+// The launch's workspace: the blocks' partial results and cuts and, with mass, the scores and the
+// rows' references. Nothing in it has to be zero.
 struct AttentionPlan {
   int grid = 0;
-  size_t counters = 0, partial = 0, ml = 0, scores = 0;
-  size_t bytes() const { return counters + partial + ml + scores; }
+  size_t cuts = 0, partial = 0, ml = 0, scores = 0;
+  size_t bytes() const { return cuts + partial + ml + scores; }
 };
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -135,7 +141,7 @@ int attention_blocks() {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem) != cudaSuccess ||
         cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, L::kThreads, L::kSmem) != cudaSuccess || n < 1)
       return -1;
-    blocks[dev] = n * sm_count();
+    blocks[dev] = std::min(n, L::kBlocks) * sm_count();
   }
   return blocks[dev];
 }
@@ -149,7 +155,7 @@ int attention_plan(const KabKvPagesAttention* p, const PagesAttnArgs& g, Attenti
   plan->grid = attention_blocks(p->q_dtype, p->cache.head_dim);
   if (plan->grid < 0) return fail(KAB_ECUDA, "cannot configure the paged attention kernel");
   const size_t items = static_cast<size_t>(p->cache.batch * p->cache.heads_kv);
-  plan->counters = round256(items * g.row_tiles * 4);
+  plan->cuts = round256(static_cast<size_t>(plan->grid) * sizeof(PagesCut));
   plan->partial = round256(static_cast<size_t>(plan->grid) * 2 * 16 * (p->cache.head_dim + 2) * 4);
   if (p->use_mass) {
     plan->ml = round256(items * g.rows * 8);
@@ -158,14 +164,32 @@ int attention_plan(const KabKvPagesAttention* p, const PagesAttnArgs& g, Attenti
   return KAB_OK;
 }
 
+// A launch that may be set up while the one before it runs (it waits by itself).
+template <typename... Args>
+cudaError_t launch_after(void (*kern)(Args...), dim3 grid, int threads, cudaStream_t s, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
 template <int T, int D>
 int launch_attention(const PagesAttnArgs& g, int grid, unsigned* status, cudaStream_t s) {
   using L = PagesLayout<D, T == kF32>;
   pages_attention_kernel<T, D><<<grid, L::kThreads, L::kSmem, s>>>(g, status);
   if (int e = check_launch("kab_kv_pages_attention")) return e;
+  const dim3 merges(static_cast<unsigned>(grid), static_cast<unsigned>((std::min(g.rows, 16) + 3) / 4));
+  launch_after(pages_merge_kernel<T, D>, merges, 512, s, g);
+  if (int e = check_launch("kab_kv_pages_attention merge")) return e;
   if (g.scores == nullptr || g.capacity == 0) return KAB_OK;
   const dim3 blocks(static_cast<unsigned>((g.capacity + 255) / 256), g.pool.heads, g.pool.batch);
-  pages_mass_kernel<<<blocks, 256, 0, s>>>(g);
+  launch_after(pages_mass_kernel, blocks, 256, s, g);
   return check_launch("kab_kv_pages_attention mass");
 }
 
@@ -230,7 +254,7 @@ int kab_kv_pages_attention_workspace(const KabKvPagesAttention* params, size_t* 
   if (params->cache.batch > 0 && g.rows > 0)
     if (int e = attention_plan(params, g, &plan)) return e;
   *bytes = plan.bytes();
-  *zero_bytes = plan.counters;
+  *zero_bytes = 0;
   return KAB_OK;
 }
 
@@ -246,11 +270,11 @@ int kab_kv_pages_attention(const KabKvPagesAttention* params, void* workspace, s
   unsigned* status = status_word();
   KAB_REQUIRE(status != nullptr, "no device status word");
   uint8_t* w = static_cast<uint8_t*>(workspace);
-  g.counters = reinterpret_cast<unsigned*>(w);
-  g.partial = reinterpret_cast<float*>(w + plan.counters);
+  g.cuts = reinterpret_cast<PagesCut*>(w);
+  g.partial = reinterpret_cast<float*>(w + plan.cuts);
   if (params->use_mass) {
-    g.ml = reinterpret_cast<float*>(w + plan.counters + plan.partial);
-    g.scores = reinterpret_cast<float*>(w + plan.counters + plan.partial + plan.ml);
+    g.ml = reinterpret_cast<float*>(w + plan.cuts + plan.partial);
+    g.scores = reinterpret_cast<float*>(w + plan.cuts + plan.partial + plan.ml);
   }
   const cudaStream_t s = as_stream(stream);
 #define KAB_PAGES_D(TT)                                                              \
