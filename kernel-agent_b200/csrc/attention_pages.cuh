@@ -19,9 +19,9 @@
 //    [2^14, 2^15): bf16 and f16 values keep all their bits down to 2^-29 of the row's largest;
 //    fp32 ones are split into two f16 terms (22 bits) and the product is taken twice.
 //  * The running maximum is that of t = s + log2(V scale), s the score in log2 units: the weight
-//    that multiplies the V codes is w = 2^(s - m) * V scale <= 2^15 with m = max t - 15, so w fits
-//    f16 with 11 bits down to 2^-29 of the largest and the page's scale costs one multiplication.
-//    Sums use 2^(s - m) itself, in fp32. (Adding every slab's product to the output with its own
+//    that multiplies the V codes is w = 2^(s - m) * V scale, with m = t - 10 at a slab's largest t,
+//    so w fits f16 with 11 bits down to 2^-24 of the largest at least and the page's scale costs
+//    one multiplication. Sums use 2^(s - m) itself, in fp32. (Adding every slab's product to the output with its own
 //    scale instead would cost 64 more multiply-adds per lane and slab.) log2(V scale) is cut at
 //    -80, which keeps the sums finite; values below 2^-80 * 448 round to zero beside it.
 #pragma once
@@ -89,6 +89,19 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// (a, b) * c and (a, b) + c in one instruction.
+__device__ __forceinline__ void scale_pair(float& a, float& b, float c) {
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%0, %1};\n mov.b64 y, {%2, %2};\n mul.rn.f32x2 x, x, y;\n"
+      " mov.b64 {%0, %1}, x;\n}"
+      : "+f"(a), "+f"(b)
+      : "f"(c));
+}
+__device__ __forceinline__ void add_pair(float& a, float& b, float c) {
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%0, %1};\n mov.b64 y, {%2, %2};\n add.rn.f32x2 x, x, y;\n"
+      " mov.b64 {%0, %1}, x;\n}"
+      : "+f"(a), "+f"(b)
+      : "f"(c));
+}
 // 16 bytes to shared memory without waiting; `bytes` 0 writes zeros.
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -131,7 +144,10 @@ __device__ __forceinline__ uint32_t slab_offset(int row, int chunk) {
 
 constexpr int kItemCost = 6;  // an item's queries, merge and output cost about as much as six slabs
 constexpr float kNoScore = -3.3e38f;  // below every finite score
-constexpr float kWeightBits = 15.0f;  // the largest weight is 2^15 in f16
+// A row's weights are at most 2^10 when its reference is set; the reference moves again only when
+// one would pass 2^15.9, the end of f16: rarely after the first slab, while every row's running
+// maximum would move often enough to rescale the 64 outputs of a lane in most slabs.
+constexpr float kWeightBits = 10.0f, kWeightRoom = 5.9f;
 constexpr float kLeastLogScale = -80.0f;
 
 // ------------------------------------------------------------------ the kernel
@@ -139,7 +155,7 @@ constexpr float kLeastLogScale = -80.0f;
 // Where a position of the line of slabs lies: sequence, head, row tile, and the item's first slab.
 struct PagesItem {
   int b, h, tile, length, slabs;
-  int64_t first;
+  unsigned first;
 };
 
 // Four output elements of row r (of a KV head's rows) from their weighted sum and the row's sum.
@@ -176,7 +192,6 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
   float* sc_all = reinterpret_cast<float*>(ring + L::kRing);
   float* q_unit = sc_all + L::kWarps * ST * 2;                     // [16] units of the query rows
   int* shared_i = reinterpret_cast<int*>(q_unit + 16);             // [8..] broadcast words
-  int64_t* shared_l = reinterpret_cast<int64_t*>(shared_i + 12);
   constexpr int PITCH = L::kPitch;
   float* merge_o = reinterpret_cast<float*>(ring);                 // [8][16][PITCH]
   float* merge_ml = merge_o + L::kWarps * 16 * PITCH;              // [8][16][2]
@@ -189,50 +204,54 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
   // the merge may be set up while this kernel runs: it waits for its end by itself
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // ---- this block's part of the line
-  auto units_of = [&](int b) -> int64_t {
+  auto units_of = [&](int b) -> unsigned {
     const int n = min(max(__ldg(p.lengths + b), 0), cap);
     return max((n + 15) >> 4, 1) + kItemCost;  // an empty sequence is one empty slab: its output is written too
   };
   const int chunk = (p.batch + NT - 1) / NT;
-  int64_t mine = 0;
+  unsigned mine = 0;
   for (int i = 0; i < chunk; ++i) {
     const int b = tid * chunk + i;
     if (b < p.batch) mine += units_of(b) * per_seq;
   }
-  int64_t upto = mine;
+  unsigned upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+    const unsigned y = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += y;
   }
-  int64_t* warp_sum = reinterpret_cast<int64_t*>(ring);
+  unsigned* warp_sum = reinterpret_cast<unsigned*>(ring);
   if (lane == 31) warp_sum[warp] = upto;
   __syncthreads();
-  int64_t total = 0, before = upto - mine;
+  unsigned total = 0, before = upto - mine;
 #pragma unroll
   for (int w = 0; w < NW; ++w) {
     if (w < warp) before += warp_sum[w];
     total += warp_sum[w];
   }
-  const int64_t grid = min(static_cast<int64_t>(gridDim.x), total);
+  const unsigned grid = min(gridDim.x, total), share = total / grid, longer = total % grid;
   if (blockIdx.x >= grid) {
     if (tid == 0) a.cuts[blockIdx.x].last = -1;
     return;
   }
-  const int64_t lo = total * blockIdx.x / grid, hi = total * (blockIdx.x + 1) / grid;
+  // the first `longer` blocks take one unit more
+  const unsigned lo = share * blockIdx.x + min(blockIdx.x, longer), hi = lo + share + (blockIdx.x < longer);
+  auto block_of = [&](unsigned unit) -> unsigned {
+    const unsigned split = longer * (share + 1);
+    return unit < split ? unit / (share + 1) : longer + (unit - split) / share;
+  };
   if (lo >= before && lo < before + mine) {  // one thread: the sequence that `lo` lies in
-    int64_t at = before;
+    unsigned at = before;
     int b = tid * chunk;
     while (lo >= at + units_of(b) * per_seq) at += units_of(b++) * per_seq;
     shared_i[0] = b;
-    shared_l[0] = at;
+    shared_i[1] = static_cast<int>(at);
   }
   __syncthreads();
   PagesItem it;
   it.b = shared_i[0];
   {
-    const int64_t at = shared_l[0], n = units_of(it.b);
-    const int i = static_cast<int>((lo - at) / n);
+    const unsigned at = shared_i[1], n = units_of(it.b), i = (lo - at) / n;
     it.h = i / a.row_tiles;
     it.tile = i % a.row_tiles;
     it.first = at + i * n;
@@ -254,9 +273,9 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
   auto share_off = [&](int i) -> uint32_t { return (D == 128 && (i & 1) ? lane_off ^ 64u : lane_off) + i * 512; };
 
   PagesCut cut{0, 0, 0, -1, 0};
-  for (int64_t pos = lo; pos < hi;) {
+  for (unsigned pos = lo; pos < hi;) {
     it.length = page_length(p, it.b, status);
-    const int64_t end = it.first + units_of(it.b);
+    const unsigned end = it.first + units_of(it.b);
     it.slabs = static_cast<int>(end - it.first) - kItemCost;
     // the item's first kItemCost units stand for what an item costs beside its slabs
     const int s0 = max(0, static_cast<int>(pos - it.first) - kItemCost);
@@ -406,10 +425,8 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
         const float c0 = unit0 * ksc, c1 = unit1 * ksc;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          s[i][0] *= c0;
-          s[i][1] *= c0;
-          s[i][2] *= c1;
-          s[i][3] *= c1;
+          scale_pair(s[i][0], s[i][1], c0);
+          scale_pair(s[i][2], s[i][3], c1);
         }
         if (slab * 16 + 16 > seen_by_all) {
           const int seen0 = seen_of(0), seen1 = seen_of(1);
@@ -438,8 +455,8 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
         t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 1));
         t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 2)) + (lv - kWeightBits);
         t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 2)) + (lv - kWeightBits);
-        if (__any_sync(0xffffffffu, t0 > m0 || t1 > m1)) {
-          const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
+        if (__any_sync(0xffffffffu, t0 > m0 + kWeightRoom || t1 > m1 + kWeightRoom)) {
+          const float n0 = t0 > m0 + kWeightRoom ? t0 : m0, n1 = t1 > m1 + kWeightRoom ? t1 : m1;
           const float f0 = exp2_approx(m0 - n0), f1 = exp2_approx(m1 - n1);
           m0 = n0;
           m1 = n1;
@@ -447,25 +464,23 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
           l1 *= f1;
 #pragma unroll
           for (int j = 0; j < TILES; ++j) {
-            o[j][0] *= f0;
-            o[j][1] *= f0;
-            o[j][2] *= f1;
-            o[j][3] *= f1;
+            scale_pair(o[j][0], o[j][1], f0);
+            scale_pair(o[j][2], o[j][3], f1);
           }
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          s[i][0] = exp2_approx(s[i][0] - m0);
-          s[i][1] = exp2_approx(s[i][1] - m0);
-          s[i][2] = exp2_approx(s[i][2] - m1);
-          s[i][3] = exp2_approx(s[i][3] - m1);
+          add_pair(s[i][0], s[i][1], -m0);
+          add_pair(s[i][2], s[i][3], -m1);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[i][e] = exp2_approx(s[i][e]);
         }
         l0 += (s[0][0] + s[0][1]) + (s[1][0] + s[1][1]);
         l1 += (s[0][2] + s[0][3]) + (s[1][2] + s[1][3]);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[i][e] *= vsc;
+          scale_pair(s[i][0], s[i][1], vsc);
+          scale_pair(s[i][2], s[i][3], vsc);
         }
         const uint32_t pa[4] = {f16x2_of(s[0][0], s[0][1]), f16x2_of(s[0][2], s[0][3]), f16x2_of(s[1][0], s[1][1]),
                                 f16x2_of(s[1][2], s[1][3])};
@@ -583,7 +598,7 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
     }
     if (s0 == 0 && !whole) {
       // the merge goes from this block to the one that holds the item's last unit
-      cut = PagesCut{it.b, it.h, it.tile, static_cast<int>((end * grid + total - 1) / total - 1), it.first <= lo ? 0 : 1};
+      cut = PagesCut{it.b, it.h, it.tile, static_cast<int>(block_of(end - 1)), it.first <= lo ? 0 : 1};
     }
     }
     // ---- the next item

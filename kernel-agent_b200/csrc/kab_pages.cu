@@ -155,6 +155,8 @@ int attention_plan(const KabKvPagesAttention* p, const PagesAttnArgs& g, Attenti
   plan->grid = attention_blocks(p->q_dtype, p->cache.head_dim);
   if (plan->grid < 0) return fail(KAB_ECUDA, "cannot configure the paged attention kernel");
   const size_t items = static_cast<size_t>(p->cache.batch * p->cache.heads_kv);
+  KAB_REQUIRE(items * g.row_tiles * (static_cast<size_t>(g.capacity) / 16 + 1 + kItemCost) < (size_t(1) << 31),
+              "sequences x KV heads x row tiles x tokens of the page table is too large");
   plan->cuts = round256(static_cast<size_t>(plan->grid) * sizeof(PagesCut));
   plan->partial = round256(static_cast<size_t>(plan->grid) * 2 * 16 * (p->cache.head_dim + 2) * 4);
   if (p->use_mass) {
