@@ -10,8 +10,8 @@
 // the warp. What has to be fast is the stream: every warp keeps its own ring of 16-token slabs of
 // K and V in flight with cp.async and never waits for another warp inside a segment.
 //
-//  * Work is cut into equal parts whatever the lengths: the slabs of all (sequence, KV head, 16
-//    rows) items stand in one line, and each block takes a contiguous part of it. A block's first
+//  * Work is cut into equal parts whatever the lengths: the slabs of all (sequence, KV head, row
+//    tile) items stand in one line, and each block takes a contiguous part of it. A block's first
 //    and last item may be shared with its neighbours: their partial results (maximum, sum,
 //    output) go to two slots of the block's own, and a second small launch merges them in an
 //    order of their own, so the same inputs give the same bits.
@@ -43,7 +43,7 @@ struct PagesAttnArgs {
   float scale_log2;  // sm_scale * log2(e)
   int heads_q, q_len, causal;
   int rows, row_tiles;   // rows of one KV head (query heads x query tokens), tiles of 16 of them
-  float* partial;        // [grid, 2 slots, 16 rows, D + 2]: output, maximum, sum
+  float* partial;        // [grid, 2 slots, a tile's rows, D + 2]: output, maximum, sum
   PagesCut* cuts;        // [grid]: the item that begins in a block and goes on in the next ones
   float* scores;         // [batch, heads, rows, capacity] in log2 units, or NULL
   float* ml;             // [batch, heads, rows, 2]: reference and reciprocal sum, with scores
@@ -89,18 +89,18 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// (a, b) * c and (a, b) + c in one instruction.
+// (a, b) * c in one instruction.
 __device__ __forceinline__ void scale_pair(float& a, float& b, float c) {
   asm("{\n .reg .b64 x, y;\n mov.b64 x, {%0, %1};\n mov.b64 y, {%2, %2};\n mul.rn.f32x2 x, x, y;\n"
       " mov.b64 {%0, %1}, x;\n}"
       : "+f"(a), "+f"(b)
       : "f"(c));
 }
-__device__ __forceinline__ void add_pair(float& a, float& b, float c) {
-  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%0, %1};\n mov.b64 y, {%2, %2};\n add.rn.f32x2 x, x, y;\n"
-      " mov.b64 {%0, %1}, x;\n}"
-      : "+f"(a), "+f"(b)
-      : "f"(c));
+// An 8 x 8 matrix of f16 over the warp (lane (g, t) holds row g, columns 2 t and 2 t + 1), transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 // 16 bytes to shared memory without waiting; `bytes` 0 writes zeros.
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
@@ -117,20 +117,21 @@ __device__ __forceinline__ void copies_wait() {
 
 // ------------------------------------------------------------------ layout
 
-template <int D, bool SPLIT>
+// NR: groups of 8 query rows that share one pass over the cache (the MMA's N).
+template <int D, int NR, bool SPLIT>
 struct PagesLayout {
-  static constexpr int kWarps = 4, kThreads = kWarps * 32, kStages = 3, kSlab = 16;
-  static constexpr int kBlocks = 16 / kWarps;  // per SM: 16 warps of 128 registers
-  static constexpr int kSlabBytes = kSlab * D;              // K or V of one slab
+  static constexpr int kWarps = 4, kThreads = kWarps * 32, kRows = 8 * NR;
+  static constexpr int kBlocks = NR == 1 && !SPLIT ? 5 : 4;  // per SM, by registers
+  static constexpr int kStages = NR == 1 && !SPLIT ? 2 : 3;
+  static constexpr int kSlabBytes = 16 * D;  // K or V of one slab
   static constexpr int kStageBytes = 2 * kSlabBytes;
-  static constexpr int kQBytes = D / 16 * 32 * 16 * (SPLIT ? 2 : 1);
-  static constexpr int kRing = kWarps * kStages * kStageBytes;
+  static constexpr int kQBytes = D / 16 * 32 * 8 * NR * (SPLIT ? 2 : 1);
+  // a row of the warps' outputs in the merge: its pitch keeps the fragments' float4 stores two to a bank
+  static constexpr int kPitch = D + 4;
+  static constexpr int kMergeBytes = kWarps * kRows * (kPitch + 2) * 4;
+  static constexpr int kRing = kWarps * kStages * kStageBytes > kMergeBytes ? kWarps * kStages * kStageBytes : kMergeBytes;
   static constexpr int kScales = kWarps * kStages * 2 * 4;
-  static constexpr int kSmem = kQBytes + kRing + kScales + 256;
-  // a row of the warps' outputs in the merge: 4 floats of padding per 32 and a pitch that shifts
-  // the next row by 16 (8) banks, so that the fragments' float4 stores touch all banks
-  static constexpr int kPitch = D + D / 32 * 4;
-  static_assert(kRing >= kWarps * 16 * (kPitch + 2) * 4, "the merge reuses the ring");
+  static constexpr int kSmem = kQBytes + kRing + kScales + kRows * 4 + 32;
 };
 
 // Byte offset of 16-byte chunk `chunk` of token `row` in a slab: the chunks are permuted so that
@@ -146,13 +147,13 @@ constexpr int kItemCost = 6;  // an item's queries, merge and output cost about 
 constexpr float kNoScore = -3.3e38f;  // below every finite score
 // A row's weights are at most 2^10 when its reference is set; the reference moves again only when
 // one would pass 2^15.9, the end of f16: rarely after the first slab, while every row's running
-// maximum would move often enough to rescale the 64 outputs of a lane in most slabs.
+// maximum would move often enough to rescale a lane's outputs in most slabs.
 constexpr float kWeightBits = 10.0f, kWeightRoom = 5.9f;
 constexpr float kLeastLogScale = -80.0f;
 
 // ------------------------------------------------------------------ the kernel
 
-// Where a position of the line of slabs lies: sequence, head, row tile, and the item's first slab.
+// Where a position of the line of slabs lies: sequence, head, row tile, and the item's first unit.
 struct PagesItem {
   int b, h, tile, length, slabs;
   unsigned first;
@@ -180,21 +181,21 @@ __device__ __forceinline__ void pages_finish(const PagesAttnArgs& a, int b, int 
   }
 }
 
-template <int T, int D>
-__global__ void __launch_bounds__(PagesLayout<D, T == kF32>::kThreads, PagesLayout<D, T == kF32>::kBlocks)
+template <int T, int D, int NR>
+__global__ void __launch_bounds__(PagesLayout<D, NR, T == kF32>::kThreads, PagesLayout<D, NR, T == kF32>::kBlocks)
 pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
-  constexpr bool SPLIT = T == kF32;
-  using L = PagesLayout<D, SPLIT>;
-  constexpr int ST = L::kStages, NW = L::kWarps, NT = L::kThreads, TILES = D / 8, CHUNKS = D / 16, COPIES = D / 32;
+  constexpr bool SPLIT = T == kF32, Q_HELD = NR == 1 && !SPLIT;
+  using L = PagesLayout<D, NR, SPLIT>;
+  constexpr int ST = L::kStages, NW = L::kWarps, NT = L::kThreads, ROWS = L::kRows, PITCH = L::kPitch;
+  constexpr int STEPS = D / 16, MT = D / 16, CHUNKS = D / 16, COPIES = D / 32;
   extern __shared__ __align__(128) uint8_t smem[];
-  uint4* q_frag = reinterpret_cast<uint4*>(smem);
+  uint2* q_frag = reinterpret_cast<uint2*>(smem);                  // [hi, lo][NR][STEPS][32]
   uint8_t* ring = smem + L::kQBytes;
   float* sc_all = reinterpret_cast<float*>(ring + L::kRing);
-  float* q_unit = sc_all + L::kWarps * ST * 2;                     // [16] units of the query rows
-  int* shared_i = reinterpret_cast<int*>(q_unit + 16);             // [8..] broadcast words
-  constexpr int PITCH = L::kPitch;
-  float* merge_o = reinterpret_cast<float*>(ring);                 // [8][16][PITCH]
-  float* merge_ml = merge_o + L::kWarps * 16 * PITCH;              // [8][16][2]
+  float* q_unit = sc_all + NW * ST * 2;                            // [ROWS] units of the query rows
+  int* shared_i = reinterpret_cast<int*>(q_unit + ROWS);
+  float* merge_o = reinterpret_cast<float*>(ring);                 // [NW][ROWS][PITCH]
+  float* merge_ml = merge_o + NW * ROWS * PITCH;                   // [NW][ROWS][2]
 
   const PagePool& p = a.pool;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -282,324 +283,346 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
     const int s1 = static_cast<int>(min(end, hi) - it.first) - kItemCost;
     pos = end;
     const int n = it.length;
-    const int rows = min(16, a.rows - it.tile * 16);
+    const int rows = min(ROWS, a.rows - it.tile * ROWS);
     const int seen_by_all = a.causal ? max(0, n - a.q_len + 1) : n;
-
     if (s1 > 0) {
-    // tokens that row g (half 0) or g + 8 (half 1) of the tile sees
-    auto seen_of = [&](int half) -> int {
-      return a.causal ? max(0, n - a.q_len + 1 + (it.tile * 16 + g + 8 * half) % a.q_len) : n;
-    };
+      // tokens that row r of the tile sees
+      auto seen_of = [&](int r) -> int {
+        return a.causal ? max(0, n - a.q_len + 1 + (it.tile * ROWS + r) % a.q_len) : n;
+      };
 
-    const uint8_t* kbase = p.codes[0] + it.h * p.sh[0];
-    const uint8_t* vbase = p.codes[1] + it.h * p.sh[1];
-    const int32_t* table = p.table + it.b * p.table_stride;
-    // lane 0 fetches K's scales, lane 1 V's
-    const float* sc_base = lane & 1 ? p.scale[1] + it.h * p.ssh[1] : p.scale[0] + it.h * p.ssh[0];
-    uint32_t valid = 0;  // bit s: stage s holds a page of the pool
+      const uint8_t* kbase = p.codes[0] + it.h * p.sh[0];
+      const uint8_t* vbase = p.codes[1] + it.h * p.sh[1];
+      const int32_t* table = p.table + it.b * p.table_stride;
+      // lane 0 fetches K's scales, lane 1 V's
+      const float* sc_base = lane & 1 ? p.scale[1] + it.h * p.ssh[1] : p.scale[0] + it.h * p.ssh[0];
+      uint32_t valid = 0;  // bit s: stage s holds a page of the pool
 
-    auto page_at = [&](int slab) -> int {
-      if (slab >= s1 || slab * 16 >= n) return -1;
-      const int page = __ldg(table + (slab >> (p.page_shift - 4)));
-      if (static_cast<unsigned>(page) < static_cast<unsigned>(p.num_pages)) return page;
-      if (lane == 0) atomicOr(status, kDevBounds);
-      return -1;
-    };
-    auto issue = [&](int slab, int page, int stage) {
-      if (page >= 0) {
-        const int slot = (slab << 4) & (P - 1);
-        const uint8_t* ks = kbase + static_cast<int64_t>(page) * k_page + (slot * k_tok + k_lane);
-        const uint8_t* vs = vbase + static_cast<int64_t>(page) * v_page + (slot * v_tok + v_lane);
-        const uint32_t dst = my_ring_s + stage * L::kStageBytes;
-        if (slab * 16 + 16 <= seen_by_all) {
+      auto page_at = [&](int slab) -> int {
+        if (slab >= s1 || slab * 16 >= n) return -1;
+        const int page = __ldg(table + (slab >> (p.page_shift - 4)));
+        if (static_cast<unsigned>(page) < static_cast<unsigned>(p.num_pages)) return page;
+        if (lane == 0) atomicOr(status, kDevBounds);
+        return -1;
+      };
+      auto issue = [&](int slab, int page, int stage) {
+        if (page >= 0) {
+          const int slot = (slab << 4) & (P - 1);
+          const uint8_t* ks = kbase + static_cast<int64_t>(page) * k_page + (slot * k_tok + k_lane);
+          const uint8_t* vs = vbase + static_cast<int64_t>(page) * v_page + (slot * v_tok + v_lane);
+          const uint32_t dst = my_ring_s + stage * L::kStageBytes;
+          if (slab * 16 + 16 <= seen_by_all) {
 #pragma unroll
-          for (int i = 0; i < COPIES; ++i) {
-            copy16(dst + share_off(i), ks + i * STEP * k_tok, 16);
-            copy16(dst + share_off(i) + L::kSlabBytes, vs + i * STEP * v_tok, 16);
+            for (int i = 0; i < COPIES; ++i) {
+              copy16(dst + share_off(i), ks + i * STEP * k_tok, 16);
+              copy16(dst + share_off(i) + L::kSlabBytes, vs + i * STEP * v_tok, 16);
+            }
+          } else {
+            // zeros past the sequence's end; V of tokens that not every row sees is added apart, so
+            // that a NaN there stays with the rows that see it
+#pragma unroll
+            for (int i = 0; i < COPIES; ++i) {
+              const int tok = slab * 16 + lane / CHUNKS + i * STEP;
+              copy16(dst + share_off(i), ks + i * STEP * k_tok, tok < n ? 16 : 0);
+              copy16(dst + share_off(i) + L::kSlabBytes, vs + i * STEP * v_tok, tok < seen_by_all ? 16 : 0);
+            }
           }
+          if (lane < 2) copy4(my_sc_s + (stage * 2 + lane) * 4, sc_base + static_cast<int64_t>(page) * sc_page);
+          valid |= 1u << stage;
         } else {
-          // zeros past the sequence's end; V of tokens that not every row sees is added apart, so
-          // that a NaN there stays with the rows that see it
+          valid &= ~(1u << stage);
+        }
+        copies_commit();
+      };
+
+      __syncthreads();  // the previous item's readers of the ring, q_frag and q_unit are done
+      const int first = s0 + warp;
 #pragma unroll
-          for (int i = 0; i < COPIES; ++i) {
-            const int tok = slab * 16 + lane / CHUNKS + i * STEP;
-            copy16(dst + share_off(i), ks + i * STEP * k_tok, tok < n ? 16 : 0);
-            copy16(dst + share_off(i) + L::kSlabBytes, vs + i * STEP * v_tok, tok < seen_by_all ? 16 : 0);
+      for (int i = 0; i < ST - 1; ++i) issue(first + NW * i, page_at(first + NW * i), i);
+      int next_page = page_at(first + NW * (ST - 1));
+
+      // ---- the queries, as B fragments: b0 / b1 of step j are dims chunk * 16 + 4 i + {0, 1} / {2, 3}
+      // of row g, where lane t reads K's chunks 2 t and 2 t + 1 (D = 128) or t (D = 64)
+      {
+        constexpr int PARTS = NT / ROWS, E = D / PARTS;
+        const int r = tid / PARTS, part = tid % PARTS, rr = it.tile * ROWS + r;
+        float v[E];
+        uint32_t top = 0;
+        if (r < rows) {
+          const int hq = it.h * group + rr / a.q_len, qi = rr % a.q_len;
+          const int64_t base = it.b * a.qb + hq * a.qh + qi * a.qt + part * E;
+#pragma unroll
+          for (int e = 0; e < E; ++e) v[e] = load_elem<T>(a.q, base + e);
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e) v[e] = 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+#pragma unroll
+        for (int o = PARTS / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        // 2^(14 - e): the largest value lands in [2^14, 2^15); rows of zeros, infinities or NaN as they are
+        const int e = static_cast<int>(top >> 23) - 127;
+        const bool plain = top == 0 || top >= 0x7F800000u;
+        const float up = plain ? 1.0f : __uint_as_float((127u + 14u - max(e, -100)) << 23);
+        if (part == 0) q_unit[r] = 1.0f / up;
+#pragma unroll
+        for (int e2 = 0; e2 < E; e2 += 2) {
+          const int d = part * E + e2, c = d >> 4, i = (d & 15) >> 2, pair = (d >> 1) & 1;
+          const int tt = D == 128 ? c >> 1 : c, j = (D == 128 ? (c & 1) * 4 : 0) + i;
+          const float x0 = v[e2] * up, x1 = v[e2 + 1] * up;
+          uint32_t* slot = reinterpret_cast<uint32_t*>(&q_frag[((r >> 3) * STEPS + j) * 32 + (r & 7) * 4 + tt]) + pair;
+          const uint32_t hi2 = f16x2_of(x0, x1);
+          *slot = hi2;
+          if constexpr (SPLIT) {
+            const float2 h = f16x2_values(hi2);
+            slot[NR * STEPS * 32 * 2] = plain ? 0u : f16x2_of(x0 - h.x, x1 - h.y);
           }
         }
-        if (lane < 2) copy4(my_sc_s + (stage * 2 + lane) * 4, sc_base + static_cast<int64_t>(page) * sc_page);
-        valid |= 1u << stage;
-      } else {
-        valid &= ~(1u << stage);
+        __syncthreads();
       }
-      copies_commit();
-    };
-
-    __syncthreads();  // the previous item's readers of the ring, q_frag and q_unit are done
-    const int first = s0 + warp;
+      uint2 q_held[Q_HELD ? STEPS : 1];
+      if constexpr (Q_HELD) {
 #pragma unroll
-    for (int i = 0; i < ST - 1; ++i) issue(first + NW * i, page_at(first + NW * i), i);
-    int next_page = page_at(first + NW * (ST - 1));
-
-    // ---- the queries, as fragments
-    {
-      constexpr int PARTS = NT / 16, E = D / PARTS;
-      const int r = tid / PARTS, part = tid % PARTS, rr = it.tile * 16 + r;
-      float v[E];
-      uint32_t top = 0;
-      if (r < rows) {
-        const int hq = it.h * group + rr / a.q_len, qi = rr % a.q_len;
-        const int64_t base = it.b * a.qb + hq * a.qh + qi * a.qt + part * E;
-#pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = load_elem<T>(a.q, base + e);
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = 0.0f;
+        for (int j = 0; j < STEPS; ++j) q_held[j] = q_frag[j * 32 + lane];
       }
+      // rows 2 t and 2 t + 1 of group r: units, reference, sum; O^T fragments of 16 dims x 8 rows
+      float unit[NR][2], m[NR][2], l[NR][2], o[NR][MT][4];
 #pragma unroll
-      for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+      for (int r = 0; r < NR; ++r) {
 #pragma unroll
-      for (int o = PARTS / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      // 2^(14 - e): the largest value lands in [2^14, 2^15); rows of zeros, infinities or NaN as they are
-      const int e = static_cast<int>(top >> 23) - 127;
-      const bool plain = top == 0 || top >= 0x7F800000u;
-      const float up = plain ? 1.0f : e >= 0 ? __uint_as_float((127u + 14u - min(e, 127)) << 23)
-                                             : __uint_as_float((127u + min(14 - max(e, -100), 127)) << 23);
-      if (part == 0) q_unit[r] = 1.0f / up;
-      // dims of (step j, lane t): chunk * 16 + 4 i + {0, 1} in a0 / a1, {2, 3} in a2 / a3
+        for (int e = 0; e < 2; ++e) {
+          unit[r][e] = q_unit[r * 8 + 2 * t + e] * a.scale_log2;
+          m[r][e] = kNoScore;
+          l[r][e] = 0.0f;
+        }
 #pragma unroll
-      for (int e2 = 0; e2 < E; e2 += 2) {
-        const int d = part * E + e2, c = d >> 4, i = (d & 15) >> 2, pair = (d >> 1) & 1;
-        const int tt = D == 128 ? c >> 1 : c, j = (D == 128 ? (c & 1) * 4 : 0) + i;
-        const float x0 = v[e2] * up, x1 = v[e2 + 1] * up;
-        uint32_t* slot = reinterpret_cast<uint32_t*>(&q_frag[j * 32 + (r & 7) * 4 + tt]) + 2 * pair + (r >> 3);
-        const uint32_t hi2 = f16x2_of(x0, x1);
-        *slot = hi2;
-        if constexpr (SPLIT) {
-          const float2 h = f16x2_values(hi2);
-          slot[D / 16 * 32 * 4] = plain ? 0u : f16x2_of(x0 - h.x, x1 - h.y);
+        for (int j = 0; j < MT; ++j) o[r][j][0] = o[r][j][1] = o[r][j][2] = o[r][j][3] = 0.0f;
+      }
+
+      int stage = 0;
+      for (int slab = first; slab < s1; slab += NW) {
+        copies_wait<ST - 2>();
+        __syncwarp();
+        const int ahead = slab + NW * (ST - 1);
+        issue(ahead, next_page, stage == 0 ? ST - 1 : stage - 1);
+        next_page = page_at(ahead + NW);
+        if ((valid >> stage) & 1u) {
+          const uint8_t* kb = my_ring + stage * L::kStageBytes;
+          const uint8_t* vb = kb + L::kSlabBytes;
+          const float ksc = my_sc[stage * 2], vsc = my_sc[stage * 2 + 1];
+          // ---- S^T: tokens g and g + 8, rows 2 t and 2 t + 1. Two accumulators per group halve the
+          // chain of dependent products.
+          float s[NR][4], s2[NR][4];
+#pragma unroll
+          for (int r = 0; r < NR; ++r) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[r][e] = s2[r][e] = 0.0f;
+          }
+#pragma unroll
+          for (int h = 0; h < D / 64; ++h) {
+            const int ch = D == 128 ? 2 * t + h : t;
+            const uint4 k0 = *reinterpret_cast<const uint4*>(kb + slab_offset<D>(g, ch));
+            const uint4 k1 = *reinterpret_cast<const uint4*>(kb + slab_offset<D>(g + 8, ch));
+            const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int j = h * 4 + i;
+              const uint32_t ka[4] = {e4m3x2_f16(w0[i]), e4m3x2_f16(w1[i]), e4m3x2_f16_high(w0[i]),
+                                      e4m3x2_f16_high(w1[i])};
+#pragma unroll
+              for (int r = 0; r < NR; ++r) {
+                const uint2 q = Q_HELD ? q_held[Q_HELD ? j : 0] : q_frag[(r * STEPS + j) * 32 + lane];
+                mma_f16(i & 1 ? s2[r] : s[r], ka, q.x, q.y);
+                if constexpr (SPLIT) {
+                  const uint2 ql = q_frag[((NR + r) * STEPS + j) * 32 + lane];
+                  mma_f16(i & 1 ? s2[r] : s[r], ka, ql.x, ql.y);
+                }
+              }
+            }
+          }
+          const float size = fabsf(vsc), lv = size > 0.0f ? fmaxf(__log2f(size), kLeastLogScale) : kLeastLogScale;
+          const int tok = slab * 16 + g;
+          uint32_t pb[NR][2], pl[NR][2];
+#pragma unroll
+          for (int r = 0; r < NR; ++r) {
+            const float c0 = unit[r][0] * ksc, c1 = unit[r][1] * ksc;
+            s[r][0] = (s[r][0] + s2[r][0]) * c0;
+            s[r][1] = (s[r][1] + s2[r][1]) * c1;
+            s[r][2] = (s[r][2] + s2[r][2]) * c0;
+            s[r][3] = (s[r][3] + s2[r][3]) * c1;
+            if (slab * 16 + 16 > seen_by_all) {
+              const int seen0 = seen_of(r * 8 + 2 * t), seen1 = seen_of(r * 8 + 2 * t + 1);
+              if (tok >= seen0) s[r][0] = -INFINITY;
+              if (tok >= seen1) s[r][1] = -INFINITY;
+              if (tok + 8 >= seen0) s[r][2] = -INFINITY;
+              if (tok + 8 >= seen1) s[r][3] = -INFINITY;
+            }
+            if (a.scores != nullptr) {
+              float* at = a.scores +
+                          ((static_cast<int64_t>(it.b) * p.heads + it.h) * a.rows + it.tile * ROWS + r * 8 + 2 * t) * a.capacity + tok;
+              if (r * 8 + 2 * t < rows) at[0] = s[r][0], at[8] = s[r][2];
+              if (r * 8 + 2 * t + 1 < rows) at[a.capacity] = s[r][1], at[a.capacity + 8] = s[r][3];
+            }
+            float t0 = fmaxf(s[r][0], s[r][2]), t1 = fmaxf(s[r][1], s[r][3]);
+#pragma unroll
+            for (int x = 4; x <= 16; x <<= 1) {
+              t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, x));
+              t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, x));
+            }
+            t0 += lv - kWeightBits;
+            t1 += lv - kWeightBits;
+            if (__any_sync(0xffffffffu, t0 > m[r][0] + kWeightRoom || t1 > m[r][1] + kWeightRoom)) {
+              const float n0 = t0 > m[r][0] + kWeightRoom ? t0 : m[r][0];
+              const float n1 = t1 > m[r][1] + kWeightRoom ? t1 : m[r][1];
+              const float f0 = exp2_approx(m[r][0] - n0), f1 = exp2_approx(m[r][1] - n1);
+              m[r][0] = n0;
+              m[r][1] = n1;
+              l[r][0] *= f0;
+              l[r][1] *= f1;
+#pragma unroll
+              for (int j = 0; j < MT; ++j) {
+                o[r][j][0] *= f0;
+                o[r][j][1] *= f1;
+                o[r][j][2] *= f0;
+                o[r][j][3] *= f1;
+              }
+            }
+            s[r][0] = exp2_approx(s[r][0] - m[r][0]);
+            s[r][1] = exp2_approx(s[r][1] - m[r][1]);
+            s[r][2] = exp2_approx(s[r][2] - m[r][0]);
+            s[r][3] = exp2_approx(s[r][3] - m[r][1]);
+            l[r][0] += s[r][0] + s[r][2];
+            l[r][1] += s[r][1] + s[r][3];
+            scale_pair(s[r][0], s[r][1], vsc);
+            scale_pair(s[r][2], s[r][3], vsc);
+            // the weights of 8 tokens x 8 rows, transposed into the B fragment of O^T = V^T P^T
+            const uint32_t w0 = f16x2_of(s[r][0], s[r][1]), w1 = f16x2_of(s[r][2], s[r][3]);
+            pb[r][0] = transpose8(w0);
+            pb[r][1] = transpose8(w1);
+            if constexpr (SPLIT) {
+              const float2 h0 = f16x2_values(w0), h1 = f16x2_values(w1);
+              pl[r][0] = transpose8(f16x2_of(s[r][0] - h0.x, s[r][1] - h0.y));
+              pl[r][1] = transpose8(f16x2_of(s[r][2] - h1.x, s[r][3] - h1.y));
+            }
+          }
+          // ---- O^T: row g of MMA tile j is dim g * D / 8 + 2 j, row g + 8 the next one, so a lane's
+          // bytes of a token are consecutive; tokens 2 t, 2 t + 1 and 2 t + 8, 2 t + 9
+          constexpr int W = D / 32;  // 4-byte words per lane and token
+          uint32_t r0[W], r1[W], r2[W], r3[W];
+          auto take = [&](int row, uint32_t(&r)[W]) {
+            if constexpr (D == 128) {
+              const uint4 x = *reinterpret_cast<const uint4*>(vb + slab_offset<D>(row, g));
+              r[0] = x.x, r[1] = x.y, r[2] = x.z, r[3] = x.w;
+            } else {
+              const uint2 x = *reinterpret_cast<const uint2*>(vb + slab_offset<D>(row, g >> 1) + (g & 1) * 8);
+              r[0] = x.x, r[1] = x.y;
+            }
+          };
+          take(2 * t, r0);
+          take(2 * t + 1, r1);
+          take(2 * t + 8, r2);
+          take(2 * t + 9, r3);
+#pragma unroll
+          for (int w = 0; w < W; ++w) {
+            const uint32_t x0 = __byte_perm(r0[w], r1[w], 0x5140), x1 = __byte_perm(r0[w], r1[w], 0x7362);
+            const uint32_t y0 = __byte_perm(r2[w], r3[w], 0x5140), y1 = __byte_perm(r2[w], r3[w], 0x7362);
+            const uint32_t va[4] = {e4m3x2_f16(x0), e4m3x2_f16_high(x0), e4m3x2_f16(y0), e4m3x2_f16_high(y0)};
+            const uint32_t vc[4] = {e4m3x2_f16(x1), e4m3x2_f16_high(x1), e4m3x2_f16(y1), e4m3x2_f16_high(y1)};
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+              mma_f16(o[r][2 * w], va, pb[r][0], pb[r][1]);
+              mma_f16(o[r][2 * w + 1], vc, pb[r][0], pb[r][1]);
+              if constexpr (SPLIT) {
+                mma_f16(o[r][2 * w], va, pl[r][0], pl[r][1]);
+                mma_f16(o[r][2 * w + 1], vc, pl[r][0], pl[r][1]);
+              }
+            }
+          }
+          // the tokens that only some rows see (fewer than q_len of them)
+          for (int x = max(seen_by_all, slab * 16); x < min(n, slab * 16 + 16); ++x) {
+            const int k = x - slab * 16, from = ((k & 7) << 2) | t;
+            const int page = __ldg(table + (x >> p.page_shift));
+            const uint8_t* v = vbase + page * p.sp[1] + (x & (P - 1)) * p.st[1] + g * (D / 8);
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+              const float w0 = __shfl_sync(0xffffffffu, k < 8 ? s[r][0] : s[r][2], from);
+              const float w1 = __shfl_sync(0xffffffffu, k < 8 ? s[r][1] : s[r][3], from);
+              const bool sees0 = x < seen_of(r * 8 + 2 * t), sees1 = x < seen_of(r * 8 + 2 * t + 1);
+#pragma unroll
+              for (int j = 0; j < MT; ++j) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const float value = e4m3_value_hw(__ldg(v + 2 * j + e));
+                  if (sees0) o[r][j][2 * e] = fmaf(w0, value, o[r][j][2 * e]);
+                  if (sees1) o[r][j][2 * e + 1] = fmaf(w1, value, o[r][j][2 * e + 1]);
+                }
+              }
+            }
+          }
+        }
+        stage = stage == ST - 1 ? 0 : stage + 1;
+      }
+      copies_wait<0>();
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+#pragma unroll
+        for (int x = 4; x <= 16; x <<= 1) {
+          l[r][0] += __shfl_xor_sync(0xffffffffu, l[r][0], x);
+          l[r][1] += __shfl_xor_sync(0xffffffffu, l[r][1], x);
+        }
+      }
+
+      // ---- the warps' parts of this block's share of the item
+      __syncthreads();  // the ring is free
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = r * 8 + 2 * t + e;
+          if (row < rows) {
+            float* at = merge_o + (warp * ROWS + row) * PITCH + g * (D / 8);
+#pragma unroll
+            for (int j = 0; j < MT; j += 2)
+              *reinterpret_cast<float4*>(at + 2 * j) =
+                  make_float4(o[r][j][e], o[r][j][2 + e], o[r][j + 1][e], o[r][j + 1][2 + e]);
+            if (g == 0) {
+              merge_ml[(warp * ROWS + row) * 2] = m[r][e];
+              merge_ml[(warp * ROWS + row) * 2 + 1] = l[r][e];
+            }
+          }
         }
       }
       __syncthreads();
-    }
-    const float unit0 = q_unit[g] * a.scale_log2, unit1 = q_unit[g + 8] * a.scale_log2;
-    float o[TILES][4], m0 = kNoScore, m1 = kNoScore, l0 = 0.0f, l1 = 0.0f;
+      const bool whole = s0 == 0 && s1 == it.slabs;
+      float* my_part = a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (it.first <= lo ? 0 : 1)) * ROWS * (D + 2);
+      for (int i = tid; i < rows * (D / 4); i += NT) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        float ref = kNoScore, sum = 0.0f;
 #pragma unroll
-    for (int j = 0; j < TILES; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-
-    int stage = 0;
-    for (int slab = first; slab < s1; slab += NW) {
-      copies_wait<ST - 2>();
-      __syncwarp();
-      const int ahead = slab + NW * (ST - 1);
-      issue(ahead, next_page, stage == 0 ? ST - 1 : stage - 1);
-      next_page = page_at(ahead + NW);
-      if ((valid >> stage) & 1u) {
-        const uint8_t* kb = my_ring + stage * L::kStageBytes;
-        const uint8_t* vb = kb + L::kSlabBytes;
-        const float ksc = my_sc[stage * 2], vsc = my_sc[stage * 2 + 1];
-        float s[2][4] = {};
+        for (int w = 0; w < NW; ++w) ref = fmaxf(ref, merge_ml[(w * ROWS + r) * 2]);
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int h = 0; h < D / 64; ++h) {
-          const int ch = D == 128 ? 2 * t + h : t;
-          const uint4 k0 = *reinterpret_cast<const uint4*>(kb + slab_offset<D>(g, ch));
-          const uint4 k1 = *reinterpret_cast<const uint4*>(kb + slab_offset<D>(g + 8, ch));
-          const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint4 af = q_frag[(h * 4 + i) * 32 + lane];
-            const uint32_t aq[4] = {af.x, af.y, af.z, af.w};
-            const uint32_t b00 = e4m3x2_f16(w0[i]), b01 = e4m3x2_f16_high(w0[i]);
-            const uint32_t b10 = e4m3x2_f16(w1[i]), b11 = e4m3x2_f16_high(w1[i]);
-            mma_f16(s[0], aq, b00, b01);
-            mma_f16(s[1], aq, b10, b11);
-            if constexpr (SPLIT) {
-              const uint4 lf = q_frag[D / 16 * 32 + (h * 4 + i) * 32 + lane];
-              const uint32_t al[4] = {lf.x, lf.y, lf.z, lf.w};
-              mma_f16(s[0], al, b00, b01);
-              mma_f16(s[1], al, b10, b11);
-            }
-          }
+        for (int w = 0; w < NW; ++w) {
+          const float f = exp2_approx(merge_ml[(w * ROWS + r) * 2] - ref);
+          sum = fmaf(f, merge_ml[(w * ROWS + r) * 2 + 1], sum);
+          const float4 x = *reinterpret_cast<const float4*>(merge_o + (w * ROWS + r) * PITCH + d);
+          acc.x = fmaf(f, x.x, acc.x);
+          acc.y = fmaf(f, x.y, acc.y);
+          acc.z = fmaf(f, x.z, acc.z);
+          acc.w = fmaf(f, x.w, acc.w);
         }
-        const int tok = slab * 16 + 2 * t;
-        const float c0 = unit0 * ksc, c1 = unit1 * ksc;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          scale_pair(s[i][0], s[i][1], c0);
-          scale_pair(s[i][2], s[i][3], c1);
-        }
-        if (slab * 16 + 16 > seen_by_all) {
-          const int seen0 = seen_of(0), seen1 = seen_of(1);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              if (tok + 8 * i + e >= seen0) s[i][e] = -INFINITY;
-              if (tok + 8 * i + e >= seen1) s[i][2 + e] = -INFINITY;
-            }
-          }
-        }
-        if (a.scores != nullptr) {
-          const int64_t base = ((static_cast<int64_t>(it.b) * p.heads + it.h) * a.rows + it.tile * 16) * a.capacity + tok;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (g < rows) *reinterpret_cast<float2*>(a.scores + base + g * a.capacity + 8 * i) = make_float2(s[i][0], s[i][1]);
-            if (g + 8 < rows)
-              *reinterpret_cast<float2*>(a.scores + base + (g + 8) * a.capacity + 8 * i) = make_float2(s[i][2], s[i][3]);
-          }
-        }
-        const float size = fabsf(vsc), lv = size > 0.0f ? fmaxf(__log2f(size), kLeastLogScale) : kLeastLogScale;
-        float t0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-        float t1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
-        t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 1));
-        t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 1));
-        t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 2)) + (lv - kWeightBits);
-        t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 2)) + (lv - kWeightBits);
-        if (__any_sync(0xffffffffu, t0 > m0 + kWeightRoom || t1 > m1 + kWeightRoom)) {
-          const float n0 = t0 > m0 + kWeightRoom ? t0 : m0, n1 = t1 > m1 + kWeightRoom ? t1 : m1;
-          const float f0 = exp2_approx(m0 - n0), f1 = exp2_approx(m1 - n1);
-          m0 = n0;
-          m1 = n1;
-          l0 *= f0;
-          l1 *= f1;
-#pragma unroll
-          for (int j = 0; j < TILES; ++j) {
-            scale_pair(o[j][0], o[j][1], f0);
-            scale_pair(o[j][2], o[j][3], f1);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          add_pair(s[i][0], s[i][1], -m0);
-          add_pair(s[i][2], s[i][3], -m1);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[i][e] = exp2_approx(s[i][e]);
-        }
-        l0 += (s[0][0] + s[0][1]) + (s[1][0] + s[1][1]);
-        l1 += (s[0][2] + s[0][3]) + (s[1][2] + s[1][3]);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          scale_pair(s[i][0], s[i][1], vsc);
-          scale_pair(s[i][2], s[i][3], vsc);
-        }
-        const uint32_t pa[4] = {f16x2_of(s[0][0], s[0][1]), f16x2_of(s[0][2], s[0][3]), f16x2_of(s[1][0], s[1][1]),
-                                f16x2_of(s[1][2], s[1][3])};
-        uint32_t pl[4];
-        if constexpr (SPLIT) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 h = f16x2_values(pa[i]);
-            const float x0 = s[i >> 1][(i & 1) * 2], x1 = s[i >> 1][(i & 1) * 2 + 1];
-            pl[i] = f16x2_of(x0 - h.x, x1 - h.y);
-          }
-        }
-        // V codes of tokens 2t, 2t + 1 (b0) and 2t + 8, 2t + 9 (b1); column g of tile j is dim
-        // g * D / 8 + j, so a lane's bytes of a token are consecutive
-        constexpr int W = D / 32;  // 4-byte words per lane and token
-        uint32_t r0[W], r1[W], r2[W], r3[W];
-        auto take = [&](int row, uint32_t(&r)[W]) {
-          if constexpr (D == 128) {
-            const uint4 x = *reinterpret_cast<const uint4*>(vb + slab_offset<D>(row, g));
-            r[0] = x.x, r[1] = x.y, r[2] = x.z, r[3] = x.w;
-          } else {
-            const uint2 x = *reinterpret_cast<const uint2*>(vb + slab_offset<D>(row, g >> 1) + (g & 1) * 8);
-            r[0] = x.x, r[1] = x.y;
-          }
-        };
-        take(2 * t, r0);
-        take(2 * t + 1, r1);
-        take(2 * t + 8, r2);
-        take(2 * t + 9, r3);
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-          const uint32_t x0 = __byte_perm(r0[w], r1[w], 0x5140), x1 = __byte_perm(r0[w], r1[w], 0x7362);
-          const uint32_t y0 = __byte_perm(r2[w], r3[w], 0x5140), y1 = __byte_perm(r2[w], r3[w], 0x7362);
-          const uint32_t bx[4] = {e4m3x2_f16(x0), e4m3x2_f16_high(x0), e4m3x2_f16(x1), e4m3x2_f16_high(x1)};
-          const uint32_t by[4] = {e4m3x2_f16(y0), e4m3x2_f16_high(y0), e4m3x2_f16(y1), e4m3x2_f16_high(y1)};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            mma_f16(o[4 * w + i], pa, bx[i], by[i]);
-            if constexpr (SPLIT) mma_f16(o[4 * w + i], pl, bx[i], by[i]);
-          }
-        }
-        // the tokens that only some rows see (fewer than q_len of them)
-        for (int x = max(seen_by_all, slab * 16); x < min(n, slab * 16 + 16); ++x) {
-          const int k = x - slab * 16, from = (g << 2) | ((k & 7) >> 1);
-          const float e0 = k & 1 ? (k < 8 ? s[0][1] : s[1][1]) : (k < 8 ? s[0][0] : s[1][0]);
-          const float e1 = k & 1 ? (k < 8 ? s[0][3] : s[1][3]) : (k < 8 ? s[0][2] : s[1][2]);
-          const float w0 = __shfl_sync(0xffffffffu, e0, from), w1 = __shfl_sync(0xffffffffu, e1, from);
-          const int page = __ldg(table + (x >> p.page_shift));
-          const uint8_t* v = vbase + page * p.sp[1] + (x & (P - 1)) * p.st[1];
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {  // columns 2t and 2t + 1 of every tile
-#pragma unroll
-            for (int j = 0; j < TILES; ++j) {
-              const float value = e4m3_value_hw(__ldg(v + (2 * t + c) * (D / 8) + j));
-              if (x < seen_of(0)) o[j][c] = fmaf(w0, value, o[j][c]);
-              if (x < seen_of(1)) o[j][2 + c] = fmaf(w1, value, o[j][2 + c]);
-            }
-          }
+        if (whole) {
+          pages_finish<T, D>(a, it.b, it.h, it.tile * ROWS + r, d, n, acc, ref, sum);
+        } else {
+          __stcg(reinterpret_cast<float4*>(my_part + r * D + d), acc);
+          if (d == 0) __stcg(reinterpret_cast<float2*>(my_part + ROWS * D + 2 * r), make_float2(ref, sum));
         }
       }
-      stage = stage == ST - 1 ? 0 : stage + 1;
-    }
-    copies_wait<0>();
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-
-    // ---- the warps' parts of this block's share of the item
-    __syncthreads();  // the ring is free
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      if (g + 8 * half >= rows) break;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-#pragma unroll
-        for (int j = 0; j < TILES; j += 4) {
-          const int d = (2 * t + c) * (D / 8) + j, e = 2 * half + c;
-          *reinterpret_cast<float4*>(&merge_o[(warp * 16 + g + 8 * half) * PITCH + d + d / 32 * 4]) =
-              make_float4(o[j][e], o[j + 1][e], o[j + 2][e], o[j + 3][e]);
-        }
+      if (s0 == 0 && !whole) {
+        // the merge goes from this block to the one that holds the item's last unit
+        cut = PagesCut{it.b, it.h, it.tile, static_cast<int>(block_of(end - 1)), it.first <= lo ? 0 : 1};
       }
-    }
-    if (t == 0) {
-      merge_ml[(warp * 16 + g) * 2] = m0;
-      merge_ml[(warp * 16 + g) * 2 + 1] = l0;
-      merge_ml[(warp * 16 + g + 8) * 2] = m1;
-      merge_ml[(warp * 16 + g + 8) * 2 + 1] = l1;
-    }
-    __syncthreads();
-    const bool whole = s0 == 0 && s1 == it.slabs;
-    float* my_part = a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (it.first <= lo ? 0 : 1)) * 16 * (D + 2);
-    for (int i = tid; i < rows * (D / 4); i += NT) {
-      const int r = i / (D / 4), d = i % (D / 4) * 4;
-      float ref = kNoScore, sum = 0.0f;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) ref = fmaxf(ref, merge_ml[(w * 16 + r) * 2]);
-      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        const float f = exp2_approx(merge_ml[(w * 16 + r) * 2] - ref);
-        sum = fmaf(f, merge_ml[(w * 16 + r) * 2 + 1], sum);
-        const float4 x = *reinterpret_cast<const float4*>(&merge_o[(w * 16 + r) * PITCH + d + d / 32 * 4]);
-        acc.x = fmaf(f, x.x, acc.x);
-        acc.y = fmaf(f, x.y, acc.y);
-        acc.z = fmaf(f, x.z, acc.z);
-        acc.w = fmaf(f, x.w, acc.w);
-      }
-      if (whole) {
-        pages_finish<T, D>(a, it.b, it.h, it.tile * 16 + r, d, n, acc, ref, sum);
-      } else {
-        __stcg(reinterpret_cast<float4*>(my_part + r * D + d), acc);
-        if (d == 0) __stcg(reinterpret_cast<float2*>(my_part + 16 * D + 2 * r), make_float2(ref, sum));
-      }
-    }
-    if (s0 == 0 && !whole) {
-      // the merge goes from this block to the one that holds the item's last unit
-      cut = PagesCut{it.b, it.h, it.tile, static_cast<int>(block_of(end - 1)), it.first <= lo ? 0 : 1};
-    }
     }
     // ---- the next item
     it.first = end;
@@ -616,7 +639,7 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
 
 // The items that several blocks share: four warps per row add the blocks' outputs, each with its
 // weight, in an order that depends on nothing but their number. A block per cut and four rows.
-template <int T, int D>
+template <int T, int D, int ROWS>
 __global__ void __launch_bounds__(512) pages_merge_kernel(PagesAttnArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const PagesCut cut = a.cuts[blockIdx.x];
@@ -624,20 +647,20 @@ __global__ void __launch_bounds__(512) pages_merge_kernel(PagesAttnArgs a) {
   constexpr int LANES = D / 4, SIDES = 32 / LANES, SHARES = 4 * SIDES;  // lanes per part, parts side by side
   __shared__ float4 sums[4][SHARES][LANES];
   const int lane = threadIdx.x & 31, group = threadIdx.x >> 7, share = (threadIdx.x >> 5 & 3) * SIDES + lane / LANES;
-  const int row = blockIdx.y * 4 + group, r = cut.tile * 16 + row, parts = cut.last - static_cast<int>(blockIdx.x) + 1;
-  const bool live = row < 16 && r < a.rows;
+  const int row = blockIdx.y * 4 + group, r = cut.tile * ROWS + row, parts = cut.last - static_cast<int>(blockIdx.x) + 1;
+  const bool live = row < ROWS && r < a.rows;
   auto part_of = [&](int i) -> const float* {
     const int64_t slot = i == 0 ? 2 * static_cast<int64_t>(blockIdx.x) + cut.slot : 2 * (static_cast<int64_t>(blockIdx.x) + i);
-    return a.partial + slot * 16 * (D + 2);
+    return a.partial + slot * ROWS * (D + 2);
   };
   float ref = kNoScore, sum = 0.0f;
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   if (live) {
-    for (int i = lane; i < parts; i += 32) ref = fmaxf(ref, __ldg(part_of(i) + 16 * D + 2 * row));
+    for (int i = lane; i < parts; i += 32) ref = fmaxf(ref, __ldg(part_of(i) + ROWS * D + 2 * row));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, o));
     for (int i = lane; i < parts; i += 32) {
-      const float2 ml = __ldg(reinterpret_cast<const float2*>(part_of(i) + 16 * D + 2 * row));
+      const float2 ml = __ldg(reinterpret_cast<const float2*>(part_of(i) + ROWS * D + 2 * row));
       sum = fmaf(exp2_approx(ml.x - ref), ml.y, sum);
     }
 #pragma unroll
@@ -646,7 +669,7 @@ __global__ void __launch_bounds__(512) pages_merge_kernel(PagesAttnArgs a) {
 #pragma unroll 8
     for (int i = share; i < parts; i += SHARES) {
       const float* part = part_of(i);
-      const float f = exp2_approx(__ldg(part + 16 * D + 2 * row) - ref);
+      const float f = exp2_approx(__ldg(part + ROWS * D + 2 * row) - ref);
       const float4 x = __ldg(reinterpret_cast<const float4*>(part + row * D + d));
       acc.x = fmaf(f, x.x, acc.x);
       acc.y = fmaf(f, x.y, acc.y);

@@ -2,6 +2,7 @@
 // append, the attention over the pages and the eviction, and this translation unit's device
 // status word.
 #include <algorithm>
+#include <type_traits>
 
 #include "kab_host.h"
 
@@ -94,6 +95,9 @@ void launch_append(const AppendArgs& a, dim3 grid, int ch, unsigned* status, cud
   else append_pages_kernel<T, 8><<<grid, 256, 0, s>>>(a, status);
 }
 
+// Query rows that share one pass over the cache: one group of 8 where that is all, else two.
+int tile_rows(int rows) { return rows <= 8 ? 8 : 16; }
+
 int attention_check(const KabKvPagesAttention* p, PagesAttnArgs* g) {
   KAB_REQUIRE(p != nullptr, "null parameters");
   if (int e = pool_check(&p->cache, &g->pool)) return e;
@@ -113,7 +117,8 @@ int attention_check(const KabKvPagesAttention* p, PagesAttnArgs* g) {
   g->q_len = static_cast<int>(p->q_len);
   g->causal = p->causal != 0;
   g->rows = static_cast<int>(p->heads_q / p->cache.heads_kv * p->q_len);
-  g->row_tiles = (g->rows + 15) / 16;
+  const int tile = tile_rows(g->rows);
+  g->row_tiles = (g->rows + tile - 1) / tile;
   g->capacity = p->cache.max_pages * p->cache.page_tokens;
   return KAB_OK;
 }
@@ -129,14 +134,14 @@ size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
 // Opts the kernel instance into its shared memory and returns the blocks of it that fit on the
 // GPU at once (asked once per device), or -1.
-template <int T, int D>
+template <int T, int D, int NR>
 int attention_blocks() {
-  using L = PagesLayout<D, T == kF32>;
+  using L = PagesLayout<D, NR, T == kF32>;
   static int blocks[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
   if (blocks[dev] == 0) {
-    auto kern = pages_attention_kernel<T, D>;
+    auto kern = pages_attention_kernel<T, D, NR>;
     int n = 0;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem) != cudaSuccess ||
         cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, L::kThreads, L::kSmem) != cudaSuccess || n < 1)
@@ -145,20 +150,31 @@ int attention_blocks() {
   }
   return blocks[dev];
 }
-int attention_blocks(int dtype, int64_t d) {
-  if (dtype == KAB_BF16) return d == 128 ? attention_blocks<kBF16, 128>() : attention_blocks<kBF16, 64>();
-  if (dtype == KAB_F16) return d == 128 ? attention_blocks<kF16, 128>() : attention_blocks<kF16, 64>();
-  return d == 128 ? attention_blocks<kF32, 128>() : attention_blocks<kF32, 64>();
+// Runs `f` with the kernel instance's types: f(type, head_dim, groups of rows).
+template <int T, int D, typename F>
+auto with_groups(int rows, F&& f) {
+  return tile_rows(rows) == 8 ? f(std::integral_constant<int, T>(), std::integral_constant<int, D>(),
+                                  std::integral_constant<int, 1>())
+                              : f(std::integral_constant<int, T>(), std::integral_constant<int, D>(),
+                                  std::integral_constant<int, 2>());
+}
+template <typename F>
+auto with_instance(int dtype, int64_t d, int rows, F&& f) {
+  if (dtype == KAB_BF16) return d == 128 ? with_groups<kBF16, 128>(rows, f) : with_groups<kBF16, 64>(rows, f);
+  if (dtype == KAB_F16) return d == 128 ? with_groups<kF16, 128>(rows, f) : with_groups<kF16, 64>(rows, f);
+  return d == 128 ? with_groups<kF32, 128>(rows, f) : with_groups<kF32, 64>(rows, f);
 }
 
 int attention_plan(const KabKvPagesAttention* p, const PagesAttnArgs& g, AttentionPlan* plan) {
-  plan->grid = attention_blocks(p->q_dtype, p->cache.head_dim);
+  plan->grid = with_instance(p->q_dtype, p->cache.head_dim, g.rows, [](auto T, auto D, auto NR) {
+    return attention_blocks<decltype(T)::value, decltype(D)::value, decltype(NR)::value>();
+  });
   if (plan->grid < 0) return fail(KAB_ECUDA, "cannot configure the paged attention kernel");
   const size_t items = static_cast<size_t>(p->cache.batch * p->cache.heads_kv);
   KAB_REQUIRE(items * g.row_tiles * (static_cast<size_t>(g.capacity) / 16 + 1 + kItemCost) < (size_t(1) << 31),
               "sequences x KV heads x row tiles x tokens of the page table is too large");
   plan->cuts = round256(static_cast<size_t>(plan->grid) * sizeof(PagesCut));
-  plan->partial = round256(static_cast<size_t>(plan->grid) * 2 * 16 * (p->cache.head_dim + 2) * 4);
+  plan->partial = round256(static_cast<size_t>(plan->grid) * 2 * tile_rows(g.rows) * (p->cache.head_dim + 2) * 4);
   if (p->use_mass) {
     plan->ml = round256(items * g.rows * 8);
     plan->scores = round256(items * g.rows * static_cast<size_t>(g.capacity) * 4);
@@ -181,13 +197,13 @@ cudaError_t launch_after(void (*kern)(Args...), dim3 grid, int threads, cudaStre
   return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
-template <int T, int D>
+template <int T, int D, int NR>
 int launch_attention(const PagesAttnArgs& g, int grid, unsigned* status, cudaStream_t s) {
-  using L = PagesLayout<D, T == kF32>;
-  pages_attention_kernel<T, D><<<grid, L::kThreads, L::kSmem, s>>>(g, status);
+  using L = PagesLayout<D, NR, T == kF32>;
+  pages_attention_kernel<T, D, NR><<<grid, L::kThreads, L::kSmem, s>>>(g, status);
   if (int e = check_launch("kab_kv_pages_attention")) return e;
-  const dim3 merges(static_cast<unsigned>(grid), static_cast<unsigned>((std::min(g.rows, 16) + 3) / 4));
-  launch_after(pages_merge_kernel<T, D>, merges, 512, s, g);
+  const dim3 merges(static_cast<unsigned>(grid), static_cast<unsigned>((std::min(g.rows, L::kRows) + 3) / 4));
+  launch_after(pages_merge_kernel<T, D, L::kRows>, merges, 512, s, g);
   if (int e = check_launch("kab_kv_pages_attention merge")) return e;
   if (g.scores == nullptr || g.capacity == 0) return KAB_OK;
   const dim3 blocks(static_cast<unsigned>((g.capacity + 255) / 256), g.pool.heads, g.pool.batch);
@@ -279,13 +295,9 @@ int kab_kv_pages_attention(const KabKvPagesAttention* params, void* workspace, s
     g.scores = reinterpret_cast<float*>(w + plan.cuts + plan.partial + plan.ml);
   }
   const cudaStream_t s = as_stream(stream);
-#define KAB_PAGES_D(TT)                                                              \
-  return params->cache.head_dim == 128 ? launch_attention<TT, 128>(g, plan.grid, status, s) \
-                                       : launch_attention<TT, 64>(g, plan.grid, status, s)
-  if (params->q_dtype == KAB_BF16) KAB_PAGES_D(kBF16);
-  if (params->q_dtype == KAB_F16) KAB_PAGES_D(kF16);
-  KAB_PAGES_D(kF32);
-#undef KAB_PAGES_D
+  return with_instance(params->q_dtype, params->cache.head_dim, g.rows, [&](auto T, auto D, auto NR) {
+    return launch_attention<decltype(T)::value, decltype(D)::value, decltype(NR)::value>(g, plan.grid, status, s);
+  });
 }
 
 int kab_kv_pages_evict(const KabKvPages* cache, const int32_t* out_table, int64_t out_stride, int64_t budget,
