@@ -7,7 +7,7 @@
 // head x query tokens) of a decode step. So the products run on mma.sync.m16n8k16 (f16 in, fp32
 // accumulators), 16 rows at a time: e4m3 -> f16 is one exact conversion per two codes, and the
 // instruction's fragments let the codes go from shared memory to the tensor core without leaving
-// the warp. What has to be fast is the stream: every warp keeps its own ring of 16-token slabs of
+// the warp. What has to be fast is the stream: every warp keeps its own ring of slabs of 32 (16 where a page has no more) tokens of
 // K and V in flight with cp.async and never waits for another warp inside a segment.
 //
 //  * Work is cut into equal parts whatever the lengths: the slabs of all (sequence, KV head, row
@@ -30,9 +30,10 @@
 
 namespace kab {
 
-// An item that several blocks share: which one, and the last of the blocks (-1: none begins here).
+// An item that several blocks share: which one, the first and the last of the blocks and the slot of
+// the first (the others' is 0); last -1: no such item.
 struct PagesCut {
-  int b, h, tile, last, slot;
+  int b, h, tile, first, last, slot;
 };
 
 struct PagesAttnArgs {
@@ -44,7 +45,8 @@ struct PagesAttnArgs {
   int heads_q, q_len, causal;
   int rows, row_tiles;   // rows of one KV head (query heads x query tokens), tiles of 16 of them
   float* partial;        // [grid, 2 slots, a tile's rows, D + 2]: output, maximum, sum
-  PagesCut* cuts;        // [grid]: the item that begins in a block and goes on in the next ones
+  PagesCut* cuts;        // [items or grid]: the shared items, by item or by the block that begins them
+  int cuts_by_item;
   float* scores;         // [batch, heads, rows, capacity] in log2 units, or NULL
   float* ml;             // [batch, heads, rows, 2]: reference and reciprocal sum, with scores
   int64_t capacity;      // max_pages * page_tokens
@@ -89,12 +91,12 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// (a, b) * c in one instruction.
-__device__ __forceinline__ void scale_pair(float& a, float& b, float c) {
-  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%0, %1};\n mov.b64 y, {%2, %2};\n mul.rn.f32x2 x, x, y;\n"
+// a *= c, b *= d in one instruction.
+__device__ __forceinline__ void scale_pair(float& a, float& b, float c, float d) {
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%0, %1};\n mov.b64 y, {%2, %3};\n mul.rn.f32x2 x, x, y;\n"
       " mov.b64 {%0, %1}, x;\n}"
       : "+f"(a), "+f"(b)
-      : "f"(c));
+      : "f"(c), "f"(d));
 }
 // An 8 x 8 matrix of f16 over the warp (lane (g, t) holds row g, columns 2 t and 2 t + 1), transposed.
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
@@ -117,14 +119,16 @@ __device__ __forceinline__ void copies_wait() {
 
 // ------------------------------------------------------------------ layout
 
-// NR: groups of 8 query rows that share one pass over the cache (the MMA's N).
-template <int D, int NR, bool SPLIT>
+// NR: groups of 8 query rows that share one pass over the cache (the MMA's N). SL: tokens of a slab.
+template <int D, int NR, int SL, bool SPLIT>
 struct PagesLayout {
   static constexpr int kWarps = 4, kThreads = kWarps * 32, kRows = 8 * NR;
-  static constexpr int kBlocks = NR == 1 && !SPLIT ? 5 : 4;  // per SM, by registers
-  static constexpr int kStages = NR == 1 && !SPLIT ? 2 : 3;
-  static constexpr int kSlabBytes = 16 * D;  // K or V of one slab
+  static constexpr bool kLight = NR == 1 && !SPLIT;
+  static constexpr int kSlabBytes = SL * D;  // K or V of one slab
   static constexpr int kStageBytes = 2 * kSlabBytes;
+  // blocks per SM by registers and shared memory, and as many stages as fit beside them
+  static constexpr int kBlocks = SL == 16 ? (kLight ? 5 : 4) : 3;
+  static constexpr int kStages = SL * D == 4096 || (SL == 16 && kLight) ? 2 : 3;
   static constexpr int kQBytes = D / 16 * 32 * 8 * NR * (SPLIT ? 2 : 1);
   // a row of the warps' outputs in the merge: its pitch keeps the fragments' float4 stores two to a bank
   static constexpr int kPitch = D + 4;
@@ -181,13 +185,15 @@ __device__ __forceinline__ void pages_finish(const PagesAttnArgs& a, int b, int 
   }
 }
 
-template <int T, int D, int NR>
-__global__ void __launch_bounds__(PagesLayout<D, NR, T == kF32>::kThreads, PagesLayout<D, NR, T == kF32>::kBlocks)
+template <int T, int D, int NR, int SL>
+__global__ void __launch_bounds__(PagesLayout<D, NR, SL, T == kF32>::kThreads, PagesLayout<D, NR, SL, T == kF32>::kBlocks)
 pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
   constexpr bool SPLIT = T == kF32, Q_HELD = NR == 1 && !SPLIT;
-  using L = PagesLayout<D, NR, SPLIT>;
+  using L = PagesLayout<D, NR, SL, SPLIT>;
+  constexpr int U = SL / 16, SHIFT = SL == 16 ? 4 : 5;  // 16-token parts of a slab
+  constexpr int COST = kItemCost * 16 / SL;
   constexpr int ST = L::kStages, NW = L::kWarps, NT = L::kThreads, ROWS = L::kRows, PITCH = L::kPitch;
-  constexpr int STEPS = D / 16, MT = D / 16, CHUNKS = D / 16, COPIES = D / 32;
+  constexpr int STEPS = D / 16, MT = D / 16, CHUNKS = D / 16, COPIES = SL * D / 512;
   extern __shared__ __align__(128) uint8_t smem[];
   uint2* q_frag = reinterpret_cast<uint2*>(smem);                  // [hi, lo][NR][STEPS][32]
   uint8_t* ring = smem + L::kQBytes;
@@ -207,7 +213,7 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
   // ---- this block's part of the line
   auto units_of = [&](int b) -> unsigned {
     const int n = min(max(__ldg(p.lengths + b), 0), cap);
-    return max((n + 15) >> 4, 1) + kItemCost;  // an empty sequence is one empty slab: its output is written too
+    return max((n + SL - 1) >> SHIFT, 1) + COST;  // an empty sequence is one empty slab: its output is written too
   };
   const int chunk = (p.batch + NT - 1) / NT;
   unsigned mine = 0;
@@ -232,7 +238,7 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
   }
   const unsigned grid = min(gridDim.x, total), share = total / grid, longer = total % grid;
   if (blockIdx.x >= grid) {
-    if (tid == 0) a.cuts[blockIdx.x].last = -1;
+    if (tid == 0 && !a.cuts_by_item) a.cuts[blockIdx.x].last = -1;
     return;
   }
   // the first `longer` blocks take one unit more
@@ -273,14 +279,14 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
   // slab_offset of the share's i-th token: for D = 128 the tokens are 4 apart, which flips bit 2 of the chunk
   auto share_off = [&](int i) -> uint32_t { return (D == 128 && (i & 1) ? lane_off ^ 64u : lane_off) + i * 512; };
 
-  PagesCut cut{0, 0, 0, -1, 0};
+  PagesCut cut{0, 0, 0, 0, -1, 0};
   for (unsigned pos = lo; pos < hi;) {
     it.length = page_length(p, it.b, status);
     const unsigned end = it.first + units_of(it.b);
-    it.slabs = static_cast<int>(end - it.first) - kItemCost;
-    // the item's first kItemCost units stand for what an item costs beside its slabs
-    const int s0 = max(0, static_cast<int>(pos - it.first) - kItemCost);
-    const int s1 = static_cast<int>(min(end, hi) - it.first) - kItemCost;
+    it.slabs = static_cast<int>(end - it.first) - COST;
+    // the item's first COST units stand for what an item costs beside its slabs
+    const int s0 = max(0, static_cast<int>(pos - it.first) - COST);
+    const int s1 = static_cast<int>(min(end, hi) - it.first) - COST;
     pos = end;
     const int n = it.length;
     const int rows = min(ROWS, a.rows - it.tile * ROWS);
@@ -299,19 +305,19 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
       uint32_t valid = 0;  // bit s: stage s holds a page of the pool
 
       auto page_at = [&](int slab) -> int {
-        if (slab >= s1 || slab * 16 >= n) return -1;
-        const int page = __ldg(table + (slab >> (p.page_shift - 4)));
+        if (slab >= s1 || slab * SL >= n) return -1;
+        const int page = __ldg(table + (slab >> (p.page_shift - SHIFT)));
         if (static_cast<unsigned>(page) < static_cast<unsigned>(p.num_pages)) return page;
         if (lane == 0) atomicOr(status, kDevBounds);
         return -1;
       };
       auto issue = [&](int slab, int page, int stage) {
         if (page >= 0) {
-          const int slot = (slab << 4) & (P - 1);
+          const int slot = (slab << SHIFT) & (P - 1);
           const uint8_t* ks = kbase + static_cast<int64_t>(page) * k_page + (slot * k_tok + k_lane);
           const uint8_t* vs = vbase + static_cast<int64_t>(page) * v_page + (slot * v_tok + v_lane);
           const uint32_t dst = my_ring_s + stage * L::kStageBytes;
-          if (slab * 16 + 16 <= seen_by_all) {
+          if (slab * SL + SL <= seen_by_all) {
 #pragma unroll
             for (int i = 0; i < COPIES; ++i) {
               copy16(dst + share_off(i), ks + i * STEP * k_tok, 16);
@@ -322,7 +328,7 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
             // that a NaN there stays with the rows that see it
 #pragma unroll
             for (int i = 0; i < COPIES; ++i) {
-              const int tok = slab * 16 + lane / CHUNKS + i * STEP;
+              const int tok = slab * SL + lane / CHUNKS + i * STEP;
               copy16(dst + share_off(i), ks + i * STEP * k_tok, tok < n ? 16 : 0);
               copy16(dst + share_off(i) + L::kSlabBytes, vs + i * STEP * v_tok, tok < seen_by_all ? 16 : 0);
             }
@@ -411,60 +417,85 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
           const uint8_t* kb = my_ring + stage * L::kStageBytes;
           const uint8_t* vb = kb + L::kSlabBytes;
           const float ksc = my_sc[stage * 2], vsc = my_sc[stage * 2 + 1];
-          // ---- S^T: tokens g and g + 8, rows 2 t and 2 t + 1. Two accumulators per group halve the
-          // chain of dependent products.
-          float s[NR][4], s2[NR][4];
+          // ---- S^T: tokens g and g + 8 of each 16-token part, rows 2 t and 2 t + 1. Where a slab is
+          // one part, two accumulators halve the chain of dependent products.
+          constexpr int ACC = U == 1 ? 2 : 1;
+          float s[NR][U][4], s2[NR][4];
 #pragma unroll
           for (int r = 0; r < NR; ++r) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[r][e] = s2[r][e] = 0.0f;
+            for (int e = 0; e < 4; ++e) {
+              s2[r][e] = 0.0f;
+#pragma unroll
+              for (int u = 0; u < U; ++u) s[r][u][e] = 0.0f;
+            }
           }
 #pragma unroll
           for (int h = 0; h < D / 64; ++h) {
             const int ch = D == 128 ? 2 * t + h : t;
-            const uint4 k0 = *reinterpret_cast<const uint4*>(kb + slab_offset<D>(g, ch));
-            const uint4 k1 = *reinterpret_cast<const uint4*>(kb + slab_offset<D>(g + 8, ch));
-            const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int j = h * 4 + i;
-              const uint32_t ka[4] = {e4m3x2_f16(w0[i]), e4m3x2_f16(w1[i]), e4m3x2_f16_high(w0[i]),
-                                      e4m3x2_f16_high(w1[i])};
+            for (int u = 0; u < U; ++u) {
+              const uint4 k0 = *reinterpret_cast<const uint4*>(kb + u * 16 * D + slab_offset<D>(g, ch));
+              const uint4 k1 = *reinterpret_cast<const uint4*>(kb + u * 16 * D + slab_offset<D>(g + 8, ch));
+              const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
-              for (int r = 0; r < NR; ++r) {
-                const uint2 q = Q_HELD ? q_held[Q_HELD ? j : 0] : q_frag[(r * STEPS + j) * 32 + lane];
-                mma_f16(i & 1 ? s2[r] : s[r], ka, q.x, q.y);
-                if constexpr (SPLIT) {
-                  const uint2 ql = q_frag[((NR + r) * STEPS + j) * 32 + lane];
-                  mma_f16(i & 1 ? s2[r] : s[r], ka, ql.x, ql.y);
+              for (int i = 0; i < 4; ++i) {
+                const int j = h * 4 + i;
+                const uint32_t ka[4] = {e4m3x2_f16(w0[i]), e4m3x2_f16(w1[i]), e4m3x2_f16_high(w0[i]),
+                                        e4m3x2_f16_high(w1[i])};
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                  const uint2 q = Q_HELD ? q_held[Q_HELD ? j : 0] : q_frag[(r * STEPS + j) * 32 + lane];
+                  mma_f16(ACC == 2 && (i & 1) ? s2[r] : s[r][u], ka, q.x, q.y);
+                  if constexpr (SPLIT) {
+                    const uint2 ql = q_frag[((NR + r) * STEPS + j) * 32 + lane];
+                    mma_f16(ACC == 2 && (i & 1) ? s2[r] : s[r][u], ka, ql.x, ql.y);
+                  }
                 }
               }
             }
           }
           const float size = fabsf(vsc), lv = size > 0.0f ? fmaxf(__log2f(size), kLeastLogScale) : kLeastLogScale;
-          const int tok = slab * 16 + g;
-          uint32_t pb[NR][2], pl[NR][2];
+          const int tok = slab * SL + g;
+          uint32_t pb[NR][U][2], pl[NR][U][2];
 #pragma unroll
           for (int r = 0; r < NR; ++r) {
             const float c0 = unit[r][0] * ksc, c1 = unit[r][1] * ksc;
-            s[r][0] = (s[r][0] + s2[r][0]) * c0;
-            s[r][1] = (s[r][1] + s2[r][1]) * c1;
-            s[r][2] = (s[r][2] + s2[r][2]) * c0;
-            s[r][3] = (s[r][3] + s2[r][3]) * c1;
-            if (slab * 16 + 16 > seen_by_all) {
+            float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              if constexpr (ACC == 2) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[r][u][e] += s2[r][e];
+              }
+              scale_pair(s[r][u][0], s[r][u][1], c0, c1);
+              scale_pair(s[r][u][2], s[r][u][3], c0, c1);
+            }
+            if (slab * SL + SL > seen_by_all) {
               const int seen0 = seen_of(r * 8 + 2 * t), seen1 = seen_of(r * 8 + 2 * t + 1);
-              if (tok >= seen0) s[r][0] = -INFINITY;
-              if (tok >= seen1) s[r][1] = -INFINITY;
-              if (tok + 8 >= seen0) s[r][2] = -INFINITY;
-              if (tok + 8 >= seen1) s[r][3] = -INFINITY;
+#pragma unroll
+              for (int u = 0; u < U; ++u) {
+                if (tok + 16 * u >= seen0) s[r][u][0] = -INFINITY;
+                if (tok + 16 * u >= seen1) s[r][u][1] = -INFINITY;
+                if (tok + 16 * u + 8 >= seen0) s[r][u][2] = -INFINITY;
+                if (tok + 16 * u + 8 >= seen1) s[r][u][3] = -INFINITY;
+              }
             }
             if (a.scores != nullptr) {
               float* at = a.scores +
                           ((static_cast<int64_t>(it.b) * p.heads + it.h) * a.rows + it.tile * ROWS + r * 8 + 2 * t) * a.capacity + tok;
-              if (r * 8 + 2 * t < rows) at[0] = s[r][0], at[8] = s[r][2];
-              if (r * 8 + 2 * t + 1 < rows) at[a.capacity] = s[r][1], at[a.capacity + 8] = s[r][3];
+#pragma unroll
+              for (int u = 0; u < U; ++u) {
+                if (r * 8 + 2 * t < rows) at[16 * u] = s[r][u][0], at[16 * u + 8] = s[r][u][2];
+                if (r * 8 + 2 * t + 1 < rows)
+                  at[a.capacity + 16 * u] = s[r][u][1], at[a.capacity + 16 * u + 8] = s[r][u][3];
+              }
             }
-            float t0 = fmaxf(s[r][0], s[r][2]), t1 = fmaxf(s[r][1], s[r][3]);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              t0 = fmaxf(t0, fmaxf(s[r][u][0], s[r][u][2]));
+              t1 = fmaxf(t1, fmaxf(s[r][u][1], s[r][u][3]));
+            }
 #pragma unroll
             for (int x = 4; x <= 16; x <<= 1) {
               t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, x));
@@ -482,72 +513,83 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
               l[r][1] *= f1;
 #pragma unroll
               for (int j = 0; j < MT; ++j) {
-                o[r][j][0] *= f0;
-                o[r][j][1] *= f1;
-                o[r][j][2] *= f0;
-                o[r][j][3] *= f1;
+                scale_pair(o[r][j][0], o[r][j][1], f0, f1);
+                scale_pair(o[r][j][2], o[r][j][3], f0, f1);
               }
             }
-            s[r][0] = exp2_approx(s[r][0] - m[r][0]);
-            s[r][1] = exp2_approx(s[r][1] - m[r][1]);
-            s[r][2] = exp2_approx(s[r][2] - m[r][0]);
-            s[r][3] = exp2_approx(s[r][3] - m[r][1]);
-            l[r][0] += s[r][0] + s[r][2];
-            l[r][1] += s[r][1] + s[r][3];
-            scale_pair(s[r][0], s[r][1], vsc);
-            scale_pair(s[r][2], s[r][3], vsc);
-            // the weights of 8 tokens x 8 rows, transposed into the B fragment of O^T = V^T P^T
-            const uint32_t w0 = f16x2_of(s[r][0], s[r][1]), w1 = f16x2_of(s[r][2], s[r][3]);
-            pb[r][0] = transpose8(w0);
-            pb[r][1] = transpose8(w1);
-            if constexpr (SPLIT) {
-              const float2 h0 = f16x2_values(w0), h1 = f16x2_values(w1);
-              pl[r][0] = transpose8(f16x2_of(s[r][0] - h0.x, s[r][1] - h0.y));
-              pl[r][1] = transpose8(f16x2_of(s[r][2] - h1.x, s[r][3] - h1.y));
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              float(&x)[4] = s[r][u];
+              x[0] = exp2_approx(x[0] - m[r][0]);
+              x[1] = exp2_approx(x[1] - m[r][1]);
+              x[2] = exp2_approx(x[2] - m[r][0]);
+              x[3] = exp2_approx(x[3] - m[r][1]);
+              l[r][0] += x[0] + x[2];
+              l[r][1] += x[1] + x[3];
+              scale_pair(x[0], x[1], vsc, vsc);
+              scale_pair(x[2], x[3], vsc, vsc);
+              // the weights of 8 tokens x 8 rows, transposed into the B fragment of O^T = V^T P^T
+              const uint32_t w0 = f16x2_of(x[0], x[1]), w1 = f16x2_of(x[2], x[3]);
+              pb[r][u][0] = transpose8(w0);
+              pb[r][u][1] = transpose8(w1);
+              if constexpr (SPLIT) {
+                const float2 h0 = f16x2_values(w0), h1 = f16x2_values(w1);
+                pl[r][u][0] = transpose8(f16x2_of(x[0] - h0.x, x[1] - h0.y));
+                pl[r][u][1] = transpose8(f16x2_of(x[2] - h1.x, x[3] - h1.y));
+              }
             }
           }
           // ---- O^T: row g of MMA tile j is dim g * D / 8 + 2 j, row g + 8 the next one, so a lane's
-          // bytes of a token are consecutive; tokens 2 t, 2 t + 1 and 2 t + 8, 2 t + 9
+          // bytes of a token are consecutive; tokens 2 t, 2 t + 1 and 2 t + 8, 2 t + 9 of each part
           constexpr int W = D / 32;  // 4-byte words per lane and token
-          uint32_t r0[W], r1[W], r2[W], r3[W];
-          auto take = [&](int row, uint32_t(&r)[W]) {
-            if constexpr (D == 128) {
-              const uint4 x = *reinterpret_cast<const uint4*>(vb + slab_offset<D>(row, g));
-              r[0] = x.x, r[1] = x.y, r[2] = x.z, r[3] = x.w;
-            } else {
-              const uint2 x = *reinterpret_cast<const uint2*>(vb + slab_offset<D>(row, g >> 1) + (g & 1) * 8);
-              r[0] = x.x, r[1] = x.y;
-            }
-          };
-          take(2 * t, r0);
-          take(2 * t + 1, r1);
-          take(2 * t + 8, r2);
-          take(2 * t + 9, r3);
 #pragma unroll
-          for (int w = 0; w < W; ++w) {
-            const uint32_t x0 = __byte_perm(r0[w], r1[w], 0x5140), x1 = __byte_perm(r0[w], r1[w], 0x7362);
-            const uint32_t y0 = __byte_perm(r2[w], r3[w], 0x5140), y1 = __byte_perm(r2[w], r3[w], 0x7362);
-            const uint32_t va[4] = {e4m3x2_f16(x0), e4m3x2_f16_high(x0), e4m3x2_f16(y0), e4m3x2_f16_high(y0)};
-            const uint32_t vc[4] = {e4m3x2_f16(x1), e4m3x2_f16_high(x1), e4m3x2_f16(y1), e4m3x2_f16_high(y1)};
+          for (int u = 0; u < U; ++u) {
+            uint32_t r0[W], r1[W], r2[W], r3[W];
+            auto take = [&](int row, uint32_t(&r)[W]) {
+              if constexpr (D == 128) {
+                const uint4 x = *reinterpret_cast<const uint4*>(vb + u * 16 * D + slab_offset<D>(row, g));
+                r[0] = x.x, r[1] = x.y, r[2] = x.z, r[3] = x.w;
+              } else {
+                const uint2 x = *reinterpret_cast<const uint2*>(vb + u * 16 * D + slab_offset<D>(row, g >> 1) + (g & 1) * 8);
+                r[0] = x.x, r[1] = x.y;
+              }
+            };
+            take(2 * t, r0);
+            take(2 * t + 1, r1);
+            take(2 * t + 8, r2);
+            take(2 * t + 9, r3);
 #pragma unroll
-            for (int r = 0; r < NR; ++r) {
-              mma_f16(o[r][2 * w], va, pb[r][0], pb[r][1]);
-              mma_f16(o[r][2 * w + 1], vc, pb[r][0], pb[r][1]);
-              if constexpr (SPLIT) {
-                mma_f16(o[r][2 * w], va, pl[r][0], pl[r][1]);
-                mma_f16(o[r][2 * w + 1], vc, pl[r][0], pl[r][1]);
+            for (int w = 0; w < W; ++w) {
+              const uint32_t x0 = __byte_perm(r0[w], r1[w], 0x5140), x1 = __byte_perm(r0[w], r1[w], 0x7362);
+              const uint32_t y0 = __byte_perm(r2[w], r3[w], 0x5140), y1 = __byte_perm(r2[w], r3[w], 0x7362);
+              const uint32_t va[4] = {e4m3x2_f16(x0), e4m3x2_f16_high(x0), e4m3x2_f16(y0), e4m3x2_f16_high(y0)};
+              const uint32_t vc[4] = {e4m3x2_f16(x1), e4m3x2_f16_high(x1), e4m3x2_f16(y1), e4m3x2_f16_high(y1)};
+#pragma unroll
+              for (int r = 0; r < NR; ++r) {
+                mma_f16(o[r][2 * w], va, pb[r][u][0], pb[r][u][1]);
+                mma_f16(o[r][2 * w + 1], vc, pb[r][u][0], pb[r][u][1]);
+                if constexpr (SPLIT) {
+                  mma_f16(o[r][2 * w], va, pl[r][u][0], pl[r][u][1]);
+                  mma_f16(o[r][2 * w + 1], vc, pl[r][u][0], pl[r][u][1]);
+                }
               }
             }
           }
           // the tokens that only some rows see (fewer than q_len of them)
-          for (int x = max(seen_by_all, slab * 16); x < min(n, slab * 16 + 16); ++x) {
-            const int k = x - slab * 16, from = ((k & 7) << 2) | t;
+          for (int x = max(seen_by_all, slab * SL); x < min(n, slab * SL + SL); ++x) {
+            const int k = x - slab * SL, from = ((k & 7) << 2) | t;
             const int page = __ldg(table + (x >> p.page_shift));
             const uint8_t* v = vbase + page * p.sp[1] + (x & (P - 1)) * p.st[1] + g * (D / 8);
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
-              const float w0 = __shfl_sync(0xffffffffu, k < 8 ? s[r][0] : s[r][2], from);
-              const float w1 = __shfl_sync(0xffffffffu, k < 8 ? s[r][1] : s[r][3], from);
+              float w0 = 0.0f, w1 = 0.0f;
+#pragma unroll
+              for (int i = 0; i < 2 * U; ++i) {
+                if (k >> 3 == i) {  // the same for all lanes
+                  w0 = __shfl_sync(0xffffffffu, s[r][i >> 1][(i & 1) * 2], from);
+                  w1 = __shfl_sync(0xffffffffu, s[r][i >> 1][(i & 1) * 2 + 1], from);
+                }
+              }
               const bool sees0 = x < seen_of(r * 8 + 2 * t), sees1 = x < seen_of(r * 8 + 2 * t + 1);
 #pragma unroll
               for (int j = 0; j < MT; ++j) {
@@ -619,9 +661,12 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
           if (d == 0) __stcg(reinterpret_cast<float2*>(my_part + ROWS * D + 2 * r), make_float2(ref, sum));
         }
       }
-      if (s0 == 0 && !whole) {
+      if (s0 == 0) {
         // the merge goes from this block to the one that holds the item's last unit
-        cut = PagesCut{it.b, it.h, it.tile, static_cast<int>(block_of(end - 1)), it.first <= lo ? 0 : 1};
+        const PagesCut c{it.b, it.h, it.tile, static_cast<int>(blockIdx.x),
+                         whole ? -1 : static_cast<int>(block_of(end - 1)), it.first <= lo ? 0 : 1};
+        if (!whole) cut = c;
+        if (a.cuts_by_item && tid == 0) a.cuts[(it.b * p.heads + it.h) * a.row_tiles + it.tile] = c;
       }
     }
     // ---- the next item
@@ -634,37 +679,36 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
       }
     }
   }
-  if (tid == 0) a.cuts[blockIdx.x] = cut;
+  if (tid == 0 && !a.cuts_by_item) a.cuts[blockIdx.x] = cut;
 }
 
-// The items that several blocks share: four warps per row add the blocks' outputs, each with its
-// weight, in an order that depends on nothing but their number. A block per cut and four rows.
-template <int T, int D, int ROWS>
+// The items that several blocks share: WARPS warps per row add the blocks' outputs, each with its
+// weight, in an order that depends on nothing but their number. A block per item (16 warps per row:
+// few items, shared by many blocks) or per block of the attention (4: many items, few shared by more
+// than two) and 16 / WARPS rows.
+template <int T, int D, int ROWS, int WARPS>
 __global__ void __launch_bounds__(512) pages_merge_kernel(PagesAttnArgs a) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const PagesCut cut = a.cuts[blockIdx.x];
   if (cut.last < 0) return;
-  constexpr int LANES = D / 4, SIDES = 32 / LANES, SHARES = 4 * SIDES;  // lanes per part, parts side by side
-  __shared__ float4 sums[4][SHARES][LANES];
-  const int lane = threadIdx.x & 31, group = threadIdx.x >> 7, share = (threadIdx.x >> 5 & 3) * SIDES + lane / LANES;
-  const int row = blockIdx.y * 4 + group, r = cut.tile * ROWS + row, parts = cut.last - static_cast<int>(blockIdx.x) + 1;
+  constexpr int LANES = D / 4, SIDES = 32 / LANES, SHARES = WARPS * SIDES;  // lanes per part, parts side by side
+  constexpr int GROUPS = 16 / WARPS;
+  __shared__ float4 sums[GROUPS][SHARES][LANES];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = warp / WARPS;
+  const int share = warp % WARPS * SIDES + lane / LANES;
+  const int row = blockIdx.y * GROUPS + group, r = cut.tile * ROWS + row, parts = cut.last - cut.first + 1;
   const bool live = row < ROWS && r < a.rows;
   auto part_of = [&](int i) -> const float* {
-    const int64_t slot = i == 0 ? 2 * static_cast<int64_t>(blockIdx.x) + cut.slot : 2 * (static_cast<int64_t>(blockIdx.x) + i);
-    return a.partial + slot * ROWS * (D + 2);
+    return a.partial + static_cast<int64_t>(2 * (cut.first + i) + (i == 0 ? cut.slot : 0)) * (ROWS * (D + 2));
   };
   float ref = kNoScore, sum = 0.0f;
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   if (live) {
+#pragma unroll 4
     for (int i = lane; i < parts; i += 32) ref = fmaxf(ref, __ldg(part_of(i) + ROWS * D + 2 * row));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, o));
-    for (int i = lane; i < parts; i += 32) {
-      const float2 ml = __ldg(reinterpret_cast<const float2*>(part_of(i) + ROWS * D + 2 * row));
-      sum = fmaf(exp2_approx(ml.x - ref), ml.y, sum);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const int d = lane % LANES * 4;
 #pragma unroll 8
     for (int i = share; i < parts; i += SHARES) {
@@ -677,6 +721,15 @@ __global__ void __launch_bounds__(512) pages_merge_kernel(PagesAttnArgs a) {
       acc.w = fmaf(f, x.w, acc.w);
     }
     sums[group][share][lane % LANES] = acc;
+    if (warp % WARPS == 0) {
+#pragma unroll 4
+      for (int i = lane; i < parts; i += 32) {
+        const float2 ml = __ldg(reinterpret_cast<const float2*>(part_of(i) + ROWS * D + 2 * row));
+        sum = fmaf(exp2_approx(ml.x - ref), ml.y, sum);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
   }
   __syncthreads();
   if (!live || share != 0) return;

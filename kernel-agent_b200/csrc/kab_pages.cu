@@ -126,7 +126,7 @@ int attention_check(const KabKvPagesAttention* p, PagesAttnArgs* g) {
 // The launch's workspace: the blocks' partial results and cuts and, with mass, the scores and the
 // rows' references. Nothing in it has to be zero.
 struct AttentionPlan {
-  int grid = 0;
+  int grid = 0, merges = 0;  // blocks of the attention; items, or blocks where those are fewer
   size_t cuts = 0, partial = 0, ml = 0, scores = 0;
   size_t bytes() const { return cuts + partial + ml + scores; }
 };
@@ -134,14 +134,14 @@ size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
 // Opts the kernel instance into its shared memory and returns the blocks of it that fit on the
 // GPU at once (asked once per device), or -1.
-template <int T, int D, int NR>
+template <int T, int D, int NR, int SL>
 int attention_blocks() {
-  using L = PagesLayout<D, NR, T == kF32>;
+  using L = PagesLayout<D, NR, SL, T == kF32>;
   static int blocks[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
   if (blocks[dev] == 0) {
-    auto kern = pages_attention_kernel<T, D, NR>;
+    auto kern = pages_attention_kernel<T, D, NR, SL>;
     int n = 0;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem) != cudaSuccess ||
         cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, L::kThreads, L::kSmem) != cudaSuccess || n < 1)
@@ -150,30 +150,33 @@ int attention_blocks() {
   }
   return blocks[dev];
 }
-// Runs `f` with the kernel instance's types: f(type, head_dim, groups of rows).
+
+// The kernel instance of a call: f(type, head_dim, groups of rows, tokens of a slab).
+template <int V>
+using Int = std::integral_constant<int, V>;
 template <int T, int D, typename F>
-auto with_groups(int rows, F&& f) {
-  return tile_rows(rows) == 8 ? f(std::integral_constant<int, T>(), std::integral_constant<int, D>(),
-                                  std::integral_constant<int, 1>())
-                              : f(std::integral_constant<int, T>(), std::integral_constant<int, D>(),
-                                  std::integral_constant<int, 2>());
+auto with_groups(int rows, int64_t page, F&& f) {
+  if (page == 16) return tile_rows(rows) == 8 ? f(Int<T>(), Int<D>(), Int<1>(), Int<16>()) : f(Int<T>(), Int<D>(), Int<2>(), Int<16>());
+  return tile_rows(rows) == 8 ? f(Int<T>(), Int<D>(), Int<1>(), Int<32>()) : f(Int<T>(), Int<D>(), Int<2>(), Int<32>());
 }
 template <typename F>
-auto with_instance(int dtype, int64_t d, int rows, F&& f) {
-  if (dtype == KAB_BF16) return d == 128 ? with_groups<kBF16, 128>(rows, f) : with_groups<kBF16, 64>(rows, f);
-  if (dtype == KAB_F16) return d == 128 ? with_groups<kF16, 128>(rows, f) : with_groups<kF16, 64>(rows, f);
-  return d == 128 ? with_groups<kF32, 128>(rows, f) : with_groups<kF32, 64>(rows, f);
+auto with_instance(const KabKvPagesAttention* p, int rows, F&& f) {
+  const int64_t d = p->cache.head_dim, page = p->cache.page_tokens;
+  if (p->q_dtype == KAB_BF16) return d == 128 ? with_groups<kBF16, 128>(rows, page, f) : with_groups<kBF16, 64>(rows, page, f);
+  if (p->q_dtype == KAB_F16) return d == 128 ? with_groups<kF16, 128>(rows, page, f) : with_groups<kF16, 64>(rows, page, f);
+  return d == 128 ? with_groups<kF32, 128>(rows, page, f) : with_groups<kF32, 64>(rows, page, f);
 }
 
 int attention_plan(const KabKvPagesAttention* p, const PagesAttnArgs& g, AttentionPlan* plan) {
-  plan->grid = with_instance(p->q_dtype, p->cache.head_dim, g.rows, [](auto T, auto D, auto NR) {
-    return attention_blocks<decltype(T)::value, decltype(D)::value, decltype(NR)::value>();
+  plan->grid = with_instance(p, g.rows, [](auto T, auto D, auto NR, auto SL) {
+    return attention_blocks<decltype(T)::value, decltype(D)::value, decltype(NR)::value, decltype(SL)::value>();
   });
   if (plan->grid < 0) return fail(KAB_ECUDA, "cannot configure the paged attention kernel");
   const size_t items = static_cast<size_t>(p->cache.batch * p->cache.heads_kv);
   KAB_REQUIRE(items * g.row_tiles * (static_cast<size_t>(g.capacity) / 16 + 1 + kItemCost) < (size_t(1) << 31),
               "sequences x KV heads x row tiles x tokens of the page table is too large");
-  plan->cuts = round256(static_cast<size_t>(plan->grid) * sizeof(PagesCut));
+  plan->merges = static_cast<int>(std::min(items * g.row_tiles, static_cast<size_t>(plan->grid)));
+  plan->cuts = round256(static_cast<size_t>(plan->merges) * sizeof(PagesCut));
   plan->partial = round256(static_cast<size_t>(plan->grid) * 2 * tile_rows(g.rows) * (p->cache.head_dim + 2) * 4);
   if (p->use_mass) {
     plan->ml = round256(items * g.rows * 8);
@@ -197,13 +200,16 @@ cudaError_t launch_after(void (*kern)(Args...), dim3 grid, int threads, cudaStre
   return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
-template <int T, int D, int NR>
-int launch_attention(const PagesAttnArgs& g, int grid, unsigned* status, cudaStream_t s) {
-  using L = PagesLayout<D, NR, T == kF32>;
-  pages_attention_kernel<T, D, NR><<<grid, L::kThreads, L::kSmem, s>>>(g, status);
+template <int T, int D, int NR, int SL>
+int launch_attention(const PagesAttnArgs& g, const AttentionPlan& plan, unsigned* status, cudaStream_t s) {
+  using L = PagesLayout<D, NR, SL, T == kF32>;
+  pages_attention_kernel<T, D, NR, SL><<<plan.grid, L::kThreads, L::kSmem, s>>>(g, status);
   if (int e = check_launch("kab_kv_pages_attention")) return e;
-  const dim3 merges(static_cast<unsigned>(grid), static_cast<unsigned>((std::min(g.rows, L::kRows) + 3) / 4));
-  launch_after(pages_merge_kernel<T, D, L::kRows>, merges, 512, s, g);
+  const int rows = std::min(g.rows, L::kRows);
+  if (g.cuts_by_item)
+    launch_after(pages_merge_kernel<T, D, L::kRows, 16>, dim3(plan.merges, rows), 512, s, g);
+  else
+    launch_after(pages_merge_kernel<T, D, L::kRows, 4>, dim3(plan.merges, (rows + 3) / 4), 512, s, g);
   if (int e = check_launch("kab_kv_pages_attention merge")) return e;
   if (g.scores == nullptr || g.capacity == 0) return KAB_OK;
   const dim3 blocks(static_cast<unsigned>((g.capacity + 255) / 256), g.pool.heads, g.pool.batch);
@@ -289,14 +295,16 @@ int kab_kv_pages_attention(const KabKvPagesAttention* params, void* workspace, s
   KAB_REQUIRE(status != nullptr, "no device status word");
   uint8_t* w = static_cast<uint8_t*>(workspace);
   g.cuts = reinterpret_cast<PagesCut*>(w);
+  g.cuts_by_item = params->cache.batch * params->cache.heads_kv * g.row_tiles <= plan.grid;
   g.partial = reinterpret_cast<float*>(w + plan.cuts);
   if (params->use_mass) {
     g.ml = reinterpret_cast<float*>(w + plan.cuts + plan.partial);
     g.scores = reinterpret_cast<float*>(w + plan.cuts + plan.partial + plan.ml);
   }
   const cudaStream_t s = as_stream(stream);
-  return with_instance(params->q_dtype, params->cache.head_dim, g.rows, [&](auto T, auto D, auto NR) {
-    return launch_attention<decltype(T)::value, decltype(D)::value, decltype(NR)::value>(g, plan.grid, status, s);
+  return with_instance(params, g.rows, [&](auto T, auto D, auto NR, auto SL) {
+    return launch_attention<decltype(T)::value, decltype(D)::value, decltype(NR)::value, decltype(SL)::value>(
+        g, plan, status, s);
   });
 }
 
