@@ -1,4 +1,6 @@
 // extern "C" entry points of the weight-only FP4 linear (gemv_fp4.cuh).
+#include <algorithm>
+
 #include "kab_host.h"
 
 #include "gemv_fp4.cuh"
@@ -11,15 +13,76 @@ int gemv_check(int64_t m, int64_t n, int64_t k, int fmt, int dtype) {
   KAB_REQUIRE(valid_dtype(dtype), "unknown dtype %d", dtype);
   KAB_REQUIRE(m >= 0 && n >= 0 && k >= 0, "negative shape");
   KAB_REQUIRE(k % (fmt == KAB_NVFP4 ? 16 : 32) == 0, "K = %lld is not a multiple of the block", (long long)k);
-  KAB_REQUIRE(m < (int64_t(1) << 18) && n < (int64_t(1) << 31) && k < (int64_t(1) << 31), "problem too large");
+  KAB_REQUIRE(m < (int64_t(1) << 18) && n < (int64_t(1) << 30) && k < (int64_t(1) << 30), "problem too large");
   return KAB_OK;
 }
 
+// How a shape is cut: slices of K so that a slice of x fits in shared memory beside a second block
+// (kXBytes), more of them where the rows alone cannot occupy the GPU, and blocks per slice.
+constexpr int kXBytes = 72 * 1024;
+struct GemvPlan {
+  int nt, tokens, chunks, slice_chunks, slices, k_warps, blocks;
+  size_t partial;
+};
+GemvPlan gemv_plan(int64_t m, int64_t n, int64_t k, int dtype) {
+  GemvPlan p{};
+  p.nt = m <= 8 ? 1 : m <= 16 ? 2 : 4;
+  p.tokens = static_cast<int>(std::min<int64_t>(m, 8 * p.nt));
+  p.chunks = static_cast<int>(std::max<int64_t>(1, (k + 127) / 128));
+  const int64_t per_chunk = static_cast<int64_t>(p.tokens) * 256 * (dtype == KAB_F32 ? 2 : 1);
+  const int fit = static_cast<int>(std::max<int64_t>(1, kXBytes / per_chunk));
+  const int64_t tiles = (n + 15) / 16;
+  int want = (p.chunks + fit - 1) / fit;
+  p.slice_chunks = (p.chunks + want - 1) / want;
+  p.slices = (p.chunks + p.slice_chunks - 1) / p.slice_chunks;
+  p.k_warps = p.slice_chunks >= 8 ? 8 : p.slice_chunks >= 4 ? 4 : p.slice_chunks >= 2 ? 2 : 1;
+  const int64_t units = (tiles + kGemvWarps / p.k_warps - 1) / (kGemvWarps / p.k_warps);
+  p.blocks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(units, 2 * sm_count() / p.slices)));
+  p.partial = p.slices > 1 ? static_cast<size_t>(p.slices) * m * n * 4 : 0;
+  return p;
+}
+
+template <int T, int MX, int NT, int WIDE>
+int launch_gemv(const GemvArgs& a, const GemvPlan& p, cudaStream_t s) {
+  auto kern = gemv_fp4_kernel<T, MX, NT, WIDE>;
+  const int bytes = gemv_smem(p.tokens, p.slice_chunks, NT, T == kF32);
+  static bool configured[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(KAB_ECUDA, "no current device");
+  if (!configured[dev]) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 113 * 1024) != cudaSuccess)
+      return fail(KAB_ECUDA, "cannot configure the FP4 linear");
+    configured[dev] = true;
+  }
+  const dim3 grid(p.blocks, p.slices, (a.m + 8 * NT - 1) / (8 * NT));
+  kern<<<grid, kGemvThreads, bytes, s>>>(a);
+  if (int e = check_launch("kab_gemv_fp4")) return e;
+  if (p.slices == 1) return KAB_OK;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((a.n + 255) / 256, a.m);
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, gemv_join_kernel<T>, a);
+  return check_launch("kab_gemv_fp4 join");
+}
+template <int T, int MX, int NT>
+int launch_gemv(const GemvArgs& a, const GemvPlan& p, cudaStream_t s) {
+  const bool wide = a.k % 32 == 0 && aligned(a.codes, 16) && aligned(a.scales, 2);
+  return wide ? launch_gemv<T, MX, NT, 1>(a, p, s) : launch_gemv<T, MX, NT, 0>(a, p, s);
+}
+template <int T, int MX>
+int launch_gemv(const GemvArgs& a, const GemvPlan& p, cudaStream_t s) {
+  return p.nt == 1 ? launch_gemv<T, MX, 1>(a, p, s) : p.nt == 2 ? launch_gemv<T, MX, 2>(a, p, s)
+                                                                : launch_gemv<T, MX, 4>(a, p, s);
+}
 template <int T>
-void launch_gemv(const GemvArgs& a, int fmt, cudaStream_t s) {
-  const dim3 grid(static_cast<unsigned>((a.n + 7) / 8), static_cast<unsigned>((a.m + 7) / 8));
-  if (fmt == KAB_MXFP4) gemv_fp4_kernel<T, 1><<<grid, 256, 0, s>>>(a);
-  else gemv_fp4_kernel<T, 0><<<grid, 256, 0, s>>>(a);
+int launch_gemv(const GemvArgs& a, const GemvPlan& p, int fmt, cudaStream_t s) {
+  return fmt == KAB_MXFP4 ? launch_gemv<T, 1>(a, p, s) : launch_gemv<T, 0>(a, p, s);
 }
 
 }  // namespace
@@ -33,7 +96,7 @@ int kab_gemv_fp4_workspace(int64_t m, int64_t n, int64_t k, int fmt, int dtype, 
                            size_t* zero_bytes) {
   if (int e = gemv_check(m, n, k, fmt, dtype)) return e;
   KAB_REQUIRE(bytes != nullptr && zero_bytes != nullptr, "null pointer");
-  *bytes = 0;
+  *bytes = m == 0 || n == 0 ? 0 : gemv_plan(m, n, k, dtype).partial;
   *zero_bytes = 0;
   return KAB_OK;
 }
@@ -42,21 +105,28 @@ int kab_gemv_fp4(const void* x, int dtype, int64_t ldx, const uint8_t* codes, co
                  int fmt, const float* tensor_scale, int scale_per_row, int64_t m, int64_t n, int64_t k,
                  const void* bias, int bias_dtype, void* out, int64_t ldo, void* workspace, size_t workspace_bytes,
                  void* stream) {
-  (void)workspace;
-  (void)workspace_bytes;
   if (int e = gemv_check(m, n, k, fmt, dtype)) return e;
   if (m == 0 || n == 0) return KAB_OK;
   KAB_REQUIRE(out != nullptr && tensor_scale != nullptr && (k == 0 || (x && codes && scales)), "null pointer");
   KAB_REQUIRE(bias == nullptr || valid_dtype(bias_dtype), "unknown bias dtype %d", bias_dtype);
   KAB_REQUIRE(aligned(x, 16) && ldx % 8 == 0, "x must be 16-byte aligned, its row stride a multiple of 8");
   KAB_REQUIRE(aligned(codes, 8), "codes must be 8-byte aligned");
+  KAB_REQUIRE(!swizzle || aligned(scales, 4), "swizzled scales must be 4-byte aligned");
   KAB_REQUIRE(ldo >= n && ldx >= k, "ldx %lld or ldo %lld is too short", (long long)ldx, (long long)ldo);
-  GemvArgs a{x, ldx, codes, scales, swizzle, tensor_scale, scale_per_row, m, n, k, bias, bias_dtype, out, ldo};
+  const GemvPlan p = gemv_plan(m, n, k, dtype);
+  KAB_REQUIRE(p.partial == 0 || (workspace != nullptr && workspace_bytes >= p.partial && aligned(workspace, 256)),
+              "the workspace needs %zu bytes, 256-byte aligned (kab_gemv_fp4_workspace)", p.partial);
+  GemvArgs a{};
+  a.x = x, a.ldx = ldx, a.codes = codes, a.scales = scales, a.swizzle = swizzle;
+  a.ts = tensor_scale, a.ts_per_row = scale_per_row;
+  a.m = static_cast<int>(m), a.n = static_cast<int>(n), a.k = static_cast<int>(k);
+  a.bias = bias, a.bias_dtype = bias_dtype, a.out = out, a.ldo = ldo;
+  a.chunks = p.chunks, a.slice_chunks = p.slice_chunks, a.slices = p.slices, a.k_warps = p.k_warps;
+  a.blocks = p.blocks, a.partial = static_cast<float*>(workspace);
   const cudaStream_t s = as_stream(stream);
-  if (dtype == KAB_BF16) launch_gemv<kBF16>(a, fmt, s);
-  else if (dtype == KAB_F16) launch_gemv<kF16>(a, fmt, s);
-  else launch_gemv<kF32>(a, fmt, s);
-  return check_launch("kab_gemv_fp4");
+  if (dtype == KAB_BF16) return launch_gemv<kBF16>(a, p, fmt, s);
+  if (dtype == KAB_F16) return launch_gemv<kF16>(a, p, fmt, s);
+  return launch_gemv<kF32>(a, p, fmt, s);
 }
 
 }  // extern "C"

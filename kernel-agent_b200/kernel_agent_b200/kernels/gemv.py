@@ -76,6 +76,8 @@ def fp4_w4a16_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     c, s = codes.contiguous(), scales.contiguous()
     if c.data_ptr() % 8:
         c = c.clone()
+    if s.data_ptr() % 4:
+        s = s.clone()
     ts = tensor_scale
     if not isinstance(ts, torch.Tensor) or ts.dtype != torch.float32 or ts.get_device() != device \
             or not ts.is_contiguous():
