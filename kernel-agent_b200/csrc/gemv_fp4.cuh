@@ -20,10 +20,12 @@
 //    finite value in [2^14, 2^15): bf16 and f16 keep all their bits down to 2^-29 of it; fp32 is
 //    split into two f16 terms (22 bits) and multiplied twice. It is converted once per block and
 //    stays in shared memory while the block streams its rows.
-//  * Each warp keeps four 128-code chunks of its rows in flight in registers, across the block's row
-//    tiles; the warps of a block share a tile's K and add their sums in shared memory. Blocks take
-//    equal numbers of rows (not of tiles). Where x does not fit, or the rows are too few to occupy
-//    the GPU, K is cut into slices whose sums meet in a second launch.
+//  * The (16-row tile, 128-code chunk) pairs of a K slice stand in one line, cut into equal parts for
+//    the blocks and again for their warps: every warp streams its part with kGemvDepth chunks in
+//    flight in registers and waits for nobody. Tiles that lie within a warp are written by it; those
+//    that several warps of a block share are added in shared memory at the end, those that two
+//    blocks share (and the slices of K, where x does not fit in shared memory) in a second launch.
+//    Always in the order of the line.
 #pragma once
 
 #include "codes.cuh"
@@ -44,9 +46,19 @@ struct GemvArgs {
   void* out;
   int64_t ldo;
   int chunks, slice_chunks, slices;  // 128-code chunks of K, of a slice of it, and slices
-  int k_warps;                       // warps of a block that share a tile's K
-  int blocks;                        // blocks per slice
-  float* partial;                    // [slices, m, n] where there is more than one slice
+  int tiles, blocks;                 // 16-row tiles; blocks per slice
+  float* partial;                    // [2, slices, m, n]: a tile's sum or its first part, and its second part
+};
+
+// The line of `total` units cut into `parts`: the first total % parts take one more.
+struct GemvCut {
+  int share, longer;
+  __host__ __device__ GemvCut(int total, int parts) : share(total / parts), longer(total % parts) {}
+  __host__ __device__ int begin(int part) const { return share * part + (part < longer ? part : longer); }
+  __host__ __device__ int part_of(int unit) const {
+    const int split = longer * (share + 1);
+    return unit < split ? unit / (share + 1) : longer + (unit - split) / share;
+  }
 };
 
 // ------------------------------------------------------------------ instructions
@@ -111,7 +123,8 @@ constexpr int kGemvThreads = 256, kGemvWarps = 8, kGemvDepth = 4;
 // so that the tokens of a group lie in different banks.
 __host__ __device__ constexpr int gemv_pitch(int slice_chunks) { return slice_chunks * 256 + 64; }
 __host__ __device__ constexpr int gemv_smem(int m, int slice_chunks, int nt, bool split) {
-  return m * gemv_pitch(slice_chunks) * (split ? 2 : 1) + 2 * kGemvWarps * 16 * 8 * nt * 4 + 8 * nt * 4;
+  return m * gemv_pitch(slice_chunks) * (split ? 2 : 1) + 2 * kGemvWarps * 16 * 8 * nt * 4 + 8 * nt * 4 +
+         2 * kGemvWarps * 4;
 }
 
 // ------------------------------------------------------------------ the kernel
@@ -127,74 +140,88 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
   const int slice = blockIdx.y, m0 = blockIdx.z * COLS, tokens = min(COLS, a.m - m0);
   const int c_first = slice * a.slice_chunks, c_count = min(a.slice_chunks, a.chunks - c_first);
   const int pitch = gemv_pitch(a.slice_chunks);
-  float* sums = reinterpret_cast<float*>(smem + tokens * pitch * (SPLIT ? 2 : 1));  // [2][8 warps][16][COLS]
+  float* sums = reinterpret_cast<float*>(smem + tokens * pitch * (SPLIT ? 2 : 1));  // [8 warps][2][16][COLS]
   float* unit = sums + 2 * kGemvWarps * 16 * COLS;                                  // [COLS]
 
-  // ---- this warp's stream: rows of the block's tiles, chunks kw, kw + KW, ... of the slice
-  const int KW = a.k_warps, RW = kGemvWarps / KW, kw = warp & (KW - 1), rw = warp / KW;
-  const int64_t row_lo = static_cast<int64_t>(a.n) * blockIdx.x / a.blocks;
-  const int64_t row_hi = static_cast<int64_t>(a.n) * (blockIdx.x + 1) / a.blocks;
-  const int tiles = static_cast<int>((row_hi - row_lo + 16 * RW - 1) / (16 * RW));
-  const int mine = kw < c_count ? (c_count - kw + KW - 1) / KW : 0;  // chunks per tile
+  int* seg_tile = reinterpret_cast<int*>(unit + COLS);  // [8 warps][2]: 2 * tile + (its end is here), or -1
+
+  // ---- this warp's part of the line
+  const GemvCut cut(a.tiles * c_count, a.blocks);
+  const int b_lo = cut.begin(blockIdx.x), b_hi = cut.begin(blockIdx.x + 1);
+  const GemvCut warps(b_hi - b_lo, kGemvWarps);
+  const int u_lo = b_lo + warps.begin(warp), u_hi = b_lo + warps.begin(warp + 1);
   const int cols = a.k >> (MX ? 5 : 4), half = a.k >> 1;
+  if (tid < 2 * kGemvWarps) seg_tile[tid] = -1;
 
   struct Slot {
     uint4 w0, w1;      // 32 codes of rows g and g + 8
     uint32_t s0, s1;   // their scales: two e4m3 bytes, or one e8m0
   };
-  const int k_last = max(0, (a.k - 1) / 32 * 32);  // the last 32 codes (or 16) of a row
   Slot slots[kGemvDepth] = {};
-  int is_tile = 0, is_chunk = 0;  // what the next issue loads
-  // the first scale of 32 codes; NVFP4 has two
-  auto scale_at = [&](int64_t row, int col) -> uint32_t {
-    if constexpr (MX) {
-      return __ldg(a.scales + (a.swizzle ? scale_offset_swizzled(row, col, cols) : row * cols + col));
-    } else if constexpr (WIDE) {  // col is even: both lie in one 4-column block
-      return __ldg(reinterpret_cast<const uint16_t*>(
-          a.scales + (a.swizzle ? scale_offset_swizzled(row, col, cols) : row * cols + col)));
-    } else {
-      const int next = min(col + 1, cols - 1);
-      const uint32_t s0 = __ldg(a.scales + (a.swizzle ? scale_offset_swizzled(row, col, cols) : row * cols + col));
-      const uint32_t s1 = __ldg(a.scales + (a.swizzle ? scale_offset_swizzled(row, next, cols) : row * cols + next));
-      return s0 | s1 << 8;
-    }
+  int is_unit = u_lo, is_tile = u_lo / c_count, is_chunk = u_lo % c_count;  // what the next issue loads
+  const uint8_t *code0, *code1, *scale0, *scale1;  // the tile's rows g and g + 8
+  auto point = [&]() {
+    const int r0 = min(is_tile * 16 + g, a.n - 1), r1 = min(is_tile * 16 + g + 8, a.n - 1);
+    code0 = a.codes + static_cast<int64_t>(r0) * half;
+    code1 = a.codes + static_cast<int64_t>(r1) * half;
+    scale0 = a.scales + (a.swizzle ? scale_offset_swizzled(r0, 0, cols) : static_cast<int64_t>(r0) * cols);
+    scale1 = a.scales + (a.swizzle ? scale_offset_swizzled(r1, 0, cols) : static_cast<int64_t>(r1) * cols);
   };
-  // Every load is made, at the nearest place that exists: rows past the block's are not written, and
-  // x is zero past K. (Loads under conditions were waited for at once: 98 us where these take 40 at
-  // 1 x 28672 x 8192.)
+  point();
+  // Every load is made, at the nearest place that exists: rows past n are not written, and x is zero
+  // past K. (Loads under conditions were waited for at once: 98 us against 53 at 1 x 28672 x 8192.)
+  const int last = max(0, (a.k - 1) / 32);  // the last 32 codes (or 16) of a row
   auto issue = [&](Slot& s) {
-    const int64_t row = row_lo + (static_cast<int64_t>(is_tile) * RW + rw) * 16 + g;
-    const int k0 = min((c_first + kw + is_chunk * KW) * 128 + t * 32, k_last), col = k0 >> (MX ? 5 : 4);
-    const int64_t r0 = min(row, row_hi - 1), r1 = min(row + 8, row_hi - 1);
-    const uint8_t* p0 = a.codes + r0 * half + (k0 >> 1);
-    const uint8_t* p1 = a.codes + r1 * half + (k0 >> 1);
+    if (is_unit >= u_hi) return;
+    const int at = min((c_first + is_chunk) * 4 + t, last);  // in 32 codes
     if constexpr (WIDE) {
-      s.w0 = load_stream16(p0);
-      s.w1 = load_stream16(p1);
+      s.w0 = load_stream16(code0 + at * 16);
+      s.w1 = load_stream16(code1 + at * 16);
     } else {
-      const int next = k0 + 16 < a.k ? 8 : 0;
-      const uint2 x0 = load_stream8(p0), y0 = load_stream8(p0 + next), x1 = load_stream8(p1), y1 = load_stream8(p1 + next);
+      const int next = at * 32 + 16 < a.k ? 8 : 0;
+      const uint2 x0 = load_stream8(code0 + at * 16), y0 = load_stream8(code0 + at * 16 + next);
+      const uint2 x1 = load_stream8(code1 + at * 16), y1 = load_stream8(code1 + at * 16 + next);
       s.w0 = make_uint4(x0.x, x0.y, y0.x, y0.y);
       s.w1 = make_uint4(x1.x, x1.y, y1.x, y1.y);
     }
-    s.s0 = scale_at(r0, col);
-    s.s1 = scale_at(r1, col);
-    if (++is_chunk >= mine) {
+    const int col = MX ? at : 2 * at, off = a.swizzle ? (col >> 2) * 512 + (col & 3) : col;
+    if constexpr (MX) {
+      s.s0 = __ldg(scale0 + off);
+      s.s1 = __ldg(scale1 + off);
+    } else if constexpr (WIDE) {  // col is even: both scales lie in one 4-column block
+      s.s0 = __ldg(reinterpret_cast<const uint16_t*>(scale0 + off));
+      s.s1 = __ldg(reinterpret_cast<const uint16_t*>(scale1 + off));
+    } else {
+      const int next = col + 1 < cols ? 1 : 0;
+      s.s0 = __ldg(scale0 + off) | static_cast<uint32_t>(__ldg(scale0 + off + next)) << 8;
+      s.s1 = __ldg(scale1 + off) | static_cast<uint32_t>(__ldg(scale1 + off + next)) << 8;
+    }
+    ++is_unit;
+    if (++is_chunk == c_count) {
       is_chunk = 0;
       ++is_tile;
+      point();
     }
   };
-  if (a.k > 0)
+  if (a.k > 0) {
 #pragma unroll
-  for (int i = 0; i < kGemvDepth; ++i) issue(slots[i]);
+    for (int i = 0; i < kGemvDepth; ++i) issue(slots[i]);
+  }
 
   // ---- x: the slice's largest finite value per token, then f16 terms in units of it. A lane reads
   // its 8 codes' worth of two MMAs (16 bytes) at unit (k % 32 / 8) * 4 + k % 128 / 32 of a chunk.
   {
     const int k_lo = c_first * 128, count = c_count * 16;  // groups of 8 values
-    for (int mt = warp; mt < tokens; mt += kGemvWarps) {
+    uint32_t* tops = reinterpret_cast<uint32_t*>(unit);
+    if (tid < COLS) tops[tid] = 0;
+    __syncthreads();
+    // eight warps share the tokens, or a token where there are fewer
+    const int per = tokens > 4 ? 1 : tokens > 2 ? 2 : tokens > 1 ? 4 : 8, step = per * 32;
+    const int first = warp % per * 32 + lane;
+    for (int mt = warp / per; mt < tokens; mt += kGemvWarps / per) {
       uint32_t top = 0;
-      for (int i = lane; i < count; i += 32) {
+#pragma unroll 4
+      for (int i = first; i < count; i += step) {
         const int k = k_lo + i * 8;
         if (k < a.k) {
           float v[8];
@@ -207,11 +234,16 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
         }
       }
       top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0 && top != 0) atomicMax(tops + mt, top);
+    }
+    __syncthreads();
+    for (int mt = warp / per; mt < tokens; mt += kGemvWarps / per) {
+      const uint32_t top = tops[mt];
       const int e = max(static_cast<int>(top >> 23) - 127, -100);
       const float up = top == 0 ? 1.0f : __uint_as_float((127u + 14u - e) << 23);
-      if (lane == 0) unit[mt] = 1.0f / up;
       uint8_t* row = smem + mt * pitch;
-      for (int i = lane; i < count; i += 32) {
+#pragma unroll 4
+      for (int i = first; i < count; i += step) {
         const int k = k_lo + i * 8;
         float v[8] = {};
         if (k < a.k) load8<T>(a.x, (m0 + mt) * a.ldx + k, v);
@@ -233,6 +265,11 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
         if constexpr (SPLIT) *reinterpret_cast<uint4*>(row + tokens * pitch + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
     }
+    __syncthreads();
+    if (tid < tokens) {
+      const uint32_t top = tops[tid];
+      unit[tid] = top == 0 ? 1.0f : 1.0f / __uint_as_float((127u + 14u - max(static_cast<int>(top >> 23) - 127, -100)) << 23);
+    }
   }
   __syncthreads();
 
@@ -249,6 +286,7 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
   // products of 128 codes, scaled by f16 pairs m0 / m1 (rows g, g + 8; first and second 16 codes)
   auto products = [&](const Slot& s, int chunk, const uint32_t (&f0)[2], const uint32_t (&f1)[2], float (&c)[NT][4]) {
     const uint32_t w0[4] = {s.w0.x, s.w0.y, s.w0.z, s.w0.w}, w1[4] = {s.w1.x, s.w1.y, s.w1.z, s.w1.w};
+    float c2[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // halves the chain of dependent products
 #pragma unroll
     for (int i = 0; i < 4; ++i) {  // 8 codes of each row: two MMAs
       const uint32_t a00 = mul_f16x2(e2m1_f16<0>(w0[i]), f0[i >> 1]), a01 = mul_f16x2(e2m1_f16<1>(w0[i]), f0[i >> 1]);
@@ -259,13 +297,17 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
       for (int j = 0; j < NT; ++j) {
         const uint4 b = *reinterpret_cast<const uint4*>(x_at[j] + chunk * 256 + i * 64);
         mma_m16n8k16(c[j], a00, a10, a01, a11, b.x, b.y);
-        mma_m16n8k16(c[j], a02, a12, a03, a13, b.z, b.w);
+        mma_m16n8k16(NT == 1 ? c2 : c[j], a02, a12, a03, a13, b.z, b.w);
         if constexpr (SPLIT) {
           const uint4 l = *reinterpret_cast<const uint4*>(x_at[j] + lo_at + chunk * 256 + i * 64);
           mma_m16n8k16(c[j], a00, a10, a01, a11, l.x, l.y);
-          mma_m16n8k16(c[j], a02, a12, a03, a13, l.z, l.w);
+          mma_m16n8k16(NT == 1 ? c2 : c[j], a02, a12, a03, a13, l.z, l.w);
         }
       }
+    }
+    if constexpr (NT == 1) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c[0][e] += c2[e];
     }
   };
   auto consume = [&](const Slot& s, int chunk) {
@@ -323,65 +365,89 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
     }
   };
 
-  // the sums of a tile: every warp's fragments to shared memory, then one thread per output
-  int done_chunks = 0, tile = 0;
-  auto finish_tile = [&]() {
-    float* buf = sums + (tile & 1) * kGemvWarps * 16 * COLS;
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      float* at = buf + (warp * 16 + g) * COLS + j * 8 + 2 * t;
-      *reinterpret_cast<float2*>(at) = make_float2(acc[j][0], acc[j][1]);
-      *reinterpret_cast<float2*>(at + 8 * COLS) = make_float2(acc[j][2], acc[j][3]);
-      acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
+  // one output of a tile: the final value, or one of its two partial sums
+  auto put = [&](int tile, int r, int mt, float y, int part) {
+    const int64_t row = static_cast<int64_t>(tile) * 16 + r;
+    if (row >= a.n || mt >= tokens) return;
+    y *= unit[mt] * a.ts[a.ts_per_row ? row : 0];
+    if (part < 0 && a.slices == 1) {
+      if (a.bias != nullptr) y += load_any(a.bias, a.bias_dtype, row);
+      store_any<T>(a.out, (m0 + mt) * a.ldo + row, y);
+    } else {
+      a.partial[((static_cast<int64_t>(max(part, 0)) * a.slices + slice) * a.m + m0 + mt) * a.n + row] = y;
     }
-    __syncthreads();  // the other buffer is free once every warp is here again
-    for (int i = tid; i < RW * 16 * tokens; i += kGemvThreads) {
-      const int r = i % (RW * 16), mt = i / (RW * 16);
-      const int64_t row = row_lo + static_cast<int64_t>(tile) * RW * 16 + r;
-      if (row < row_hi) {
-        const float* from = buf + (r >> 4) * KW * 16 * COLS + (r & 15) * COLS + mt;
-        float y = from[0];
-        for (int w = 1; w < KW; ++w) y += from[w * 16 * COLS];
-        y *= unit[mt] * a.ts[a.ts_per_row ? row : 0];
-        if (a.slices > 1) {
-          a.partial[(static_cast<int64_t>(slice) * a.m + m0 + mt) * a.n + row] = y;
-        } else {
-          if (a.bias != nullptr) y += load_any(a.bias, a.bias_dtype, row);
-          store_any<T>(a.out, (m0 + mt) * a.ldo + row, y);
-        }
-      }
-    }
-    ++tile;
   };
-  if (mine == 0) {  // no chunk of the slice is left for this warp: its sums are zeros
-    while (tile < tiles) finish_tile();
-    return;
-  }
-  const int total = tiles * mine;
-  for (int i0 = 0; i0 < total; i0 += kGemvDepth) {
+  int tile = u_lo / c_count, chunk = u_lo % c_count, begun = chunk;
+  auto end_segment = [&]() {
+    const bool ends = chunk == c_count - 1;
+    if (begun == 0 && ends) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) put(tile, g + 8 * (e >> 1), j * 8 + 2 * t + (e & 1), acc[j][e], -1);
+      }
+    } else {
+      const int seg = warp * 2 + (begun == 0);  // 0: the tile began before this warp, 1: it begins here
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        float* at = sums + (seg * 16 + g) * COLS + j * 8 + 2 * t;
+        *reinterpret_cast<float2*>(at) = make_float2(acc[j][0], acc[j][1]);
+        *reinterpret_cast<float2*>(at + 8 * COLS) = make_float2(acc[j][2], acc[j][3]);
+      }
+      if (lane == 0) seg_tile[seg] = 2 * tile + ends;
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
+    begun = 0;
+  };
+  for (int u = u_lo; u < u_hi; u += kGemvDepth) {
 #pragma unroll
     for (int i = 0; i < kGemvDepth; ++i) {
-      if (i0 + i < total) {
-        consume(slots[i], kw + done_chunks * KW);
+      if (u + i < u_hi) {
+        consume(slots[i], chunk);
         if (a.k > 0) issue(slots[i]);
-        if (++done_chunks == mine) {
-          done_chunks = 0;
-          finish_tile();
+        if (chunk == c_count - 1 || u + i == u_hi - 1) end_segment();
+        if (++chunk == c_count) {
+          chunk = 0;
+          ++tile;
         }
       }
     }
+  }
+  __syncthreads();
+  // the tiles that warps share: from where they begin in this block (a warp's second segment, or the
+  // first warp's first), through the following warps' first segments
+  for (int i = tid; i < (kGemvWarps + 1) * 16 * COLS; i += kGemvThreads) {
+    const int head = i / (16 * COLS), cell = i % (16 * COLS);
+    const int seg = head == 0 ? 0 : (head - 1) * 2 + 1, first = seg_tile[seg];
+    if (first < 0) continue;
+    float y = sums[seg * 16 * COLS + cell];
+    int end = first & 1;
+    for (int w = (seg >> 1) + 1; w < kGemvWarps && seg_tile[2 * w] >= 0 && seg_tile[2 * w] >> 1 == first >> 1; ++w) {
+      y += sums[2 * w * 16 * COLS + cell];
+      end = seg_tile[2 * w] & 1;
+    }
+    put(first >> 1, cell / COLS, cell % COLS, y, head == 0 ? 1 : end ? -1 : 0);
   }
 }
 
-// The slices' sums (each in units already undone and times the tensor scale), added in order.
+// The tiles that two blocks share and the slices of K, added in order (units and the tensor scale
+// are in the sums already).
 template <int T>
 __global__ void __launch_bounds__(256) gemv_join_kernel(GemvArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int row = blockIdx.x * 256 + threadIdx.x, mt = blockIdx.y;
+  const int row = blockIdx.x * 256 + threadIdx.x, mt = blockIdx.y, tile = row / 16;
   if (row >= a.n) return;
   float y = 0.0f;
-#pragma unroll 4
-  for (int s = 0; s < a.slices; ++s) y += __ldg(a.partial + (static_cast<int64_t>(s) * a.m + mt) * a.n + row);
+  for (int s = 0; s < a.slices; ++s) {
+    const int count = min(a.slice_chunks, a.chunks - s * a.slice_chunks);
+    const GemvCut cut(a.tiles * count, a.blocks);
+    const bool shared = cut.part_of(tile * count) != cut.part_of(tile * count + count - 1);
+    if (a.slices == 1 && !shared) return;
+    const float* at = a.partial + (static_cast<int64_t>(s) * a.m + mt) * a.n + row;
+    y += __ldg(at);
+    if (shared) y += __ldg(at + static_cast<int64_t>(a.slices) * a.m * a.n);
+  }
   if (a.bias != nullptr) y += load_any(a.bias, a.bias_dtype, row);
   store_any<T>(a.out, mt * a.ldo + row, y);
 }

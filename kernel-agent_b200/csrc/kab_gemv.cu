@@ -13,15 +13,17 @@ int gemv_check(int64_t m, int64_t n, int64_t k, int fmt, int dtype) {
   KAB_REQUIRE(valid_dtype(dtype), "unknown dtype %d", dtype);
   KAB_REQUIRE(m >= 0 && n >= 0 && k >= 0, "negative shape");
   KAB_REQUIRE(k % (fmt == KAB_NVFP4 ? 16 : 32) == 0, "K = %lld is not a multiple of the block", (long long)k);
+  KAB_REQUIRE((n + 15) / 16 * ((k + 127) / 128) < (int64_t(1) << 31), "problem too large");
   KAB_REQUIRE(m < (int64_t(1) << 18) && n < (int64_t(1) << 30) && k < (int64_t(1) << 30), "problem too large");
   return KAB_OK;
 }
 
 // How a shape is cut: slices of K so that a slice of x fits in shared memory beside a second block
-// (kXBytes), more of them where the rows alone cannot occupy the GPU, and blocks per slice.
+// (kXBytes), and blocks per slice.
 constexpr int kXBytes = 72 * 1024;
 struct GemvPlan {
-  int nt, tokens, chunks, slice_chunks, slices, k_warps, blocks;
+  int nt, tokens, chunks, slice_chunks, slices, tiles, blocks;
+  bool join;
   size_t partial;
 };
 GemvPlan gemv_plan(int64_t m, int64_t n, int64_t k, int dtype) {
@@ -31,14 +33,13 @@ GemvPlan gemv_plan(int64_t m, int64_t n, int64_t k, int dtype) {
   p.chunks = static_cast<int>(std::max<int64_t>(1, (k + 127) / 128));
   const int64_t per_chunk = static_cast<int64_t>(p.tokens) * 256 * (dtype == KAB_F32 ? 2 : 1);
   const int fit = static_cast<int>(std::max<int64_t>(1, kXBytes / per_chunk));
-  const int64_t tiles = (n + 15) / 16;
-  int want = (p.chunks + fit - 1) / fit;
+  const int want = (p.chunks + fit - 1) / fit;
   p.slice_chunks = (p.chunks + want - 1) / want;
   p.slices = (p.chunks + p.slice_chunks - 1) / p.slice_chunks;
-  p.k_warps = p.slice_chunks >= 8 ? 8 : p.slice_chunks >= 4 ? 4 : p.slice_chunks >= 2 ? 2 : 1;
-  const int64_t units = (tiles + kGemvWarps / p.k_warps - 1) / (kGemvWarps / p.k_warps);
-  p.blocks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(units, 2 * sm_count() / p.slices)));
-  p.partial = p.slices > 1 ? static_cast<size_t>(p.slices) * m * n * 4 : 0;
+  p.tiles = static_cast<int>((n + 15) / 16);
+  p.blocks = std::max(1, std::min(p.tiles, 2 * sm_count() / p.slices));
+  p.join = p.slices > 1 || p.tiles % p.blocks != 0;  // else every block has whole tiles
+  p.partial = p.join ? static_cast<size_t>(2) * p.slices * m * n * 4 : 0;
   return p;
 }
 
@@ -57,7 +58,7 @@ int launch_gemv(const GemvArgs& a, const GemvPlan& p, cudaStream_t s) {
   const dim3 grid(p.blocks, p.slices, (a.m + 8 * NT - 1) / (8 * NT));
   kern<<<grid, kGemvThreads, bytes, s>>>(a);
   if (int e = check_launch("kab_gemv_fp4")) return e;
-  if (p.slices == 1) return KAB_OK;
+  if (!p.join) return KAB_OK;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((a.n + 255) / 256, a.m);
   cfg.blockDim = dim3(256);
@@ -121,8 +122,8 @@ int kab_gemv_fp4(const void* x, int dtype, int64_t ldx, const uint8_t* codes, co
   a.ts = tensor_scale, a.ts_per_row = scale_per_row;
   a.m = static_cast<int>(m), a.n = static_cast<int>(n), a.k = static_cast<int>(k);
   a.bias = bias, a.bias_dtype = bias_dtype, a.out = out, a.ldo = ldo;
-  a.chunks = p.chunks, a.slice_chunks = p.slice_chunks, a.slices = p.slices, a.k_warps = p.k_warps;
-  a.blocks = p.blocks, a.partial = static_cast<float*>(workspace);
+  a.chunks = p.chunks, a.slice_chunks = p.slice_chunks, a.slices = p.slices;
+  a.tiles = p.tiles, a.blocks = p.blocks, a.partial = static_cast<float*>(workspace);
   const cudaStream_t s = as_stream(stream);
   if (dtype == KAB_BF16) return launch_gemv<kBF16>(a, p, fmt, s);
   if (dtype == KAB_F16) return launch_gemv<kF16>(a, p, fmt, s);
