@@ -10,12 +10,20 @@
 //    lane's share of eight consecutive MMAs; nothing is exchanged between lanes. (tcgen05 would want
 //    the scales in its own layout and M padded to its tile; at these M the tensor pipe is idle either
 //    way.)
-//  * e2m1 -> f16 is one exact conversion per two codes. An NVFP4 code times its e4m3 scale has at
-//    most 6 significant bits and lies in [2^-10, 2688]: exact in f16, one packed multiplication per
-//    two codes. An MXFP4 scale does not fit f16: the four 32-code blocks of a row's 128 codes are
-//    taken in units of the first one's scale where they lie within 2^-20 .. 2^13 of it (exact), and
-//    the 16 x 8 products of the 128 codes are added in fp32 with that scale; otherwise each block is
-//    taken by itself.
+//  * e2m1 -> f16 is one exact conversion per two codes. For few tokens (GROUPED) the scales never
+//    touch the codes: the MMA's 8 columns hold one token's blocks apart. A lane's 32 codes are the two
+//    NVFP4 blocks 2 t and 2 t + 1 of the 128 of the quad (or MXFP4's block t), and column n carries x
+//    only in the lane that owns block n, zeros elsewhere, so column n sums block n alone; one
+//    multiply-add per row and block then applies the scale in fp32, exactly for every scale. NVFP4
+//    fills the columns with one token, MXFP4 with two; more tokens take more MMAs on the same
+//    converted codes. (Scaling the codes costs 32 packed multiplications per chunk instead: 37 us
+//    against GROUPED's 29 for one token at 28672 x 8192.)
+//  * For more tokens the codes are scaled. An NVFP4 code times its e4m3 scale has at most 6
+//    significant bits and lies in [2^-10, 2688]: exact in f16, one packed multiplication per two
+//    codes. An MXFP4 scale does not fit f16: the four 32-code blocks of a row's 128 codes are taken in
+//    units of the first one's scale where they lie within 2^-20 .. 2^13 of it (exact), and the 16 x 8
+//    products of the 128 codes are added in fp32 with that scale; otherwise each block is taken by
+//    itself.
 //  * x enters as f16, each token (and K slice) in units of a power of two that puts its largest
 //    finite value in [2^14, 2^15): bf16 and f16 keep all their bits down to 2^-29 of it; fp32 is
 //    split into two f16 terms (22 bits) and multiplied twice. It is converted once per block and
@@ -122,25 +130,29 @@ constexpr int kGemvThreads = 256, kGemvWarps = 8, kGemvDepth = 4;
 // Bytes of one token's slice of x (hi terms, and lo terms for fp32): a multiple of 256 and 64 more,
 // so that the tokens of a group lie in different banks.
 __host__ __device__ constexpr int gemv_pitch(int slice_chunks) { return slice_chunks * 256 + 64; }
-__host__ __device__ constexpr int gemv_smem(int m, int slice_chunks, int nt, bool split) {
-  return m * gemv_pitch(slice_chunks) * (split ? 2 : 1) + 2 * kGemvWarps * 16 * 8 * nt * 4 + 8 * nt * 4 +
+__host__ __device__ constexpr int gemv_smem(int m, int slice_chunks, int columns, bool split) {
+  return m * gemv_pitch(slice_chunks) * (split ? 2 : 1) + 256 + 2 * kGemvWarps * 16 * columns * 4 + columns * 4 +
          2 * kGemvWarps * 4;
 }
 
 // ------------------------------------------------------------------ the kernel
 
-// MX: MXFP4 (e8m0 per 32), else NVFP4 (e4m3 per 16). NT: groups of 8 tokens. WIDE: rows of codes
+// Tokens that NT groups of the MMA's columns take.
+constexpr int gemv_columns(bool mx, int nt, bool grouped) { return grouped ? (mx ? 2 * nt : nt) : 8 * nt; }
+
+// MX: MXFP4 (e8m0 per 32), else NVFP4 (e4m3 per 16). NT: groups of 8 MMA columns. WIDE: rows of codes
 // start on 16 bytes (K a multiple of 32 and an aligned weight), else on 8.
-template <int T, int MX, int NT, int WIDE>
+template <int T, int MX, int NT, int WIDE, int GROUPED>
 __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
   constexpr bool SPLIT = T == kF32;
-  constexpr int COLS = 8 * NT;
+  constexpr int COLS = gemv_columns(MX, NT, GROUPED);
   extern __shared__ __align__(128) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int slice = blockIdx.y, m0 = blockIdx.z * COLS, tokens = min(COLS, a.m - m0);
   const int c_first = slice * a.slice_chunks, c_count = min(a.slice_chunks, a.chunks - c_first);
   const int pitch = gemv_pitch(a.slice_chunks);
-  float* sums = reinterpret_cast<float*>(smem + tokens * pitch * (SPLIT ? 2 : 1));  // [8 warps][2][16][COLS]
+  uint8_t* zeros = smem + tokens * pitch * (SPLIT ? 2 : 1);  // 256 bytes: what a column's other lanes read
+  float* sums = reinterpret_cast<float*>(zeros + 256);  // [8 warps][2][16][COLS]
   float* unit = sums + 2 * kGemvWarps * 16 * COLS;                                  // [COLS]
 
   int* seg_tile = reinterpret_cast<int*>(unit + COLS);  // [8 warps][2]: 2 * tile + (its end is here), or -1
@@ -152,6 +164,7 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
   const int u_lo = b_lo + warps.begin(warp), u_hi = b_lo + warps.begin(warp + 1);
   const int cols = a.k >> (MX ? 5 : 4), half = a.k >> 1;
   if (tid < 2 * kGemvWarps) seg_tile[tid] = -1;
+  if (tid < 16) reinterpret_cast<uint4*>(zeros)[tid] = make_uint4(0, 0, 0, 0);
 
   struct Slot {
     uint4 w0, w1;      // 32 codes of rows g and g + 8
@@ -273,33 +286,49 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
   }
   __syncthreads();
 
-  // columns past the tokens repeat the last one; nobody reads them
-  const uint8_t* x_at[NT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) x_at[j] = smem + min(j * 8 + g, tokens - 1) * pitch + t * 16;
   const int lo_at = tokens * pitch;
+  // where a lane reads column g of group j; `step`: 256 bytes per chunk, or none in the zeros. With
+  // NVFP4 blocks apart the lane's first block and its second have a column each.
+  constexpr int SIDES = GROUPED && !MX ? 2 : 1;
+  const uint8_t* x_at[NT][SIDES];
+  int x_step[NT][SIDES];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+#pragma unroll
+    for (int side = 0; side < SIDES; ++side) {
+      // columns past the tokens repeat the last one; nobody reads them
+      const int token = !GROUPED ? j * 8 + g : MX ? 2 * j + (g & 1) : j;
+      const bool here = !GROUPED || (MX ? t == g >> 1 : g == 2 * t + side);
+      x_at[j][side] = here ? smem + min(token, tokens - 1) * pitch + t * 16 : zeros;
+      x_step[j][side] = here ? 256 : 0;
+    }
+  }
 
   float acc[NT][4];
 #pragma unroll
   for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
 
-  // products of 128 codes, scaled by f16 pairs m0 / m1 (rows g, g + 8; first and second 16 codes)
+  // products of 128 codes, in GROUPED as they are, else scaled by f16 pairs f0 / f1 (rows g, g + 8;
+  // first and second 16 codes)
   auto products = [&](const Slot& s, int chunk, const uint32_t (&f0)[2], const uint32_t (&f1)[2], float (&c)[NT][4]) {
     const uint32_t w0[4] = {s.w0.x, s.w0.y, s.w0.z, s.w0.w}, w1[4] = {s.w1.x, s.w1.y, s.w1.z, s.w1.w};
-    float c2[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // halves the chain of dependent products
+    float c2[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // with one group: halves the chain of dependent products
+    auto scaled = [&](uint32_t v, uint32_t f) { return GROUPED ? v : mul_f16x2(v, f); };
 #pragma unroll
     for (int i = 0; i < 4; ++i) {  // 8 codes of each row: two MMAs
-      const uint32_t a00 = mul_f16x2(e2m1_f16<0>(w0[i]), f0[i >> 1]), a01 = mul_f16x2(e2m1_f16<1>(w0[i]), f0[i >> 1]);
-      const uint32_t a02 = mul_f16x2(e2m1_f16<2>(w0[i]), f0[i >> 1]), a03 = mul_f16x2(e2m1_f16<3>(w0[i]), f0[i >> 1]);
-      const uint32_t a10 = mul_f16x2(e2m1_f16<0>(w1[i]), f1[i >> 1]), a11 = mul_f16x2(e2m1_f16<1>(w1[i]), f1[i >> 1]);
-      const uint32_t a12 = mul_f16x2(e2m1_f16<2>(w1[i]), f1[i >> 1]), a13 = mul_f16x2(e2m1_f16<3>(w1[i]), f1[i >> 1]);
+      const uint32_t a00 = scaled(e2m1_f16<0>(w0[i]), f0[i >> 1]), a01 = scaled(e2m1_f16<1>(w0[i]), f0[i >> 1]);
+      const uint32_t a02 = scaled(e2m1_f16<2>(w0[i]), f0[i >> 1]), a03 = scaled(e2m1_f16<3>(w0[i]), f0[i >> 1]);
+      const uint32_t a10 = scaled(e2m1_f16<0>(w1[i]), f1[i >> 1]), a11 = scaled(e2m1_f16<1>(w1[i]), f1[i >> 1]);
+      const uint32_t a12 = scaled(e2m1_f16<2>(w1[i]), f1[i >> 1]), a13 = scaled(e2m1_f16<3>(w1[i]), f1[i >> 1]);
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        const uint4 b = *reinterpret_cast<const uint4*>(x_at[j] + chunk * 256 + i * 64);
+        const int side = SIDES == 2 ? i >> 1 : 0;
+        const uint8_t* at = x_at[j][side] + chunk * x_step[j][side] + i * 64;
+        const uint4 b = *reinterpret_cast<const uint4*>(at);
         mma_m16n8k16(c[j], a00, a10, a01, a11, b.x, b.y);
         mma_m16n8k16(NT == 1 ? c2 : c[j], a02, a12, a03, a13, b.z, b.w);
         if constexpr (SPLIT) {
-          const uint4 l = *reinterpret_cast<const uint4*>(x_at[j] + lo_at + chunk * 256 + i * 64);
+          const uint4 l = *reinterpret_cast<const uint4*>(x_step[j][side] ? at + lo_at : at);
           mma_m16n8k16(c[j], a00, a10, a01, a11, l.x, l.y);
           mma_m16n8k16(NT == 1 ? c2 : c[j], a02, a12, a03, a13, l.z, l.w);
         }
@@ -311,7 +340,35 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
     }
   };
   auto consume = [&](const Slot& s, int chunk) {
-    if constexpr (!MX) {
+    if constexpr (GROUPED) {
+      const uint32_t none[2] = {0, 0};
+      float c[NT][4];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.0f;
+      products(s, chunk, none, none, c);
+      if constexpr (MX) {  // columns 2 t and 2 t + 1: block t, two tokens
+        const float u0 = e8m0_value(static_cast<uint8_t>(s.s0)), u1 = e8m0_value(static_cast<uint8_t>(s.s1));
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          acc[j][0] = fmaf(c[j][0], u0, acc[j][0]);
+          acc[j][1] = fmaf(c[j][1], u0, acc[j][1]);
+          acc[j][2] = fmaf(c[j][2], u1, acc[j][2]);
+          acc[j][3] = fmaf(c[j][3], u1, acc[j][3]);
+        }
+      } else {  // columns 2 t and 2 t + 1: the lane's two blocks
+        const __half2_raw h0 = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(s.s0), __NV_E4M3);
+        const __half2_raw h1 = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(s.s1), __NV_E4M3);
+        const float2 u0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
+        const float2 u1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          acc[j][0] = fmaf(c[j][0], u0.x, acc[j][0]);
+          acc[j][1] = fmaf(c[j][1], u0.y, acc[j][1]);
+          acc[j][2] = fmaf(c[j][2], u1.x, acc[j][2]);
+          acc[j][3] = fmaf(c[j][3], u1.y, acc[j][3]);
+        }
+      }
+    } else if constexpr (!MX) {
       const __half2_raw h0 = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(s.s0), __NV_E4M3);
       const __half2_raw h1 = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(s.s1), __NV_E4M3);
       const uint32_t p0 = *reinterpret_cast<const uint32_t*>(&h0), p1 = *reinterpret_cast<const uint32_t*>(&h1);
@@ -379,25 +436,44 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
   };
   int tile = u_lo / c_count, chunk = u_lo % c_count, begun = chunk;
   auto end_segment = [&]() {
-    const bool ends = chunk == c_count - 1;
-    if (begun == 0 && ends) {
+    const bool ends = chunk == c_count - 1, whole = begun == 0 && ends;
+    const int seg = warp * 2 + (begun == 0);  // 0: the tile began before this warp, 1: it begins here
+    auto one = [&](int r, int mt, float y) {
+      if (whole) put(tile, r, mt, y, -1);
+      else sums[(seg * 16 + r) * COLS + mt] = y;
+    };
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
+    for (int j = 0; j < NT; ++j) {
+      if constexpr (GROUPED) {
+        // the blocks' sums meet: over the quad, and with NVFP4 over a lane's two blocks
+        float v[4] = {acc[j][0], acc[j][1], acc[j][2], acc[j][3]};
+        if constexpr (!MX) {
+          v[0] += v[1];
+          v[2] += v[3];
+        }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) put(tile, g + 8 * (e >> 1), j * 8 + 2 * t + (e & 1), acc[j][e], -1);
+        for (int e = 0; e < 4; ++e) {
+          v[e] += __shfl_xor_sync(0xffffffffu, v[e], 1);
+          v[e] += __shfl_xor_sync(0xffffffffu, v[e], 2);
+        }
+        if (t == 0) {
+          if constexpr (MX) {
+            one(g, 2 * j, v[0]);
+            one(g, 2 * j + 1, v[1]);
+            one(g + 8, 2 * j, v[2]);
+            one(g + 8, 2 * j + 1, v[3]);
+          } else {
+            one(g, j, v[0]);
+            one(g + 8, j, v[2]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) one(g + 8 * (e >> 1), j * 8 + 2 * t + (e & 1), acc[j][e]);
       }
-    } else {
-      const int seg = warp * 2 + (begun == 0);  // 0: the tile began before this warp, 1: it begins here
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        float* at = sums + (seg * 16 + g) * COLS + j * 8 + 2 * t;
-        *reinterpret_cast<float2*>(at) = make_float2(acc[j][0], acc[j][1]);
-        *reinterpret_cast<float2*>(at + 8 * COLS) = make_float2(acc[j][2], acc[j][3]);
-      }
-      if (lane == 0) seg_tile[seg] = 2 * tile + ends;
+      acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
     }
-#pragma unroll
-    for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
+    if (!whole && lane == 0) seg_tile[seg] = 2 * tile + ends;
     begun = 0;
   };
   for (int u = u_lo; u < u_hi; u += kGemvDepth) {

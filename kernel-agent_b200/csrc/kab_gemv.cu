@@ -22,14 +22,21 @@ int gemv_check(int64_t m, int64_t n, int64_t k, int fmt, int dtype) {
 // (kXBytes), and blocks per slice.
 constexpr int kXBytes = 72 * 1024;
 struct GemvPlan {
-  int nt, tokens, chunks, slice_chunks, slices, tiles, blocks;
+  bool grouped;
+  int nt, columns, tokens, chunks, slice_chunks, slices, tiles, blocks;
   bool join;
   size_t partial;
 };
-GemvPlan gemv_plan(int64_t m, int64_t n, int64_t k, int dtype) {
+// Blocks apart (GROUPED) while its MMAs (8 per chunk and group) stay below the stream's time: one or
+// two tokens of NVFP4, up to eight of MXFP4 (half of that in fp32, whose x has two terms).
+GemvPlan gemv_plan(int64_t m, int64_t n, int64_t k, int fmt, int dtype) {
   GemvPlan p{};
-  p.nt = m <= 8 ? 1 : m <= 16 ? 2 : 4;
-  p.tokens = static_cast<int>(std::min<int64_t>(m, 8 * p.nt));
+  const bool mx = fmt == KAB_MXFP4;
+  const int most = (mx ? 8 : 2) / (dtype == KAB_F32 ? 2 : 1);
+  p.grouped = m <= most;
+  p.nt = p.grouped ? (mx ? (m <= 2 ? 1 : m <= 4 ? 2 : 4) : static_cast<int>(m)) : m <= 8 ? 1 : m <= 16 ? 2 : 4;
+  p.columns = gemv_columns(mx, p.nt, p.grouped);
+  p.tokens = static_cast<int>(std::min<int64_t>(m, p.columns));
   p.chunks = static_cast<int>(std::max<int64_t>(1, (k + 127) / 128));
   const int64_t per_chunk = static_cast<int64_t>(p.tokens) * 256 * (dtype == KAB_F32 ? 2 : 1);
   const int fit = static_cast<int>(std::max<int64_t>(1, kXBytes / per_chunk));
@@ -43,10 +50,10 @@ GemvPlan gemv_plan(int64_t m, int64_t n, int64_t k, int dtype) {
   return p;
 }
 
-template <int T, int MX, int NT, int WIDE>
+template <int T, int MX, int NT, int WIDE, int GROUPED>
 int launch_gemv(const GemvArgs& a, const GemvPlan& p, cudaStream_t s) {
-  auto kern = gemv_fp4_kernel<T, MX, NT, WIDE>;
-  const int bytes = gemv_smem(p.tokens, p.slice_chunks, NT, T == kF32);
+  auto kern = gemv_fp4_kernel<T, MX, NT, WIDE, GROUPED>;
+  const int bytes = gemv_smem(p.tokens, p.slice_chunks, p.columns, T == kF32);
   static bool configured[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(KAB_ECUDA, "no current device");
@@ -55,7 +62,7 @@ int launch_gemv(const GemvArgs& a, const GemvPlan& p, cudaStream_t s) {
       return fail(KAB_ECUDA, "cannot configure the FP4 linear");
     configured[dev] = true;
   }
-  const dim3 grid(p.blocks, p.slices, (a.m + 8 * NT - 1) / (8 * NT));
+  const dim3 grid(p.blocks, p.slices, (a.m + p.columns - 1) / p.columns);
   kern<<<grid, kGemvThreads, bytes, s>>>(a);
   if (int e = check_launch("kab_gemv_fp4")) return e;
   if (!p.join) return KAB_OK;
@@ -71,15 +78,23 @@ int launch_gemv(const GemvArgs& a, const GemvPlan& p, cudaStream_t s) {
   cudaLaunchKernelEx(&cfg, gemv_join_kernel<T>, a);
   return check_launch("kab_gemv_fp4 join");
 }
-template <int T, int MX, int NT>
+template <int T, int MX, int NT, int GROUPED>
 int launch_gemv(const GemvArgs& a, const GemvPlan& p, cudaStream_t s) {
   const bool wide = a.k % 32 == 0 && aligned(a.codes, 16) && aligned(a.scales, 2);
-  return wide ? launch_gemv<T, MX, NT, 1>(a, p, s) : launch_gemv<T, MX, NT, 0>(a, p, s);
+  return wide ? launch_gemv<T, MX, NT, 1, GROUPED>(a, p, s) : launch_gemv<T, MX, NT, 0, GROUPED>(a, p, s);
 }
 template <int T, int MX>
 int launch_gemv(const GemvArgs& a, const GemvPlan& p, cudaStream_t s) {
-  return p.nt == 1 ? launch_gemv<T, MX, 1>(a, p, s) : p.nt == 2 ? launch_gemv<T, MX, 2>(a, p, s)
-                                                                : launch_gemv<T, MX, 4>(a, p, s);
+  if (p.grouped) {
+    if (p.nt == 1) return launch_gemv<T, MX, 1, 1>(a, p, s);
+    if constexpr (MX || T != kF32) {
+      if (p.nt == 2) return launch_gemv<T, MX, 2, 1>(a, p, s);
+    }
+    if constexpr (MX && T != kF32) return launch_gemv<T, MX, 4, 1>(a, p, s);
+    return fail(KAB_EUNSUPPORTED, "no kernel for this plan");
+  }
+  return p.nt == 1 ? launch_gemv<T, MX, 1, 0>(a, p, s) : p.nt == 2 ? launch_gemv<T, MX, 2, 0>(a, p, s)
+                                                                   : launch_gemv<T, MX, 4, 0>(a, p, s);
 }
 template <int T>
 int launch_gemv(const GemvArgs& a, const GemvPlan& p, int fmt, cudaStream_t s) {
@@ -97,7 +112,7 @@ int kab_gemv_fp4_workspace(int64_t m, int64_t n, int64_t k, int fmt, int dtype, 
                            size_t* zero_bytes) {
   if (int e = gemv_check(m, n, k, fmt, dtype)) return e;
   KAB_REQUIRE(bytes != nullptr && zero_bytes != nullptr, "null pointer");
-  *bytes = m == 0 || n == 0 ? 0 : gemv_plan(m, n, k, dtype).partial;
+  *bytes = m == 0 || n == 0 ? 0 : gemv_plan(m, n, k, fmt, dtype).partial;
   *zero_bytes = 0;
   return KAB_OK;
 }
@@ -114,7 +129,7 @@ int kab_gemv_fp4(const void* x, int dtype, int64_t ldx, const uint8_t* codes, co
   KAB_REQUIRE(aligned(codes, 8), "codes must be 8-byte aligned");
   KAB_REQUIRE(!swizzle || aligned(scales, 4), "swizzled scales must be 4-byte aligned");
   KAB_REQUIRE(ldo >= n && ldx >= k, "ldx %lld or ldo %lld is too short", (long long)ldx, (long long)ldo);
-  const GemvPlan p = gemv_plan(m, n, k, dtype);
+  const GemvPlan p = gemv_plan(m, n, k, fmt, dtype);
   KAB_REQUIRE(p.partial == 0 || (workspace != nullptr && workspace_bytes >= p.partial && aligned(workspace, 256)),
               "the workspace needs %zu bytes, 256-byte aligned (kab_gemv_fp4_workspace)", p.partial);
   GemvArgs a{};
