@@ -26,14 +26,16 @@
 //    itself.
 //  * x enters as f16, each token (and K slice) in units of a power of two that puts its largest
 //    finite value in [2^14, 2^15): bf16 and f16 keep all their bits down to 2^-29 of it; fp32 is
-//    split into two f16 terms (22 bits) and multiplied twice. It is converted once per block and
-//    stays in shared memory while the block streams its rows.
-//  * The (16-row tile, 128-code chunk) pairs of a K slice stand in one line, cut into equal parts for
-//    the blocks and again for their warps: every warp streams its part with kGemvDepth chunks in
-//    flight in registers and waits for nobody. Tiles that lie within a warp are written by it; those
-//    that several warps of a block share are added in shared memory at the end, those that two
-//    blocks share (and the slices of K, where x does not fit in shared memory) in a second launch.
-//    Always in the order of the line.
+//    split into two f16 terms (22 bits) and multiplied twice. It stays in shared memory while a block
+//    streams its rows, converted there for one token, by a launch before for more.
+//  * The (32-row tile, 256-code chunk) pairs of a K slice stand in one line, cut into equal parts for
+//    the blocks and again for their warps: every warp streams its part through a ring of its own in
+//    shared memory (cp.async, whole 128-byte lines of a row) and waits for nobody. 32 rows share one
+//    read of x, and lines in place of 64-byte pieces keep L1's data pipe, which bounded the kernel
+//    before (66 % busy at 3.9 TB/s), below the stream. Tiles that lie within a warp are written by it;
+//    those that several warps of a block share are added in shared memory at the end, those that two
+//    blocks share (and the slices of K, where x does not fit in shared memory) in another launch,
+//    always in the order of the line.
 #pragma once
 
 #include "codes.cuh"
@@ -53,9 +55,11 @@ struct GemvArgs {
   int bias_dtype;
   void* out;
   int64_t ldo;
-  int chunks, slice_chunks, slices;  // 128-code chunks of K, of a slice of it, and slices
-  int tiles, blocks;                 // 16-row tiles; blocks per slice
+  int chunks, slice_chunks, slices;  // 256-code chunks of K, of a slice of it, and slices
+  int tiles, blocks;                 // 32-row tiles; blocks per slice
   float* partial;                    // [2, slices, m, n]: a tile's sum or its first part, and its second part
+  uint8_t* x_terms;                  // [slices, m, 1 or 2 terms, slice_chunks * 512]: x as f16, or NULL
+  float* x_units;                    // [slices, m]
 };
 
 // The line of `total` units cut into `parts`: the first total % parts take one more.
@@ -98,16 +102,14 @@ __device__ __forceinline__ void mma_m16n8k16(float (&c)[4], uint32_t a0, uint32_
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint4 load_stream16(const uint8_t* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
+template <int BYTES>
+__device__ __forceinline__ void gemv_copy(uint32_t dst, const void* src) {
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
-__device__ __forceinline__ uint2 load_stream8(const uint8_t* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+__device__ __forceinline__ uint4 load_shared16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
   return v;
 }
 
@@ -125,37 +127,108 @@ __device__ __forceinline__ void store_any(void* p, int64_t i, float v) {
 
 // ------------------------------------------------------------------ layout
 
-constexpr int kGemvThreads = 256, kGemvWarps = 8, kGemvDepth = 4;
+constexpr int kGemvThreads = 256, kGemvWarps = 8, kGemvRows = 32, kGemvCodes = 256;
+// A warp's ring: 32 rows x 128 bytes of codes, and for each row the 4-byte words that hold its scales
+// of these codes (one word more than needed where they do not start on 4 bytes).
+constexpr int kGemvStages = 2;
+__host__ __device__ constexpr int gemv_scale_pitch(bool mx) { return mx ? 12 : 20; }
+__host__ __device__ constexpr int gemv_stage_bytes(bool mx) { return kGemvRows * (128 + gemv_scale_pitch(mx)); }
 
-// Bytes of one token's slice of x (hi terms, and lo terms for fp32): a multiple of 256 and 64 more,
+// Bytes of one token's slice of x (hi terms, and lo terms for fp32): a multiple of 512 and 64 more,
 // so that the tokens of a group lie in different banks.
-__host__ __device__ constexpr int gemv_pitch(int slice_chunks) { return slice_chunks * 256 + 64; }
-__host__ __device__ constexpr int gemv_smem(int m, int slice_chunks, int columns, bool split) {
-  return m * gemv_pitch(slice_chunks) * (split ? 2 : 1) + 256 + 2 * kGemvWarps * 16 * columns * 4 + columns * 4 +
-         2 * kGemvWarps * 4;
+__host__ __device__ constexpr int gemv_pitch(int slice_chunks) { return slice_chunks * 512 + 64; }
+__host__ __device__ constexpr int gemv_smem(bool mx, int m, int slice_chunks, int columns, bool split) {
+  return kGemvWarps * kGemvStages * gemv_stage_bytes(mx) + m * gemv_pitch(slice_chunks) * (split ? 2 : 1) + 256 +
+         2 * kGemvWarps * kGemvRows * columns * 4 + columns * 4 + 2 * kGemvWarps * 4;
+}
+// Tokens that NT groups of the MMA's columns take.
+constexpr int gemv_columns(bool mx, int nt, bool grouped) { return grouped ? (mx ? 2 * nt : nt) : 8 * nt; }
+
+// ------------------------------------------------------------------ x as f16
+
+// The largest finite value's bits -> the power of two that puts it in [2^14, 2^15).
+__device__ __forceinline__ float gemv_up(uint32_t top) {
+  return top == 0 ? 1.0f : __uint_as_float((127u + 14u - max(static_cast<int>(top >> 23) - 127, -100)) << 23);
+}
+template <int T>
+__device__ __forceinline__ uint32_t gemv_top8(const GemvArgs& a, int64_t row, int k, uint32_t top) {
+  if (k >= a.k) return top;
+  float v[8];
+  load8<T>(a.x, row * a.ldx + k, v);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t b = __float_as_uint(v[e]) & 0x7FFFFFFFu;
+    top = max(top, b < 0x7F800000u ? b : 0u);
+  }
+  return top;
+}
+// Eight values (the i-th eight of a slice) as f16 terms, at their place: a lane reads its 8 codes'
+// worth of two MMAs (16 bytes) at unit (k % 32 / 8) * 4 + k % 128 / 32 of each 128 values.
+template <int T>
+__device__ __forceinline__ void gemv_convert8(const GemvArgs& a, int64_t row, int k, float up, int i, uint8_t* hi_to,
+                                              uint8_t* lo_to) {
+  float v[8] = {};
+  if (k < a.k) load8<T>(a.x, row * a.ldx + k, v);
+  uint32_t hi[4], lo[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float x0 = v[2 * e] * up, x1 = v[2 * e + 1] * up;
+    const __half2 h = __floats2half2_rn(x0, x1);
+    hi[e] = *reinterpret_cast<const uint32_t*>(&h);
+    if constexpr (T == kF32) {
+      const float2 f = __half22float2(h);
+      // an infinity has no second term
+      const __half2 l = __floats2half2_rn(isinf(f.x) ? 0.0f : x0 - f.x, isinf(f.y) ? 0.0f : x1 - f.y);
+      lo[e] = *reinterpret_cast<const uint32_t*>(&l);
+    }
+  }
+  const int at = (i >> 4) * 256 + ((i & 3) * 4 + ((i >> 2) & 3)) * 16;
+  *reinterpret_cast<uint4*>(hi_to + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+  if constexpr (T == kF32) *reinterpret_cast<uint4*>(lo_to + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+}
+
+// One block per slice and token: x's terms and unit for every block of the product.
+template <int T>
+__global__ void __launch_bounds__(256) gemv_x_kernel(GemvArgs a) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  __shared__ uint32_t red[8];
+  const int slice = blockIdx.x, mt = blockIdx.y, tid = threadIdx.x;
+  const int k_lo = slice * a.slice_chunks * kGemvCodes, count = a.slice_chunks * (kGemvCodes / 8);
+  uint32_t top = 0;
+#pragma unroll 8
+  for (int i = tid; i < count; i += 256) top = gemv_top8<T>(a, mt, k_lo + i * 8, top);
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((tid & 31) == 0) red[tid >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) top = max(top, red[w]);
+  const float up = gemv_up(top);
+  const int64_t at = static_cast<int64_t>(slice) * a.m + mt, bytes = a.slice_chunks * 512;
+  uint8_t* hi = a.x_terms + at * bytes * (T == kF32 ? 2 : 1);
+#pragma unroll 4
+  for (int i = tid; i < count; i += 256) gemv_convert8<T>(a, mt, k_lo + i * 8, up, i, hi, hi + bytes);
+  if (tid == 0) a.x_units[at] = 1.0f / up;
 }
 
 // ------------------------------------------------------------------ the kernel
 
-// Tokens that NT groups of the MMA's columns take.
-constexpr int gemv_columns(bool mx, int nt, bool grouped) { return grouped ? (mx ? 2 * nt : nt) : 8 * nt; }
-
 // MX: MXFP4 (e8m0 per 32), else NVFP4 (e4m3 per 16). NT: groups of 8 MMA columns. WIDE: rows of codes
-// start on 16 bytes (K a multiple of 32 and an aligned weight), else on 8.
+// start on 16 bytes and rows of scales on 4 (K a multiple of 64 for NVFP4, 128 for MXFP4, and an aligned
+// weight), else on 8 and 1.
 template <int T, int MX, int NT, int WIDE, int GROUPED>
 __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
   constexpr bool SPLIT = T == kF32;
-  constexpr int COLS = gemv_columns(MX, NT, GROUPED);
-  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int COLS = gemv_columns(MX, NT, GROUPED), STAGE = gemv_stage_bytes(MX), SPITCH = gemv_scale_pitch(MX);
+  extern __shared__ __align__(128) uint8_t smem_all[];
+  uint8_t* smem = smem_all + kGemvWarps * kGemvStages * STAGE;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int slice = blockIdx.y, m0 = blockIdx.z * COLS, tokens = min(COLS, a.m - m0);
   const int c_first = slice * a.slice_chunks, c_count = min(a.slice_chunks, a.chunks - c_first);
   const int pitch = gemv_pitch(a.slice_chunks);
   uint8_t* zeros = smem + tokens * pitch * (SPLIT ? 2 : 1);  // 256 bytes: what a column's other lanes read
-  float* sums = reinterpret_cast<float*>(zeros + 256);  // [8 warps][2][16][COLS]
-  float* unit = sums + 2 * kGemvWarps * 16 * COLS;                                  // [COLS]
-
-  int* seg_tile = reinterpret_cast<int*>(unit + COLS);  // [8 warps][2]: 2 * tile + (its end is here), or -1
+  float* sums = reinterpret_cast<float*>(zeros + 256);       // [8 warps][2][32][COLS]
+  float* unit = sums + 2 * kGemvWarps * kGemvRows * COLS;    // [COLS]
+  int* seg_tile = reinterpret_cast<int*>(unit + COLS);       // [8 warps][2]: 2 * tile + (its end is here), or -1
 
   // ---- this warp's part of the line
   const GemvCut cut(a.tiles * c_count, a.blocks);
@@ -166,131 +239,104 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
   if (tid < 2 * kGemvWarps) seg_tile[tid] = -1;
   if (tid < 16) reinterpret_cast<uint4*>(zeros)[tid] = make_uint4(0, 0, 0, 0);
 
-  struct Slot {
-    uint4 w0, w1;      // 32 codes of rows g and g + 8
-    uint32_t s0, s1;   // their scales: two e4m3 bytes, or one e8m0
-  };
-  Slot slots[kGemvDepth] = {};
   int is_unit = u_lo, is_tile = u_lo / c_count, is_chunk = u_lo % c_count;  // what the next issue loads
-  const uint8_t *code0, *code1, *scale0, *scale1;  // the tile's rows g and g + 8
-  auto point = [&]() {
-    const int r0 = min(is_tile * 16 + g, a.n - 1), r1 = min(is_tile * 16 + g + 8, a.n - 1);
-    code0 = a.codes + static_cast<int64_t>(r0) * half;
-    code1 = a.codes + static_cast<int64_t>(r1) * half;
-    scale0 = a.scales + (a.swizzle ? scale_offset_swizzled(r0, 0, cols) : static_cast<int64_t>(r0) * cols);
-    scale1 = a.scales + (a.swizzle ? scale_offset_swizzled(r1, 0, cols) : static_cast<int64_t>(r1) * cols);
-  };
-  point();
-  // Every load is made, at the nearest place that exists: rows past n are not written, and x is zero
-  // past K. (Loads under conditions were waited for at once: 98 us against 53 at 1 x 28672 x 8192.)
-  const int last = max(0, (a.k - 1) / 32);  // the last 32 codes (or 16) of a row
-  auto issue = [&](Slot& s) {
-    if (is_unit >= u_hi) return;
-    const int at = min((c_first + is_chunk) * 4 + t, last);  // in 32 codes
-    if constexpr (WIDE) {
-      s.w0 = load_stream16(code0 + at * 16);
-      s.w1 = load_stream16(code1 + at * 16);
-    } else {
-      const int next = at * 32 + 16 < a.k ? 8 : 0;
-      const uint2 x0 = load_stream8(code0 + at * 16), y0 = load_stream8(code0 + at * 16 + next);
-      const uint2 x1 = load_stream8(code1 + at * 16), y1 = load_stream8(code1 + at * 16 + next);
-      s.w0 = make_uint4(x0.x, x0.y, y0.x, y0.y);
-      s.w1 = make_uint4(x1.x, x1.y, y1.x, y1.y);
-    }
-    const int col = MX ? at : 2 * at, off = a.swizzle ? (col >> 2) * 512 + (col & 3) : col;
-    if constexpr (MX) {
-      s.s0 = __ldg(scale0 + off);
-      s.s1 = __ldg(scale1 + off);
-    } else if constexpr (WIDE) {  // col is even: both scales lie in one 4-column block
-      s.s0 = __ldg(reinterpret_cast<const uint16_t*>(scale0 + off));
-      s.s1 = __ldg(reinterpret_cast<const uint16_t*>(scale1 + off));
-    } else {
-      const int next = col + 1 < cols ? 1 : 0;
-      s.s0 = __ldg(scale0 + off) | static_cast<uint32_t>(__ldg(scale0 + off + next)) << 8;
-      s.s1 = __ldg(scale1 + off) | static_cast<uint32_t>(__ldg(scale1 + off + next)) << 8;
-    }
-    ++is_unit;
-    if (++is_chunk == c_count) {
-      is_chunk = 0;
-      ++is_tile;
-      point();
-    }
-  };
-  if (a.k > 0) {
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem_all)) + warp * kGemvStages * STAGE;
+  const int64_t scale_bytes = static_cast<int64_t>(a.n) * cols;
+  // A quarter of a row's 16-byte pieces change places on odd rows, so that the fragments' reads (two
+  // neighbouring rows x four pieces) touch all banks. Every copy is made at the nearest place that
+  // exists: rows past n are not written, and x is zero past K.
+  auto issue = [&](int stage) {
+    if (is_unit < u_hi) {
+      const uint32_t to = ring + stage * STAGE;
+      const int chunk = c_first + is_chunk, row0 = is_tile * kGemvRows;
+      {
+        const int piece = lane & 7, byte = min(chunk * 128 + piece * 16, (half - 1) & ~15);
 #pragma unroll
-    for (int i = 0; i < kGemvDepth; ++i) issue(slots[i]);
-  }
-
-  // ---- x: the slice's largest finite value per token, then f16 terms in units of it. A lane reads
-  // its 8 codes' worth of two MMAs (16 bytes) at unit (k % 32 / 8) * 4 + k % 128 / 32 of a chunk.
-  {
-    const int k_lo = c_first * 128, count = c_count * 16;  // groups of 8 values
-    uint32_t* tops = reinterpret_cast<uint32_t*>(unit);
-    if (tid < COLS) tops[tid] = 0;
-    __syncthreads();
-    // eight warps share the tokens, or a token where there are fewer
-    const int per = tokens > 4 ? 1 : tokens > 2 ? 2 : tokens > 1 ? 4 : 8, step = per * 32;
-    const int first = warp % per * 32 + lane;
-    for (int mt = warp / per; mt < tokens; mt += kGemvWarps / per) {
-      uint32_t top = 0;
-#pragma unroll 4
-      for (int i = first; i < count; i += step) {
-        const int k = k_lo + i * 8;
-        if (k < a.k) {
-          float v[8];
-          load8<T>(a.x, (m0 + mt) * a.ldx + k, v);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint32_t b = __float_as_uint(v[e]) & 0x7FFFFFFFu;
-            top = max(top, b < 0x7F800000u ? b : 0u);
+        for (int i = 0; i < 8; ++i) {
+          const int r = i * 4 + (lane >> 3);
+          const uint8_t* from = a.codes + static_cast<int64_t>(min(row0 + r, a.n - 1)) * half + byte;
+          const uint32_t at = to + r * 128 + ((piece ^ ((r & 1) << 2)) << 4);
+          if constexpr (WIDE) {
+            gemv_copy<16>(at, from);
+          } else {
+            gemv_copy<8>(at, from);
+            gemv_copy<8>(at + 8, byte + 8 < half ? from + 8 : from);
           }
         }
       }
+      constexpr int WORDS = (MX ? 2 : 4) + (WIDE ? 0 : 1);  // per row
+      const int col0 = chunk * (MX ? 8 : 16);
+#pragma unroll
+      for (int i = 0; i < (kGemvRows * WORDS + 31) / 32; ++i) {
+        const int item = i * 32 + lane, r = item / WORDS, w = item % WORDS;
+        const int row = min(row0 + r, a.n - 1);
+        const uint32_t at = to + kGemvRows * 128 + r * SPITCH + w * 4;
+        if (a.swizzle) {
+          const int col = min(col0 + w * 4, (cols - 1) & ~3);
+          gemv_copy<4>(at, a.scales + scale_offset_swizzled(row, col, cols));
+        } else if constexpr (WIDE) {
+          gemv_copy<4>(at, a.scales + static_cast<int64_t>(row) * cols + min(col0 + w * 4, cols - 4));
+        } else {
+          // the aligned words around the row's scales; the weight's last word may be short
+          const int64_t word = (static_cast<int64_t>(row) * cols + col0) / 4 * 4 + w * 4;
+          const int64_t there = min(word, (scale_bytes - 1) / 4 * 4);
+          const int bytes = static_cast<int>(min(static_cast<int64_t>(4), scale_bytes - there));
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(at), "l"(a.scales + there), "r"(bytes) : "memory");
+        }
+      }
+      ++is_unit;
+      if (++is_chunk == c_count) {
+        is_chunk = 0;
+        ++is_tile;
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if (a.k > 0) {
+#pragma unroll
+    for (int i = 0; i < kGemvStages - 1; ++i) issue(i);
+  }
+
+  // ---- x: from the launch before, or converted here
+  if (a.x_terms != nullptr) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int bytes = a.slice_chunks * 512, pieces = bytes / 16, terms = SPLIT ? 2 : 1;
+    for (int i = tid; i < tokens * terms * pieces; i += kGemvThreads) {
+      const int row = i / pieces, piece = i % pieces, mt = row / terms, term = row % terms;
+      const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(smem + (term * tokens + mt) * pitch + piece * 16));
+      gemv_copy<16>(at, a.x_terms + ((static_cast<int64_t>(slice) * a.m + m0 + mt) * terms + term) * bytes + piece * 16);
+    }
+    asm volatile("cp.async.commit_group;\n cp.async.wait_group 0;" ::: "memory");
+    if (tid < tokens) unit[tid] = __ldg(a.x_units + static_cast<int64_t>(slice) * a.m + m0 + tid);
+  } else {
+    const int k_lo = c_first * kGemvCodes, count = c_count * (kGemvCodes / 8);
+    uint32_t* tops = reinterpret_cast<uint32_t*>(unit);
+    if (tid < COLS) tops[tid] = 0;
+    __syncthreads();
+    for (int mt = 0; mt < tokens; ++mt) {
+      uint32_t top = 0;
+#pragma unroll 4
+      for (int i = tid; i < count; i += kGemvThreads) top = gemv_top8<T>(a, m0 + mt, k_lo + i * 8, top);
       top = __reduce_max_sync(0xffffffffu, top);
       if (lane == 0 && top != 0) atomicMax(tops + mt, top);
     }
     __syncthreads();
-    for (int mt = warp / per; mt < tokens; mt += kGemvWarps / per) {
-      const uint32_t top = tops[mt];
-      const int e = max(static_cast<int>(top >> 23) - 127, -100);
-      const float up = top == 0 ? 1.0f : __uint_as_float((127u + 14u - e) << 23);
-      uint8_t* row = smem + mt * pitch;
+    for (int mt = 0; mt < tokens; ++mt) {
+      const float up = gemv_up(tops[mt]);
 #pragma unroll 4
-      for (int i = first; i < count; i += step) {
-        const int k = k_lo + i * 8;
-        float v[8] = {};
-        if (k < a.k) load8<T>(a.x, (m0 + mt) * a.ldx + k, v);
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int e2 = 0; e2 < 4; ++e2) {
-          const __half2 h = __floats2half2_rn(v[2 * e2] * up, v[2 * e2 + 1] * up);
-          hi[e2] = *reinterpret_cast<const uint32_t*>(&h);
-          if constexpr (SPLIT) {
-            const float2 f = __half22float2(h);
-            // an infinity has no second term
-            const __half2 l = __floats2half2_rn(isinf(f.x) ? 0.0f : v[2 * e2] * up - f.x,
-                                                isinf(f.y) ? 0.0f : v[2 * e2 + 1] * up - f.y);
-            lo[e2] = *reinterpret_cast<const uint32_t*>(&l);
-          }
-        }
-        const int at = (i >> 4) * 256 + ((i & 3) * 4 + ((i >> 2) & 3)) * 16;
-        *reinterpret_cast<uint4*>(row + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if constexpr (SPLIT) *reinterpret_cast<uint4*>(row + tokens * pitch + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-      }
+      for (int i = tid; i < count; i += kGemvThreads)
+        gemv_convert8<T>(a, m0 + mt, k_lo + i * 8, up, i, smem + mt * pitch, smem + (tokens + mt) * pitch);
     }
     __syncthreads();
-    if (tid < tokens) {
-      const uint32_t top = tops[tid];
-      unit[tid] = top == 0 ? 1.0f : 1.0f / __uint_as_float((127u + 14u - max(static_cast<int>(top >> 23) - 127, -100)) << 23);
-    }
+    if (tid < tokens) unit[tid] = 1.0f / gemv_up(tops[tid]);
   }
   __syncthreads();
 
   const int lo_at = tokens * pitch;
-  // where a lane reads column g of group j; `step`: 256 bytes per chunk, or none in the zeros. With
+  // where a lane reads column g of group j; `step`: 256 bytes per 128 codes, or none in the zeros. With
   // NVFP4 blocks apart the lane's first block and its second have a column each.
   constexpr int SIDES = GROUPED && !MX ? 2 : 1;
-  const uint8_t* x_at[NT][SIDES];
+  uint32_t x_at[NT][SIDES];
   int x_step[NT][SIDES];
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
@@ -299,124 +345,152 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
       // columns past the tokens repeat the last one; nobody reads them
       const int token = !GROUPED ? j * 8 + g : MX ? 2 * j + (g & 1) : j;
       const bool here = !GROUPED || (MX ? t == g >> 1 : g == 2 * t + side);
-      x_at[j][side] = here ? smem + min(token, tokens - 1) * pitch + t * 16 : zeros;
+      x_at[j][side] = static_cast<uint32_t>(
+          __cvta_generic_to_shared(here ? smem + min(token, tokens - 1) * pitch + t * 16 : zeros));
       x_step[j][side] = here ? 256 : 0;
     }
   }
 
-  float acc[NT][4];
+  // two 16-row tiles: [tile][group][rows g, g + 8 x columns 2 t, 2 t + 1]
+  using Sums = float[2][NT][4];
+  Sums acc;
+  auto clear = [&](Sums& c) {
 #pragma unroll
-  for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
+    for (int q = 0; q < 2; ++q) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) c[q][j][0] = c[q][j][1] = c[q][j][2] = c[q][j][3] = 0.0f;
+    }
+  };
+  clear(acc);
 
-  // products of 128 codes, in GROUPED as they are, else scaled by f16 pairs f0 / f1 (rows g, g + 8;
-  // first and second 16 codes)
-  auto products = [&](const Slot& s, int chunk, const uint32_t (&f0)[2], const uint32_t (&f1)[2], float (&c)[NT][4]) {
-    const uint32_t w0[4] = {s.w0.x, s.w0.y, s.w0.z, s.w0.w}, w1[4] = {s.w1.x, s.w1.y, s.w1.z, s.w1.w};
-    float c2[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // with one group: halves the chain of dependent products
-    auto scaled = [&](uint32_t v, uint32_t f) { return GROUPED ? v : mul_f16x2(v, f); };
+  // 128 codes of both tiles: w[tile][row half], in GROUPED as they are, else scaled by the f16 pairs
+  // f[tile][row half][first, second 16 codes]
+  auto products = [&](const uint4 (&w)[2][2], int half_chunk, const uint32_t (&f)[2][2][2], Sums& c) {
+    auto scaled = [&](uint32_t v, uint32_t m) { return GROUPED ? v : mul_f16x2(v, m); };
 #pragma unroll
     for (int i = 0; i < 4; ++i) {  // 8 codes of each row: two MMAs
-      const uint32_t a00 = scaled(e2m1_f16<0>(w0[i]), f0[i >> 1]), a01 = scaled(e2m1_f16<1>(w0[i]), f0[i >> 1]);
-      const uint32_t a02 = scaled(e2m1_f16<2>(w0[i]), f0[i >> 1]), a03 = scaled(e2m1_f16<3>(w0[i]), f0[i >> 1]);
-      const uint32_t a10 = scaled(e2m1_f16<0>(w1[i]), f1[i >> 1]), a11 = scaled(e2m1_f16<1>(w1[i]), f1[i >> 1]);
-      const uint32_t a12 = scaled(e2m1_f16<2>(w1[i]), f1[i >> 1]), a13 = scaled(e2m1_f16<3>(w1[i]), f1[i >> 1]);
+      uint4 b[NT], l[NT];
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         const int side = SIDES == 2 ? i >> 1 : 0;
-        const uint8_t* at = x_at[j][side] + chunk * x_step[j][side] + i * 64;
-        const uint4 b = *reinterpret_cast<const uint4*>(at);
-        mma_m16n8k16(c[j], a00, a10, a01, a11, b.x, b.y);
-        mma_m16n8k16(NT == 1 ? c2 : c[j], a02, a12, a03, a13, b.z, b.w);
-        if constexpr (SPLIT) {
-          const uint4 l = *reinterpret_cast<const uint4*>(x_step[j][side] ? at + lo_at : at);
-          mma_m16n8k16(c[j], a00, a10, a01, a11, l.x, l.y);
-          mma_m16n8k16(NT == 1 ? c2 : c[j], a02, a12, a03, a13, l.z, l.w);
+        const uint32_t at = x_at[j][side] + half_chunk * x_step[j][side] + i * 64;
+        b[j] = load_shared16(at);
+        if constexpr (SPLIT) l[j] = load_shared16(x_step[j][side] ? at + lo_at : at);
+      }
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const uint32_t w0 = i == 0 ? w[q][0].x : i == 1 ? w[q][0].y : i == 2 ? w[q][0].z : w[q][0].w;
+        const uint32_t w1 = i == 0 ? w[q][1].x : i == 1 ? w[q][1].y : i == 2 ? w[q][1].z : w[q][1].w;
+        const uint32_t f0 = f[q][0][i >> 1], f1 = f[q][1][i >> 1];
+        const uint32_t a00 = scaled(e2m1_f16<0>(w0), f0), a01 = scaled(e2m1_f16<1>(w0), f0);
+        const uint32_t a02 = scaled(e2m1_f16<2>(w0), f0), a03 = scaled(e2m1_f16<3>(w0), f0);
+        const uint32_t a10 = scaled(e2m1_f16<0>(w1), f1), a11 = scaled(e2m1_f16<1>(w1), f1);
+        const uint32_t a12 = scaled(e2m1_f16<2>(w1), f1), a13 = scaled(e2m1_f16<3>(w1), f1);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          mma_m16n8k16(c[q][j], a00, a10, a01, a11, b[j].x, b[j].y);
+          mma_m16n8k16(c[q][j], a02, a12, a03, a13, b[j].z, b[j].w);
+          if constexpr (SPLIT) {
+            mma_m16n8k16(c[q][j], a00, a10, a01, a11, l[j].x, l[j].y);
+            mma_m16n8k16(c[q][j], a02, a12, a03, a13, l[j].z, l[j].w);
+          }
         }
       }
     }
-    if constexpr (NT == 1) {
+  };
+  // acc += c, rows times u[tile][row half]
+  auto add_scaled = [&](const Sums& c, const float (&u)[2][2]) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) c[0][e] += c2[e];
+    for (int q = 0; q < 2; ++q) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[q][j][e] = fmaf(c[q][j][e], u[q][e >> 1], acc[q][j][e]);
+      }
     }
   };
-  auto consume = [&](const Slot& s, int chunk) {
+  // s[tile][row half]: the lane's two e4m3 bytes, or its e8m0
+  auto consume = [&](const uint4 (&w)[2][2], const uint32_t (&s)[2][2], int half_chunk) {
     if constexpr (GROUPED) {
-      const uint32_t none[2] = {0, 0};
-      float c[NT][4];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.0f;
-      products(s, chunk, none, none, c);
+      const uint32_t none[2][2][2] = {};
+      Sums c;
+      clear(c);
+      products(w, half_chunk, none, c);
       if constexpr (MX) {  // columns 2 t and 2 t + 1: block t, two tokens
-        const float u0 = e8m0_value(static_cast<uint8_t>(s.s0)), u1 = e8m0_value(static_cast<uint8_t>(s.s1));
+        float u[2][2];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          acc[j][0] = fmaf(c[j][0], u0, acc[j][0]);
-          acc[j][1] = fmaf(c[j][1], u0, acc[j][1]);
-          acc[j][2] = fmaf(c[j][2], u1, acc[j][2]);
-          acc[j][3] = fmaf(c[j][3], u1, acc[j][3]);
+        for (int q = 0; q < 2; ++q) {
+          u[q][0] = e8m0_value(static_cast<uint8_t>(s[q][0]));
+          u[q][1] = e8m0_value(static_cast<uint8_t>(s[q][1]));
         }
+        add_scaled(c, u);
       } else {  // columns 2 t and 2 t + 1: the lane's two blocks
-        const __half2_raw h0 = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(s.s0), __NV_E4M3);
-        const __half2_raw h1 = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(s.s1), __NV_E4M3);
-        const float2 u0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
-        const float2 u1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          acc[j][0] = fmaf(c[j][0], u0.x, acc[j][0]);
-          acc[j][1] = fmaf(c[j][1], u0.y, acc[j][1]);
-          acc[j][2] = fmaf(c[j][2], u1.x, acc[j][2]);
-          acc[j][3] = fmaf(c[j][3], u1.y, acc[j][3]);
+        for (int q = 0; q < 2; ++q) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const __half2_raw p = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(s[q][h]), __NV_E4M3);
+            const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&p));
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              acc[q][j][2 * h] = fmaf(c[q][j][2 * h], u.x, acc[q][j][2 * h]);
+              acc[q][j][2 * h + 1] = fmaf(c[q][j][2 * h + 1], u.y, acc[q][j][2 * h + 1]);
+            }
+          }
         }
       }
     } else if constexpr (!MX) {
-      const __half2_raw h0 = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(s.s0), __NV_E4M3);
-      const __half2_raw h1 = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(s.s1), __NV_E4M3);
-      const uint32_t p0 = *reinterpret_cast<const uint32_t*>(&h0), p1 = *reinterpret_cast<const uint32_t*>(&h1);
-      const uint32_t f0[2] = {__byte_perm(p0, p0, 0x1010), __byte_perm(p0, p0, 0x3232)};
-      const uint32_t f1[2] = {__byte_perm(p1, p1, 0x1010), __byte_perm(p1, p1, 0x3232)};
-      products(s, chunk, f0, f1, acc);
+      uint32_t f[2][2][2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const __half2_raw p = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(s[q][h]), __NV_E4M3);
+          const uint32_t v = *reinterpret_cast<const uint32_t*>(&p);
+          f[q][h][0] = __byte_perm(v, v, 0x1010);
+          f[q][h][1] = __byte_perm(v, v, 0x3232);
+        }
+      }
+      products(w, half_chunk, f, acc);
     } else {
-      const int e0 = s.s0, e1 = s.s1;
-      const int r0 = __shfl_sync(0xffffffffu, e0, lane & 28), r1 = __shfl_sync(0xffffffffu, e1, lane & 28);
       auto pow2 = [](int d) -> uint32_t {  // 2^d as an f16 pair, d in -24 .. 15
         const uint32_t h = d >= -14 ? static_cast<uint32_t>(d + 15) << 10 : 1u << (d + 24);
         return h | (h << 16);
       };
-      // the scale of 32 zeros does not count
-      const bool near0 = e0 - r0 >= -20 && e0 - r0 <= 13, near1 = e1 - r1 >= -20 && e1 - r1 <= 13;
-      const bool ok0 = near0 || (s.w0.x | s.w0.y | s.w0.z | s.w0.w) == 0, ok1 = near1 || (s.w1.x | s.w1.y | s.w1.z | s.w1.w) == 0;
-      if (__all_sync(0xffffffffu, ok0 && ok1 && e0 != 255 && e1 != 255)) {
-        const uint32_t m_0 = near0 ? pow2(e0 - r0) : 0u, m_1 = near1 ? pow2(e1 - r1) : 0u;
-        const uint32_t f0[2] = {m_0, m_0}, f1[2] = {m_1, m_1};
-        float c[NT][4];
+      uint32_t f[2][2][2];
+      float u[2][2];
+      bool ok = true;
 #pragma unroll
-        for (int j = 0; j < NT; ++j) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.0f;
-        products(s, chunk, f0, f1, c);
-        const float u0 = e8m0_value(static_cast<uint8_t>(r0)), u1 = e8m0_value(static_cast<uint8_t>(r1));
+      for (int q = 0; q < 2; ++q) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          acc[j][0] = fmaf(c[j][0], u0, acc[j][0]);
-          acc[j][1] = fmaf(c[j][1], u0, acc[j][1]);
-          acc[j][2] = fmaf(c[j][2], u1, acc[j][2]);
-          acc[j][3] = fmaf(c[j][3], u1, acc[j][3]);
+        for (int h = 0; h < 2; ++h) {
+          const int e = s[q][h], r = __shfl_sync(0xffffffffu, e, lane & 28), d = e - r;
+          const bool near = d >= -20 && d <= 13;
+          // the scale of 32 zeros does not count
+          ok = ok && e != 255 && (near || (w[q][h].x | w[q][h].y | w[q][h].z | w[q][h].w) == 0);
+          f[q][h][0] = f[q][h][1] = near ? pow2(d) : 0u;
+          u[q][h] = e8m0_value(static_cast<uint8_t>(r));
         }
+      }
+      if (__all_sync(0xffffffffu, ok)) {
+        Sums c;
+        clear(c);
+        products(w, half_chunk, f, c);
+        add_scaled(c, u);
       } else {
-        for (int q = 0; q < 4; ++q) {  // lane q's blocks of every row
-          const uint32_t one = t == q ? 0x3C003C00u : 0u;
-          const uint32_t f[2] = {one, one};
-          float c[NT][4];
+        for (int x = 0; x < 4; ++x) {  // lane x's blocks of every row
+          Sums c;
+          clear(c);
 #pragma unroll
-          for (int j = 0; j < NT; ++j) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.0f;
-          products(s, chunk, f, f, c);
-          const float u0 = e8m0_value(static_cast<uint8_t>(__shfl_sync(0xffffffffu, e0, (lane & 28) | q)));
-          const float u1 = e8m0_value(static_cast<uint8_t>(__shfl_sync(0xffffffffu, e1, (lane & 28) | q)));
+          for (int q = 0; q < 2; ++q) {
 #pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            acc[j][0] = fmaf(c[j][0], u0, acc[j][0]);
-            acc[j][1] = fmaf(c[j][1], u0, acc[j][1]);
-            acc[j][2] = fmaf(c[j][2], u1, acc[j][2]);
-            acc[j][3] = fmaf(c[j][3], u1, acc[j][3]);
+            for (int h = 0; h < 2; ++h) {
+              f[q][h][0] = f[q][h][1] = t == x ? 0x3C003C00u : 0u;
+              u[q][h] = e8m0_value(static_cast<uint8_t>(__shfl_sync(0xffffffffu, s[q][h], (lane & 28) | x)));
+            }
           }
+          products(w, half_chunk, f, c);
+          add_scaled(c, u);
         }
       }
     }
@@ -424,9 +498,9 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
 
   // one output of a tile: the final value, or one of its two partial sums
   auto put = [&](int tile, int r, int mt, float y, int part) {
-    const int64_t row = static_cast<int64_t>(tile) * 16 + r;
+    const int64_t row = static_cast<int64_t>(tile) * kGemvRows + r;
     if (row >= a.n || mt >= tokens) return;
-    y *= unit[mt] * a.ts[a.ts_per_row ? row : 0];
+    y *= unit[mt] * __ldg(a.ts + (a.ts_per_row ? row : 0));
     if (part < 0 && a.slices == 1) {
       if (a.bias != nullptr) y += load_any(a.bias, a.bias_dtype, row);
       store_any<T>(a.out, (m0 + mt) * a.ldo + row, y);
@@ -440,67 +514,107 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
     const int seg = warp * 2 + (begun == 0);  // 0: the tile began before this warp, 1: it begins here
     auto one = [&](int r, int mt, float y) {
       if (whole) put(tile, r, mt, y, -1);
-      else sums[(seg * 16 + r) * COLS + mt] = y;
+      else sums[(seg * kGemvRows + r) * COLS + mt] = y;
     };
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      if constexpr (GROUPED) {
-        // the blocks' sums meet: over the quad, and with NVFP4 over a lane's two blocks
-        float v[4] = {acc[j][0], acc[j][1], acc[j][2], acc[j][3]};
-        if constexpr (!MX) {
-          v[0] += v[1];
-          v[2] += v[3];
-        }
+    for (int q = 0; q < 2; ++q) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] += __shfl_xor_sync(0xffffffffu, v[e], 1);
-          v[e] += __shfl_xor_sync(0xffffffffu, v[e], 2);
-        }
-        if (t == 0) {
-          if constexpr (MX) {
-            one(g, 2 * j, v[0]);
-            one(g, 2 * j + 1, v[1]);
-            one(g + 8, 2 * j, v[2]);
-            one(g + 8, 2 * j + 1, v[3]);
-          } else {
-            one(g, j, v[0]);
-            one(g + 8, j, v[2]);
+      for (int j = 0; j < NT; ++j) {
+        const int r = q * 16 + g;
+        if constexpr (GROUPED) {
+          // the blocks' sums meet: over the quad, and with NVFP4 over a lane's two blocks
+          float v[4] = {acc[q][j][0], acc[q][j][1], acc[q][j][2], acc[q][j][3]};
+          if constexpr (!MX) {
+            v[0] += v[1];
+            v[2] += v[3];
           }
-        }
-      } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) one(g + 8 * (e >> 1), j * 8 + 2 * t + (e & 1), acc[j][e]);
+          for (int e = 0; e < 4; ++e) {
+            v[e] += __shfl_xor_sync(0xffffffffu, v[e], 1);
+            v[e] += __shfl_xor_sync(0xffffffffu, v[e], 2);
+          }
+          if (t == 0) {
+            if constexpr (MX) {
+              one(r, 2 * j, v[0]);
+              one(r, 2 * j + 1, v[1]);
+              one(r + 8, 2 * j, v[2]);
+              one(r + 8, 2 * j + 1, v[3]);
+            } else {
+              one(r, j, v[0]);
+              one(r + 8, j, v[2]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) one(r + 8 * (e >> 1), j * 8 + 2 * t + (e & 1), acc[q][j][e]);
+        }
       }
-      acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
     }
+    clear(acc);
     if (!whole && lane == 0) seg_tile[seg] = 2 * tile + ends;
     begun = 0;
   };
-  for (int u = u_lo; u < u_hi; u += kGemvDepth) {
+
+  int stage = 0;
+  for (int u = u_lo; u < u_hi; ++u) {
+    if (a.k > 0) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kGemvStages - 2) : "memory");
+      __syncwarp();
+      issue(stage == 0 ? kGemvStages - 1 : stage - 1);  // the stage that was consumed before this one
+      const uint32_t from = ring + stage * STAGE;
+      const uint8_t* sc = smem_all + (warp * kGemvStages + stage) * STAGE + kGemvRows * 128;
 #pragma unroll
-    for (int i = 0; i < kGemvDepth; ++i) {
-      if (u + i < u_hi) {
-        consume(slots[i], chunk);
-        if (a.k > 0) issue(slots[i]);
-        if (chunk == c_count - 1 || u + i == u_hi - 1) end_segment();
-        if (++chunk == c_count) {
-          chunk = 0;
-          ++tile;
+      for (int h = 0; h < 2; ++h) {  // 128 codes
+        uint4 w[2][2];
+        uint32_t s[2][2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int r = q * 16 + i * 8 + g;
+            w[q][i] = load_shared16(from + r * 128 + (((h * 4 + t) ^ ((g & 1) << 2)) << 4));
+            int off = r * SPITCH + h * (MX ? 4 : 8) + t * (MX ? 1 : 2);
+            if constexpr (WIDE) {
+              s[q][i] = MX ? sc[off] : *reinterpret_cast<const uint16_t*>(sc + off);
+            } else {
+              if (!a.swizzle) {  // the row's scales begin within the first word
+                const int row = min(tile * kGemvRows + r, a.n - 1);
+                off += static_cast<int>((static_cast<int64_t>(row) * cols + (c_first + chunk) * (MX ? 8 : 16)) & 3);
+              }
+              s[q][i] = sc[off] | (MX ? 0u : static_cast<uint32_t>(sc[off + 1]) << 8);
+            }
+          }
         }
+        if constexpr (!WIDE) {
+          // past K there may be any byte: no scale
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int k = (c_first + chunk) * kGemvCodes + h * 128 + t * 32;
+            if (k >= a.k) s[i >> 1][i & 1] = 0;
+            else if (!MX && k + 16 >= a.k) s[i >> 1][i & 1] &= 0xFFu;
+          }
+        }
+        consume(w, s, chunk * 2 + h);
       }
     }
+    if (chunk == c_count - 1 || u == u_hi - 1) end_segment();
+    if (++chunk == c_count) {
+      chunk = 0;
+      ++tile;
+    }
+    stage = stage == kGemvStages - 1 ? 0 : stage + 1;
   }
   __syncthreads();
   // the tiles that warps share: from where they begin in this block (a warp's second segment, or the
   // first warp's first), through the following warps' first segments
-  for (int i = tid; i < (kGemvWarps + 1) * 16 * COLS; i += kGemvThreads) {
-    const int head = i / (16 * COLS), cell = i % (16 * COLS);
+  for (int i = tid; i < (kGemvWarps + 1) * kGemvRows * COLS; i += kGemvThreads) {
+    const int head = i / (kGemvRows * COLS), cell = i % (kGemvRows * COLS);
     const int seg = head == 0 ? 0 : (head - 1) * 2 + 1, first = seg_tile[seg];
     if (first < 0) continue;
-    float y = sums[seg * 16 * COLS + cell];
+    float y = sums[seg * kGemvRows * COLS + cell];
     int end = first & 1;
     for (int w = (seg >> 1) + 1; w < kGemvWarps && seg_tile[2 * w] >= 0 && seg_tile[2 * w] >> 1 == first >> 1; ++w) {
-      y += sums[2 * w * 16 * COLS + cell];
+      y += sums[2 * w * kGemvRows * COLS + cell];
       end = seg_tile[2 * w] & 1;
     }
     put(first >> 1, cell / COLS, cell % COLS, y, head == 0 ? 1 : end ? -1 : 0);
@@ -512,7 +626,7 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
 template <int T>
 __global__ void __launch_bounds__(256) gemv_join_kernel(GemvArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int row = blockIdx.x * 256 + threadIdx.x, mt = blockIdx.y, tile = row / 16;
+  const int row = blockIdx.x * 256 + threadIdx.x, mt = blockIdx.y, tile = row / kGemvRows;
   if (row >= a.n) return;
   float y = 0.0f;
   for (int s = 0; s < a.slices; ++s) {

@@ -13,74 +13,97 @@ int gemv_check(int64_t m, int64_t n, int64_t k, int fmt, int dtype) {
   KAB_REQUIRE(valid_dtype(dtype), "unknown dtype %d", dtype);
   KAB_REQUIRE(m >= 0 && n >= 0 && k >= 0, "negative shape");
   KAB_REQUIRE(k % (fmt == KAB_NVFP4 ? 16 : 32) == 0, "K = %lld is not a multiple of the block", (long long)k);
-  KAB_REQUIRE((n + 15) / 16 * ((k + 127) / 128) < (int64_t(1) << 31), "problem too large");
-  KAB_REQUIRE(m < (int64_t(1) << 18) && n < (int64_t(1) << 30) && k < (int64_t(1) << 30), "problem too large");
+  KAB_REQUIRE((n + 31) / 32 * ((k + 255) / 256 + 1) < (int64_t(1) << 31), "problem too large");
+  KAB_REQUIRE(m < 65536 && n < (int64_t(1) << 30) && k < (int64_t(1) << 30), "problem too large");
   return KAB_OK;
 }
 
-// How a shape is cut: slices of K so that a slice of x fits in shared memory beside a second block
-// (kXBytes), and blocks per slice.
-constexpr int kXBytes = 72 * 1024;
+// How a shape is cut: slices of K so that a slice of x fits in shared memory, and blocks per slice,
+// two per SM where their shared memory allows.
+constexpr int kSmemOne = 226 * 1024, kSmemTwo = 113 * 1024;
 struct GemvPlan {
-  bool grouped;
-  int nt, columns, tokens, chunks, slice_chunks, slices, tiles, blocks;
-  bool join;
-  size_t partial;
+  bool grouped, join, terms;
+  int nt, columns, tokens, chunks, slice_chunks, slices, tiles, blocks, smem;
+  size_t partial, x_terms, x_units;  // workspace bytes
+  size_t bytes() const { return partial + x_terms + x_units; }
 };
-// Blocks apart (GROUPED) while its MMAs (8 per chunk and group) stay below the stream's time: one or
-// two tokens of NVFP4, up to eight of MXFP4 (half of that in fp32, whose x has two terms).
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+// Blocks apart (GROUPED) while its MMAs (8 per 128 codes and group) stay below the stream's time: one
+// or two tokens of NVFP4, up to eight of MXFP4 (half of that in fp32, whose x has two terms).
 GemvPlan gemv_plan(int64_t m, int64_t n, int64_t k, int fmt, int dtype) {
   GemvPlan p{};
-  const bool mx = fmt == KAB_MXFP4;
-  const int most = (mx ? 8 : 2) / (dtype == KAB_F32 ? 2 : 1);
+  const bool mx = fmt == KAB_MXFP4, split = dtype == KAB_F32;
+  const int most = (mx ? 8 : 2) / (split ? 2 : 1);
   p.grouped = m <= most;
   p.nt = p.grouped ? (mx ? (m <= 2 ? 1 : m <= 4 ? 2 : 4) : static_cast<int>(m)) : m <= 8 ? 1 : m <= 16 ? 2 : 4;
   p.columns = gemv_columns(mx, p.nt, p.grouped);
   p.tokens = static_cast<int>(std::min<int64_t>(m, p.columns));
-  p.chunks = static_cast<int>(std::max<int64_t>(1, (k + 127) / 128));
-  const int64_t per_chunk = static_cast<int64_t>(p.tokens) * 256 * (dtype == KAB_F32 ? 2 : 1);
-  const int fit = static_cast<int>(std::max<int64_t>(1, kXBytes / per_chunk));
+  p.chunks = static_cast<int>(std::max<int64_t>(1, (k + kGemvCodes - 1) / kGemvCodes));
+  p.tiles = static_cast<int>((n + kGemvRows - 1) / kGemvRows);
+  const int64_t per_chunk = static_cast<int64_t>(p.tokens) * 512 * (split ? 2 : 1);
+  const int fixed = gemv_smem(mx, 0, 0, p.columns, split) + p.tokens * 64 * (split ? 2 : 1);
+  // two blocks per SM with at least 8 chunks of x each (or all of it), else one
+  const int need = std::min(p.chunks, 8);
+  const int room = fixed + need * per_chunk <= kSmemTwo ? kSmemTwo : kSmemOne;
+  const int fit = static_cast<int>(std::max<int64_t>(1, (room - fixed) / per_chunk));
   const int want = (p.chunks + fit - 1) / fit;
   p.slice_chunks = (p.chunks + want - 1) / want;
   p.slices = (p.chunks + p.slice_chunks - 1) / p.slice_chunks;
-  p.tiles = static_cast<int>((n + 15) / 16);
-  p.blocks = std::max(1, std::min(p.tiles, 2 * sm_count() / p.slices));
+  p.smem = gemv_smem(mx, p.tokens, p.slice_chunks, p.columns, split);
+  const int resident = room == kSmemTwo ? 2 : 1;
+  p.blocks = std::max(1, std::min(p.tiles, resident * sm_count() / p.slices));
   p.join = p.slices > 1 || p.tiles % p.blocks != 0;  // else every block has whole tiles
-  p.partial = p.join ? static_cast<size_t>(2) * p.slices * m * n * 4 : 0;
+  p.partial = p.join ? round256(static_cast<size_t>(2) * p.slices * m * n * 4) : 0;
+  // x converted by a launch of its own where every block would have to convert more than one token
+  p.terms = m > 1;
+  p.x_terms = p.terms ? round256(static_cast<size_t>(p.slices) * m * p.slice_chunks * 512 * (split ? 2 : 1)) : 0;
+  p.x_units = p.terms ? round256(static_cast<size_t>(p.slices) * m * 4) : 0;
   return p;
 }
 
-template <int T, int MX, int NT, int WIDE, int GROUPED>
-int launch_gemv(const GemvArgs& a, const GemvPlan& p, cudaStream_t s) {
-  auto kern = gemv_fp4_kernel<T, MX, NT, WIDE, GROUPED>;
-  const int bytes = gemv_smem(p.tokens, p.slice_chunks, p.columns, T == kF32);
-  static bool configured[64] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(KAB_ECUDA, "no current device");
-  if (!configured[dev]) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 113 * 1024) != cudaSuccess)
-      return fail(KAB_ECUDA, "cannot configure the FP4 linear");
-    configured[dev] = true;
-  }
-  const dim3 grid(p.blocks, p.slices, (a.m + p.columns - 1) / p.columns);
-  kern<<<grid, kGemvThreads, bytes, s>>>(a);
-  if (int e = check_launch("kab_gemv_fp4")) return e;
-  if (!p.join) return KAB_OK;
+// A launch that may be set up while the one before it runs (it waits by itself).
+cudaError_t launch_after(void (*kern)(GemvArgs), dim3 grid, int smem, cudaStream_t s, const GemvArgs& a) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((a.n + 255) / 256, a.m);
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kGemvThreads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, gemv_join_kernel<T>, a);
+  return cudaLaunchKernelEx(&cfg, kern, a);
+}
+
+template <int T, int MX, int NT, int WIDE, int GROUPED>
+int launch_gemv(const GemvArgs& a, const GemvPlan& p, cudaStream_t s) {
+  auto kern = gemv_fp4_kernel<T, MX, NT, WIDE, GROUPED>;
+  static bool configured[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(KAB_ECUDA, "no current device");
+  if (!configured[dev]) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemOne) != cudaSuccess)
+      return fail(KAB_ECUDA, "cannot configure the FP4 linear");
+    configured[dev] = true;
+  }
+  const dim3 grid(p.blocks, p.slices, (a.m + p.columns - 1) / p.columns);
+  if (p.terms) {
+    gemv_x_kernel<T><<<dim3(p.slices, a.m), kGemvThreads, 0, s>>>(a);
+    if (int e = check_launch("kab_gemv_fp4 x")) return e;
+    launch_after(kern, grid, p.smem, s, a);
+  } else {
+    kern<<<grid, kGemvThreads, p.smem, s>>>(a);
+  }
+  if (int e = check_launch("kab_gemv_fp4")) return e;
+  if (!p.join) return KAB_OK;
+  launch_after(gemv_join_kernel<T>, dim3((a.n + 255) / 256, a.m), 0, s, a);
   return check_launch("kab_gemv_fp4 join");
 }
 template <int T, int MX, int NT, int GROUPED>
 int launch_gemv(const GemvArgs& a, const GemvPlan& p, cudaStream_t s) {
-  const bool wide = a.k % 32 == 0 && aligned(a.codes, 16) && aligned(a.scales, 2);
+  const bool wide = a.k % (MX ? 128 : 64) == 0 && aligned(a.codes, 16) && aligned(a.scales, 4);
   return wide ? launch_gemv<T, MX, NT, 1, GROUPED>(a, p, s) : launch_gemv<T, MX, NT, 0, GROUPED>(a, p, s);
 }
 template <int T, int MX>
@@ -112,7 +135,7 @@ int kab_gemv_fp4_workspace(int64_t m, int64_t n, int64_t k, int fmt, int dtype, 
                            size_t* zero_bytes) {
   if (int e = gemv_check(m, n, k, fmt, dtype)) return e;
   KAB_REQUIRE(bytes != nullptr && zero_bytes != nullptr, "null pointer");
-  *bytes = m == 0 || n == 0 ? 0 : gemv_plan(m, n, k, fmt, dtype).partial;
+  *bytes = m == 0 || n == 0 ? 0 : gemv_plan(m, n, k, fmt, dtype).bytes();
   *zero_bytes = 0;
   return KAB_OK;
 }
@@ -127,11 +150,11 @@ int kab_gemv_fp4(const void* x, int dtype, int64_t ldx, const uint8_t* codes, co
   KAB_REQUIRE(bias == nullptr || valid_dtype(bias_dtype), "unknown bias dtype %d", bias_dtype);
   KAB_REQUIRE(aligned(x, 16) && ldx % 8 == 0, "x must be 16-byte aligned, its row stride a multiple of 8");
   KAB_REQUIRE(aligned(codes, 8), "codes must be 8-byte aligned");
-  KAB_REQUIRE(!swizzle || aligned(scales, 4), "swizzled scales must be 4-byte aligned");
+  KAB_REQUIRE(aligned(scales, 4), "scales must be 4-byte aligned");
   KAB_REQUIRE(ldo >= n && ldx >= k, "ldx %lld or ldo %lld is too short", (long long)ldx, (long long)ldo);
   const GemvPlan p = gemv_plan(m, n, k, fmt, dtype);
-  KAB_REQUIRE(p.partial == 0 || (workspace != nullptr && workspace_bytes >= p.partial && aligned(workspace, 256)),
-              "the workspace needs %zu bytes, 256-byte aligned (kab_gemv_fp4_workspace)", p.partial);
+  KAB_REQUIRE(p.bytes() == 0 || (workspace != nullptr && workspace_bytes >= p.bytes() && aligned(workspace, 256)),
+              "the workspace needs %zu bytes, 256-byte aligned (kab_gemv_fp4_workspace)", p.bytes());
   GemvArgs a{};
   a.x = x, a.ldx = ldx, a.codes = codes, a.scales = scales, a.swizzle = swizzle;
   a.ts = tensor_scale, a.ts_per_row = scale_per_row;
@@ -139,6 +162,10 @@ int kab_gemv_fp4(const void* x, int dtype, int64_t ldx, const uint8_t* codes, co
   a.bias = bias, a.bias_dtype = bias_dtype, a.out = out, a.ldo = ldo;
   a.chunks = p.chunks, a.slice_chunks = p.slice_chunks, a.slices = p.slices;
   a.tiles = p.tiles, a.blocks = p.blocks, a.partial = static_cast<float*>(workspace);
+  if (p.terms) {
+    a.x_terms = static_cast<uint8_t*>(workspace) + p.partial;
+    a.x_units = reinterpret_cast<float*>(a.x_terms + p.x_terms);
+  }
   const cudaStream_t s = as_stream(stream);
   if (dtype == KAB_BF16) return launch_gemv<kBF16>(a, p, fmt, s);
   if (dtype == KAB_F16) return launch_gemv<kF16>(a, p, fmt, s);
