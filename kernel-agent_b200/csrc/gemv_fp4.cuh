@@ -139,7 +139,7 @@ __host__ __device__ constexpr int gemv_stage_bytes(bool mx) { return kGemvRows *
 __host__ __device__ constexpr int gemv_pitch(int slice_chunks) { return slice_chunks * 512 + 64; }
 __host__ __device__ constexpr int gemv_smem(bool mx, int m, int slice_chunks, int columns, bool split) {
   return kGemvWarps * kGemvStages * gemv_stage_bytes(mx) + m * gemv_pitch(slice_chunks) * (split ? 2 : 1) + 256 +
-         2 * kGemvWarps * kGemvRows * columns * 4 + columns * 4 + 2 * kGemvWarps * 4;
+         kGemvWarps * kGemvRows * columns * 4 + columns * 4 + 2 * kGemvWarps * 4;
 }
 // Tokens that NT groups of the MMA's columns take.
 constexpr int gemv_columns(bool mx, int nt, bool grouped) { return grouped ? (mx ? 2 * nt : nt) : 8 * nt; }
@@ -226,9 +226,15 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
   const int c_first = slice * a.slice_chunks, c_count = min(a.slice_chunks, a.chunks - c_first);
   const int pitch = gemv_pitch(a.slice_chunks);
   uint8_t* zeros = smem + tokens * pitch * (SPLIT ? 2 : 1);  // 256 bytes: what a column's other lanes read
-  float* sums = reinterpret_cast<float*>(zeros + 256);       // [8 warps][2][32][COLS]
-  float* unit = sums + 2 * kGemvWarps * kGemvRows * COLS;    // [COLS]
+  float* sums = reinterpret_cast<float*>(zeros + 256);       // [8 warps][32][COLS]: tiles begun before a warp
+  float* unit = sums + kGemvWarps * kGemvRows * COLS;        // [COLS]
   int* seg_tile = reinterpret_cast<int*>(unit + COLS);       // [8 warps][2]: 2 * tile + (its end is here), or -1
+  // the sums of a tile that began before warp w (first), or of the one it leaves unfinished: its last,
+  // so they fit in its ring
+  auto sums_of = [&](int w, int first) -> float* {
+    return first ? sums + w * kGemvRows * COLS : reinterpret_cast<float*>(smem_all + w * kGemvStages * STAGE);
+  };
+  static_assert(kGemvStages * STAGE >= kGemvRows * COLS * 4, "a tile's sums fit in a ring");
 
   // ---- this warp's part of the line
   const GemvCut cut(a.tiles * c_count, a.blocks);
@@ -512,9 +518,11 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
   auto end_segment = [&]() {
     const bool ends = chunk == c_count - 1, whole = begun == 0 && ends;
     const int seg = warp * 2 + (begun == 0);  // 0: the tile began before this warp, 1: it begins here
+    float* mine = sums_of(warp, begun != 0);
+    __syncwarp();  // the ring's last reads
     auto one = [&](int r, int mt, float y) {
       if (whole) put(tile, r, mt, y, -1);
-      else sums[(seg * kGemvRows + r) * COLS + mt] = y;
+      else mine[r * COLS + mt] = y;
     };
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
@@ -563,8 +571,8 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
       issue(stage == 0 ? kGemvStages - 1 : stage - 1);  // the stage that was consumed before this one
       const uint32_t from = ring + stage * STAGE;
       const uint8_t* sc = smem_all + (warp * kGemvStages + stage) * STAGE + kGemvRows * 128;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {  // 128 codes
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {  // 128 codes; once in the code, which short streams fetch cold
         uint4 w[2][2];
         uint32_t s[2][2];
 #pragma unroll
@@ -611,10 +619,10 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
     const int head = i / (kGemvRows * COLS), cell = i % (kGemvRows * COLS);
     const int seg = head == 0 ? 0 : (head - 1) * 2 + 1, first = seg_tile[seg];
     if (first < 0) continue;
-    float y = sums[seg * kGemvRows * COLS + cell];
+    float y = sums_of(seg >> 1, head == 0)[cell];
     int end = first & 1;
     for (int w = (seg >> 1) + 1; w < kGemvWarps && seg_tile[2 * w] >= 0 && seg_tile[2 * w] >> 1 == first >> 1; ++w) {
-      y += sums[2 * w * kGemvRows * COLS + cell];
+      y += sums_of(w, 1)[cell];
       end = seg_tile[2 * w] & 1;
     }
     put(first >> 1, cell / COLS, cell % COLS, y, head == 0 ? 1 : end ? -1 : 0);

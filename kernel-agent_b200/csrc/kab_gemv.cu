@@ -43,8 +43,8 @@ GemvPlan gemv_plan(int64_t m, int64_t n, int64_t k, int fmt, int dtype) {
   p.tiles = static_cast<int>((n + kGemvRows - 1) / kGemvRows);
   const int64_t per_chunk = static_cast<int64_t>(p.tokens) * 512 * (split ? 2 : 1);
   const int fixed = gemv_smem(mx, 0, 0, p.columns, split) + p.tokens * 64 * (split ? 2 : 1);
-  // two blocks per SM with at least 8 chunks of x each (or all of it), else one
-  const int need = std::min(p.chunks, 8);
+  // two blocks per SM with at least 4 chunks of x each (or all of it), else one
+  const int need = std::min(p.chunks, 4);
   const int room = fixed + need * per_chunk <= kSmemTwo ? kSmemTwo : kSmemOne;
   const int fit = static_cast<int>(std::max<int64_t>(1, (room - fixed) / per_chunk));
   const int want = (p.chunks + fit - 1) / fit;
@@ -63,10 +63,10 @@ GemvPlan gemv_plan(int64_t m, int64_t n, int64_t k, int fmt, int dtype) {
 }
 
 // A launch that may be set up while the one before it runs (it waits by itself).
-cudaError_t launch_after(void (*kern)(GemvArgs), dim3 grid, int smem, cudaStream_t s, const GemvArgs& a) {
+cudaError_t launch_after(void (*kern)(GemvArgs), dim3 grid, int threads, int smem, cudaStream_t s, const GemvArgs& a) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(kGemvThreads);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
   cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = s;
   cudaLaunchAttribute at[1];
@@ -90,15 +90,15 @@ int launch_gemv(const GemvArgs& a, const GemvPlan& p, cudaStream_t s) {
   }
   const dim3 grid(p.blocks, p.slices, (a.m + p.columns - 1) / p.columns);
   if (p.terms) {
-    gemv_x_kernel<T><<<dim3(p.slices, a.m), kGemvThreads, 0, s>>>(a);
+    gemv_x_kernel<T><<<dim3(p.slices, a.m), 256, 0, s>>>(a);
     if (int e = check_launch("kab_gemv_fp4 x")) return e;
-    launch_after(kern, grid, p.smem, s, a);
+    launch_after(kern, grid, kGemvThreads, p.smem, s, a);
   } else {
     kern<<<grid, kGemvThreads, p.smem, s>>>(a);
   }
   if (int e = check_launch("kab_gemv_fp4")) return e;
   if (!p.join) return KAB_OK;
-  launch_after(gemv_join_kernel<T>, dim3((a.n + 255) / 256, a.m), 0, s, a);
+  launch_after(gemv_join_kernel<T>, dim3((a.n + 255) / 256, a.m), 256, 0, s, a);
   return check_launch("kab_gemv_fp4 join");
 }
 template <int T, int MX, int NT, int GROUPED>
