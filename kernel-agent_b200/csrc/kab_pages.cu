@@ -330,17 +330,31 @@ int kab_kv_pages_evict(const KabKvPages* cache, const int32_t* out_table, int64_
   a.sinks = static_cast<int>(sinks);
   const cudaStream_t s = as_stream(stream);
   const unsigned heads = static_cast<unsigned>(cache->heads_kv), batch = static_cast<unsigned>(cache->batch);
-  evict_select_kernel<<<dim3(heads, batch), 1024, 0, s>>>(a, status);
+  // blocks of a head's cluster: 4096 tokens each where 8 of them suffice
+  const int64_t capacity = cache->max_pages * cache->page_tokens;
+  const int blocks = capacity <= 4096 ? 1 : capacity <= 8192 ? 2 : capacity <= 16384 ? 4 : 8;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks), heads, batch);
+  cfg.blockDim = dim3(kSelectThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = static_cast<unsigned>(blocks);
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, evict_select_kernel, a, blocks, status);
   if (int e = check_launch("kab_kv_pages_evict select")) return e;
   const int64_t P = cache->page_tokens;
   const int64_t pages = std::min((budget + P - 1) / P, std::max<int64_t>(cache->max_pages, 1));
   const dim3 grid(static_cast<unsigned>(pages), heads, batch);
   const int half = cache->head_dim == 64 ? 2 : 3;
   const int ch = static_cast<int>((P << half) / 128);
-  if (ch <= 1) evict_move_kernel<1><<<grid, 128, 0, s>>>(a, half, status);
-  else if (ch <= 2) evict_move_kernel<2><<<grid, 128, 0, s>>>(a, half, status);
-  else if (ch <= 4) evict_move_kernel<4><<<grid, 128, 0, s>>>(a, half, status);
-  else evict_move_kernel<8><<<grid, 128, 0, s>>>(a, half, status);
+  if (ch <= 1) launch_after(evict_move_kernel<1>, grid, 128, s, a, half, status);
+  else if (ch <= 2) launch_after(evict_move_kernel<2>, grid, 128, s, a, half, status);
+  else if (ch <= 4) launch_after(evict_move_kernel<4>, grid, 128, s, a, half, status);
+  else launch_after(evict_move_kernel<8>, grid, 128, s, a, half, status);
   return check_launch("kab_kv_pages_evict move");
 }
 
