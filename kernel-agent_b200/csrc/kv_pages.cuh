@@ -218,6 +218,50 @@ __device__ __forceinline__ uint32_t mass_key(float m) {
   return (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 
+// The largest finite magnitude of 16 codes. Codes order like their magnitudes, so the maximum is
+// taken on the codes, two at a time; only a NaN (0x7F) needs the values.
+__device__ __forceinline__ float e4m3_amax16(const uint4& raw) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = __vmaxu2(top, __vmaxu2(w[i] & 0x007F007Fu, (w[i] >> 8) & 0x007F007Fu));
+  const uint32_t code = max(top & 0xFFFFu, top >> 16);
+  if (code != 0x7Fu) return e4m3_value_hw(static_cast<uint8_t>(code));
+  float v[16], most = 0.0f;
+  e4m3_unpack16(raw, v);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) most = fmaxf(most, fabsf(v[e]));  // fmaxf leaves NaN out
+  return most;
+}
+// e4m3(code * from / s) of 16 codes. Where from / s is a power of two 2^k with -15 <= k <= 15 the
+// products are exact in f16 (a code's last bit is at least 2^-9, and no result is above 448), two at a
+// time; otherwise in fp32.
+__device__ __forceinline__ uint4 e4m3_rescale16(const uint4& raw, float from, const PageDivisor& by) {
+  const float ratio = by(from);
+  const uint32_t bits = __float_as_uint(ratio);
+  if ((bits & 0x7FFFFFu) == 0 && bits >= (112u << 23) && bits <= (142u << 23) && by.inv != 0.0f) {
+    const __half2 f = __float2half2_rn(ratio);
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i]), __NV_E4M3);
+      const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i] >> 16), __NV_E4M3);
+      const __half2 l = __hmul2(*reinterpret_cast<const __half2*>(&lo), f);
+      const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&hi), f);
+      const uint32_t a = __nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&l), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t b = __nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&h), __NV_SATFINITE, __NV_E4M3);
+      o[i] = a | b << 16;
+    }
+    return make_uint4(o[0], o[1], o[2], o[3]);
+  }
+  float v[16];
+  e4m3_unpack16(raw, v);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) v[e] = by(__fmul_rn(v[e], from));
+  return e4m3_pack16(v);
+}
+
 struct EvictArgs {
   PagePool pool;
   const int32_t* out_table;
@@ -433,24 +477,17 @@ __global__ void __launch_bounds__(128) evict_move_kernel(EvictArgs a, int half, 
   for (int kv = 0; kv < 2; ++kv) {
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      float v[16];
-      e4m3_unpack16(raw[kv][i], v);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) top = max(top, finite_bits(__fmul_rn(v[e], from[kv][i])));
-    }
+    for (int i = 0; i < CH; ++i) top = max(top, finite_bits(__fmul_rn(e4m3_amax16(raw[kv][i]), from[kv][i])));
     const float s = page_scale_of(block_max(top, red));
     const PageDivisor by(s);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int c = tid + i * 128;
       if (c < chunks) {
-        float v[16];
-        e4m3_unpack16(raw[kv][i], v);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = by(__fmul_rn(v[e], from[kv][i]));
+        uint4 out = raw[kv][i];
+        if (from[kv][i] != s) out = e4m3_rescale16(out, from[kv][i], by);
         *reinterpret_cast<uint4*>(p.codes[kv] + to * p.sp[kv] + h * p.sh[kv] + (c >> half) * p.st[kv] +
-                                  (c & mask) * 16) = e4m3_pack16(v);
+                                  (c & mask) * 16) = out;
       }
     }
     if (tid == 0) p.scale[kv][to * p.ssp[kv] + h * p.ssh[kv]] = s;
