@@ -330,7 +330,8 @@ int kab_kv_pages_evict(const KabKvPages* cache, const int32_t* out_table, int64_
   a.sinks = static_cast<int>(sinks);
   const cudaStream_t s = as_stream(stream);
   const unsigned heads = static_cast<unsigned>(cache->heads_kv), batch = static_cast<unsigned>(cache->batch);
-  // blocks of a head's cluster: 4096 tokens each where 8 of them suffice
+  // blocks of a head's cluster: 4096 tokens each (8 keys per thread) where 8 of them suffice, else 8 of
+  // 16384 (32 keys)
   const int64_t capacity = cache->max_pages * cache->page_tokens;
   const int blocks = capacity <= 4096 ? 1 : capacity <= 8192 ? 2 : capacity <= 16384 ? 4 : 8;
   cudaLaunchConfig_t cfg = {};
@@ -344,7 +345,7 @@ int kab_kv_pages_evict(const KabKvPages* cache, const int32_t* out_table, int64_
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, evict_select_kernel, a, blocks, status);
+  cudaLaunchKernelEx(&cfg, capacity <= 32768 ? evict_select_kernel<8> : evict_select_kernel<32>, a, blocks, status);
   if (int e = check_launch("kab_kv_pages_evict select")) return e;
   const int64_t P = cache->page_tokens;
   const int64_t pages = std::min((budget + P - 1) / P, std::max<int64_t>(cache->max_pages, 1));

@@ -272,27 +272,32 @@ struct EvictArgs {
 };
 
 // One cluster of blocks per (sequence, KV head), each block with an equal run of the tokens that
-// compete, kSelectKeys keys per thread in registers (tokens past that are read again in each pass).
+// compete, KEYS keys per thread in registers (tokens past that are read again in each pass).
 // The key of the last token that stays is found 11, 11 and 10 bits at a time, from the top: a histogram
 // per block of the keys that share the bits found so far, the cluster's histograms summed through
 // distributed shared memory by every block. A pass over the tokens in order then writes those above
 // the key and, of those equal to it, the first ones. (One block per head, eight bits at a time and
-// the masses read again in each of five passes, took 113 us at 32768 tokens and 8 heads.)
-constexpr int kSelectThreads = 1024, kSelectKeys = 8;
+// the masses read again in each of five passes, took 113 us at 32768 tokens and 8 heads with its move.)
+constexpr int kSelectThreads = 512;
 
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
 }
-// The word at the same shared-memory address of block `rank` of the cluster.
-__device__ __forceinline__ uint32_t load_cluster(const uint32_t* p, int rank) {
-  uint32_t at, v;
+// The four words at the same shared-memory address (16-byte aligned) of block `rank` of the cluster.
+__device__ __forceinline__ uint4 load_cluster(const uint32_t* p, int rank) {
+  uint32_t at;
+  uint4 v;
   const uint32_t mine = static_cast<uint32_t>(__cvta_generic_to_shared(p));
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(mine), "r"(rank));
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(at)
+               : "memory");
   return v;
 }
 
-__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(EvictArgs a, int blocks, unsigned* status) {
+template <int KEYS>
+__global__ void __launch_bounds__(kSelectThreads, KEYS == 8 ? 2 : 1) evict_select_kernel(EvictArgs a, int blocks, unsigned* status) {
   // the move may be set up while this kernel runs: it waits for its end by itself
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const PagePool& p = a.pool;
@@ -304,10 +309,11 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(EvictArgs 
     for (int i = rank * kSelectThreads + tid; i < a.budget; i += blocks * kSelectThreads) kept[i] = i < n ? i : -1;
     return;
   }
-  __shared__ uint32_t hist[3][2048];
-  __shared__ uint32_t totals[2];       // this block's keys above the last one that stays, and equal to it
-  __shared__ uint32_t found[2], sums[32];
-  __shared__ int above[32], equal[32];
+  __shared__ __align__(16) uint32_t hist[3][2048];
+  __shared__ __align__(16) uint32_t totals[4];      // this block's keys above the last one that stays, and equal to it
+  constexpr int WARPS = kSelectThreads / 32;
+  __shared__ uint32_t found[2], sums[WARPS];
+  __shared__ int above[WARPS], equal[WARPS];
   const int lo = a.sinks, hi = n - a.recent;  // the tokens that compete
   for (int i = rank * kSelectThreads + tid; i < a.sinks; i += blocks * kSelectThreads) kept[i] = i;
   for (int i = rank * kSelectThreads + tid; i < a.recent; i += blocks * kSelectThreads)
@@ -320,20 +326,20 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(EvictArgs 
     const int page = page_of(p, b, t >> p.page_shift, status);
     return page < 0 ? 0u : mass_key(p.mass[page * p.msp + h * p.msh + (t & (P - 1))]);
   };
-  uint32_t keys[kSelectKeys];
+  uint32_t keys[KEYS];
 #pragma unroll
-  for (int i = 0; i < kSelectKeys; ++i) {
+  for (int i = 0; i < KEYS; ++i) {
     const int t = first + i * kSelectThreads + tid;
     keys[i] = t < last ? key_at(t) : 0u;
   }
   // f(token, key) for every token of this thread, in its order
   auto each = [&](auto&& f) {
 #pragma unroll
-    for (int i = 0; i < kSelectKeys; ++i) {
+    for (int i = 0; i < KEYS; ++i) {
       const int t = first + i * kSelectThreads + tid;
       if (t < last) f(t, keys[i]);
     }
-    for (int t = first + kSelectKeys * kSelectThreads + tid; t < last; t += kSelectThreads) f(t, key_at(t));
+    for (int t = first + KEYS * kSelectThreads + tid; t < last; t += kSelectThreads) f(t, key_at(t));
   };
   for (int i = tid; i < 3 * 2048; i += kSelectThreads) (&hist[0][0])[i] = 0;
   if (tid < 2) totals[tid] = 0;
@@ -345,14 +351,22 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(EvictArgs 
       if (done == 32 || (k >> done) == (prefix >> done)) atomicAdd(&hist[pass][(k >> shift) & mask], 1u);
     });
     cluster_barrier();
-    // bins 2047 - 2 tid and the one below, over the cluster; the largest digit with at least `want`
+    // bins 2047 - 4 tid and the three below, over the cluster; the largest digit with at least `want`
     // keys at or above it
-    uint32_t c[2] = {0, 0};
-    for (int r = 0; r < blocks; ++r) {
-      c[0] += load_cluster(&hist[pass][2047 - 2 * tid], r);
-      c[1] += load_cluster(&hist[pass][2046 - 2 * tid], r);
+    static_assert(kSelectThreads * 4 == 2048, "four bins per thread");
+    uint4 bins[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) bins[r] = r < blocks ? load_cluster(&hist[pass][2044 - 4 * tid], r) : make_uint4(0, 0, 0, 0);
+    uint32_t c[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      c[0] += bins[r].w;
+      c[1] += bins[r].z;
+      c[2] += bins[r].y;
+      c[3] += bins[r].x;
     }
-    uint32_t upto = c[0] + c[1];
+    const uint32_t here = c[0] + c[1] + c[2] + c[3];
+    uint32_t upto = here;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
@@ -360,13 +374,11 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(EvictArgs 
     }
     if (lane == 31) sums[warp] = upto;
     __syncthreads();
-    uint32_t lower = lane < warp ? sums[lane] : 0u;
-    lower = __reduce_add_sync(0xffffffffu, lower);
-    uint32_t before = lower + upto - c[0] - c[1];
+    uint32_t before = __reduce_add_sync(0xffffffffu, lane < warp ? sums[lane] : 0u) + upto - here;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       if (before < want && before + c[i] >= want) {
-        found[0] = prefix | (static_cast<uint32_t>(2047 - 2 * tid - i) << shift);
+        found[0] = prefix | (static_cast<uint32_t>(2047 - 4 * tid - i) << shift);
         found[1] = want - before;
       }
       before += c[i];
@@ -389,8 +401,9 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(EvictArgs 
   const int limit = static_cast<int>(want);
   int out = a.sinks, ties = 0;  // places and equal keys taken by the blocks before this one
   for (int r = 0; r < rank; ++r) {
-    out += static_cast<int>(load_cluster(&totals[0], r));
-    ties += static_cast<int>(load_cluster(&totals[1], r));
+    const uint4 there = load_cluster(totals, r);
+    out += static_cast<int>(there.x);
+    ties += static_cast<int>(there.y);
   }
   out += min(ties, limit);
   cluster_barrier();  // no block leaves while another may still read its shared memory
@@ -402,7 +415,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(EvictArgs 
       equal[warp] = __popc(me);
     }
     __syncthreads();
-    const int va = above[lane], ve = equal[lane];
+    const int va = lane < WARPS ? above[lane] : 0, ve = lane < WARPS ? equal[lane] : 0;
     const int pa = __reduce_add_sync(0xffffffffu, lane < warp ? va : 0), pe = __reduce_add_sync(0xffffffffu, lane < warp ? ve : 0);
     const int ta = __reduce_add_sync(0xffffffffu, va), te = __reduce_add_sync(0xffffffffu, ve);
     const uint32_t below = (1u << lane) - 1u;
@@ -415,11 +428,11 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(EvictArgs 
     __syncthreads();
   };
 #pragma unroll
-  for (int i = 0; i < kSelectKeys; ++i) {
+  for (int i = 0; i < KEYS; ++i) {
     const int t0 = first + i * kSelectThreads;
     if (t0 < last) tile(t0 + tid, keys[i]);
   }
-  for (int t0 = first + kSelectKeys * kSelectThreads; t0 < last; t0 += kSelectThreads) {
+  for (int t0 = first + KEYS * kSelectThreads; t0 < last; t0 += kSelectThreads) {
     const int t = t0 + tid;
     tile(t, t < last ? key_at(t) : 0u);
   }
