@@ -488,14 +488,12 @@ int kab_kv_decode_fp8(const KabKvDecodeParams* params, void* workspace, size_t w
 /* out[m, n] = tensor_scale[n or 0] * sum_k x[m, k] * e2m1(codes[n, k]) * scales[n, k / block]
  * (+ bias[n]): a weight-only FP4 linear for a few tokens, the activations as they are. codes
  * [n, k / 2] (low nibble = even k, 8-byte aligned rows), scales e4m3 per 16 (KAB_NVFP4) or e8m0
- * per 32 (KAB_MXFP4), [n, k / block] row-major or, with `swizzle`, in the 128 x 4 blocked layout
+ * per 32 (KAB_MXFP4), 4-byte aligned, [n, k / block] row-major or, with `swizzle`, in the 128 x 4 blocked layout
  * the GEMMs read. x [m, k] of `dtype` (row stride ldx elements, 16-byte aligned rows), bias of
- * `bias_dtype` or NULL, out [m, ldo] of `dtype`. Products are exact, sums fp32. The workspace
- * (kab_gemv_fp4_workspace; `bytes` may be 0) holds fp32 partial sums and, in its first
- * `zero_bytes`, counters: zero those once when it is allocated; every launch leaves them at zero.
- * It serves one stream at a time and one shape: another shape's counters may lie elsewhere. */
-int kab_gemv_fp4_workspace(int64_t m, int64_t n, int64_t k, int fmt, int dtype, size_t* bytes,
-                           size_t* zero_bytes);
+ * `bias_dtype` or NULL, out [m, ldo] of `dtype`. Products are exact, sums fp32. Rows of x past
+ * 32 read the weight again. The workspace (kab_gemv_fp4_workspace; may be 0 bytes, 256-byte aligned)
+ * is scratch of one launch: it serves one stream at a time and need not be cleared. */
+int kab_gemv_fp4_workspace(int64_t m, int64_t n, int64_t k, int fmt, int dtype, size_t* bytes);
 int kab_gemv_fp4(const void* x, int dtype, int64_t ldx, const uint8_t* codes, const uint8_t* scales,
                  int swizzle, int fmt, const float* tensor_scale, int scale_per_row, int64_t m,
                  int64_t n, int64_t k, const void* bias, int bias_dtype, void* out, int64_t ldo,
@@ -545,7 +543,7 @@ int kab_kv_pages_append(const KabKvPages* cache, const void* k, const void* v, i
  * the first lengths[b] - q_len + 1 + i; otherwise every query sees all. A query that sees
  * nothing gives zeros. With `use_mass`, every cached token's weight, summed over the query heads
  * of its KV head and the query tokens, is added to its mass. head_dim 64 or 128. The workspace:
- * as for kab_gemv_fp4. */
+ * as for kab_gemv_fp4 (with mass it holds the scores of every row and token of the page table). */
 typedef struct KabKvPagesAttention {
   KabKvPages cache;
   const void* q;
@@ -557,7 +555,7 @@ typedef struct KabKvPagesAttention {
   int64_t heads_q, q_len;
   void* out;
 } KabKvPagesAttention;
-int kab_kv_pages_attention_workspace(const KabKvPagesAttention* params, size_t* bytes, size_t* zero_bytes);
+int kab_kv_pages_attention_workspace(const KabKvPagesAttention* params, size_t* bytes);
 int kab_kv_pages_attention(const KabKvPagesAttention* params, void* workspace, size_t workspace_bytes,
                            void* stream);
 

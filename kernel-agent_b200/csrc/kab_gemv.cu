@@ -131,12 +131,10 @@ using namespace kab;
 
 extern "C" {
 
-int kab_gemv_fp4_workspace(int64_t m, int64_t n, int64_t k, int fmt, int dtype, size_t* bytes,
-                           size_t* zero_bytes) {
+int kab_gemv_fp4_workspace(int64_t m, int64_t n, int64_t k, int fmt, int dtype, size_t* bytes) {
   if (int e = gemv_check(m, n, k, fmt, dtype)) return e;
-  KAB_REQUIRE(bytes != nullptr && zero_bytes != nullptr, "null pointer");
+  KAB_REQUIRE(bytes != nullptr, "null pointer");
   *bytes = m == 0 || n == 0 ? 0 : gemv_plan(m, n, k, fmt, dtype).bytes();
-  *zero_bytes = 0;
   return KAB_OK;
 }
 

@@ -270,15 +270,14 @@ int kab_kv_pages_append(const KabKvPages* cache, const void* k, const void* v, i
   return KAB_OK;
 }
 
-int kab_kv_pages_attention_workspace(const KabKvPagesAttention* params, size_t* bytes, size_t* zero_bytes) {
+int kab_kv_pages_attention_workspace(const KabKvPagesAttention* params, size_t* bytes) {
   PagesAttnArgs g{};
   if (int e = attention_check(params, &g)) return e;
-  KAB_REQUIRE(bytes != nullptr && zero_bytes != nullptr, "null pointer");
+  KAB_REQUIRE(bytes != nullptr, "null pointer");
   AttentionPlan plan;
   if (params->cache.batch > 0 && g.rows > 0)
     if (int e = attention_plan(params, g, &plan)) return e;
   *bytes = plan.bytes();
-  *zero_bytes = 0;
   return KAB_OK;
 }
 

@@ -175,12 +175,12 @@ _SIGNATURES: dict[str, list] = {
                          c_void_p, c_int64, c_int64, c_void_p],
     "kab_kv_decode_workspace": [POINTER(KabKvDecodeParams), POINTER(c_int), POINTER(c_size_t)],
     "kab_kv_decode_fp8": [POINTER(KabKvDecodeParams), c_void_p, c_size_t, c_void_p],
-    "kab_gemv_fp4_workspace": [c_int64, c_int64, c_int64, c_int, c_int, POINTER(c_size_t), POINTER(c_size_t)],
+    "kab_gemv_fp4_workspace": [c_int64, c_int64, c_int64, c_int, c_int, POINTER(c_size_t)],
     "kab_gemv_fp4": [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_int64, c_int64,
                      c_int64, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_size_t, c_void_p],
     "kab_kv_pages_append": [POINTER(KabKvPages), c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64,
                             c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p],
-    "kab_kv_pages_attention_workspace": [POINTER(KabKvPagesAttention), POINTER(c_size_t), POINTER(c_size_t)],
+    "kab_kv_pages_attention_workspace": [POINTER(KabKvPagesAttention), POINTER(c_size_t)],
     "kab_kv_pages_attention": [POINTER(KabKvPagesAttention), c_void_p, c_size_t, c_void_p],
     "kab_kv_pages_evict": [POINTER(KabKvPages), c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p,
                            c_void_p],

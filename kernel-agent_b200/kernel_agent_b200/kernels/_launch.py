@@ -1,6 +1,5 @@
 """What a launch needs from torch, at a decode step's pace: the tensors' device, the current
-stream as the C ABI takes it, a device guard only where one is needed, and scratch buffers of the
-kernels that leave counters at zero after every launch."""
+stream as the C ABI takes it, a device guard only where one is needed, and scratch buffers."""
 
 from __future__ import annotations
 
@@ -42,23 +41,19 @@ def stream_of(device: int) -> int:
     return torch._C._cuda_getCurrentRawStream(device)
 
 
-def workspace(op: tuple | str, device: int, stream: int, nbytes: int, zero_bytes: int) -> torch.Tensor:
-    """``nbytes`` of scratch for ``op`` on ``stream`` whose first ``zero_bytes`` are zero. The
-    kernels put their counters there and leave them at zero, so a buffer is zeroed only when it
-    is made, on the stream that uses it; ``op`` names everything that decides where the counters
-    lie. While a CUDA graph is captured every call makes its own (it belongs to the graph, which
-    zeroes it at every replay)."""
+def workspace(op: str, device: int, stream: int, nbytes: int) -> torch.Tensor:
+    """``nbytes`` of scratch for ``op`` on ``stream``, kept for its next call there (a call's contents
+    mean nothing to the next). While a CUDA graph is captured every call makes its own: it belongs to
+    the graph, which may be replayed beside other work."""
     if torch._C._cuda_isCurrentStreamCapturing():
-        return _make(device, nbytes, zero_bytes)
-    key = (op, device, stream, zero_bytes)
+        return torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", device))
+    key = (op, device, stream)
     buf = _BUFFERS.get(key)
     if buf is None or buf.numel() < nbytes:
-        buf = _BUFFERS[key] = _make(device, nbytes, zero_bytes)
+        buf = _BUFFERS[key] = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", device))
     return buf
 
 
-def _make(device: int, nbytes: int, zero_bytes: int) -> torch.Tensor:
-    buf = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", device))
-    if zero_bytes:
-        buf[:zero_bytes].zero_()
-    return buf
+def to_device(values: list, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """A small host list as a device tensor, without waiting for the GPU (through pinned memory)."""
+    return torch.tensor(values, dtype=dtype).pin_memory().to(device, non_blocking=True)

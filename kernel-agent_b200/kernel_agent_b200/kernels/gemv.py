@@ -20,18 +20,18 @@ from ._launch import device_of, guard, stream_of, workspace
 from .gemm import _bias
 
 _FORMATS = {"nvfp4": (nat.KAB_NVFP4, 16), "mxfp4": (nat.KAB_MXFP4, 32)}
-_PLANS: dict[tuple, tuple[int, int]] = {}
+_PLANS: dict[tuple, int] = {}
 
 
-def _plan(m: int, n: int, k: int, fmt: int, dtype: int, device: int | None) -> tuple[int, int]:
-    """Workspace bytes of a shape, and how many of them start at zero (asked once)."""
+def _plan(m: int, n: int, k: int, fmt: int, dtype: int, device: int) -> int:
+    """Workspace bytes of a shape (asked once)."""
     key = (m, n, k, fmt, dtype, device)
-    plan = _PLANS.get(key)
-    if plan is None:
-        nbytes, zero = ctypes.c_size_t(0), ctypes.c_size_t(0)
-        nat.call("kab_gemv_fp4_workspace", m, n, k, fmt, dtype, ctypes.byref(nbytes), ctypes.byref(zero))
-        plan = _PLANS[key] = (int(nbytes.value), int(zero.value))
-    return plan
+    nbytes = _PLANS.get(key)
+    if nbytes is None:
+        found = ctypes.c_size_t(0)
+        nat.call("kab_gemv_fp4_workspace", m, n, k, fmt, dtype, ctypes.byref(found))
+        nbytes = _PLANS[key] = int(found.value)
+    return nbytes
 
 
 def fp4_w4a16_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, tensor_scale: torch.Tensor | float,
@@ -44,7 +44,7 @@ def fp4_w4a16_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     block]`` (e4m3 per 16 for ``fmt="nvfp4"``, e8m0 per 32 for ``"mxfp4"``) or the same already
     swizzled (flat, 128 x 4 blocks); ``tensor_scale`` one value or one per row of the weight.
     Made for up to about 32 rows of ``x``, where the weight's bytes bound it; more rows work, the
-    weight being read again for every 8."""
+    weight being read again for every 32."""
     if fmt not in _FORMATS:
         raise ValueError(f"unknown FP4 format {fmt!r} (one of {', '.join(_FORMATS)})")
     code, block = _FORMATS[fmt]
@@ -85,14 +85,17 @@ def fp4_w4a16_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     per_row = ts.numel() > 1
     if ts.numel() != (n if per_row else 1):
         raise ValueError(f"tensor_scale has {ts.numel()} values, expected 1 or {n}")
-    b, bias_code = (None, nat.KAB_F32) if bias is None else _bias(bias, n, x.device)
-    out = torch.empty((m, n), dtype=x2.dtype, device=x.device)
+    if bias is None or (bias.dtype in nat.DTYPES and bias.shape == (n,) and bias.is_contiguous()):
+        b, bias_code = bias, nat.KAB_F32 if bias is None else nat.DTYPES[bias.dtype]
+    else:
+        b, bias_code = _bias(bias, n, x.device)
+    out = x2.new_empty((m, n))
     if m and n:
         dtype = nat.DTYPES[x2.dtype]
         with guard(device):
             stream = stream_of(device)
-            nbytes, zero = _plan(m, n, k, code, dtype, device)
-            ws = workspace("gemv", device, stream, nbytes, zero) if nbytes else None
+            nbytes = _plan(m, n, k, code, dtype, device)
+            ws = workspace("gemv", device, stream, nbytes) if nbytes else None
             nat.call("kab_gemv_fp4", x2.data_ptr(), dtype, x2.stride(0) if m > 1 else max(k, 8), c.data_ptr(),
                      s.data_ptr(), swizzle, code, ts.data_ptr(), per_row, m, n, k, None if b is None else b.data_ptr(),
                      bias_code, out.data_ptr(), n, None if ws is None else ws.data_ptr(), nbytes, stream)

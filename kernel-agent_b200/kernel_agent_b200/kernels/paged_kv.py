@@ -26,7 +26,7 @@ import ctypes
 import torch
 
 from .. import _native as nat
-from ._launch import device_of, guard, stream_of, workspace
+from ._launch import device_of, guard, stream_of, to_device, workspace
 
 _E4M3 = torch.float8_e4m3fn
 PAGE_TOKENS = (16, 32, 64, 128)
@@ -154,7 +154,8 @@ def paged_kv_attention(q: torch.Tensor, k_pages: torch.Tensor, k_scale: torch.Te
     ``lengths[b] - Lq + 1 + i`` tokens; without it every query sees every token. A query that sees
     nothing gives zeros. With ``mass``, the weight of every cached token, summed over the query
     heads of its KV head and the query tokens, is added to its entry. Made for the few rows (query
-    heads per KV head x query tokens) of a decode step: each 16 rows read the cache once more.
+    heads per KV head x query tokens) of a decode step: each 16 rows (8 where there are no more) read
+    the cache once.
     Results do not depend on the other sequences' lengths but in the last bits (the cache is cut
     into equal parts for the GPU, whose softmax sums are merged), and are the same for the same
     inputs."""
@@ -181,13 +182,13 @@ def paged_kv_attention(q: torch.Tensor, k_pages: torch.Tensor, k_scale: torch.Te
         t.q_stride_b, t.q_stride_h, t.q_stride_t = q4.stride()[:3]
         t.heads_q, t.q_len = hq, lq
         _pointers(t.cache, *cache)
-        nbytes, zero = ctypes.c_size_t(0), ctypes.c_size_t(0)
+        nbytes = ctypes.c_size_t(0)
         with guard(device):
-            nat.call("kab_kv_pages_attention_workspace", ctypes.byref(t), ctypes.byref(nbytes), ctypes.byref(zero))
-        made = _TEMPLATES[key] = (bytes(t), int(nbytes.value), int(zero.value))
-    template, nbytes, zero = made
+            nat.call("kab_kv_pages_attention_workspace", ctypes.byref(t), ctypes.byref(nbytes))
+        made = _TEMPLATES[key] = (bytes(t), int(nbytes.value))
+    template, nbytes = made
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
         raise ValueError(f"out must be {q.dtype} {list(q.shape)}, contiguous; got {out.dtype} {tuple(out.shape)}")
     p = nat.KabKvPagesAttention.from_buffer_copy(template)
@@ -195,7 +196,7 @@ def paged_kv_attention(q: torch.Tensor, k_pages: torch.Tensor, k_scale: torch.Te
     p.q, p.out = q4.data_ptr(), out.data_ptr()
     with guard(device):
         stream = stream_of(device)
-        ws = workspace("pages attention", device, stream, nbytes, zero) if nbytes else None
+        ws = workspace("pages attention", device, stream, nbytes) if nbytes else None
         nat.call("kab_kv_pages_attention", ctypes.byref(p), nat.ptr(ws), nbytes, stream)
     return out
 
@@ -226,9 +227,126 @@ def evict_kv_pages(k_pages: torch.Tensor, k_scale: torch.Tensor, v_pages: torch.
                          f"{out_page_table.dtype} {tuple(out_page_table.shape)}")
     if out_page_table.data_ptr() == page_table.data_ptr() and page_table.numel():
         raise ValueError("out_page_table must name other pages than page_table")
-    kept = torch.empty(p.batch, p.heads_kv, budget, dtype=torch.int32, device=mass.device)
+    kept = lengths.new_empty((p.batch, p.heads_kv, budget))
     out = torch.empty_like(lengths)
     with guard(device):
         nat.call("kab_kv_pages_evict", ctypes.byref(p), out_page_table.data_ptr(), out_page_table.stride(0), budget,
                  recent, sinks, kept.data_ptr(), out.data_ptr(), stream_of(device))
     return kept, out
+
+
+class PagedFp8KVCache:
+    """A pool of FP8 pages with the page table, lengths and free pages of ``batch`` sequences.
+
+    :meth:`append` takes pages as sequences grow, :meth:`attend` reads the cache (and, with ``mass``,
+    keeps every token's received weight), :meth:`evict` cuts sequences to a budget of tokens and
+    frees the pages they leave, :meth:`free` ends a sequence. Page numbers are kept on the host, so
+    nothing waits for the GPU; the calls follow one another on the current stream. A step captured
+    in a CUDA graph calls the functions of this module on :attr:`pool` after :meth:`reserve`."""
+
+    def __init__(self, batch: int, kv_heads: int, head_dim: int, num_pages: int, page_tokens: int = 64,
+                 max_pages: int | None = None, mass: bool = True, device: torch.device | str | None = None) -> None:
+        if page_tokens not in PAGE_TOKENS:
+            raise ValueError(f"page_tokens {page_tokens}: one of {', '.join(map(str, PAGE_TOKENS))}")
+        if head_dim not in HEAD_DIMS:
+            raise ValueError(f"head_dim {head_dim}: the paged cache takes 64 or 128")
+        dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        if dev.type != "cuda":
+            raise ValueError("CUDA device required (kernel_agent_b200 runs on the GPU only)")
+        shape = (num_pages, kv_heads, page_tokens, head_dim)
+        self.k_pages = torch.zeros(shape, dtype=_E4M3, device=dev)
+        self.v_pages = torch.zeros(shape, dtype=_E4M3, device=dev)
+        self.k_scale = torch.ones(shape[:2], dtype=torch.float32, device=dev)
+        self.v_scale = torch.ones(shape[:2], dtype=torch.float32, device=dev)
+        self.mass = torch.zeros(shape[:3], dtype=torch.float32, device=dev) if mass else None
+        self.max_pages = num_pages if max_pages is None else max_pages
+        self.page_table = torch.zeros(batch, self.max_pages, dtype=torch.int32, device=dev)
+        self.lengths = torch.zeros(batch, dtype=torch.int32, device=dev)
+        self.page_tokens = page_tokens
+        #: Cached tokens of each sequence, as the host knows them.
+        self.tokens = [0] * batch
+        self._pages: list[list[int]] = [[] for _ in range(batch)]
+        self._free = list(range(num_pages - 1, -1, -1))
+
+    @property
+    def pool(self) -> tuple[torch.Tensor, ...]:
+        """``(k_pages, k_scale, v_pages, v_scale, page_table, lengths)``, as the functions take them."""
+        return self.k_pages, self.k_scale, self.v_pages, self.v_scale, self.page_table, self.lengths
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def _write_table(self) -> None:
+        rows = [pages + [0] * (self.max_pages - len(pages)) for pages in self._pages]
+        self.page_table.copy_(to_device(rows, torch.int32, self.page_table.device).reshape(self.page_table.shape))
+
+    def reserve(self, counts: list[int]) -> None:
+        """Take the pages that ``counts[b]`` more tokens of each sequence need."""
+        if len(counts) != len(self.tokens) or min(counts, default=0) < 0:
+            raise ValueError(f"counts must be {len(self.tokens)} numbers of tokens; got {counts}")
+        need = [max(0, -(-(t + c) // self.page_tokens) - len(p)) for t, c, p in zip(self.tokens, counts, self._pages)]
+        if sum(need) > len(self._free):
+            raise ValueError(f"paged KV cache full: {sum(need)} pages wanted, {len(self._free)} free")
+        if any(len(p) + n > self.max_pages for p, n in zip(self._pages, need)):
+            raise ValueError(f"a sequence would pass {self.max_pages} pages")
+        if any(need):
+            for pages, n in zip(self._pages, need):
+                pages += [self._free.pop() for _ in range(n)]
+            self._write_table()
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, counts: list[int] | None = None) -> None:
+        """Append ``k``, ``v [batch, kv_heads, new, head_dim]``, the first ``counts[b]`` tokens of each
+        sequence (default: all), as :func:`append_kv_pages` does."""
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the cache counts tokens on the host: reserve() first and capture append_kv_pages")
+        if k.dim() != 4:
+            raise ValueError(f"expected k and v [batch, kv_heads, new, head_dim]; got {tuple(k.shape)}")
+        new = k.shape[2]
+        each = [new] * len(self.tokens) if counts is None else [int(c) for c in counts]
+        if any(c < 0 or c > new for c in each):
+            raise ValueError(f"counts must lie in 0..{new}; got {each}")
+        self.reserve(each)
+        count = None if counts is None else to_device(each, torch.int32, self.lengths.device)
+        append_kv_pages(k, v, *self.pool, counts=count, mass=self.mass, out_lengths=self.lengths)
+        self.tokens = [t + c for t, c in zip(self.tokens, each)]
+
+    def attend(self, q: torch.Tensor, scale: float | None = None, causal: bool = True) -> torch.Tensor:
+        """:func:`paged_kv_attention` of ``q`` over the cache; adds to :attr:`mass` where there is one."""
+        return paged_kv_attention(q, *self.pool, scale=scale, causal=causal, mass=self.mass)
+
+    def evict(self, budget: int, recent: int = 0, sinks: int = 0) -> tuple[list[int], torch.Tensor | None]:
+        """Cut every sequence of more than ``budget`` tokens to ``budget``, as :func:`evict_kv_pages`
+        does, and free the pages it leaves. Returns ``(sequences, kept)``: which were cut, and their
+        kept token numbers ``[len(sequences), kv_heads, budget]`` (None if none were)."""
+        if self.mass is None:
+            raise ValueError("an eviction needs the tokens' mass: make the cache with mass=True")
+        if budget < 1 or recent < 0 or sinks < 0 or sinks + recent > budget:
+            raise ValueError(f"budget {budget} must be at least 1 and hold the {sinks} first and {recent} last tokens")
+        over = [b for b, n in enumerate(self.tokens) if n > budget]
+        if not over:
+            return [], None
+        each = -(-budget // self.page_tokens)
+        if each * len(over) > len(self._free):
+            raise ValueError(f"paged KV cache full: an eviction moves into {each * len(over)} pages, "
+                             f"{len(self._free)} free")
+        to = [[self._free.pop() for _ in range(each)] for _ in over]
+        dev = self.lengths.device
+        which = to_device(over, torch.int64, dev)
+        target = to_device(to, torch.int32, dev)
+        kept, lengths = evict_kv_pages(self.k_pages, self.k_scale, self.v_pages, self.v_scale, self.mass,
+                                       self.page_table[which], self.lengths[which], target, budget=budget,
+                                       recent=recent, sinks=sinks)
+        self.lengths[which] = lengths
+        for b, pages in zip(over, to):
+            self._free += self._pages[b]
+            self._pages[b], self.tokens[b] = pages, budget
+        self._write_table()
+        return over, kept
+
+    def free(self, sequence: int) -> None:
+        """End a sequence: its pages are free, its row of the batch is empty."""
+        self._free += self._pages[sequence]
+        self._pages[sequence], self.tokens[sequence] = [], 0
+        self.lengths[sequence] = 0
+        self._write_table()
