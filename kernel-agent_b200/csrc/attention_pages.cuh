@@ -746,26 +746,38 @@ __global__ void __launch_bounds__(512) pages_merge_kernel(PagesAttnArgs a) {
 }
 
 // The mass of every cached token: its weights, from the stored scores and the rows' final
-// reference and sum, added in the order of the rows. One thread per token and KV head.
+// reference and sum, added in the order of the rows. One thread per four tokens and KV head (they
+// stand in one page), one 16-byte load per row.
 __global__ void __launch_bounds__(256) pages_mass_kernel(PagesAttnArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const PagePool& p = a.pool;
   const int h = blockIdx.y, b = blockIdx.z;
   const int n = min(max(__ldg(p.lengths + b), 0), p.max_pages << p.page_shift);
-  const int x = blockIdx.x * 256 + threadIdx.x;
+  const int x = (blockIdx.x * 256 + threadIdx.x) * 4;
   if (x >= n) return;
   const int page = __ldg(p.table + b * p.table_stride + (x >> p.page_shift));
   if (page < 0 || page >= p.num_pages) return;  // reported by the attention
+  float* mass = p.mass + page * p.msp + h * p.msh + (x & ((1 << p.page_shift) - 1));
+  float held[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) held[e] = x + e < n ? mass[e] : 0.0f;
   const int64_t row0 = (static_cast<int64_t>(b) * p.heads + h) * a.rows;
   const float* s = a.scores + row0 * a.capacity + x;
   const float2* ml = reinterpret_cast<const float2*>(a.ml) + row0;
-  float received = 0.0f;
+  float received[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
   for (int r = 0; r < a.rows; ++r) {
     const float2 f = __ldg(ml + r);
-    received += exp2_approx(__ldg(s + r * a.capacity) - f.x) * f.y;
+    const float4 v = __ldg(reinterpret_cast<const float4*>(s + r * a.capacity));
+    received[0] += exp2_approx(v.x - f.x) * f.y;
+    received[1] += exp2_approx(v.y - f.x) * f.y;
+    received[2] += exp2_approx(v.z - f.x) * f.y;
+    received[3] += exp2_approx(v.w - f.x) * f.y;
   }
-  p.mass[page * p.msp + h * p.msh + (x & ((1 << p.page_shift) - 1))] += received;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (x + e < n) mass[e] = held[e] + received[e];
+  }
 }
 
 }  // namespace kab

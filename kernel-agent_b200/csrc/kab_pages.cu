@@ -212,7 +212,7 @@ int launch_attention(const PagesAttnArgs& g, const AttentionPlan& plan, unsigned
     launch_after(pages_merge_kernel<T, D, L::kRows, 4>, dim3(plan.merges, (rows + 3) / 4), 512, s, g);
   if (int e = check_launch("kab_kv_pages_attention merge")) return e;
   if (g.scores == nullptr || g.capacity == 0) return KAB_OK;
-  const dim3 blocks(static_cast<unsigned>((g.capacity + 255) / 256), g.pool.heads, g.pool.batch);
+  const dim3 blocks(static_cast<unsigned>((g.capacity + 1023) / 1024), g.pool.heads, g.pool.batch);
   launch_after(pages_mass_kernel, blocks, 256, s, g);
   return check_launch("kab_kv_pages_attention mass");
 }
