@@ -29,13 +29,14 @@
 //    split into two f16 terms (22 bits) and multiplied twice. It stays in shared memory while a block
 //    streams its rows, converted there for one token, by a launch before for more.
 //  * The (32-row tile, 256-code chunk) pairs of a K slice stand in one line, cut into equal parts for
-//    the blocks and again for their warps: every warp streams its part through a ring of its own in
-//    shared memory (cp.async, whole 128-byte lines of a row) and waits for nobody. 32 rows share one
-//    read of x, and lines in place of 64-byte pieces keep L1's data pipe, which bounded the kernel
-//    before (66 % busy at 3.9 TB/s), below the stream. Tiles that lie within a warp are written by it;
-//    those that several warps of a block share are added in shared memory at the end, those that two
-//    blocks share (and the slices of K, where x does not fit in shared memory) in another launch,
-//    always in the order of the line.
+//    the blocks. A block's warps take its units in turn, each through a ring of its own in shared
+//    memory (cp.async, whole 128-byte lines of a row), so that together they read a kilobyte of each
+//    row at a time (one warp alone after another along a row, 128 bytes at a time, read 4.3 TB/s of
+//    DRAM), and wait for nobody: every warp leaves its sums of every tile in shared memory and they are
+//    added at the end, in the order of the warps. 32 rows share one read of x, and lines in place of
+//    64-byte pieces keep L1's data pipe, which bounded an earlier form (66 % busy at 3.9 TB/s), below
+//    the stream. Tiles that two blocks share, and the slices of K where x does not fit in shared
+//    memory, are added by another launch, in the order of the line.
 #pragma once
 
 #include "codes.cuh"
@@ -137,9 +138,10 @@ __host__ __device__ constexpr int gemv_stage_bytes(bool mx) { return kGemvRows *
 // Bytes of one token's slice of x (hi terms, and lo terms for fp32): a multiple of 512 and 64 more,
 // so that the tokens of a group lie in different banks.
 __host__ __device__ constexpr int gemv_pitch(int slice_chunks) { return slice_chunks * 512 + 64; }
-__host__ __device__ constexpr int gemv_smem(bool mx, int m, int slice_chunks, int columns, bool split) {
+// `spans`: tiles that a block's part of the line can touch.
+__host__ __device__ constexpr int gemv_smem(bool mx, int m, int slice_chunks, int columns, bool split, int spans) {
   return kGemvWarps * kGemvStages * gemv_stage_bytes(mx) + m * gemv_pitch(slice_chunks) * (split ? 2 : 1) + 256 +
-         kGemvWarps * kGemvRows * columns * 4 + columns * 4 + 2 * kGemvWarps * 4;
+         spans * kGemvWarps * kGemvRows * columns * 4 + columns * 4;
 }
 // Tokens that NT groups of the MMA's columns take.
 constexpr int gemv_columns(bool mx, int nt, bool grouped) { return grouped ? (mx ? 2 * nt : nt) : 8 * nt; }
@@ -226,33 +228,27 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
   const int c_first = slice * a.slice_chunks, c_count = min(a.slice_chunks, a.chunks - c_first);
   const int pitch = gemv_pitch(a.slice_chunks);
   uint8_t* zeros = smem + tokens * pitch * (SPLIT ? 2 : 1);  // 256 bytes: what a column's other lanes read
-  float* sums = reinterpret_cast<float*>(zeros + 256);       // [8 warps][32][COLS]: tiles begun before a warp
-  float* unit = sums + kGemvWarps * kGemvRows * COLS;        // [COLS]
-  int* seg_tile = reinterpret_cast<int*>(unit + COLS);       // [8 warps][2]: 2 * tile + (its end is here), or -1
-  // the sums of a tile that began before warp w (first), or of the one it leaves unfinished: its last,
-  // so they fit in its ring
-  auto sums_of = [&](int w, int first) -> float* {
-    return first ? sums + w * kGemvRows * COLS : reinterpret_cast<float*>(smem_all + w * kGemvStages * STAGE);
-  };
-  static_assert(kGemvStages * STAGE >= kGemvRows * COLS * 4, "a tile's sums fit in a ring");
+  float* unit = reinterpret_cast<float*>(zeros + 256);        // [COLS]
+  float* sums = unit + COLS;                                  // [tiles of the block][8 warps][32][COLS]
 
-  // ---- this warp's part of the line
+  // ---- this block's part of the line
   const GemvCut cut(a.tiles * c_count, a.blocks);
   const int b_lo = cut.begin(blockIdx.x), b_hi = cut.begin(blockIdx.x + 1);
-  const GemvCut warps(b_hi - b_lo, kGemvWarps);
-  const int u_lo = b_lo + warps.begin(warp), u_hi = b_lo + warps.begin(warp + 1);
+  const int tile_lo = b_lo / c_count, spans = (b_hi - 1) / c_count - tile_lo + 1;
+  const int step_tiles = kGemvWarps / c_count, step_chunks = kGemvWarps % c_count;
+  for (int i = tid; i < spans * kGemvWarps * kGemvRows * COLS; i += kGemvThreads) sums[i] = 0.0f;
   const int cols = a.k >> (MX ? 5 : 4), half = a.k >> 1;
-  if (tid < 2 * kGemvWarps) seg_tile[tid] = -1;
   if (tid < 16) reinterpret_cast<uint4*>(zeros)[tid] = make_uint4(0, 0, 0, 0);
 
-  int is_unit = u_lo, is_tile = u_lo / c_count, is_chunk = u_lo % c_count;  // what the next issue loads
+  // what the next issue loads
+  int is_unit = b_lo + warp, is_tile = is_unit / c_count, is_chunk = is_unit % c_count;
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem_all)) + warp * kGemvStages * STAGE;
   const int64_t scale_bytes = static_cast<int64_t>(a.n) * cols;
   // A quarter of a row's 16-byte pieces change places on odd rows, so that the fragments' reads (two
   // neighbouring rows x four pieces) touch all banks. Every copy is made at the nearest place that
   // exists: rows past n are not written, and x is zero past K.
   auto issue = [&](int stage) {
-    if (is_unit < u_hi) {
+    if (is_unit < b_hi) {
       const uint32_t to = ring + stage * STAGE;
       const int chunk = c_first + is_chunk, row0 = is_tile * kGemvRows;
       {
@@ -290,9 +286,11 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
           asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(at), "l"(a.scales + there), "r"(bytes) : "memory");
         }
       }
-      ++is_unit;
-      if (++is_chunk == c_count) {
-        is_chunk = 0;
+      is_unit += kGemvWarps;
+      is_tile += step_tiles;
+      is_chunk += step_chunks;
+      if (is_chunk >= c_count) {
+        is_chunk -= c_count;
         ++is_tile;
       }
     }
@@ -514,16 +512,10 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
       a.partial[((static_cast<int64_t>(max(part, 0)) * a.slices + slice) * a.m + m0 + mt) * a.n + row] = y;
     }
   };
-  int tile = u_lo / c_count, chunk = u_lo % c_count, begun = chunk;
-  auto end_segment = [&]() {
-    const bool ends = chunk == c_count - 1, whole = begun == 0 && ends;
-    const int seg = warp * 2 + (begun == 0);  // 0: the tile began before this warp, 1: it begins here
-    float* mine = sums_of(warp, begun != 0);
-    __syncwarp();  // the ring's last reads
-    auto one = [&](int r, int mt, float y) {
-      if (whole) put(tile, r, mt, y, -1);
-      else mine[r * COLS + mt] = y;
-    };
+  int tile = (b_lo + warp) / c_count, chunk = (b_lo + warp) % c_count;
+  // this warp's sums of a tile
+  auto leave = [&]() {
+    float* at = sums + ((tile - tile_lo) * kGemvWarps + warp) * kGemvRows * COLS;
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
 #pragma unroll
@@ -543,28 +535,26 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
           }
           if (t == 0) {
             if constexpr (MX) {
-              one(r, 2 * j, v[0]);
-              one(r, 2 * j + 1, v[1]);
-              one(r + 8, 2 * j, v[2]);
-              one(r + 8, 2 * j + 1, v[3]);
+              at[r * COLS + 2 * j] = v[0];
+              at[r * COLS + 2 * j + 1] = v[1];
+              at[(r + 8) * COLS + 2 * j] = v[2];
+              at[(r + 8) * COLS + 2 * j + 1] = v[3];
             } else {
-              one(r, j, v[0]);
-              one(r + 8, j, v[2]);
+              at[r * COLS + j] = v[0];
+              at[(r + 8) * COLS + j] = v[2];
             }
           }
         } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) one(r + 8 * (e >> 1), j * 8 + 2 * t + (e & 1), acc[q][j][e]);
+          for (int e = 0; e < 4; ++e) at[(r + 8 * (e >> 1)) * COLS + j * 8 + 2 * t + (e & 1)] = acc[q][j][e];
         }
       }
     }
     clear(acc);
-    if (!whole && lane == 0) seg_tile[seg] = 2 * tile + ends;
-    begun = 0;
   };
 
   int stage = 0;
-  for (int u = u_lo; u < u_hi; ++u) {
+  for (int u = b_lo + warp; u < b_hi; u += kGemvWarps) {
     if (a.k > 0) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kGemvStages - 2) : "memory");
       __syncwarp();
@@ -605,27 +595,21 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
         consume(w, s, chunk * 2 + h);
       }
     }
-    if (chunk == c_count - 1 || u == u_hi - 1) end_segment();
-    if (++chunk == c_count) {
-      chunk = 0;
-      ++tile;
-    }
+    const int next_chunk = chunk + step_chunks, next_tile = tile + step_tiles + (next_chunk >= c_count);
+    if (next_tile != tile || u + kGemvWarps >= b_hi) leave();
+    tile = next_tile;
+    chunk = next_chunk >= c_count ? next_chunk - c_count : next_chunk;
     stage = stage == kGemvStages - 1 ? 0 : stage + 1;
   }
   __syncthreads();
-  // the tiles that warps share: from where they begin in this block (a warp's second segment, or the
-  // first warp's first), through the following warps' first segments
-  for (int i = tid; i < (kGemvWarps + 1) * kGemvRows * COLS; i += kGemvThreads) {
-    const int head = i / (kGemvRows * COLS), cell = i % (kGemvRows * COLS);
-    const int seg = head == 0 ? 0 : (head - 1) * 2 + 1, first = seg_tile[seg];
-    if (first < 0) continue;
-    float y = sums_of(seg >> 1, head == 0)[cell];
-    int end = first & 1;
-    for (int w = (seg >> 1) + 1; w < kGemvWarps && seg_tile[2 * w] >= 0 && seg_tile[2 * w] >> 1 == first >> 1; ++w) {
-      y += sums_of(w, 1)[cell];
-      end = seg_tile[2 * w] & 1;
-    }
-    put(first >> 1, cell / COLS, cell % COLS, y, head == 0 ? 1 : end ? -1 : 0);
+  for (int i = tid; i < spans * kGemvRows * COLS; i += kGemvThreads) {
+    const int s = i / (kGemvRows * COLS), cell = i % (kGemvRows * COLS), first = (tile_lo + s) * c_count;
+    const float* at = sums + s * kGemvWarps * kGemvRows * COLS + cell;
+    float y = at[0];
+#pragma unroll
+    for (int w = 1; w < kGemvWarps; ++w) y += at[w * kGemvRows * COLS];
+    // begun in the block before: its second part; ended in the next one: its first
+    put(tile_lo + s, cell / COLS, cell % COLS, y, first < b_lo ? 1 : first + c_count > b_hi ? 0 : -1);
   }
 }
 
