@@ -33,7 +33,9 @@
 //    memory (cp.async, whole 128-byte lines of a row), so that together they read a kilobyte of each
 //    row at a time (one warp alone after another along a row, 128 bytes at a time, read 4.3 TB/s of
 //    DRAM), and wait for nobody: every warp leaves its sums of every tile in shared memory and they are
-//    added at the end, in the order of the warps. 32 rows share one read of x, and lines in place of
+//    added at the end, in the order of the warps. (With 16 or 32 tokens those sums would not fit: there
+//    each warp takes a contiguous part of the block's, and leaves only the sums of a tile that began
+//    before its part, beside its ring, and of the one that it does not finish, in it.) 32 rows share one read of x, and lines in place of
 //    64-byte pieces keep L1's data pipe, which bounded an earlier form (66 % busy at 3.9 TB/s), below
 //    the stream. Tiles that two blocks share, and the slices of K where x does not fit in shared
 //    memory, are added by another launch, in the order of the line.
@@ -138,10 +140,12 @@ __host__ __device__ constexpr int gemv_stage_bytes(bool mx) { return kGemvRows *
 // Bytes of one token's slice of x (hi terms, and lo terms for fp32): a multiple of 512 and 64 more,
 // so that the tokens of a group lie in different banks.
 __host__ __device__ constexpr int gemv_pitch(int slice_chunks) { return slice_chunks * 512 + 64; }
-// `spans`: tiles that a block's part of the line can touch.
+// Whether a block's warps take its units in turn, or a contiguous part each.
+__host__ __device__ constexpr bool gemv_turns(int columns) { return columns <= 8; }
+// `spans`: tiles that a block's part of the line can touch, where its warps take turns.
 __host__ __device__ constexpr int gemv_smem(bool mx, int m, int slice_chunks, int columns, bool split, int spans) {
   return kGemvWarps * kGemvStages * gemv_stage_bytes(mx) + m * gemv_pitch(slice_chunks) * (split ? 2 : 1) + 256 +
-         spans * kGemvWarps * kGemvRows * columns * 4 + columns * 4;
+         (gemv_turns(columns) ? spans : 1) * kGemvWarps * kGemvRows * columns * 4 + columns * 4 + 2 * kGemvWarps * 4;
 }
 // Tokens that NT groups of the MMA's columns take.
 constexpr int gemv_columns(bool mx, int nt, bool grouped) { return grouped ? (mx ? 2 * nt : nt) : 8 * nt; }
@@ -218,7 +222,7 @@ __global__ void __launch_bounds__(256) gemv_x_kernel(GemvArgs a) {
 // start on 16 bytes and rows of scales on 4 (K a multiple of 64 for NVFP4, 128 for MXFP4, and an aligned
 // weight), else on 8 and 1.
 template <int T, int MX, int NT, int WIDE, int GROUPED>
-__global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
+__global__ void __launch_bounds__(kGemvThreads, gemv_columns(MX, NT, GROUPED) > 8 ? 1 : 2) gemv_fp4_kernel(GemvArgs a) {
   constexpr bool SPLIT = T == kF32;
   constexpr int COLS = gemv_columns(MX, NT, GROUPED), STAGE = gemv_stage_bytes(MX), SPITCH = gemv_scale_pitch(MX);
   extern __shared__ __align__(128) uint8_t smem_all[];
@@ -229,26 +233,41 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
   const int pitch = gemv_pitch(a.slice_chunks);
   uint8_t* zeros = smem + tokens * pitch * (SPLIT ? 2 : 1);  // 256 bytes: what a column's other lanes read
   float* unit = reinterpret_cast<float*>(zeros + 256);        // [COLS]
-  float* sums = unit + COLS;                                  // [tiles of the block][8 warps][32][COLS]
+  int* seg_tile = reinterpret_cast<int*>(unit + COLS);        // [8 warps][2]: 2 * tile + (its end is here), or -1
+  float* sums = reinterpret_cast<float*>(seg_tile + 2 * kGemvWarps);  // [tiles of the block or 1][8 warps][32][COLS]
 
   // ---- this block's part of the line
   const GemvCut cut(a.tiles * c_count, a.blocks);
   const int b_lo = cut.begin(blockIdx.x), b_hi = cut.begin(blockIdx.x + 1);
+  constexpr bool TURNS = gemv_turns(COLS);
+  constexpr int STEP = TURNS ? kGemvWarps : 1;
+  const GemvCut warps(b_hi - b_lo, kGemvWarps);
+  const int u_lo = TURNS ? b_lo + warp : b_lo + warps.begin(warp), u_hi = TURNS ? b_hi : b_lo + warps.begin(warp + 1);
   const int tile_lo = b_lo / c_count, spans = (b_hi - 1) / c_count - tile_lo + 1;
-  const int step_tiles = kGemvWarps / c_count, step_chunks = kGemvWarps % c_count;
-  for (int i = tid; i < spans * kGemvWarps * kGemvRows * COLS; i += kGemvThreads) sums[i] = 0.0f;
+  const int step_tiles = STEP / c_count, step_chunks = STEP % c_count;
+  if constexpr (TURNS) {
+    for (int i = tid; i < spans * kGemvWarps * kGemvRows * COLS; i += kGemvThreads) sums[i] = 0.0f;
+  } else {
+    if (tid < 2 * kGemvWarps) seg_tile[tid] = -1;
+  }
+  // without turns: the sums of a tile that began before warp w, or of the one that it leaves unfinished:
+  // its last, so they fit in its ring
+  auto sums_of = [&](int w, bool before) -> float* {
+    return before ? sums + w * kGemvRows * COLS : reinterpret_cast<float*>(smem_all + w * kGemvStages * STAGE);
+  };
+  static_assert(kGemvStages * STAGE >= kGemvRows * COLS * 4, "a tile's sums fit in a ring");
   const int cols = a.k >> (MX ? 5 : 4), half = a.k >> 1;
   if (tid < 16) reinterpret_cast<uint4*>(zeros)[tid] = make_uint4(0, 0, 0, 0);
 
   // what the next issue loads
-  int is_unit = b_lo + warp, is_tile = is_unit / c_count, is_chunk = is_unit % c_count;
+  int is_unit = u_lo, is_tile = is_unit / c_count, is_chunk = is_unit % c_count;
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem_all)) + warp * kGemvStages * STAGE;
   const int64_t scale_bytes = static_cast<int64_t>(a.n) * cols;
   // A quarter of a row's 16-byte pieces change places on odd rows, so that the fragments' reads (two
   // neighbouring rows x four pieces) touch all banks. Every copy is made at the nearest place that
   // exists: rows past n are not written, and x is zero past K.
   auto issue = [&](int stage) {
-    if (is_unit < b_hi) {
+    if (is_unit < u_hi) {
       const uint32_t to = ring + stage * STAGE;
       const int chunk = c_first + is_chunk, row0 = is_tile * kGemvRows;
       {
@@ -286,7 +305,7 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
           asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(at), "l"(a.scales + there), "r"(bytes) : "memory");
         }
       }
-      is_unit += kGemvWarps;
+      is_unit += STEP;
       is_tile += step_tiles;
       is_chunk += step_chunks;
       if (is_chunk >= c_count) {
@@ -512,10 +531,16 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
       a.partial[((static_cast<int64_t>(max(part, 0)) * a.slices + slice) * a.m + m0 + mt) * a.n + row] = y;
     }
   };
-  int tile = (b_lo + warp) / c_count, chunk = (b_lo + warp) % c_count;
-  // this warp's sums of a tile
-  auto leave = [&]() {
-    float* at = sums + ((tile - tile_lo) * kGemvWarps + warp) * kGemvRows * COLS;
+  int tile = u_lo / c_count, chunk = u_lo % c_count, begun = chunk;
+  // this warp's sums of a tile; `ends`: its last chunk is among them
+  auto leave = [&](bool ends) {
+    const bool whole = !TURNS && begun == 0 && ends;
+    float* at = TURNS ? sums + ((tile - tile_lo) * kGemvWarps + warp) * kGemvRows * COLS : sums_of(warp, begun != 0);
+    if constexpr (!TURNS) __syncwarp();  // the ring's last reads
+    auto one = [&](int r, int mt, float y) {
+      if (whole) put(tile, r, mt, y, -1);
+      else at[r * COLS + mt] = y;
+    };
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
 #pragma unroll
@@ -535,26 +560,28 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
           }
           if (t == 0) {
             if constexpr (MX) {
-              at[r * COLS + 2 * j] = v[0];
-              at[r * COLS + 2 * j + 1] = v[1];
-              at[(r + 8) * COLS + 2 * j] = v[2];
-              at[(r + 8) * COLS + 2 * j + 1] = v[3];
+              one(r, 2 * j, v[0]);
+              one(r, 2 * j + 1, v[1]);
+              one(r + 8, 2 * j, v[2]);
+              one(r + 8, 2 * j + 1, v[3]);
             } else {
-              at[r * COLS + j] = v[0];
-              at[(r + 8) * COLS + j] = v[2];
+              one(r, j, v[0]);
+              one(r + 8, j, v[2]);
             }
           }
         } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) at[(r + 8 * (e >> 1)) * COLS + j * 8 + 2 * t + (e & 1)] = acc[q][j][e];
+          for (int e = 0; e < 4; ++e) one(r + 8 * (e >> 1), j * 8 + 2 * t + (e & 1), acc[q][j][e]);
         }
       }
     }
+    if (!TURNS && !whole && lane == 0) seg_tile[2 * warp + (begun == 0)] = 2 * tile + ends;
+    begun = 0;
     clear(acc);
   };
 
   int stage = 0;
-  for (int u = b_lo + warp; u < b_hi; u += kGemvWarps) {
+  for (int u = u_lo; u < u_hi; u += STEP) {
     if (a.k > 0) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kGemvStages - 2) : "memory");
       __syncwarp();
@@ -596,20 +623,37 @@ __global__ void __launch_bounds__(kGemvThreads, 2) gemv_fp4_kernel(GemvArgs a) {
       }
     }
     const int next_chunk = chunk + step_chunks, next_tile = tile + step_tiles + (next_chunk >= c_count);
-    if (next_tile != tile || u + kGemvWarps >= b_hi) leave();
+    if (next_tile != tile || u + STEP >= u_hi) leave(chunk == c_count - 1);
     tile = next_tile;
     chunk = next_chunk >= c_count ? next_chunk - c_count : next_chunk;
     stage = stage == kGemvStages - 1 ? 0 : stage + 1;
   }
   __syncthreads();
-  for (int i = tid; i < spans * kGemvRows * COLS; i += kGemvThreads) {
-    const int s = i / (kGemvRows * COLS), cell = i % (kGemvRows * COLS), first = (tile_lo + s) * c_count;
-    const float* at = sums + s * kGemvWarps * kGemvRows * COLS + cell;
-    float y = at[0];
+  if constexpr (TURNS) {
+    for (int i = tid; i < spans * kGemvRows * COLS; i += kGemvThreads) {
+      const int s = i / (kGemvRows * COLS), cell = i % (kGemvRows * COLS), first = (tile_lo + s) * c_count;
+      const float* at = sums + s * kGemvWarps * kGemvRows * COLS + cell;
+      float y = at[0];
 #pragma unroll
-    for (int w = 1; w < kGemvWarps; ++w) y += at[w * kGemvRows * COLS];
-    // begun in the block before: its second part; ended in the next one: its first
-    put(tile_lo + s, cell / COLS, cell % COLS, y, first < b_lo ? 1 : first + c_count > b_hi ? 0 : -1);
+      for (int w = 1; w < kGemvWarps; ++w) y += at[w * kGemvRows * COLS];
+      // begun in the block before: its second part; ended in the next one: its first
+      put(tile_lo + s, cell / COLS, cell % COLS, y, first < b_lo ? 1 : first + c_count > b_hi ? 0 : -1);
+    }
+  } else {
+    // the tiles that warps share: from where they begin in this block (a warp's unfinished one, or the
+    // one that began before the block), through the following warps' first sums
+    for (int i = tid; i < (kGemvWarps + 1) * kGemvRows * COLS; i += kGemvThreads) {
+      const int head = i / (kGemvRows * COLS), cell = i % (kGemvRows * COLS);
+      const int seg = head == 0 ? 0 : (head - 1) * 2 + 1, first = seg_tile[seg];
+      if (first < 0) continue;
+      float y = sums_of(seg >> 1, head == 0)[cell];
+      int end = first & 1;
+      for (int w = (seg >> 1) + 1; w < kGemvWarps && seg_tile[2 * w] >= 0 && seg_tile[2 * w] >> 1 == first >> 1; ++w) {
+        y += sums_of(w, true)[cell];
+        end = seg_tile[2 * w] & 1;
+      }
+      put(first >> 1, cell / COLS, cell % COLS, y, head == 0 ? 1 : end ? -1 : 0);
+    }
   }
 }
 

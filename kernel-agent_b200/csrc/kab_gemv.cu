@@ -44,20 +44,21 @@ GemvPlan gemv_plan(int64_t m, int64_t n, int64_t k, int fmt, int dtype) {
   p.tiles = static_cast<int>((n + kGemvRows - 1) / kGemvRows);
   const int64_t per_chunk = static_cast<int64_t>(p.tokens) * 512 * (split ? 2 : 1);
   // the tiles that a block's part may touch: their sums stay in shared memory
-  const int spans = p.columns <= 2 ? 8 : p.columns <= 8 ? 4 : p.columns <= 16 ? 5 : 3;
+  const bool turns = gemv_turns(p.columns);
+  const int spans = p.columns <= 2 ? 8 : 4;
   const int fixed = gemv_smem(mx, 0, 0, p.columns, split, spans) + p.tokens * 64 * (split ? 2 : 1);
   // two blocks per SM with at least 4 chunks of x each (or all of it), else one
   const int need = std::min(p.chunks, 4);
-  const int room = fixed + need * per_chunk <= kSmemTwo ? kSmemTwo : kSmemOne;
+  const int room = turns && fixed + need * per_chunk <= kSmemTwo ? kSmemTwo : kSmemOne;
   const int fit = static_cast<int>(std::max<int64_t>(1, (room - fixed) / per_chunk));
   const int want = (p.chunks + fit - 1) / fit;
   p.slice_chunks = (p.chunks + want - 1) / want;
   p.slices = (p.chunks + p.slice_chunks - 1) / p.slice_chunks;
   p.smem = gemv_smem(mx, p.tokens, p.slice_chunks, p.columns, split, spans);
   const int resident = room == kSmemTwo ? 2 : 1;
-  // whole waves of blocks, as few as keep a block's part within `spans` tiles
+  // where a block's warps take turns, whole waves of blocks, as few as keep its part within `spans` tiles
   const int wave = std::max(1, resident * sm_count() / p.slices);
-  const int waves = (p.tiles + wave * (spans - 1) - 1) / (wave * (spans - 1));
+  const int waves = turns ? (p.tiles + wave * (spans - 1) - 1) / (wave * (spans - 1)) : 1;
   p.blocks = std::min(p.tiles, waves * wave);
   p.join = p.slices > 1 || p.tiles % p.blocks != 0;  // else every block has whole tiles
   p.partial = p.join ? round256(static_cast<size_t>(2) * p.slices * m * n * 4) : 0;
