@@ -16,8 +16,8 @@
 //    only in the lane that owns block n, zeros elsewhere, so column n sums block n alone; one
 //    multiply-add per row and block then applies the scale in fp32, exactly for every scale. NVFP4
 //    fills the columns with one token, MXFP4 with two; more tokens take more MMAs on the same
-//    converted codes. (Scaling the codes costs 32 packed multiplications per chunk instead: 37 us
-//    against GROUPED's 29 for one token at 28672 x 8192.)
+//    converted codes. (With scaled codes, 32 packed multiplications per 128 x 16 codes, one token took
+//    37.0 us at 28672 x 8192, with blocks apart 34.1 in the same form of the kernel.)
 //  * For more tokens the codes are scaled. An NVFP4 code times its e4m3 scale has at most 6
 //    significant bits and lies in [2^-10, 2688]: exact in f16, one packed multiplication per two
 //    codes. An MXFP4 scale does not fit f16: the four 32-code blocks of a row's 128 codes are taken in
@@ -30,15 +30,20 @@
 //    streams its rows, converted there for one token, by a launch before for more.
 //  * The (32-row tile, 256-code chunk) pairs of a K slice stand in one line, cut into equal parts for
 //    the blocks. A block's warps take its units in turn, each through a ring of its own in shared
-//    memory (cp.async, whole 128-byte lines of a row), so that together they read a kilobyte of each
-//    row at a time (one warp alone after another along a row, 128 bytes at a time, read 4.3 TB/s of
-//    DRAM), and wait for nobody: every warp leaves its sums of every tile in shared memory and they are
-//    added at the end, in the order of the warps. (With 16 or 32 tokens those sums would not fit: there
-//    each warp takes a contiguous part of the block's, and leaves only the sums of a tile that began
-//    before its part, beside its ring, and of the one that it does not finish, in it.) 32 rows share one read of x, and lines in place of
-//    64-byte pieces keep L1's data pipe, which bounded an earlier form (66 % busy at 3.9 TB/s), below
-//    the stream. Tiles that two blocks share, and the slices of K where x does not fit in shared
-//    memory, are added by another launch, in the order of the line.
+//    memory (cp.async, whole 128-byte lines of a row), and wait for nobody: every warp leaves its sums
+//    of every tile in shared memory and they are added at the end, in the order of the warps. With 16
+//    or 32 tokens those sums would not fit: there each warp takes a contiguous part of the block's, and
+//    leaves only the sums of a tile that began before its part, beside its ring, and of the one that it
+//    does not finish, in it. (Contiguous parts for all: 39 us in place of 33 at 1 x 8192 x 28672, 28 in
+//    place of 23 at 8 x 4096 x 14336 MXFP4, 48 in place of 51 at 8 x 28672 x 8192.)
+//  * 32 rows share one read of x, and whole lines in place of 64-byte pieces keep L1's data pipe, which
+//    bounded an earlier form (66 % busy at 3.9 TB/s), below the stream.
+//  * Tiles that two blocks share, and the slices of K where x does not fit in shared memory, are added
+//    by another launch, in the order of the line.
+//
+// One token at 28672 x 8192 NVFP4: 30.8 us = 4.29 TB/s = 0.65 of the measured copy. About 5 us of it
+// are fixed (x's conversion, the join's launch); the rest streams at 5.2 TB/s, and no faster from L2:
+// 16 warps per SM, each a chain of conversions and MMAs (issue slots 45 % used, ALU 43 %), bound it.
 #pragma once
 
 #include "codes.cuh"

@@ -4,7 +4,8 @@
 scaled linears), ``kernel_agent_b200.kernels.compare`` mirrors ``kernel_agent.kernels.compare``
 (the evaluator's comparator) and ``kernel_agent_b200.kernels.scale_guard`` its scale-rule
 guard; ``kernel_agent_b200.kernels.blockwise`` and ``.attention`` add the blockwise-FP8 and
-FP8-attention APIs in the same style. Every numeric loop runs in ``libkab.so`` (CUDA for
+FP8-attention APIs in the same style, and ``.gemv`` and ``.paged_kv`` what a decode step needs
+beside them (the weight-only FP4 linear, a paged FP8 cache). Every numeric loop runs in ``libkab.so`` (CUDA for
 sm_100a, C ABI in ``include/kab.h``); CPU tensors are refused.
 """
 
