@@ -286,6 +286,7 @@ int kab_kv_pages_attention(const KabKvPagesAttention* params, void* workspace, s
   if (int e = attention_check(params, &g)) return e;
   if (params->cache.batch == 0 || params->heads_q == 0 || params->q_len == 0) return KAB_OK;
   KAB_REQUIRE(params->q != nullptr && params->out != nullptr, "null pointer");
+  KAB_REQUIRE(aligned(params->out, 16), "out must be 16-byte aligned");
   AttentionPlan plan;
   if (int e = attention_plan(params, g, &plan)) return e;
   KAB_REQUIRE(workspace != nullptr && workspace_bytes >= plan.bytes() && aligned(workspace, 256),

@@ -281,7 +281,7 @@ struct EvictArgs {
 constexpr int kSelectThreads = 512;
 
 __device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.arrive;\n barrier.cluster.wait;" ::: "memory");
 }
 // The four words at the same shared-memory address (16-byte aligned) of block `rank` of the cluster.
 __device__ __forceinline__ uint4 load_cluster(const uint32_t* p, int rank) {

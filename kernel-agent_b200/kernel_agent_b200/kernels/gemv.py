@@ -11,6 +11,7 @@ count. The reference's decode example for such weights is
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
@@ -19,7 +20,7 @@ from . import quant as q
 from ._launch import device_of, guard, stream_of, workspace
 from .gemm import _bias
 
-_FORMATS = {"nvfp4": (nat.KAB_NVFP4, 16), "mxfp4": (nat.KAB_MXFP4, 32)}
+_FORMATS = {"nvfp4": (nat.KAB_NVFP4, 16, torch.float8_e4m3fn), "mxfp4": (nat.KAB_MXFP4, 32, torch.float8_e8m0fnu)}
 _PLANS: dict[tuple, int] = {}
 
 
@@ -47,7 +48,7 @@ def fp4_w4a16_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     weight being read again for every 32."""
     if fmt not in _FORMATS:
         raise ValueError(f"unknown FP4 format {fmt!r} (one of {', '.join(_FORMATS)})")
-    code, block = _FORMATS[fmt]
+    code, block, kind = _FORMATS[fmt]
     device = device_of(x, codes, scales, bias)
     if x.dim() < 1 or codes.dim() != 2:
         raise ValueError(f"expected x [..., K] and codes [N, K / 2]; got {tuple(x.shape)}, {tuple(codes.shape)}")
@@ -58,8 +59,8 @@ def fp4_w4a16_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     if half * 2 != k or codes.element_size() != 1:
         raise ValueError(f"codes {tuple(codes.shape)} {codes.dtype} do not fit x {tuple(x.shape)}: expected "
                          f"[N, {k // 2}] bytes")
-    if scales.element_size() != 1:
-        raise ValueError(f"scales must be one byte each (e4m3 or e8m0), got {scales.dtype}")
+    if scales.dtype != kind and scales.dtype != torch.uint8:
+        raise ValueError(f"{fmt} scales are one byte each, {kind} or uint8; got {scales.dtype}")
     cols = k // block
     swizzle = scales.dim() == 1
     if swizzle and scales.numel() != -(-n // 128) * 128 * (-(-cols // 4)) * 4:
@@ -67,10 +68,10 @@ def fp4_w4a16_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
                          f"{-(-n // 128) * 128 * (-(-cols // 4)) * 4}")
     if not swizzle and scales.shape != (n, cols):
         raise ValueError(f"expected scales [{n}, {cols}], got {tuple(scales.shape)}")
-    x2 = x if x.dim() == 2 else x.reshape(-1, k)
+    x2 = x if x.dim() == 2 else x.reshape(math.prod(x.shape[:-1]), k)
     if x2.dtype not in nat.DTYPES:
         x2 = x2.float()
-    if x2.stride(1) != 1 or x2.stride(0) % 8 or x2.data_ptr() % 16:
+    if x2.stride(1) != 1 or x2.stride(0) % 8 or x2.stride(0) < k or x2.data_ptr() % 16:
         x2 = x2.contiguous()
     m = x2.shape[0]
     c, s = codes.contiguous(), scales.contiguous()
@@ -90,7 +91,11 @@ def fp4_w4a16_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     else:
         b, bias_code = _bias(bias, n, x.device)
     out = x2.new_empty((m, n))
-    if m and n:
+    if k == 0:
+        out.zero_()
+        if b is not None:
+            out += b
+    elif m and n:
         dtype = nat.DTYPES[x2.dtype]
         with guard(device):
             stream = stream_of(device)

@@ -156,7 +156,8 @@ def paged_kv_attention(q: torch.Tensor, k_pages: torch.Tensor, k_scale: torch.Te
     heads of its KV head and the query tokens, is added to its entry. Made for the few rows (query
     heads per KV head x query tokens) of a decode step: each 16 rows (8 where there are no more) read
     the cache once.
-    Results do not depend on the other sequences' lengths but in the last bits (the cache is cut
+    ``mass`` takes scratch memory of four bytes per query row and token that the page table has room
+    for. Results do not depend on the other sequences' lengths but in the last bits (the cache is cut
     into equal parts for the GPU, whose softmax sums are merged), and are the same for the same
     inputs."""
     if q.dim() not in (3, 4):

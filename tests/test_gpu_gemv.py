@@ -146,6 +146,10 @@ def test_tensor_scales_bias_and_strides(gv):
     wide = torch.randn(4, 2, 512, device=DEV).to(torch.float16)
     check(gv.fp4_w4a16_linear(wide[:, 1], codes, scales, 0.001), wide[:, 1], w, np.float32(0.001), None, torch.float16)
     assert gv.fp4_w4a16_linear(x[:0], codes, scales, ts).shape == (0, 3, 1, 80)
+    same = wide[:1, 1].expand(5, 512)  # one row five times
+    check(gv.fp4_w4a16_linear(same, codes, scales, 0.001), same, w, np.float32(0.001), None, torch.float16)
+    none = gv.fp4_w4a16_linear(x[..., :0], codes[:, :0], scales[:, :0], ts, bias)
+    assert torch.equal(none, bias.to(torch.bfloat16).expand(2, 3, 1, 80))
 
 
 def test_same_weight_as_w4a4(gv):
@@ -192,6 +196,8 @@ def test_refusals(gv):
         ((x[:, :128], codes, scales, 1.0), {}, "fit"),
         ((x, codes, scales[:, :8], 1.0), {}, "scales"),
         ((x, codes, scales.float(), 1.0), {}, "one byte"),
+        ((x, codes, scales.view(torch.float8_e8m0fnu), 1.0), {}, "nvfp4 scales"),
+        ((x, codes, scales[:, ::2].contiguous(), 1.0), {"fmt": "mxfp4"}, "mxfp4 scales"),
         ((x, codes, scales.reshape(-1), 1.0), {}, "swizzled"),
         ((x, codes, scales, torch.ones(3, device=DEV)), {}, "tensor_scale"),
         ((x, codes, scales, 1.0, torch.ones(31, device=DEV)), {}, "bias"),

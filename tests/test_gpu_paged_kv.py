@@ -483,6 +483,9 @@ def test_refusals(pk):
         pk.paged_kv_attention(q.double(), *parts, c.table, c.lengths)
     with pytest.raises(ValueError, match="out must"):
         pk.paged_kv_attention(q, *parts, c.table, c.lengths, out=q.half())
+    with pytest.raises(ValueError, match="aligned"):
+        paged = torch.empty(q.numel() + 1, device=DEV)[1:].reshape(q.shape)
+        pk.paged_kv_attention(q, *parts, c.table, c.lengths, out=paged)
     with pytest.raises(ValueError, match="expected k and v"):
         pk.append_kv_pages(x[:, :1], x[:, :1], *parts, c.table, c.lengths)
     with pytest.raises(ValueError, match="both be"):
