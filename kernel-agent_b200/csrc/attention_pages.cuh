@@ -245,7 +245,9 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
     if (w < warp) before += warp_sum[w];
     total += warp_sum[w];
   }
-  const unsigned grid = min(gridDim.x, total), share = total / grid, longer = total % grid;
+  // at least four units per block: with fewer, more parts to merge cost more than the idle blocks save
+  // (1 x 4096 tokens: 12.1 us with one, 10.5 with four, 11.2 with eight)
+  const unsigned grid = min(gridDim.x, max(total / 4u, 1u)), share = total / grid, longer = total % grid;
   if (blockIdx.x >= grid) {
     if (tid == 0 && !a.cuts_by_item) a.cuts[blockIdx.x].last = -1;
     return;
@@ -594,10 +596,9 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
               float w0 = 0.0f, w1 = 0.0f;
 #pragma unroll
               for (int i = 0; i < 2 * U; ++i) {
-                if (k >> 3 == i) {  // the same for all lanes
-                  w0 = __shfl_sync(0xffffffffu, s[r][i >> 1][(i & 1) * 2], from);
-                  w1 = __shfl_sync(0xffffffffu, s[r][i >> 1][(i & 1) * 2 + 1], from);
-                }
+                const float e0 = __shfl_sync(0xffffffffu, s[r][i >> 1][(i & 1) * 2], from);
+                const float e1 = __shfl_sync(0xffffffffu, s[r][i >> 1][(i & 1) * 2 + 1], from);
+                if (k >> 3 == i) w0 = e0, w1 = e1;
               }
               const bool sees0 = x < seen_of(r * 8 + 2 * t), sees1 = x < seen_of(r * 8 + 2 * t + 1);
 #pragma unroll
