@@ -104,7 +104,7 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
 }
 __device__ __forceinline__ void mma_m16n8k16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                              uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -115,12 +115,6 @@ __device__ __forceinline__ void gemv_copy(uint32_t dst, const void* src) {
   if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
   else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
-__device__ __forceinline__ uint4 load_shared16(uint32_t at) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
-  return v;
-}
-
 __device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
   if (dtype == KAB_F32) return static_cast<const float*>(p)[i];
   if (dtype == KAB_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
@@ -364,8 +358,7 @@ __global__ void __launch_bounds__(kGemvThreads, gemv_columns(MX, NT, GROUPED) > 
   // where a lane reads column g of group j; `step`: 256 bytes per 128 codes, or none in the zeros. With
   // NVFP4 blocks apart the lane's first block and its second have a column each.
   constexpr int SIDES = GROUPED && !MX ? 2 : 1;
-  uint32_t x_at[NT][SIDES];
-  int x_step[NT][SIDES];
+  int x_at[NT][SIDES], x_step[NT][SIDES];  // bytes from smem
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
 #pragma unroll
@@ -373,8 +366,7 @@ __global__ void __launch_bounds__(kGemvThreads, gemv_columns(MX, NT, GROUPED) > 
       // columns past the tokens repeat the last one; nobody reads them
       const int token = !GROUPED ? j * 8 + g : MX ? 2 * j + (g & 1) : j;
       const bool here = !GROUPED || (MX ? t == g >> 1 : g == 2 * t + side);
-      x_at[j][side] = static_cast<uint32_t>(
-          __cvta_generic_to_shared(here ? smem + min(token, tokens - 1) * pitch + t * 16 : zeros));
+      x_at[j][side] = here ? min(token, tokens - 1) * pitch + t * 16 : tokens * pitch * (SPLIT ? 2 : 1);
       x_step[j][side] = here ? 256 : 0;
     }
   }
@@ -401,9 +393,9 @@ __global__ void __launch_bounds__(kGemvThreads, gemv_columns(MX, NT, GROUPED) > 
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         const int side = SIDES == 2 ? i >> 1 : 0;
-        const uint32_t at = x_at[j][side] + half_chunk * x_step[j][side] + i * 64;
-        b[j] = load_shared16(at);
-        if constexpr (SPLIT) l[j] = load_shared16(x_step[j][side] ? at + lo_at : at);
+        const int at = x_at[j][side] + half_chunk * x_step[j][side] + i * 64;
+        b[j] = *reinterpret_cast<const uint4*>(smem + at);
+        if constexpr (SPLIT) l[j] = *reinterpret_cast<const uint4*>(smem + (x_step[j][side] ? at + lo_at : at));
       }
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
@@ -591,8 +583,8 @@ __global__ void __launch_bounds__(kGemvThreads, gemv_columns(MX, NT, GROUPED) > 
       asm volatile("cp.async.wait_group %0;" ::"n"(kGemvStages - 2) : "memory");
       __syncwarp();
       issue(stage == 0 ? kGemvStages - 1 : stage - 1);  // the stage that was consumed before this one
-      const uint32_t from = ring + stage * STAGE;
-      const uint8_t* sc = smem_all + (warp * kGemvStages + stage) * STAGE + kGemvRows * 128;
+      const uint8_t* from = smem_all + (warp * kGemvStages + stage) * STAGE;
+      const uint8_t* sc = from + kGemvRows * 128;
 #pragma unroll 1
       for (int h = 0; h < 2; ++h) {  // 128 codes; once in the code, which short streams fetch cold
         uint4 w[2][2];
@@ -602,7 +594,7 @@ __global__ void __launch_bounds__(kGemvThreads, gemv_columns(MX, NT, GROUPED) > 
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int r = q * 16 + i * 8 + g;
-            w[q][i] = load_shared16(from + r * 128 + (((h * 4 + t) ^ ((g & 1) << 2)) << 4));
+            w[q][i] = *reinterpret_cast<const uint4*>(from + r * 128 + (((h * 4 + t) ^ ((g & 1) << 2)) << 4));
             int off = r * SPITCH + h * (MX ? 4 : 8) + t * (MX ? 1 : 2);
             if constexpr (WIDE) {
               s[q][i] = MX ? sc[off] : *reinterpret_cast<const uint16_t*>(sc + off);
