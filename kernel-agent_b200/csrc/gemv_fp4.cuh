@@ -31,11 +31,12 @@
 //  * The (32-row tile, 256-code chunk) pairs of a K slice stand in one line, cut into equal parts for
 //    the blocks. A block's warps take its units in turn, each through a ring of its own in shared
 //    memory (cp.async, whole 128-byte lines of a row), and wait for nobody: every warp leaves its sums
-//    of every tile in shared memory and they are added at the end, in the order of the warps. With 16
-//    or 32 tokens those sums would not fit: there each warp takes a contiguous part of the block's, and
-//    leaves only the sums of a tile that began before its part, beside its ring, and of the one that it
-//    does not finish, in it. (Contiguous parts for all: 39 us in place of 33 at 1 x 8192 x 28672, 28 in
-//    place of 23 at 8 x 4096 x 14336 MXFP4, 48 in place of 51 at 8 x 28672 x 8192.)
+//    of every tile in shared memory and they are added at the end, in the order of the warps. Where
+//    those sums would leave room for one block per SM only (three tokens and more, many tiles per
+//    block) each warp takes a contiguous part of the block's instead, and leaves only the sums of a tile
+//    that began before its part, beside its ring, and of the one that it does not finish, in it. (In
+//    turns against contiguous parts: 33 us against 39 at 1 x 8192 x 28672, 22.6 against 24.8 at 8 x 4096
+//    x 14336 MXFP4; 51 against 49 at 8 x 28672 x 8192, where turns leave one block per SM.)
 //  * 32 rows share one read of x, and whole lines in place of 64-byte pieces keep L1's data pipe, which
 //    bounded an earlier form (66 % busy at 3.9 TB/s), below the stream.
 //  * Tiles that two blocks share, and the slices of K where x does not fit in shared memory, are added
@@ -139,12 +140,10 @@ __host__ __device__ constexpr int gemv_stage_bytes(bool mx) { return kGemvRows *
 // Bytes of one token's slice of x (hi terms, and lo terms for fp32): a multiple of 512 and 64 more,
 // so that the tokens of a group lie in different banks.
 __host__ __device__ constexpr int gemv_pitch(int slice_chunks) { return slice_chunks * 512 + 64; }
-// Whether a block's warps take its units in turn, or a contiguous part each.
-__host__ __device__ constexpr bool gemv_turns(int columns) { return columns <= 8; }
-// `spans`: tiles that a block's part of the line can touch, where its warps take turns.
+// `spans`: tiles that a block's part of the line can touch, where its warps take turns, else 1.
 __host__ __device__ constexpr int gemv_smem(bool mx, int m, int slice_chunks, int columns, bool split, int spans) {
   return kGemvWarps * kGemvStages * gemv_stage_bytes(mx) + m * gemv_pitch(slice_chunks) * (split ? 2 : 1) + 256 +
-         (gemv_turns(columns) ? spans : 1) * kGemvWarps * kGemvRows * columns * 4 + columns * 4 + 2 * kGemvWarps * 4;
+         spans * kGemvWarps * kGemvRows * columns * 4 + columns * 4 + 2 * kGemvWarps * 4;
 }
 // Tokens that NT groups of the MMA's columns take.
 constexpr int gemv_columns(bool mx, int nt, bool grouped) { return grouped ? (mx ? 2 * nt : nt) : 8 * nt; }
@@ -220,7 +219,8 @@ __global__ void __launch_bounds__(256) gemv_x_kernel(GemvArgs a) {
 // MX: MXFP4 (e8m0 per 32), else NVFP4 (e4m3 per 16). NT: groups of 8 MMA columns. WIDE: rows of codes
 // start on 16 bytes and rows of scales on 4 (K a multiple of 64 for NVFP4, 128 for MXFP4, and an aligned
 // weight), else on 8 and 1.
-template <int T, int MX, int NT, int WIDE, int GROUPED>
+// TURNS: a block's warps take its units in turn, else a contiguous part each.
+template <int T, int MX, int NT, int WIDE, int GROUPED, int TURNS>
 __global__ void __launch_bounds__(kGemvThreads, gemv_columns(MX, NT, GROUPED) > 8 ? 1 : 2) gemv_fp4_kernel(GemvArgs a) {
   constexpr bool SPLIT = T == kF32;
   constexpr int COLS = gemv_columns(MX, NT, GROUPED), STAGE = gemv_stage_bytes(MX), SPITCH = gemv_scale_pitch(MX);
@@ -238,7 +238,6 @@ __global__ void __launch_bounds__(kGemvThreads, gemv_columns(MX, NT, GROUPED) > 
   // ---- this block's part of the line
   const GemvCut cut(a.tiles * c_count, a.blocks);
   const int b_lo = cut.begin(blockIdx.x), b_hi = cut.begin(blockIdx.x + 1);
-  constexpr bool TURNS = gemv_turns(COLS);
   constexpr int STEP = TURNS ? kGemvWarps : 1;
   const GemvCut warps(b_hi - b_lo, kGemvWarps);
   const int u_lo = TURNS ? b_lo + warp : b_lo + warps.begin(warp), u_hi = TURNS ? b_hi : b_lo + warps.begin(warp + 1);

@@ -22,7 +22,7 @@ int gemv_check(int64_t m, int64_t n, int64_t k, int fmt, int dtype) {
 // two per SM where their shared memory allows.
 constexpr int kSmemOne = 226 * 1024, kSmemTwo = 113 * 1024;
 struct GemvPlan {
-  bool grouped, join, terms;
+  bool grouped, turns, join, terms;
   int nt, columns, tokens, chunks, slice_chunks, slices, tiles, blocks, smem;
   size_t partial, x_terms, x_units;  // workspace bytes
   size_t bytes() const { return partial + x_terms + x_units; }
@@ -43,23 +43,27 @@ GemvPlan gemv_plan(int64_t m, int64_t n, int64_t k, int fmt, int dtype) {
   p.chunks = static_cast<int>(std::max<int64_t>(1, (k + kGemvCodes - 1) / kGemvCodes));
   p.tiles = static_cast<int>((n + kGemvRows - 1) / kGemvRows);
   const int64_t per_chunk = static_cast<int64_t>(p.tokens) * 512 * (split ? 2 : 1);
-  // the tiles that a block's part may touch: their sums stay in shared memory
-  const bool turns = gemv_turns(p.columns);
-  const int spans = p.columns <= 2 ? 8 : 4;
-  const int fixed = gemv_smem(mx, 0, 0, p.columns, split, spans) + p.tokens * 64 * (split ? 2 : 1);
-  // two blocks per SM with at least 4 chunks of x each (or all of it), else one
+  // A block's warps in turns where the tiles of its part, whose sums stay in shared memory, are few
+  // enough in one wave of blocks; else a contiguous part per warp. Two blocks per SM with at least 4
+  // chunks of x each (or all of it) where that fits, one for 16 columns and more (by registers).
   const int need = std::min(p.chunks, 4);
-  const int room = turns && fixed + need * per_chunk <= kSmemTwo ? kSmemTwo : kSmemOne;
-  const int fit = static_cast<int>(std::max<int64_t>(1, (room - fixed) / per_chunk));
-  const int want = (p.chunks + fit - 1) / fit;
-  p.slice_chunks = (p.chunks + want - 1) / want;
-  p.slices = (p.chunks + p.slice_chunks - 1) / p.slice_chunks;
-  p.smem = gemv_smem(mx, p.tokens, p.slice_chunks, p.columns, split, spans);
-  const int resident = room == kSmemTwo ? 2 : 1;
-  // where a block's warps take turns, whole waves of blocks, as few as keep its part within `spans` tiles
-  const int wave = std::max(1, resident * sm_count() / p.slices);
-  const int waves = turns ? (p.tiles + wave * (spans - 1) - 1) / (wave * (spans - 1)) : 1;
-  p.blocks = std::min(p.tiles, waves * wave);
+  for (p.turns = p.columns <= 8; ; p.turns = false) {
+    const int spans = !p.turns ? 1 : p.columns <= 2 ? 8 : 4;
+    const int fixed = gemv_smem(mx, 0, 0, p.columns, split, spans) + p.tokens * 64 * (split ? 2 : 1);
+    const int room = p.columns <= 8 && fixed + need * per_chunk <= kSmemTwo ? kSmemTwo : kSmemOne;
+    const int fit = static_cast<int>(std::max<int64_t>(1, (room - fixed) / per_chunk));
+    const int want = (p.chunks + fit - 1) / fit;
+    p.slice_chunks = (p.chunks + want - 1) / want;
+    p.slices = (p.chunks + p.slice_chunks - 1) / p.slice_chunks;
+    p.smem = gemv_smem(mx, p.tokens, p.slice_chunks, p.columns, split, spans);
+    const int wave = std::max(1, (room == kSmemTwo ? 2 : 1) * sm_count() / p.slices);
+    p.blocks = std::min(p.tiles, wave);
+    if (!p.turns || p.tiles <= wave * (spans - 1)) break;
+    if (p.columns <= 2) {  // more waves, as few as keep a block's part within its tiles
+      p.blocks = std::min(p.tiles, (p.tiles + wave * (spans - 1) - 1) / (wave * (spans - 1)) * wave);
+      break;
+    }
+  }
   p.join = p.slices > 1 || p.tiles % p.blocks != 0;  // else every block has whole tiles
   p.partial = p.join ? round256(static_cast<size_t>(2) * p.slices * m * n * 4) : 0;
   // x converted by a launch of its own where every block would have to convert more than one token
@@ -84,9 +88,9 @@ cudaError_t launch_after(void (*kern)(GemvArgs), dim3 grid, int threads, int sme
   return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
-template <int T, int MX, int NT, int WIDE, int GROUPED>
+template <int T, int MX, int NT, int WIDE, int GROUPED, int TURNS>
 int launch_gemv(const GemvArgs& a, const GemvPlan& p, cudaStream_t s) {
-  auto kern = gemv_fp4_kernel<T, MX, NT, WIDE, GROUPED>;
+  auto kern = gemv_fp4_kernel<T, MX, NT, WIDE, GROUPED, TURNS>;
   static bool configured[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(KAB_ECUDA, "no current device");
@@ -111,7 +115,13 @@ int launch_gemv(const GemvArgs& a, const GemvPlan& p, cudaStream_t s) {
 template <int T, int MX, int NT, int GROUPED>
 int launch_gemv(const GemvArgs& a, const GemvPlan& p, cudaStream_t s) {
   const bool wide = a.k % (MX ? 128 : 64) == 0 && aligned(a.codes, 16) && aligned(a.scales, 4);
-  return wide ? launch_gemv<T, MX, NT, 1, GROUPED>(a, p, s) : launch_gemv<T, MX, NT, 0, GROUPED>(a, p, s);
+  constexpr int columns = gemv_columns(MX, NT, GROUPED);
+  if constexpr (columns <= 8) {
+    if (p.turns) return wide ? launch_gemv<T, MX, NT, 1, GROUPED, 1>(a, p, s) : launch_gemv<T, MX, NT, 0, GROUPED, 1>(a, p, s);
+  }
+  if constexpr (columns > 2)
+    return wide ? launch_gemv<T, MX, NT, 1, GROUPED, 0>(a, p, s) : launch_gemv<T, MX, NT, 0, GROUPED, 0>(a, p, s);
+  return fail(KAB_EUNSUPPORTED, "no kernel for this plan");
 }
 template <int T, int MX>
 int launch_gemv(const GemvArgs& a, const GemvPlan& p, cudaStream_t s) {

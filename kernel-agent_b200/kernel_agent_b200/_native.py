@@ -232,10 +232,15 @@ def call(name: str, *args) -> None:
     """Run entry point ``name``; a non-zero status raises with the library's message."""
     status = getattr(load(), name)(*args)
     if status != KAB_OK:
-        msg = f"{name}: {last_error()}"
-        if status == KAB_EINVAL:
-            raise ValueError(msg)
-        raise RuntimeError(msg)
+        refuse(name, status)
+
+
+def refuse(name: str, status: int) -> None:
+    """Raise for the non-zero ``status`` of entry point ``name``."""
+    msg = f"{name}: {last_error()}"
+    if status == KAB_EINVAL:
+        raise ValueError(msg)
+    raise RuntimeError(msg)
 
 
 def query(name: str, *args):

@@ -1,39 +1,46 @@
 """What a launch needs from torch, at a decode step's pace: the tensors' device, the current
-stream as the C ABI takes it, a device guard only where one is needed, and scratch buffers."""
+stream as the C ABI takes it, calls with that device current, and scratch buffers."""
 
 from __future__ import annotations
-
-from contextlib import nullcontext
 
 import torch
 
 from .. import _native as nat
 
 _BUFFERS: dict[tuple, torch.Tensor] = {}
-_NO_GUARD = nullcontext()
+_ENTRIES: dict[str, object] = {}
 
 
 def device_of(*tensors: torch.Tensor | None) -> int:
     """The index of the CUDA device that all given tensors are on (the checks and errors of
     :func:`kernel_agent_b200._native.require_cuda`)."""
-    dev = -1
-    for t in tensors:
-        if t is None:
-            continue
-        at = t.get_device() if isinstance(t, torch.Tensor) else -1
-        if at < 0 or (dev >= 0 and at != dev):
-            break
-        dev = at
-    else:
-        if dev in nat._checked_devices:
-            return dev
+    try:
+        dev = tensors[0].get_device()
+        for t in tensors:
+            if t is not None and t.get_device() != dev:
+                break
+        else:
+            if dev in nat._checked_devices:
+                return dev
+    except AttributeError:
+        pass  # not a tensor: refused below
     found = nat.require_cuda(*tensors)
     return torch.cuda.current_device() if found.index is None else found.index
 
 
-def guard(device: int):
-    """A context in which ``device`` is the current one."""
-    return _NO_GUARD if torch._C._cuda_getDevice() == device else torch.cuda.device(device)
+def call(name: str, device: int, *args) -> None:
+    """Entry point ``name`` with ``device`` current; a non-zero status raises as in
+    :func:`kernel_agent_b200._native.call`."""
+    entry = _ENTRIES.get(name)
+    if entry is None:
+        entry = _ENTRIES[name] = getattr(nat.load(), name)
+    if torch._C._cuda_getDevice() == device:
+        status = entry(*args)
+    else:
+        with torch.cuda.device(device):
+            status = entry(*args)
+    if status:
+        nat.refuse(name, status)
 
 
 def stream_of(device: int) -> int:

@@ -17,7 +17,7 @@ import torch
 
 from .. import _native as nat
 from . import quant as q
-from ._launch import device_of, guard, stream_of, workspace
+from ._launch import call, device_of, stream_of, workspace
 from .gemm import _bias
 
 _FORMATS = {"nvfp4": (nat.KAB_NVFP4, 16, torch.float8_e4m3fn), "mxfp4": (nat.KAB_MXFP4, 32, torch.float8_e8m0fnu)}
@@ -30,7 +30,7 @@ def _plan(m: int, n: int, k: int, fmt: int, dtype: int, device: int) -> int:
     nbytes = _PLANS.get(key)
     if nbytes is None:
         found = ctypes.c_size_t(0)
-        nat.call("kab_gemv_fp4_workspace", m, n, k, fmt, dtype, ctypes.byref(found))
+        call("kab_gemv_fp4_workspace", device, m, n, k, fmt, dtype, ctypes.byref(found))
         nbytes = _PLANS[key] = int(found.value)
     return nbytes
 
@@ -97,11 +97,10 @@ def fp4_w4a16_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
             out += b
     elif m and n:
         dtype = nat.DTYPES[x2.dtype]
-        with guard(device):
-            stream = stream_of(device)
-            nbytes = _plan(m, n, k, code, dtype, device)
-            ws = workspace("gemv", device, stream, nbytes) if nbytes else None
-            nat.call("kab_gemv_fp4", x2.data_ptr(), dtype, x2.stride(0) if m > 1 else max(k, 8), c.data_ptr(),
-                     s.data_ptr(), swizzle, code, ts.data_ptr(), per_row, m, n, k, None if b is None else b.data_ptr(),
-                     bias_code, out.data_ptr(), n, None if ws is None else ws.data_ptr(), nbytes, stream)
+        stream = stream_of(device)
+        nbytes = _plan(m, n, k, code, dtype, device)
+        ws = workspace("gemv", device, stream, nbytes) if nbytes else None
+        call("kab_gemv_fp4", device, x2.data_ptr(), dtype, x2.stride(0) if m > 1 else k, c.data_ptr(), s.data_ptr(),
+             swizzle, code, ts.data_ptr(), per_row, m, n, k, None if b is None else b.data_ptr(), bias_code,
+             out.data_ptr(), n, None if ws is None else ws.data_ptr(), nbytes, stream)
     return out if out.dtype == x.dtype and x.dim() == 2 else q._linear_out(out, x, n)

@@ -26,7 +26,7 @@ import ctypes
 import torch
 
 from .. import _native as nat
-from ._launch import device_of, guard, stream_of, to_device, workspace
+from ._launch import call, device_of, stream_of, to_device, workspace
 
 _E4M3 = torch.float8_e4m3fn
 PAGE_TOKENS = (16, 32, 64, 128)
@@ -136,9 +136,8 @@ def append_kv_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, k_s
             raise ValueError(f"{name} must be int32 [{p.batch}], contiguous; got {t.dtype} {tuple(t.shape)}")
     k, v = _rows16(k), _rows16(v)
     out = torch.empty_like(lengths) if out_lengths is None else out_lengths
-    with guard(device):
-        nat.call("kab_kv_pages_append", ctypes.byref(p), k.data_ptr(), v.data_ptr(), nat.DTYPES[k.dtype],
-                 *k.stride()[:3], *v.stride()[:3], k.shape[2], nat.ptr(counts), out.data_ptr(), stream_of(device))
+    call("kab_kv_pages_append", device, ctypes.byref(p), k.data_ptr(), v.data_ptr(), nat.DTYPES[k.dtype],
+         *k.stride()[:3], *v.stride()[:3], k.shape[2], nat.ptr(counts), out.data_ptr(), stream_of(device))
     return out
 
 
@@ -184,8 +183,7 @@ def paged_kv_attention(q: torch.Tensor, k_pages: torch.Tensor, k_scale: torch.Te
         t.heads_q, t.q_len = hq, lq
         _pointers(t.cache, *cache)
         nbytes = ctypes.c_size_t(0)
-        with guard(device):
-            nat.call("kab_kv_pages_attention_workspace", ctypes.byref(t), ctypes.byref(nbytes))
+        call("kab_kv_pages_attention_workspace", device, ctypes.byref(t), ctypes.byref(nbytes))
         made = _TEMPLATES[key] = (bytes(t), int(nbytes.value))
     template, nbytes = made
     if out is None:
@@ -195,10 +193,9 @@ def paged_kv_attention(q: torch.Tensor, k_pages: torch.Tensor, k_scale: torch.Te
     p = nat.KabKvPagesAttention.from_buffer_copy(template)
     _pointers(p.cache, *cache)
     p.q, p.out = q4.data_ptr(), out.data_ptr()
-    with guard(device):
-        stream = stream_of(device)
-        ws = workspace("pages attention", device, stream, nbytes) if nbytes else None
-        nat.call("kab_kv_pages_attention", ctypes.byref(p), nat.ptr(ws), nbytes, stream)
+    stream = stream_of(device)
+    ws = workspace("pages attention", device, stream, nbytes) if nbytes else None
+    call("kab_kv_pages_attention", device, ctypes.byref(p), nat.ptr(ws), nbytes, stream)
     return out
 
 
@@ -230,9 +227,8 @@ def evict_kv_pages(k_pages: torch.Tensor, k_scale: torch.Tensor, v_pages: torch.
         raise ValueError("out_page_table must name other pages than page_table")
     kept = lengths.new_empty((p.batch, p.heads_kv, budget))
     out = torch.empty_like(lengths)
-    with guard(device):
-        nat.call("kab_kv_pages_evict", ctypes.byref(p), out_page_table.data_ptr(), out_page_table.stride(0), budget,
-                 recent, sinks, kept.data_ptr(), out.data_ptr(), stream_of(device))
+    call("kab_kv_pages_evict", device, ctypes.byref(p), out_page_table.data_ptr(), out_page_table.stride(0), budget,
+         recent, sinks, kept.data_ptr(), out.data_ptr(), stream_of(device))
     return kept, out
 
 
