@@ -655,22 +655,40 @@ __global__ void __launch_bounds__(kGemvThreads, gemv_columns(MX, NT, GROUPED) > 
 }
 
 // The tiles that two blocks share and the slices of K, added in order (units and the tensor scale
-// are in the sums already).
+// are in the sums already). A warp has one tile and its lane i says whether two blocks share it in the i-th
+// of 32 slices, before the sums are there: at 8 x 28672 x 8192 that took 3 us less of 48.6
+// than a division by every lane for every slice.
 template <int T>
 __global__ void __launch_bounds__(256) gemv_join_kernel(GemvArgs a) {
+  static_assert(kGemvRows == 32, "a row per lane");
+  const int lane = threadIdx.x & 31, row = blockIdx.x * 256 + threadIdx.x, mt = blockIdx.y, tile = row / kGemvRows;
+  auto shared_in = [&](int s) -> uint32_t {  // slices s .. s + 31
+    bool shared = false;
+    if (s + lane < a.slices && tile < a.tiles) {
+      const int count = min(a.slice_chunks, a.chunks - (s + lane) * a.slice_chunks);
+      const GemvCut cut(a.tiles * count, a.blocks);
+      shared = cut.part_of(tile * count) != cut.part_of(tile * count + count - 1);
+    }
+    return __ballot_sync(0xffffffffu, shared);
+  };
+  uint32_t shared = shared_in(0);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int row = blockIdx.x * 256 + threadIdx.x, mt = blockIdx.y, tile = row / kGemvRows;
-  if (row >= a.n) return;
+  if (tile >= a.tiles || (a.slices == 1 && shared == 0)) return;  // the whole warp
+  const int64_t step = static_cast<int64_t>(a.m) * a.n, second = a.slices * step;
+  const float* at = a.partial + static_cast<int64_t>(mt) * a.n + min(row, a.n - 1);
   float y = 0.0f;
-  for (int s = 0; s < a.slices; ++s) {
-    const int count = min(a.slice_chunks, a.chunks - s * a.slice_chunks);
-    const GemvCut cut(a.tiles * count, a.blocks);
-    const bool shared = cut.part_of(tile * count) != cut.part_of(tile * count + count - 1);
-    if (a.slices == 1 && !shared) return;
-    const float* at = a.partial + (static_cast<int64_t>(s) * a.m + mt) * a.n + row;
-    y += __ldg(at);
-    if (shared) y += __ldg(at + static_cast<int64_t>(a.slices) * a.m * a.n);
+  for (int s = 0;;) {
+#pragma unroll 4
+    for (int i = 0; i < min(32, a.slices - s); ++i, at += step) {
+      const bool both = shared >> i & 1;
+      const float first = __ldg(at), rest = both ? __ldg(at + second) : 0.0f;
+      y += first;
+      if (both) y += rest;
+    }
+    if ((s += 32) >= a.slices) break;
+    shared = shared_in(s);
   }
+  if (row >= a.n) return;
   if (a.bias != nullptr) y += load_any(a.bias, a.bias_dtype, row);
   store_any<T>(a.out, mt * a.ldo + row, y);
 }
