@@ -7,7 +7,6 @@ import torch
 
 from .. import _native as nat
 
-_BUFFERS: dict[tuple, torch.Tensor] = {}
 _ENTRIES: dict[str, object] = {}
 
 
@@ -48,17 +47,12 @@ def stream_of(device: int) -> int:
     return torch._C._cuda_getCurrentRawStream(device)
 
 
-def workspace(op: str, device: int, stream: int, nbytes: int) -> torch.Tensor:
-    """``nbytes`` of scratch for ``op`` on ``stream``, kept for its next call there (a call's contents
-    mean nothing to the next). While a CUDA graph is captured every call makes its own: it belongs to
-    the graph, which may be replayed beside other work."""
-    if torch._C._cuda_isCurrentStreamCapturing():
-        return torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", device))
-    key = (op, device, stream)
-    buf = _BUFFERS.get(key)
-    if buf is None or buf.numel() < nbytes:
-        buf = _BUFFERS[key] = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", device))
-    return buf
+def workspace(device: int, nbytes: int) -> torch.Tensor:
+    """``nbytes`` of scratch for one call on the current stream. Each call takes its own from the
+    allocator: a call passes data from launch to launch through it, and another thread's call on the
+    same stream may enqueue its launches between them. The caller holds it until its launches are
+    enqueued; the allocator then gives it to later work of this stream only."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", device))
 
 
 def to_device(values: list, dtype: torch.dtype, device: torch.device) -> torch.Tensor:

@@ -99,7 +99,7 @@ def fp4_w4a16_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
         dtype = nat.DTYPES[x2.dtype]
         stream = stream_of(device)
         nbytes = _plan(m, n, k, code, dtype, device)
-        ws = workspace("gemv", device, stream, nbytes) if nbytes else None
+        ws = workspace(device, nbytes) if nbytes else None
         call("kab_gemv_fp4", device, x2.data_ptr(), dtype, x2.stride(0) if m > 1 else k, c.data_ptr(), s.data_ptr(),
              swizzle, code, ts.data_ptr(), per_row, m, n, k, None if b is None else b.data_ptr(), bias_code,
              out.data_ptr(), n, None if ws is None else ws.data_ptr(), nbytes, stream)

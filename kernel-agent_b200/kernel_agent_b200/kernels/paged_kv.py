@@ -194,7 +194,7 @@ def paged_kv_attention(q: torch.Tensor, k_pages: torch.Tensor, k_scale: torch.Te
     _pointers(p.cache, *cache)
     p.q, p.out = q4.data_ptr(), out.data_ptr()
     stream = stream_of(device)
-    ws = workspace("pages attention", device, stream, nbytes) if nbytes else None
+    ws = workspace(device, nbytes) if nbytes else None
     call("kab_kv_pages_attention", device, ctypes.byref(p), nat.ptr(ws), nbytes, stream)
     return out
 

@@ -1,0 +1,62 @@
+"""Host side of the decode operators without a GPU: what a wrapper hands to the C entry points, with
+the entry point itself replaced and the tensors on the CPU."""
+
+from __future__ import annotations
+
+import threading
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from kernel_agent_b200 import _native as nat
+from kernel_agent_b200.kernels import _launch, gemv, paged_kv
+
+pytestmark = pytest.mark.skipif(not nat.LIB_PATH.exists(), reason="libkab.so is not built")
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """The wrappers on CPU tensors: every entry point but the workspace queries is recorded as
+    ``(name, args)`` and handed to ``calls.seen`` where that is set."""
+    log = SimpleNamespace(made=[], seen=None)
+
+    def call(name, device, *args):
+        if name.endswith("_workspace"):
+            return nat.call(name, *args)
+        log.made.append((name, args))
+        if log.seen is not None:
+            log.seen(name, args)
+
+    for module in (gemv, paged_kv):
+        monkeypatch.setattr(module, "call", call)
+        monkeypatch.setattr(module, "device_of", lambda *tensors: -1)  # as Tensor.get_device() says on the CPU
+        monkeypatch.setattr(module, "stream_of", lambda device: 0)
+    monkeypatch.setattr(_launch, "torch", SimpleNamespace(
+        empty=torch.empty, uint8=torch.uint8, device=lambda *a: torch.device("cpu"),
+        _C=SimpleNamespace(_cuda_isCurrentStreamCapturing=lambda: False)))
+    return log
+
+
+def test_calls_of_two_threads_have_scratch_of_their_own(calls):
+    """A call enqueues several launches that pass data through its scratch memory, and the interpreter runs
+    other threads meanwhile: two calls on one stream must not share it."""
+    x = torch.zeros(5, 8192, dtype=torch.bfloat16)
+    codes, scales = torch.zeros(64, 4096, dtype=torch.uint8), torch.zeros(64, 512, dtype=torch.uint8)
+    spans = []
+    inside = threading.Barrier(2, timeout=20)
+
+    def seen(name, args):
+        spans.append((args[-3], args[-3] + args[-2]))
+        inside.wait()  # both calls are between their launches
+
+    calls.seen = seen
+    run = lambda: gemv.fp4_w4a16_linear(x, codes, scales, 1.0)  # noqa: E731
+    threads = [threading.Thread(target=run) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    (a0, a1), (b0, b1) = spans
+    assert a1 > a0 and b1 > b0
+    assert a1 <= b0 or b1 <= a0

@@ -1,0 +1,73 @@
+"""The decode operators as programs use them: from several threads, over shared pages, in captured
+steps, on inputs of unusual layout."""
+
+from __future__ import annotations
+
+import threading
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+E4M3 = torch.float8_e4m3fn
+
+
+@pytest.fixture(scope="module")
+def pk():
+    from kernel_agent_b200.kernels import paged_kv
+
+    return paged_kv
+
+
+@pytest.fixture(scope="module")
+def gv():
+    from kernel_agent_b200.kernels import gemv
+
+    return gemv
+
+
+def weight(n, k, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    codes = torch.randint(0, 256, (n, k // 2), generator=g, dtype=torch.int32).to(torch.uint8).to(DEV)
+    return codes, torch.rand(n, k // 16, generator=g).add(0.5).to(E4M3).to(DEV)
+
+
+def pool(pages, heads, page, dim, seed=0):
+    """(k_pages, k_scale, v_pages, v_scale) of normal values."""
+    g = torch.Generator().manual_seed(seed)
+    codes = [(torch.randn(pages, heads, page, dim, generator=g) * 64).clamp(-448, 448).to(E4M3).to(DEV) for _ in range(2)]
+    scale = torch.full((pages, heads), 2.0 ** -6, device=DEV)
+    return codes[0], scale, codes[1], scale.clone()
+
+
+def test_two_threads_on_one_stream(pk, gv):
+    """Calls that two threads enqueue on the default stream give what each gives alone."""
+    codes, scales = weight(4096, 4096)
+    x = torch.randn(2, 8, 4096, device=DEV).to(torch.bfloat16)
+    cache = pool(64, 2, 64, 128)
+    table = torch.arange(64, dtype=torch.int32, device=DEV).reshape(1, 64)
+    lengths = torch.tensor([4000], dtype=torch.int32, device=DEV)
+    q = torch.randn(2, 1, 8, 128, device=DEV).to(torch.bfloat16)
+    ts = torch.tensor(0.01, device=DEV)
+
+    def step(i):
+        return gv.fp4_w4a16_linear(x[i], codes, scales, ts), pk.paged_kv_attention(q[i], *cache, table, lengths)
+
+    want = [step(i) for i in range(2)]
+    got = [[], []]
+
+    def many(i):
+        for _ in range(150):
+            got[i].append(step(i))
+
+    threads = [threading.Thread(target=many, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert len(got[i]) == 150
+        for pair in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(pair, want[i]))
