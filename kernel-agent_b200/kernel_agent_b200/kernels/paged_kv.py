@@ -257,7 +257,7 @@ class PagedFp8KVCache:
         self.v_scale = torch.ones(shape[:2], dtype=torch.float32, device=dev)
         self.mass = torch.zeros(shape[:3], dtype=torch.float32, device=dev) if mass else None
         self.max_pages = num_pages if max_pages is None else max_pages
-        self.page_table = torch.zeros(batch, self.max_pages, dtype=torch.int32, device=dev)
+        self.page_table = torch.full((batch, self.max_pages), -1, dtype=torch.int32, device=dev)
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=dev)
         self.page_tokens = page_tokens
         #: Cached tokens of each sequence, as the host knows them.
@@ -275,7 +275,8 @@ class PagedFp8KVCache:
         return len(self._free)
 
     def _write_table(self) -> None:
-        rows = [pages + [0] * (self.max_pages - len(pages)) for pages in self._pages]
+        # -1 past a sequence's pages: a kernel that comes there skips it and reports it
+        rows = [pages + [-1] * (self.max_pages - len(pages)) for pages in self._pages]
         self.page_table.copy_(to_device(rows, torch.int32, self.page_table.device).reshape(self.page_table.shape))
 
     def reserve(self, counts: list[int]) -> None:

@@ -60,3 +60,43 @@ def test_calls_of_two_threads_have_scratch_of_their_own(calls):
     (a0, a1), (b0, b1) = spans
     assert a1 > a0 and b1 > b0
     assert a1 <= b0 or b1 <= a0
+
+
+@pytest.fixture
+def host_cache(monkeypatch):
+    """``PagedFp8KVCache`` with its tensors on the CPU (its functions replaced by a test where it calls them)."""
+
+    class Cpu:
+        def __getattr__(self, name):
+            return getattr(torch, name)
+
+        def device(self, *_):
+            return SimpleNamespace(type="cuda")
+
+        def zeros(self, *shape, device=None, **kw):
+            return torch.zeros(*shape, **kw)
+
+        def ones(self, *shape, device=None, **kw):
+            return torch.ones(*shape, **kw)
+
+        def full(self, *args, device=None, **kw):
+            return torch.full(*args, **kw)
+
+        cuda = SimpleNamespace(is_current_stream_capturing=lambda: False)
+
+    monkeypatch.setattr(paged_kv, "torch", Cpu())
+    monkeypatch.setattr(paged_kv, "to_device", lambda values, dtype, device: torch.tensor(values, dtype=dtype))
+    return lambda *args, **kw: paged_kv.PagedFp8KVCache(*args, device="cuda", **kw)
+
+
+def test_page_table_names_only_pages_of_the_sequence(host_cache):
+    """Entries past a sequence's pages are outside the pool, so that a kernel that reads one reports it instead
+    of touching another sequence's page."""
+    cache = host_cache(3, 1, 64, num_pages=10, page_tokens=16, max_pages=6)
+    assert (cache.page_table == -1).all()
+    cache.reserve([33, 0, 16])
+    table = cache.page_table.tolist()
+    assert [sum(p >= 0 for p in row) for row in table] == [3, 0, 1]
+    assert table[0][3:] == [-1] * 3 and table[1] == [-1] * 6 and table[2][1:] == [-1] * 5
+    cache.free(0)
+    assert cache.page_table[0].tolist() == [-1] * 6 and cache.page_table[2].tolist() == table[2]

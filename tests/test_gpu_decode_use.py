@@ -71,3 +71,18 @@ def test_two_threads_on_one_stream(pk, gv):
         assert len(got[i]) == 150
         for pair in got[i]:
             assert all(torch.equal(a, b) for a, b in zip(pair, want[i]))
+
+
+def test_append_past_the_reservation(pk):
+    """Tokens past a sequence's pages are dropped and reported; no other sequence's page changes."""
+    from kernel_agent_b200 import _native as nat
+
+    cache = pk.PagedFp8KVCache(2, 1, 64, num_pages=6, page_tokens=16)
+    x = torch.randn(2, 1, 16, 64, device=DEV)
+    cache.append(x, x)
+    before = [t.clone() for t in (cache.k_pages.view(torch.uint8), cache.k_scale, cache.mass)]
+    pk.append_kv_pages(x * 8, x * 8, *cache.pool, mass=cache.mass)
+    assert nat.device_status() == 2
+    for a, b in zip(before, (cache.k_pages.view(torch.uint8), cache.k_scale, cache.mass)):
+        assert torch.equal(a, b)
+    assert nat.device_status() == 0
