@@ -239,7 +239,9 @@ class PagedFp8KVCache:
     keeps every token's received weight), :meth:`evict` cuts sequences to a budget of tokens and
     frees the pages they leave, :meth:`free` ends a sequence. Page numbers are kept on the host, so
     nothing waits for the GPU; the calls follow one another on the current stream. A step captured
-    in a CUDA graph calls the functions of this module on :attr:`pool` after :meth:`reserve`."""
+    in a CUDA graph calls the functions of this module on :attr:`pool` after :meth:`reserve`; its replays
+    move :attr:`lengths` alone, so :meth:`advance` has to tell the host what they appended before the next
+    call of another method here."""
 
     def __init__(self, batch: int, kv_heads: int, head_dim: int, num_pages: int, page_tokens: int = 64,
                  max_pages: int | None = None, mass: bool = True, device: torch.device | str | None = None) -> None:
@@ -279,10 +281,13 @@ class PagedFp8KVCache:
         rows = [pages + [-1] * (self.max_pages - len(pages)) for pages in self._pages]
         self.page_table.copy_(to_device(rows, torch.int32, self.page_table.device).reshape(self.page_table.shape))
 
-    def reserve(self, counts: list[int]) -> None:
-        """Take the pages that ``counts[b]`` more tokens of each sequence need."""
+    def _check_counts(self, counts: list[int]) -> None:
         if len(counts) != len(self.tokens) or min(counts, default=0) < 0:
             raise ValueError(f"counts must be {len(self.tokens)} numbers of tokens; got {counts}")
+
+    def reserve(self, counts: list[int]) -> None:
+        """Take the pages that ``counts[b]`` more tokens of each sequence than :attr:`tokens` need."""
+        self._check_counts(counts)
         need = [max(0, -(-(t + c) // self.page_tokens) - len(p)) for t, c, p in zip(self.tokens, counts, self._pages)]
         if sum(need) > len(self._free):
             raise ValueError(f"paged KV cache full: {sum(need)} pages wanted, {len(self._free)} free")
@@ -292,6 +297,14 @@ class PagedFp8KVCache:
             for pages, n in zip(self._pages, need):
                 pages += [self._free.pop() for _ in range(n)]
             self._write_table()
+
+    def advance(self, counts: list[int]) -> None:
+        """Count ``counts[b]`` tokens of each sequence that replays of a captured step have appended through
+        :attr:`pool` (the device's lengths moved with them), within what :meth:`reserve` took pages for."""
+        self._check_counts(counts)
+        if any(t + c > len(p) * self.page_tokens for t, c, p in zip(self.tokens, counts, self._pages)):
+            raise ValueError(f"counts {counts} pass the pages held: reserve() before the steps that append them")
+        self.tokens = [t + c for t, c in zip(self.tokens, counts)]
 
     def append(self, k: torch.Tensor, v: torch.Tensor, counts: list[int] | None = None) -> None:
         """Append ``k``, ``v [batch, kv_heads, new, head_dim]``, the first ``counts[b]`` tokens of each

@@ -100,3 +100,23 @@ def test_page_table_names_only_pages_of_the_sequence(host_cache):
     assert table[0][3:] == [-1] * 3 and table[1] == [-1] * 6 and table[2][1:] == [-1] * 5
     cache.free(0)
     assert cache.page_table[0].tolist() == [-1] * 6 and cache.page_table[2].tolist() == table[2]
+
+
+def test_captured_steps_are_counted(host_cache):
+    """Tokens that replays appended are made known with advance(): the next reservation goes by them, and
+    no more can be counted than pages were reserved for."""
+    cache = host_cache(2, 1, 64, num_pages=10, page_tokens=16)
+    cache.reserve([40, 16])
+    assert cache.tokens == [0, 0]
+    cache.advance([40, 16])
+    assert cache.tokens == [40, 16] and [len(p) for p in cache._pages] == [3, 1]
+    cache.reserve([9, 1])
+    assert [len(p) for p in cache._pages] == [4, 2]
+    assert (cache.page_table >= 0).sum(1).tolist() == [4, 2]
+    with pytest.raises(ValueError, match="reserve"):
+        cache.advance([25, 0])
+    with pytest.raises(ValueError, match="counts"):
+        cache.advance([1])
+    with pytest.raises(ValueError, match="counts"):
+        cache.advance([1, -1])
+    assert cache.tokens == [40, 16]

@@ -86,3 +86,34 @@ def test_append_past_the_reservation(pk):
     for a, b in zip(before, (cache.k_pages.view(torch.uint8), cache.k_scale, cache.mass)):
         assert torch.equal(a, b)
     assert nat.device_status() == 0
+
+
+def test_captured_steps_then_others(pk):
+    """Replays, their count, another reservation past it and plain appends: the host and the device agree,
+    and what the other sequence holds stays."""
+    cache = pk.PagedFp8KVCache(2, 1, 64, num_pages=16, page_tokens=16)
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randn(2, 1, 20, 64, generator=g, device=DEV)
+    cache.append(x, x)
+    cache.reserve([30, 0])
+    one = torch.randn(2, 1, 1, 64, generator=g, device=DEV)
+    counts = torch.tensor([1, 0], dtype=torch.int32, device=DEV)
+    held = cache._pages[1]
+    before = cache.k_pages.view(torch.uint8)[held].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pk.append_kv_pages(one, one, *cache.pool, counts=counts, mass=cache.mass, out_lengths=cache.lengths)
+    for _ in range(28):
+        graph.replay()
+    cache.advance([28, 0])
+    assert cache.tokens == cache.lengths.tolist() == [48, 20]
+    cache.reserve([20, 0])
+    for _ in range(17):  # into the pages of the second reservation
+        graph.replay()
+    cache.advance([17, 0])
+    cache.append(one, one, counts=[1, 0])
+    assert cache.tokens == cache.lengths.tolist() == [66, 20]
+    assert torch.equal(cache.k_pages.view(torch.uint8)[held], before)
+    assert cache._pages[1] == held and len(set(cache._pages[0]) & set(held)) == 0
+    over, _ = cache.evict(40)
+    assert over == [0] and cache.tokens == cache.lengths.tolist() == [40, 20]
