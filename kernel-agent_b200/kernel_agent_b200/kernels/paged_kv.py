@@ -281,6 +281,11 @@ class PagedFp8KVCache:
         rows = [pages + [-1] * (self.max_pages - len(pages)) for pages in self._pages]
         self.page_table.copy_(to_device(rows, torch.int32, self.page_table.device).reshape(self.page_table.shape))
 
+    def _not_captured(self) -> None:
+        # neither the host's counts nor the host memory of a table's copy would be there for a replay
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the cache counts tokens on the host: reserve() first and capture append_kv_pages")
+
     def _check_counts(self, counts: list[int]) -> None:
         if len(counts) != len(self.tokens) or min(counts, default=0) < 0:
             raise ValueError(f"counts must be {len(self.tokens)} numbers of tokens; got {counts}")
@@ -294,6 +299,7 @@ class PagedFp8KVCache:
         if any(len(p) + n > self.max_pages for p, n in zip(self._pages, need)):
             raise ValueError(f"a sequence would pass {self.max_pages} pages")
         if any(need):
+            self._not_captured()
             for pages, n in zip(self._pages, need):
                 pages += [self._free.pop() for _ in range(n)]
             self._write_table()
@@ -309,8 +315,7 @@ class PagedFp8KVCache:
     def append(self, k: torch.Tensor, v: torch.Tensor, counts: list[int] | None = None) -> None:
         """Append ``k``, ``v [batch, kv_heads, new, head_dim]``, the first ``counts[b]`` tokens of each
         sequence (default: all), as :func:`append_kv_pages` does."""
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("the cache counts tokens on the host: reserve() first and capture append_kv_pages")
+        self._not_captured()
         if k.dim() != 4:
             raise ValueError(f"expected k and v [batch, kv_heads, new, head_dim]; got {tuple(k.shape)}")
         new = k.shape[2]
@@ -337,6 +342,7 @@ class PagedFp8KVCache:
         over = [b for b, n in enumerate(self.tokens) if n > budget]
         if not over:
             return [], None
+        self._not_captured()
         each = -(-budget // self.page_tokens)
         if each * len(over) > len(self._free):
             raise ValueError(f"paged KV cache full: an eviction moves into {each * len(over)} pages, "
@@ -357,6 +363,7 @@ class PagedFp8KVCache:
 
     def free(self, sequence: int) -> None:
         """End a sequence: its pages are free, its row of the batch is empty."""
+        self._not_captured()
         self._free += self._pages[sequence]
         self._pages[sequence], self.tokens[sequence] = [], 0
         self.lengths[sequence] = 0

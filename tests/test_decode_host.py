@@ -120,3 +120,18 @@ def test_captured_steps_are_counted(host_cache):
     with pytest.raises(ValueError, match="counts"):
         cache.advance([1, -1])
     assert cache.tokens == [40, 16]
+
+
+def test_no_table_is_written_inside_a_capture(host_cache, monkeypatch):
+    """A captured copy of host page numbers would be replayed from host memory that is gone by then."""
+    cache = host_cache(1, 1, 64, num_pages=8, page_tokens=16)
+    cache.reserve([40])
+    cache.advance([40])
+    pages, free, table = list(cache._pages[0]), list(cache._free), cache.page_table.clone()
+    monkeypatch.setattr(paged_kv.torch.cuda, "is_current_stream_capturing", lambda: True)
+    for method, args in ((cache.reserve, ([20],)), (cache.evict, (16,)), (cache.free, (0,))):
+        with pytest.raises(RuntimeError, match="reserve"):
+            method(*args)
+        assert cache._pages == [pages] and cache._free == free and cache.tokens == [40]
+        assert torch.equal(cache.page_table, table)
+    cache.reserve([1])  # no page needed: nothing is written
