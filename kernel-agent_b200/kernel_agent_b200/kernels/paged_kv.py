@@ -347,7 +347,8 @@ class PagedFp8KVCache:
         if each * len(over) > len(self._free):
             raise ValueError(f"paged KV cache full: an eviction moves into {each * len(over)} pages, "
                              f"{len(self._free)} free")
-        to = [[self._free.pop() for _ in range(each)] for _ in over]
+        taken = self._free[len(self._free) - each * len(over):]
+        to = [taken[i * each:(i + 1) * each] for i in range(len(over))]
         dev = self.lengths.device
         which = to_device(over, torch.int64, dev)
         target = to_device(to, torch.int32, dev)
@@ -355,6 +356,7 @@ class PagedFp8KVCache:
                                        self.page_table[which], self.lengths[which], target, budget=budget,
                                        recent=recent, sinks=sinks)
         self.lengths[which] = lengths
+        del self._free[len(self._free) - len(taken):]
         for b, pages in zip(over, to):
             self._free += self._pages[b]
             self._pages[b], self.tokens[b] = pages, budget

@@ -135,3 +135,18 @@ def test_no_table_is_written_inside_a_capture(host_cache, monkeypatch):
         assert cache._pages == [pages] and cache._free == free and cache.tokens == [40]
         assert torch.equal(cache.page_table, table)
     cache.reserve([1])  # no page needed: nothing is written
+
+
+def test_a_failed_eviction_keeps_the_free_pages(host_cache, monkeypatch):
+    cache = host_cache(1, 1, 64, num_pages=8, page_tokens=16)
+    cache.reserve([40])
+    cache.advance([40])
+    before = list(cache._free)
+
+    def fail(*args, **kw):
+        raise RuntimeError("out of memory")
+
+    monkeypatch.setattr(paged_kv, "evict_kv_pages", fail)
+    with pytest.raises(RuntimeError, match="memory"):
+        cache.evict(20)
+    assert cache._free == before and cache.tokens == [40] and len(cache._pages[0]) == 3
