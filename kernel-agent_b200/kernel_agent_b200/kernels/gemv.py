@@ -71,9 +71,9 @@ def fp4_w4a16_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     x2 = x if x.dim() == 2 else x.reshape(math.prod(x.shape[:-1]), k)
     if x2.dtype not in nat.DTYPES:
         x2 = x2.float()
-    if x2.stride(1) != 1 or x2.stride(0) % 8 or x2.stride(0) < k or x2.data_ptr() % 16:
-        x2 = x2.contiguous()
     m = x2.shape[0]
+    if x2.stride(1) != 1 or (m > 1 and (x2.stride(0) % 8 or x2.stride(0) < k)) or x2.data_ptr() % 16:
+        x2 = x2.clone(memory_format=torch.contiguous_format)  # also where x is contiguous and starts off 16 bytes
     c, s = codes.contiguous(), scales.contiguous()
     if c.data_ptr() % 8:
         c = c.clone()

@@ -150,3 +150,21 @@ def test_a_failed_eviction_keeps_the_free_pages(host_cache, monkeypatch):
     with pytest.raises(RuntimeError, match="memory"):
         cache.evict(20)
     assert cache._free == before and cache.tokens == [40] and len(cache._pages[0]) == 3
+
+
+def misaligned(shape, dtype=torch.bfloat16):
+    """A contiguous tensor one element past a 16-byte boundary."""
+    flat = torch.arange(17 + torch.Size(shape).numel(), dtype=torch.float32).to(dtype)
+    start = (16 - flat.data_ptr() % 16) % 16 // flat.element_size() + 1
+    return flat[start:start + torch.Size(shape).numel()].view(shape)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m", [1, 3])
+def test_linear_takes_x_off_16_bytes(calls, m, dtype):
+    x = misaligned((m, 64), dtype)
+    assert x.is_contiguous() and x.data_ptr() % 16
+    codes, scales = torch.zeros(8, 32, dtype=torch.uint8), torch.zeros(8, 4, dtype=torch.uint8)
+    gemv.fp4_w4a16_linear(x, codes, scales, 1.0)
+    (name, args), = calls.made
+    assert name == "kab_gemv_fp4" and args[0] % 16 == 0 and args[2] % 8 == 0

@@ -117,3 +117,12 @@ def test_captured_steps_then_others(pk):
     assert cache._pages[1] == held and len(set(cache._pages[0]) & set(held)) == 0
     over, _ = cache.evict(40)
     assert over == [0] and cache.tokens == cache.lengths.tolist() == [40, 20]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_linear_x_off_16_bytes(gv, dtype):
+    codes, scales = weight(40, 128)
+    for m in (1, 3):
+        flat = torch.randn(1 + m * 128, device=DEV).to(dtype)
+        x = flat[1:].view(m, 128)
+        assert torch.equal(gv.fp4_w4a16_linear(x, codes, scales, 0.1), gv.fp4_w4a16_linear(x.clone(), codes, scales, 0.1))
