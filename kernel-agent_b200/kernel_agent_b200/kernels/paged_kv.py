@@ -101,12 +101,13 @@ def _pool(cache: tuple) -> "nat.KabKvPages":
     return p
 
 
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """Rows that the kernels can load 16 bytes at a time."""
-    st = t.stride()
-    if st[3] != 1 or st[0] % 8 or st[1] % 8 or st[2] % 8 or t.data_ptr() % 16:
-        return t.contiguous()
-    return t
+def _rows16(t: torch.Tensor) -> tuple[torch.Tensor, list[int]]:
+    """Rows that the kernels can load 16 bytes at a time, and their strides (0 where there is one only)."""
+    strides = [s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape)]
+    if t.stride(3) != 1 or any(s % 8 for s in strides) or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)  # contiguous() would leave a tensor off 16 bytes there
+        strides = list(t.stride()[:3])
+    return t, strides
 
 
 def append_kv_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, k_scale: torch.Tensor,
@@ -134,10 +135,10 @@ def append_kv_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, k_s
     for name, t in (("counts", counts), ("out_lengths", out_lengths)):
         if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (p.batch,) or not t.is_contiguous()):
             raise ValueError(f"{name} must be int32 [{p.batch}], contiguous; got {t.dtype} {tuple(t.shape)}")
-    k, v = _rows16(k), _rows16(v)
+    (k, k_strides), (v, v_strides) = _rows16(k), _rows16(v)
     out = torch.empty_like(lengths) if out_lengths is None else out_lengths
     call("kab_kv_pages_append", device, ctypes.byref(p), k.data_ptr(), v.data_ptr(), nat.DTYPES[k.dtype],
-         *k.stride()[:3], *v.stride()[:3], k.shape[2], nat.ptr(counts), out.data_ptr(), stream_of(device))
+         *k_strides, *v_strides, k.shape[2], nat.ptr(counts), out.data_ptr(), stream_of(device))
     return out
 
 

@@ -168,3 +168,22 @@ def test_linear_takes_x_off_16_bytes(calls, m, dtype):
     gemv.fp4_w4a16_linear(x, codes, scales, 1.0)
     (name, args), = calls.made
     assert name == "kab_gemv_fp4" and args[0] % 16 == 0 and args[2] % 8 == 0
+
+
+def cpu_pool(pages=4, heads=1, page=16, dim=64):
+    codes = torch.zeros(pages, heads, page, dim, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    return codes, torch.ones(pages, heads), codes.clone(), torch.ones(pages, heads)
+
+
+def test_append_takes_rows_off_16_bytes(calls):
+    """Contiguous keys and values that start anywhere, and size-1 dimensions of any stride."""
+    table, lengths = torch.zeros(1, 4, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    off = misaligned((1, 1, 3, 64))
+    odd = torch.zeros(1, 1, 2, 70, dtype=torch.bfloat16)[:, :, 1:, :64].as_strided((1, 1, 1, 64), (70, 35, 70, 1), 0)
+    assert odd.is_contiguous() and off.is_contiguous() and off.data_ptr() % 16
+    for x in (off, odd):
+        calls.made.clear()
+        paged_kv.append_kv_pages(x, x, *cpu_pool(), table, lengths)
+        (name, args), = calls.made
+        assert name == "kab_kv_pages_append" and args[1] % 16 == args[2] % 16 == 0
+        assert all(s % 8 == 0 for s in args[4:10])

@@ -126,3 +126,20 @@ def test_linear_x_off_16_bytes(gv, dtype):
         flat = torch.randn(1 + m * 128, device=DEV).to(dtype)
         x = flat[1:].view(m, 128)
         assert torch.equal(gv.fp4_w4a16_linear(x, codes, scales, 0.1), gv.fp4_w4a16_linear(x.clone(), codes, scales, 0.1))
+
+
+def test_append_rows_off_16_bytes(pk):
+    table = torch.arange(4, dtype=torch.int32, device=DEV).reshape(1, 4)
+    lengths = torch.tensor([5], dtype=torch.int32, device=DEV)
+    for new in (1, 20):
+        flat = torch.randn(1 + new * 64, device=DEV).to(torch.bfloat16)
+        off = flat[1:].view(1, 1, new, 64)
+        got, want = pool(4, 1, 16, 64), pool(4, 1, 16, 64)
+        pk.append_kv_pages(off, off, *got, table, lengths)
+        pk.append_kv_pages(off.clone(), off.clone(), *want, table, lengths)
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, want))
+    odd = torch.randn(70, device=DEV).as_strided((1, 1, 1, 64), (70, 35, 70, 1))
+    got, want = pool(4, 1, 16, 64), pool(4, 1, 16, 64)
+    pk.append_kv_pages(odd, odd, *got, table, lengths)
+    pk.append_kv_pages(odd.clone(memory_format=torch.contiguous_format).reshape(1, 1, 1, 64), odd, *want, table, lengths)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, want))
