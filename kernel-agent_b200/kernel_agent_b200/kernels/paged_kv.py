@@ -168,6 +168,8 @@ def paged_kv_attention(q: torch.Tensor, k_pages: torch.Tensor, k_scale: torch.Te
     q4 = q if q.dim() == 4 else q.unsqueeze(2)
     if q4.stride(3) != 1:
         q4 = q4.contiguous()
+    if scale is not None:
+        scale = float(scale)  # the value: a tensor would be looked up by its identity
     cache = (k_pages, k_scale, v_pages, v_scale, mass, page_table, lengths)
     key = ("attention", q4.shape, q4.stride(), q4.dtype, device, scale, bool(causal), _layout(*cache))
     made = _TEMPLATES.get(key)
@@ -179,7 +181,7 @@ def paged_kv_attention(q: torch.Tensor, k_pages: torch.Tensor, k_scale: torch.Te
             raise ValueError(f"q {tuple(q.shape)} does not fit the cache: {t.cache.batch} sequences, "
                              f"{t.cache.heads_kv} KV heads, head_dim {t.cache.head_dim}")
         t.q_dtype, t.causal, t.use_mass = nat.DTYPES[q4.dtype], int(bool(causal)), int(mass is not None)
-        t.sm_scale = float(d ** -0.5 if scale is None else scale)
+        t.sm_scale = d ** -0.5 if scale is None else scale
         t.q_stride_b, t.q_stride_h, t.q_stride_t = q4.stride()[:3]
         t.heads_q, t.q_len = hq, lq
         _pointers(t.cache, *cache)

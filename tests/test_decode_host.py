@@ -187,3 +187,18 @@ def test_append_takes_rows_off_16_bytes(calls):
         (name, args), = calls.made
         assert name == "kab_kv_pages_append" and args[1] % 16 == args[2] % 16 == 0
         assert all(s % 8 == 0 for s in args[4:10])
+
+
+def attend(q, scale=None, heads=1, mass=None):
+    table, lengths = torch.zeros(q.shape[0], 4, dtype=torch.int32), torch.zeros(q.shape[0], dtype=torch.int32)
+    return paged_kv.paged_kv_attention(q, *cpu_pool(heads=heads), table, lengths, scale=scale, mass=mass)
+
+
+def test_attention_reads_its_scale_every_call(calls):
+    """A scale held in a tensor that changes between calls."""
+    scale = torch.tensor(0.5)
+    q = torch.zeros(1, 2, 1, 64)
+    attend(q, scale)
+    scale.fill_(0.25)
+    attend(q, scale)
+    assert [args[0]._obj.sm_scale for _, args in calls.made] == [0.5, 0.25]
