@@ -55,6 +55,15 @@ def workspace(device: int, nbytes: int) -> torch.Tensor:
     return torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", device))
 
 
+def keep(table: dict, key: tuple, value):
+    """``table[key] = value``, the table emptied first where it holds 1024 layouts: enough for a program's
+    steps, and bounded where shapes change without end. Returns ``value``."""
+    if len(table) >= 1024:
+        table.clear()
+    table[key] = value
+    return value
+
+
 def to_device(values: list, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
     """A small host list as a device tensor, without waiting for the GPU (through pinned memory)."""
     return torch.tensor(values, dtype=dtype).pin_memory().to(device, non_blocking=True)

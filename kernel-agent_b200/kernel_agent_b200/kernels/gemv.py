@@ -17,7 +17,7 @@ import torch
 
 from .. import _native as nat
 from . import quant as q
-from ._launch import call, device_of, stream_of, workspace
+from ._launch import call, device_of, keep, stream_of, workspace
 from .gemm import _bias
 
 _FORMATS = {"nvfp4": (nat.KAB_NVFP4, 16, torch.float8_e4m3fn), "mxfp4": (nat.KAB_MXFP4, 32, torch.float8_e8m0fnu)}
@@ -31,7 +31,7 @@ def _plan(m: int, n: int, k: int, fmt: int, dtype: int, device: int) -> int:
     if nbytes is None:
         found = ctypes.c_size_t(0)
         call("kab_gemv_fp4_workspace", device, m, n, k, fmt, dtype, ctypes.byref(found))
-        nbytes = _PLANS[key] = int(found.value)
+        nbytes = keep(_PLANS, key, int(found.value))
     return nbytes
 
 

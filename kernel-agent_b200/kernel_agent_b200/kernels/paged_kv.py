@@ -26,7 +26,7 @@ import ctypes
 import torch
 
 from .. import _native as nat
-from ._launch import call, device_of, stream_of, to_device, workspace
+from ._launch import call, device_of, keep, stream_of, to_device, workspace
 
 _E4M3 = torch.float8_e4m3fn
 PAGE_TOKENS = (16, 32, 64, 128)
@@ -95,7 +95,7 @@ def _pool(cache: tuple) -> "nat.KabKvPages":
     if made is None:
         p = nat.KabKvPages()
         _pool_fields(p, *cache)
-        made = _TEMPLATES[key] = (bytes(p),)
+        made = keep(_TEMPLATES, key, (bytes(p),))
     p = nat.KabKvPages.from_buffer_copy(made[0])
     _pointers(p, *cache)
     return p
@@ -187,7 +187,7 @@ def paged_kv_attention(q: torch.Tensor, k_pages: torch.Tensor, k_scale: torch.Te
         _pointers(t.cache, *cache)
         nbytes = ctypes.c_size_t(0)
         call("kab_kv_pages_attention_workspace", device, ctypes.byref(t), ctypes.byref(nbytes))
-        made = _TEMPLATES[key] = (bytes(t), int(nbytes.value))
+        made = keep(_TEMPLATES, key, (bytes(t), int(nbytes.value)))
     template, nbytes = made
     if out is None:
         out = q.new_empty(q.shape)

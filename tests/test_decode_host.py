@@ -202,3 +202,12 @@ def test_attention_reads_its_scale_every_call(calls):
     scale.fill_(0.25)
     attend(q, scale)
     assert [args[0]._obj.sm_scale for _, args in calls.made] == [0.5, 0.25]
+
+
+def test_what_is_kept_for_layouts_is_bounded(calls):
+    """Shapes that change from step to step (rows, table widths) do not grow the wrappers' tables without end."""
+    codes, scales = torch.zeros(8, 32, dtype=torch.uint8), torch.zeros(8, 4, dtype=torch.uint8)
+    for m in range(1, 1200):
+        gemv.fp4_w4a16_linear(torch.zeros(m, 64), codes, scales, 1.0)
+        attend(torch.zeros(1, 1, 1, 64), 1.0 / m)
+    assert len(gemv._PLANS) <= 1024 and len(paged_kv._TEMPLATES) <= 1024
