@@ -42,6 +42,8 @@ def _pool_fields(p, k_pages, k_scale, v_pages, v_scale, mass, page_table, length
     if k_pages.dtype != _E4M3 or v_pages.dtype != _E4M3:
         raise ValueError("the pages must be float8_e4m3fn")
     pages, heads, page, dim = k_pages.shape
+    if heads < 1:
+        raise ValueError("the pages need at least one KV head")
     if page not in PAGE_TOKENS:
         raise ValueError(f"page_tokens {page}: one of {', '.join(map(str, PAGE_TOKENS))}")
     if dim not in HEAD_DIMS:

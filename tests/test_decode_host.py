@@ -211,3 +211,8 @@ def test_what_is_kept_for_layouts_is_bounded(calls):
         gemv.fp4_w4a16_linear(torch.zeros(m, 64), codes, scales, 1.0)
         attend(torch.zeros(1, 1, 1, 64), 1.0 / m)
     assert len(gemv._PLANS) <= 1024 and len(paged_kv._TEMPLATES) <= 1024
+
+
+def test_a_pool_without_heads_is_refused(calls):
+    with pytest.raises(ValueError, match="KV head"):
+        attend(torch.zeros(1, 2, 1, 64), heads=0)
