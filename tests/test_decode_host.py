@@ -22,8 +22,11 @@ def calls(monkeypatch):
     log = SimpleNamespace(made=[], seen=None)
 
     def call(name, device, *args):
-        if name.endswith("_workspace"):
+        if name == "kab_gemv_fp4_workspace":
             return nat.call(name, *args)
+        if name == "kab_kv_pages_attention_workspace":  # the real one asks the GPU for its resident blocks
+            args[1]._obj.value = 256
+            return
         log.made.append((name, args))
         if log.seen is not None:
             log.seen(name, args)
