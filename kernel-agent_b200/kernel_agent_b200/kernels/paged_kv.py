@@ -34,6 +34,11 @@ HEAD_DIMS = (64, 128)
 _TEMPLATES: dict[tuple, tuple] = {}
 
 
+def _strides(t: torch.Tensor) -> list[int]:
+    """The strides of the first three dimensions, 0 along those of size 1, whose strides mean nothing."""
+    return [s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape)]
+
+
 def _pool_fields(p, k_pages, k_scale, v_pages, v_scale, mass, page_table, lengths) -> None:
     """Checks the cache's tensors and fills everything of ``p`` but the pointers."""
     if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
@@ -64,8 +69,8 @@ def _pool_fields(p, k_pages, k_scale, v_pages, v_scale, mass, page_table, length
     batch = page_table.shape[0]
     if lengths.dtype != torch.int32 or tuple(lengths.shape) != (batch,) or not lengths.is_contiguous():
         raise ValueError(f"lengths must be int32 [{batch}], contiguous; got {lengths.dtype} {tuple(lengths.shape)}")
-    p.k_stride_page, p.k_stride_head, p.k_stride_token = k_pages.stride()[:3]
-    p.v_stride_page, p.v_stride_head, p.v_stride_token = v_pages.stride()[:3]
+    p.k_stride_page, p.k_stride_head, p.k_stride_token = _strides(k_pages)
+    p.v_stride_page, p.v_stride_head, p.v_stride_token = _strides(v_pages)
     p.ks_stride_page, p.ks_stride_head = k_scale.stride()
     p.vs_stride_page, p.vs_stride_head = v_scale.stride()
     if mass is not None:
@@ -104,11 +109,11 @@ def _pool(cache: tuple) -> "nat.KabKvPages":
 
 
 def _rows16(t: torch.Tensor) -> tuple[torch.Tensor, list[int]]:
-    """Rows that the kernels can load 16 bytes at a time, and their strides (0 where there is one only)."""
-    strides = [s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape)]
+    """Rows that the kernels can load 16 bytes at a time, and their strides."""
+    strides = _strides(t)
     if t.stride(3) != 1 or any(s % 8 for s in strides) or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)  # contiguous() would leave a tensor off 16 bytes there
-        strides = list(t.stride()[:3])
+        strides = _strides(t)
     return t, strides
 
 

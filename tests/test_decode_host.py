@@ -219,3 +219,18 @@ def test_what_is_kept_for_layouts_is_bounded(calls):
 def test_a_pool_without_heads_is_refused(calls):
     with pytest.raises(ValueError, match="KV head"):
         attend(torch.zeros(1, 2, 1, 64), heads=0)
+
+
+def test_pool_strides_of_single_rows_do_not_count(calls):
+    """A pool of one head, or one page, whose stride along it is anything."""
+    flat = torch.zeros(4 * 16 * 64 + 64, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    pages = flat.as_strided((4, 1, 16, 64), (1024, 7, 64, 1))
+    one = flat.as_strided((1, 2, 16, 64), (1 << 33, 1024, 64, 1))
+    for codes, heads in ((pages, 1), (one, 2)):
+        scale = torch.ones(codes.shape[:2])
+        table, lengths = torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+        calls.made.clear()
+        paged_kv.paged_kv_attention(torch.zeros(1, 2, 1, 64), codes, scale, codes, scale, table, lengths)
+        cache = calls.made[0][1][0]._obj.cache
+        assert cache.k_stride_head % 16 == cache.v_stride_head % 16 == 0
+        assert cache.k_stride_page < 1 << 31 and cache.v_stride_page < 1 << 31
