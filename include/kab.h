@@ -531,7 +531,8 @@ typedef struct KabKvPages {
  * |value| <= 448 s for every finite value appended to it, or its old scale where that is larger;
  * when it grows, the codes that the page holds already are rewritten as e4m3(code * old / s).
  * Infinities become the largest code, NaN stays NaN. The new slots' mass becomes 0.
- * lengths_out[b] = lengths[b] + counts[b]; it may be `lengths` itself. */
+ * lengths_out[b] = lengths[b] + counts[b]; it may be `lengths` itself. A page that receives tokens
+ * belongs to one sequence. */
 int kab_kv_pages_append(const KabKvPages* cache, const void* k, const void* v, int dtype,
                         int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_t,
                         int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_t,
@@ -542,7 +543,8 @@ int kab_kv_pages_append(const KabKvPages* cache, const void* k, const void* v, i
  * of q's dtype, contiguous. With `causal` the queries are the newest q_len tokens: query i sees
  * the first lengths[b] - q_len + 1 + i; otherwise every query sees all. A query that sees
  * nothing gives zeros. With `use_mass`, every cached token's weight, summed over the query heads
- * of its KV head and the query tokens, is added to its mass. head_dim 64 or 128. The workspace:
+ * of its KV head and the query tokens, is added to its mass; a page that several sequences name
+ * (a common prefix) receives from each, in no fixed order. head_dim 64 or 128. The workspace:
  * as for kab_gemv_fp4 (with mass it holds the scores of every row and token of the page table). */
 typedef struct KabKvPagesAttention {
   KabKvPages cache;

@@ -759,7 +759,10 @@ __global__ void __launch_bounds__(512) pages_merge_kernel(PagesAttnArgs a) {
 
 // The mass of every cached token: its weights, from the stored scores and the rows' final
 // reference and sum, added in the order of the rows. One thread per four tokens and KV head (they
-// stand in one page), one 16-byte load per row.
+// stand in one page), one 16-byte load per row. Sequences with a common prefix may name the same page, so
+// what each of them gives is added atomically: one addition per token where a page is a sequence's own.
+// (Against a plain load and store: 9 x 4 x 1500 17.8 -> 19.1 us, 32 x 8192 64.8 us either way; four tokens in
+// one atomic addition the same.)
 __global__ void __launch_bounds__(256) pages_mass_kernel(PagesAttnArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const PagePool& p = a.pool;
@@ -770,9 +773,6 @@ __global__ void __launch_bounds__(256) pages_mass_kernel(PagesAttnArgs a) {
   const int page = __ldg(p.table + b * p.table_stride + (x >> p.page_shift));
   if (page < 0 || page >= p.num_pages) return;  // reported by the attention
   float* mass = p.mass + page * p.msp + h * p.msh + (x & ((1 << p.page_shift) - 1));
-  float held[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) held[e] = x + e < n ? mass[e] : 0.0f;
   const int64_t row0 = (static_cast<int64_t>(b) * p.heads + h) * a.rows;
   const float* s = a.scores + row0 * a.capacity + x;
   const float2* ml = reinterpret_cast<const float2*>(a.ml) + row0;
@@ -788,7 +788,7 @@ __global__ void __launch_bounds__(256) pages_mass_kernel(PagesAttnArgs a) {
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    if (x + e < n) mass[e] = held[e] + received[e];
+    if (x + e < n) atomicAdd(mass + e, received[e]);
   }
 }
 

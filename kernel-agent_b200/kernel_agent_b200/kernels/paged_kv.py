@@ -130,7 +130,7 @@ def append_kv_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, k_s
     finite value appended to it; codes are ``e4m3(x / s)``, to nearest even. Appending to a page
     that would need a larger scale rewrites the page's codes as ``e4m3(code * old / s)``. An
     infinity becomes the largest code of its sign, NaN stays NaN. ``mass`` of the new slots
-    becomes 0."""
+    becomes 0. A page that receives tokens must be one sequence's own."""
     device = device_of(k, v, k_pages, k_scale, v_pages, v_scale, page_table, lengths, counts, mass, out_lengths)
     p = _pool((k_pages, k_scale, v_pages, v_scale, mass, page_table, lengths))
     if k.dim() != 4 or v.shape != k.shape or k.shape[0] != p.batch or k.shape[1] != p.heads_kv \
@@ -160,7 +160,8 @@ def paged_kv_attention(q: torch.Tensor, k_pages: torch.Tensor, k_scale: torch.Te
     With ``causal`` the queries are the newest ``Lq`` cached tokens: query i sees the first
     ``lengths[b] - Lq + 1 + i`` tokens; without it every query sees every token. A query that sees
     nothing gives zeros. With ``mass``, the weight of every cached token, summed over the query
-    heads of its KV head and the query tokens, is added to its entry. Made for the few rows (query
+    heads of its KV head and the query tokens, is added to its entry; pages of a common prefix may stand
+    in several rows of the table and receive from each (in no fixed order). Made for the few rows (query
     heads per KV head x query tokens) of a decode step: each 16 rows (8 where there are no more) read
     the cache once.
     ``mass`` takes scratch memory of four bytes per query row and token that the page table has room

@@ -143,3 +143,25 @@ def test_append_rows_off_16_bytes(pk):
     pk.append_kv_pages(odd, odd, *got, table, lengths)
     pk.append_kv_pages(odd.clone(memory_format=torch.contiguous_format).reshape(1, 1, 1, 64), odd, *want, table, lengths)
     assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("page", [16, 64])
+def test_mass_of_pages_that_sequences_share(pk, page):
+    """Twelve sequences with a common prefix: its tokens receive from all of them. A weight is off by at most
+    2^-18 and the sums of a few of them by less (the cuts differ with the batch), so 2^-16 in all."""
+    shared, own, batch = 4, 2, 12
+    cache = pool(shared + own * batch, 2, page, 64)
+    table = torch.stack([torch.cat([torch.arange(shared), shared + own * b + torch.arange(own)]) for b in range(batch)])
+    table = table.to(torch.int32).to(DEV)
+    lengths = torch.tensor([(shared + 1) * page + 1 + b for b in range(batch)], dtype=torch.int32, device=DEV)
+    q = torch.randn(batch, 4, 1, 64, device=DEV)
+    shape = cache[1].shape + (page,)
+    want = torch.zeros(shape, dtype=torch.float64, device=DEV)
+    for b in range(batch):
+        mass = torch.zeros(shape, device=DEV)
+        pk.paged_kv_attention(q[b:b + 1], *cache, table[b:b + 1], lengths[b:b + 1], mass=mass)
+        want += mass.double()
+    for _ in range(10):
+        mass = torch.zeros(shape, device=DEV)
+        pk.paged_kv_attention(q, *cache, table, lengths, mass=mass)
+        assert ((mass.double() - want).abs() <= 2.0 ** -16 * want).all()
