@@ -777,14 +777,22 @@ __global__ void __launch_bounds__(256) pages_mass_kernel(PagesAttnArgs a) {
   const float* s = a.scores + row0 * a.capacity + x;
   const float2* ml = reinterpret_cast<const float2*>(a.ml) + row0;
   float received[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  // of the four tokens, those that row r sees: all (past n nothing is added) but near the end of several queries
+  const int first_sees = n - a.q_len + 1 - x;
+  const bool some = a.causal && first_sees < 4 && a.q_len > 1;
 #pragma unroll 4
   for (int r = 0; r < a.rows; ++r) {
     const float2 f = __ldg(ml + r);
     const float4 v = __ldg(reinterpret_cast<const float4*>(s + r * a.capacity));
-    received[0] += exp2_approx(v.x - f.x) * f.y;
-    received[1] += exp2_approx(v.y - f.x) * f.y;
-    received[2] += exp2_approx(v.z - f.x) * f.y;
-    received[3] += exp2_approx(v.w - f.x) * f.y;
+    float w[4] = {exp2_approx(v.x - f.x) * f.y, exp2_approx(v.y - f.x) * f.y, exp2_approx(v.z - f.x) * f.y,
+                  exp2_approx(v.w - f.x) * f.y};
+    if (some) {  // a row gives nothing to the others, also where its sum is NaN
+      const int left = first_sees + r % a.q_len;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = e < left ? w[e] : 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) received[e] += w[e];
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) {

@@ -165,3 +165,22 @@ def test_mass_of_pages_that_sequences_share(pk, page):
         mass = torch.zeros(shape, device=DEV)
         pk.paged_kv_attention(q, *cache, table, lengths, mass=mass)
         assert ((mass.double() - want).abs() <= 2.0 ** -16 * want).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_nan_query_gives_nothing_to_tokens_it_does_not_see(pk, dtype):
+    """Query i of 3 sees all tokens but the last 2 - i."""
+    page, n = 16, 44
+    cache = pool(3, 1, page, 64)
+    table = torch.arange(3, dtype=torch.int32, device=DEV).reshape(1, 3)
+    lengths = torch.tensor([n], dtype=torch.int32, device=DEV)
+    q = torch.randn(1, 2, 3, 64, device=DEV).to(dtype)
+    for i in range(3):
+        bad = q.clone()
+        bad[0, 1, i, 7] = float("nan")
+        mass = torch.zeros(3, 1, page, device=DEV)
+        pk.paged_kv_attention(bad, *cache, table, lengths, mass=mass)
+        flat = mass.reshape(-1)
+        seen = n - 2 + i
+        assert torch.isnan(flat[:seen]).all() and torch.isfinite(flat[seen:n]).all()
+        assert (flat[seen:n] > 0).all() and (flat[n:] == 0).all()
