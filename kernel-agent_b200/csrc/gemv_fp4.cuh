@@ -520,7 +520,9 @@ __global__ void __launch_bounds__(kGemvThreads, gemv_columns(MX, NT, GROUPED) > 
   auto put = [&](int tile, int r, int mt, float y, int part) {
     const int64_t row = static_cast<int64_t>(tile) * kGemvRows + r;
     if (row >= a.n || mt >= tokens) return;
-    y *= unit[mt] * __ldg(a.ts + (a.ts_per_row ? row : 0));
+    // one rounding: in fp32 the product of the two factors, or of y and one of them, may leave the normal range
+    // where the result does not
+    y = static_cast<float>(static_cast<double>(y) * unit[mt] * __ldg(a.ts + (a.ts_per_row ? row : 0)));
     if (part < 0 && a.slices == 1) {
       if (a.bias != nullptr) y += load_any(a.bias, a.bias_dtype, row);
       store_any<T>(a.out, (m0 + mt) * a.ldo + row, y);

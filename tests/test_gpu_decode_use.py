@@ -184,3 +184,25 @@ def test_a_nan_query_gives_nothing_to_tokens_it_does_not_see(pk, dtype):
         seen = n - 2 + i
         assert torch.isnan(flat[:seen]).all() and torch.isfinite(flat[seen:n]).all()
         assert (flat[seen:n] > 0).all() and (flat[n:] == 0).all()
+
+
+@pytest.mark.parametrize("m", [1, 2, 8, 16])
+@pytest.mark.parametrize("size,ts", [(1e-33, 1e-4), (1e-36, 3.0), (2e36, 1e-6), (1e-30, 1e-8)])
+def test_linear_far_from_one(gv, size, ts, m):
+    """fp32 activations whose unit times the tensor scale is subnormal, and sums that pass fp32 before the
+    scale: the result is normal and keeps its bits. Bound: as for any linear (a partial sum loses at most
+    2^-22 of sum |x| |w|, K / 16 + 64 of them follow one another)."""
+    codes, scales = weight(48, 1024, 5)
+    scales = (scales.float() * 128).to(E4M3)  # sums of about 2^13 of x's size
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn(m, 1024, generator=g, device=DEV) * size
+    level = torch.tensor([0.0, 0.5, 1, 1.5, 2, 3, 4, 6], dtype=torch.float64, device=DEV)
+    level = torch.cat([level, -level])
+    w = torch.stack([level[(codes & 15).long()], level[(codes >> 4).long()]], -1).reshape(48, 1024)
+    w = w * scales.double().repeat_interleave(16, 1)
+    factor = torch.tensor(ts, device=DEV)
+    want = x.double() @ w.T * factor.double()
+    bound = x.double().abs() @ w.abs().T * factor.double()
+    assert 1e-36 < want.abs().median() < 1e38
+    y = gv.fp4_w4a16_linear(x, codes, scales, factor)
+    assert ((y.double() - want).abs() <= 2.0 ** -24 * want.abs() + (1024 / 16 + 64) * 2.0 ** -22 * bound + 1e-44).all()
