@@ -73,6 +73,20 @@ GemvPlan gemv_plan(int64_t m, int64_t n, int64_t k, int fmt, int dtype) {
   return p;
 }
 
+// Rows of x that share the launches of a call: all where their partial sums and terms fit in 256 MB, else as
+// many groups of 32 as do (2048 x 28672 x 8192 would take 2.3 GB; the weight is read again for every 32 rows
+// either way).
+constexpr size_t kGemvMost = size_t(256) << 20;
+int64_t gemv_rows(int64_t m, int64_t n, int64_t k, int fmt, int dtype) {
+  if (m <= 32 || gemv_plan(m, n, k, fmt, dtype).bytes() <= kGemvMost) return m;
+  return std::max<int64_t>(1, kGemvMost / gemv_plan(32, n, k, fmt, dtype).bytes()) * 32;
+}
+size_t gemv_bytes(int64_t m, int64_t n, int64_t k, int fmt, int dtype) {
+  const int64_t rows = gemv_rows(m, n, k, fmt, dtype), rest = m % rows;
+  const size_t most = gemv_plan(rows, n, k, fmt, dtype).bytes();
+  return rest == 0 ? most : std::max(most, gemv_plan(rest, n, k, fmt, dtype).bytes());
+}
+
 // A launch that may be set up while the one before it runs (it waits by itself).
 cudaError_t launch_after(void (*kern)(GemvArgs), dim3 grid, int threads, int smem, cudaStream_t s, const GemvArgs& a) {
   cudaLaunchConfig_t cfg = {};
@@ -148,7 +162,7 @@ extern "C" {
 int kab_gemv_fp4_workspace(int64_t m, int64_t n, int64_t k, int fmt, int dtype, size_t* bytes) {
   if (int e = gemv_check(m, n, k, fmt, dtype)) return e;
   KAB_REQUIRE(bytes != nullptr, "null pointer");
-  *bytes = m == 0 || n == 0 ? 0 : gemv_plan(m, n, k, fmt, dtype).bytes();
+  *bytes = m == 0 || n == 0 ? 0 : gemv_bytes(m, n, k, fmt, dtype);
   return KAB_OK;
 }
 
@@ -164,24 +178,32 @@ int kab_gemv_fp4(const void* x, int dtype, int64_t ldx, const uint8_t* codes, co
   KAB_REQUIRE(aligned(codes, 8), "codes must be 8-byte aligned");
   KAB_REQUIRE(aligned(scales, 4), "scales must be 4-byte aligned");
   KAB_REQUIRE(ldo >= n && ldx >= k, "ldx %lld or ldo %lld is too short", (long long)ldx, (long long)ldo);
-  const GemvPlan p = gemv_plan(m, n, k, fmt, dtype);
-  KAB_REQUIRE(p.bytes() == 0 || (workspace != nullptr && workspace_bytes >= p.bytes() && aligned(workspace, 256)),
-              "the workspace needs %zu bytes, 256-byte aligned (kab_gemv_fp4_workspace)", p.bytes());
+  const size_t need = gemv_bytes(m, n, k, fmt, dtype);
+  KAB_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && aligned(workspace, 256)),
+              "the workspace needs %zu bytes, 256-byte aligned (kab_gemv_fp4_workspace)", need);
   GemvArgs a{};
-  a.x = x, a.ldx = ldx, a.codes = codes, a.scales = scales, a.swizzle = swizzle;
+  a.ldx = ldx, a.codes = codes, a.scales = scales, a.swizzle = swizzle;
   a.ts = tensor_scale, a.ts_per_row = scale_per_row;
-  a.m = static_cast<int>(m), a.n = static_cast<int>(n), a.k = static_cast<int>(k);
-  a.bias = bias, a.bias_dtype = bias_dtype, a.out = out, a.ldo = ldo;
-  a.chunks = p.chunks, a.slice_chunks = p.slice_chunks, a.slices = p.slices;
-  a.tiles = p.tiles, a.blocks = p.blocks, a.partial = static_cast<float*>(workspace);
-  if (p.terms) {
-    a.x_terms = static_cast<uint8_t*>(workspace) + p.partial;
-    a.x_units = reinterpret_cast<float*>(a.x_terms + p.x_terms);
-  }
+  a.n = static_cast<int>(n), a.k = static_cast<int>(k);
+  a.bias = bias, a.bias_dtype = bias_dtype, a.ldo = ldo;
   const cudaStream_t s = as_stream(stream);
-  if (dtype == KAB_BF16) return launch_gemv<kBF16>(a, p, fmt, s);
-  if (dtype == KAB_F16) return launch_gemv<kF16>(a, p, fmt, s);
-  return launch_gemv<kF32>(a, p, fmt, s);
+  const int64_t step = gemv_rows(m, n, k, fmt, dtype), size = dtype == KAB_F32 ? 4 : 2;
+  for (int64_t m0 = 0; m0 < m; m0 += step) {
+    const int64_t rows = std::min(step, m - m0);
+    const GemvPlan p = gemv_plan(rows, n, k, fmt, dtype);
+    a.x = static_cast<const uint8_t*>(x) + m0 * ldx * size;
+    a.out = static_cast<uint8_t*>(out) + m0 * ldo * size;
+    a.m = static_cast<int>(rows);
+    a.chunks = p.chunks, a.slice_chunks = p.slice_chunks, a.slices = p.slices;
+    a.tiles = p.tiles, a.blocks = p.blocks, a.partial = static_cast<float*>(workspace);
+    a.x_terms = p.terms ? static_cast<uint8_t*>(workspace) + p.partial : nullptr;
+    a.x_units = p.terms ? reinterpret_cast<float*>(a.x_terms + p.x_terms) : nullptr;
+    const int e = dtype == KAB_BF16 ? launch_gemv<kBF16>(a, p, fmt, s)
+                  : dtype == KAB_F16 ? launch_gemv<kF16>(a, p, fmt, s)
+                                     : launch_gemv<kF32>(a, p, fmt, s);
+    if (e != KAB_OK) return e;
+  }
+  return KAB_OK;
 }
 
 }  // extern "C"

@@ -3,6 +3,7 @@ the entry point itself replaced and the tensors on the CPU."""
 
 from __future__ import annotations
 
+import ctypes
 import threading
 from types import SimpleNamespace
 
@@ -234,3 +235,17 @@ def test_pool_strides_of_single_rows_do_not_count(calls):
         cache = calls.made[0][1][0]._obj.cache
         assert cache.k_stride_head % 16 == cache.v_stride_head % 16 == 0
         assert cache.k_stride_page < 1 << 31 and cache.v_stride_page < 1 << 31
+
+
+@pytest.mark.parametrize("m,n,k", [(2048, 28672, 8192), (65535, 57344, 8192), (1171, 28672, 2048), (4000, 4096, 131072)])
+@pytest.mark.parametrize("fmt", [nat.KAB_NVFP4, nat.KAB_MXFP4])
+def test_linear_workspace_is_bounded(m, n, k, fmt):
+    """Many rows go through in groups: 256 MB of scratch, or what 32 rows need where that is more."""
+    def size(rows):
+        found = ctypes.c_size_t(0)
+        nat.call("kab_gemv_fp4_workspace", rows, n, k, fmt, nat.KAB_BF16, ctypes.byref(found))
+        return found.value
+
+    assert size(m) <= max(256 << 20, size(32))
+    for rows in (1, 2, 5, 8, 9, 16, 17, 31):  # what is left for the last group needs no more
+        assert size(m // 32 * 32 + rows) <= max(256 << 20, size(32), size(rows))

@@ -206,3 +206,15 @@ def test_linear_far_from_one(gv, size, ts, m):
     assert 1e-36 < want.abs().median() < 1e38
     y = gv.fp4_w4a16_linear(x, codes, scales, factor)
     assert ((y.double() - want).abs() <= 2.0 ** -24 * want.abs() + (1024 / 16 + 64) * 2.0 ** -22 * bound + 1e-44).all()
+
+
+def test_linear_many_rows_in_groups(gv):
+    """More rows than one group takes: any 32 give what they give alone (fewer alone may be cut along K
+    differently)."""
+    codes, scales = weight(28672, 2048, 7)
+    x = torch.randn(1300, 2048, device=DEV).to(torch.bfloat16)
+    bias = torch.randn(28672, device=DEV)
+    ts = torch.tensor(0.01, device=DEV)
+    y = gv.fp4_w4a16_linear(x, codes, scales, ts, bias)
+    for lo in (0, 32, 1120, 1152, 1184, 1268):
+        assert torch.equal(y[lo:lo + 32], gv.fp4_w4a16_linear(x[lo:lo + 32], codes, scales, ts, bias))
