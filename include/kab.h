@@ -545,7 +545,8 @@ int kab_kv_pages_append(const KabKvPages* cache, const void* k, const void* v, i
  * nothing gives zeros. With `use_mass`, every cached token's weight, summed over the query heads
  * of its KV head and the query tokens, is added to its mass; a page that several sequences name
  * (a common prefix) receives from each, in no fixed order. head_dim 64 or 128. The workspace:
- * as for kab_gemv_fp4 (with mass it holds the scores of every row and token of the page table). */
+ * as for kab_gemv_fp4 (with mass it holds the scores of rows x tokens of the page table, for as many
+ * sequences or query tokens at a time as keep them in 256 MB). */
 typedef struct KabKvPagesAttention {
   KabKvPages cache;
   const void* q;

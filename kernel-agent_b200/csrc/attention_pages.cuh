@@ -51,7 +51,9 @@ struct PagesAttnArgs {
   int64_t qb, qh, qt;
   void* out;
   float scale_log2;  // sm_scale * log2(e)
-  int heads_q, q_len, causal;
+  int heads_q, q_len, causal;  // q_len: query tokens of this launch, of those of the call
+  int tail;                    // causal: newest tokens of every sequence that belong to later launches' queries
+  int q_skip, out_rows;        // the call's query tokens less this launch's; rows of one KV head in `out`
   int rows, row_tiles;   // rows of one KV head (query heads x query tokens), tiles of 8 or 16 of them
   float* partial;        // [grid, 2 slots, a tile's rows, D + 2]: output, maximum, sum
   PagesCut* cuts;        // [items or grid]: the shared items, by item or by the block that begins them
@@ -174,13 +176,20 @@ struct PagesItem {
   unsigned first;
 };
 
+// Tokens of sequence b that any query of this launch sees, cut to what the page table can hold.
+__device__ __forceinline__ int pages_tokens(const PagesAttnArgs& a, int b) {
+  const int cap = a.pool.max_pages << a.pool.page_shift;
+  return max(min(max(__ldg(a.pool.lengths + b), 0), cap) - a.tail, 0);
+}
+
 // Four output elements of row r (of a KV head's rows) from their weighted sum and the row's sum.
 template <int T, int D>
 __device__ __forceinline__ void pages_finish(const PagesAttnArgs& a, int b, int h, int r, int d, int n, float4 acc,
                                              float ref, float sum) {
   const int seen = a.causal ? max(0, n - a.q_len + 1 + r % a.q_len) : n;
   const float inv = seen > 0 ? 1.0f / sum : 0.0f;  // a row that sees nothing gives zeros
-  const int64_t row = (static_cast<int64_t>(b) * a.pool.heads + h) * a.rows + r, at = row * D + d;
+  const int64_t head = static_cast<int64_t>(b) * a.pool.heads + h, row = head * a.rows + r;
+  const int64_t at = (head * a.out_rows + r + (a.q_skip != 0 ? r / a.q_len * a.q_skip : 0)) * D + d;
   if constexpr (T == kF32) {
     *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) =
         make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
@@ -217,13 +226,12 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
   const PagePool& p = a.pool;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int P = 1 << p.page_shift, group = a.heads_q / p.heads, per_seq = p.heads * a.row_tiles;
-  const int cap = p.max_pages << p.page_shift;
 
   // the merge may be set up while this kernel runs: it waits for its end by itself
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // ---- this block's part of the line
   auto units_of = [&](int b) -> unsigned {
-    const int n = min(max(__ldg(p.lengths + b), 0), cap);
+    const int n = pages_tokens(a, b);
     return max((n + SL - 1) >> SHIFT, 1) + COST;  // an empty sequence is one empty slab: its output is written too
   };
   const int chunk = (p.batch + NT - 1) / NT;
@@ -294,7 +302,7 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
 
   PagesCut cut{0, 0, 0, 0, -1, 0};
   for (unsigned pos = lo; pos < hi;) {
-    it.length = page_length(p, it.b, status);
+    it.length = max(page_length(p, it.b, status) - a.tail, 0);
     const unsigned end = it.first + units_of(it.b);
     it.slabs = static_cast<int>(end - it.first) - COST;
     // the item's first COST units stand for what an item costs beside its slabs
@@ -753,7 +761,7 @@ __global__ void __launch_bounds__(512) pages_merge_kernel(PagesAttnArgs a) {
     acc.z += x.z;
     acc.w += x.w;
   }
-  const int n = min(max(__ldg(a.pool.lengths + cut.b), 0), a.pool.max_pages << a.pool.page_shift);
+  const int n = pages_tokens(a, cut.b);
   pages_finish<T, D>(a, cut.b, cut.h, r, lane * 4, n, acc, ref, sum);
 }
 
@@ -767,7 +775,7 @@ __global__ void __launch_bounds__(256) pages_mass_kernel(PagesAttnArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const PagePool& p = a.pool;
   const int h = blockIdx.y, b = blockIdx.z;
-  const int n = min(max(__ldg(p.lengths + b), 0), p.max_pages << p.page_shift);
+  const int n = pages_tokens(a, b);
   const int x = (blockIdx.x * 256 + threadIdx.x) * 4;
   if (x >= n) return;
   const int page = __ldg(p.table + b * p.table_stride + (x >> p.page_shift));

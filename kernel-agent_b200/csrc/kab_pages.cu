@@ -107,20 +107,47 @@ int attention_check(const KabKvPagesAttention* p, PagesAttnArgs* g) {
               (long long)p->heads_q, (long long)p->cache.heads_kv);
   KAB_REQUIRE(p->heads_q * p->q_len < (int64_t(1) << 20), "too many query rows per sequence");
   KAB_REQUIRE(!p->use_mass || p->cache.mass != nullptr || p->cache.num_pages == 0, "use_mass without a mass");
-  g->q = p->q;
   g->qb = p->q_stride_b;
   g->qh = p->q_stride_h;
   g->qt = p->q_stride_t;
-  g->out = p->out;
   g->scale_log2 = p->sm_scale * 1.4426950408889634f;
   g->heads_q = static_cast<int>(p->heads_q);
-  g->q_len = static_cast<int>(p->q_len);
   g->causal = p->causal != 0;
-  g->rows = static_cast<int>(p->heads_q / p->cache.heads_kv * p->q_len);
-  const int tile = tile_rows(g->rows);
-  g->row_tiles = (g->rows + tile - 1) / tile;
   g->capacity = p->cache.max_pages * p->cache.page_tokens;
   return KAB_OK;
+}
+
+// What one round of launches takes of a call: sequences and query tokens.
+struct AttentionPart {
+  int64_t batch, queries;
+};
+// All of them without mass. With it the scores of every (row, token of the page table) are kept until the
+// rows' sums are known: as many query tokens, or sequences with all of theirs, as keep those in 256 MB (a
+// prompt of 4 x 2048 tokens and 32 heads would take 2.1 GB).
+constexpr int64_t kScoresMost = int64_t(256) << 20;
+AttentionPart attention_part(const KabKvPagesAttention* p) {
+  const int64_t pair = p->heads_q * p->cache.max_pages * p->cache.page_tokens * 4;  // a sequence's query token
+  if (!p->use_mass || pair == 0) return {p->cache.batch, p->q_len};
+  const int64_t fit = std::max<int64_t>(1, kScoresMost / pair);
+  if (fit >= p->q_len) return {std::min(p->cache.batch, fit / p->q_len), p->q_len};
+  return {1, fit >= 16 ? fit / 16 * 16 : fit};
+}
+// The arguments of the part at sequence b0 and query token q0.
+void attention_args(const KabKvPagesAttention* p, int64_t b0, int64_t batch, int64_t q0, int64_t queries,
+                    PagesAttnArgs* g) {
+  const int64_t size = p->q_dtype == KAB_F32 ? 4 : 2, group = p->heads_q / p->cache.heads_kv;
+  g->pool.batch = static_cast<int>(batch);
+  g->pool.table = p->cache.page_table + b0 * p->cache.table_stride;
+  g->pool.lengths = p->cache.lengths + b0;
+  g->q = static_cast<const uint8_t*>(p->q) + (b0 * p->q_stride_b + q0 * p->q_stride_t) * size;
+  g->out = static_cast<uint8_t*>(p->out) + (b0 * p->heads_q * p->q_len + q0) * p->cache.head_dim * size;
+  g->q_len = static_cast<int>(queries);
+  g->tail = p->causal ? static_cast<int>(p->q_len - q0 - queries) : 0;
+  g->q_skip = static_cast<int>(p->q_len - queries);
+  g->out_rows = static_cast<int>(group * p->q_len);
+  g->rows = static_cast<int>(group * queries);
+  const int tile = tile_rows(g->rows);
+  g->row_tiles = (g->rows + tile - 1) / tile;
 }
 
 // The launch's workspace: the blocks' partial results and cuts and, with mass, the scores and the
@@ -172,7 +199,7 @@ int attention_plan(const KabKvPagesAttention* p, const PagesAttnArgs& g, Attenti
     return attention_blocks<decltype(T)::value, decltype(D)::value, decltype(NR)::value, decltype(SL)::value>();
   });
   if (plan->grid < 0) return fail(KAB_ECUDA, "cannot configure the paged attention kernel");
-  const size_t items = static_cast<size_t>(p->cache.batch * p->cache.heads_kv);
+  const size_t items = static_cast<size_t>(g.pool.batch) * g.pool.heads;
   KAB_REQUIRE(items * g.row_tiles * (static_cast<size_t>(g.capacity) / 16 + 1 + kItemCost) < (size_t(1) << 31),
               "sequences x KV heads x row tiles x tokens of the page table is too large");
   plan->merges = static_cast<int>(std::min(items * g.row_tiles, static_cast<size_t>(plan->grid)));
@@ -274,10 +301,16 @@ int kab_kv_pages_attention_workspace(const KabKvPagesAttention* params, size_t* 
   PagesAttnArgs g{};
   if (int e = attention_check(params, &g)) return e;
   KAB_REQUIRE(bytes != nullptr, "null pointer");
-  AttentionPlan plan;
-  if (params->cache.batch > 0 && g.rows > 0)
+  *bytes = 0;
+  if (params->cache.batch == 0 || params->heads_q == 0 || params->q_len == 0) return KAB_OK;
+  const AttentionPart part = attention_part(params);
+  for (int64_t queries : {part.queries, params->q_len % part.queries}) {  // the last query tokens may be fewer
+    if (queries == 0) continue;
+    AttentionPlan plan;
+    attention_args(params, 0, part.batch, 0, queries, &g);
     if (int e = attention_plan(params, g, &plan)) return e;
-  *bytes = plan.bytes();
+    *bytes = std::max(*bytes, plan.bytes());
+  }
   return KAB_OK;
 }
 
@@ -287,25 +320,36 @@ int kab_kv_pages_attention(const KabKvPagesAttention* params, void* workspace, s
   if (params->cache.batch == 0 || params->heads_q == 0 || params->q_len == 0) return KAB_OK;
   KAB_REQUIRE(params->q != nullptr && params->out != nullptr, "null pointer");
   KAB_REQUIRE(aligned(params->out, 16), "out must be 16-byte aligned");
-  AttentionPlan plan;
-  if (int e = attention_plan(params, g, &plan)) return e;
-  KAB_REQUIRE(workspace != nullptr && workspace_bytes >= plan.bytes() && aligned(workspace, 256),
-              "the workspace needs %zu bytes, 256-byte aligned (kab_kv_pages_attention_workspace)", plan.bytes());
+  size_t need = 0;
+  if (int e = kab_kv_pages_attention_workspace(params, &need)) return e;
+  KAB_REQUIRE(workspace != nullptr && workspace_bytes >= need && aligned(workspace, 256),
+              "the workspace needs %zu bytes, 256-byte aligned (kab_kv_pages_attention_workspace)", need);
   unsigned* status = status_word();
   KAB_REQUIRE(status != nullptr, "no device status word");
   uint8_t* w = static_cast<uint8_t*>(workspace);
-  g.cuts = reinterpret_cast<PagesCut*>(w);
-  g.cuts_by_item = params->cache.batch * params->cache.heads_kv * g.row_tiles <= plan.grid;
-  g.partial = reinterpret_cast<float*>(w + plan.cuts);
-  if (params->use_mass) {
-    g.ml = reinterpret_cast<float*>(w + plan.cuts + plan.partial);
-    g.scores = reinterpret_cast<float*>(w + plan.cuts + plan.partial + plan.ml);
-  }
   const cudaStream_t s = as_stream(stream);
-  return with_instance(params, g.rows, [&](auto T, auto D, auto NR, auto SL) {
-    return launch_attention<decltype(T)::value, decltype(D)::value, decltype(NR)::value, decltype(SL)::value>(
-        g, plan, status, s);
-  });
+  const AttentionPart part = attention_part(params);
+  for (int64_t b0 = 0; b0 < params->cache.batch; b0 += part.batch) {
+    for (int64_t q0 = 0; q0 < params->q_len; q0 += part.queries) {
+      attention_args(params, b0, std::min(part.batch, params->cache.batch - b0), q0,
+                     std::min(part.queries, params->q_len - q0), &g);
+      AttentionPlan plan;
+      if (int e = attention_plan(params, g, &plan)) return e;
+      g.cuts = reinterpret_cast<PagesCut*>(w);
+      g.cuts_by_item = static_cast<int64_t>(g.pool.batch) * g.pool.heads * g.row_tiles <= plan.grid;
+      g.partial = reinterpret_cast<float*>(w + plan.cuts);
+      if (params->use_mass) {
+        g.ml = reinterpret_cast<float*>(w + plan.cuts + plan.partial);
+        g.scores = reinterpret_cast<float*>(w + plan.cuts + plan.partial + plan.ml);
+      }
+      const int e = with_instance(params, g.rows, [&](auto T, auto D, auto NR, auto SL) {
+        return launch_attention<decltype(T)::value, decltype(D)::value, decltype(NR)::value, decltype(SL)::value>(
+            g, plan, status, s);
+      });
+      if (e != KAB_OK) return e;
+    }
+  }
+  return KAB_OK;
 }
 
 int kab_kv_pages_evict(const KabKvPages* cache, const int32_t* out_table, int64_t out_stride, int64_t budget,

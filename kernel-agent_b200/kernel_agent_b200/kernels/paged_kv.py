@@ -165,7 +165,7 @@ def paged_kv_attention(q: torch.Tensor, k_pages: torch.Tensor, k_scale: torch.Te
     heads per KV head x query tokens) of a decode step: each 16 rows (8 where there are no more) read
     the cache once.
     ``mass`` takes scratch memory of four bytes per query row and token that the page table has room
-    for. Results do not depend on the other sequences' lengths but in the last bits (the cache is cut
+    for, at most 256 MB: where that is more, sequences or query tokens go in parts. Results do not depend on the other sequences' lengths but in the last bits (the cache is cut
     into equal parts for the GPU, whose softmax sums are merged), and are the same for the same
     inputs."""
     if q.dim() not in (3, 4):

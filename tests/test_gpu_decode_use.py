@@ -218,3 +218,89 @@ def test_linear_many_rows_in_groups(gv):
     y = gv.fp4_w4a16_linear(x, codes, scales, ts, bias)
     for lo in (0, 32, 1120, 1152, 1184, 1268):
         assert torch.equal(y[lo:lo + 32], gv.fp4_w4a16_linear(x[lo:lo + 32], codes, scales, ts, bias))
+
+
+UNIT = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+
+
+def attention64(q, cache, table, lengths, causal):
+    """(out, received, size, biggest) in 64 bits: size is sum p |v|, biggest a row's largest sum |q| |k| * scale."""
+    k_pages, k_scale, v_pages, v_scale = cache
+    batch, heads_q, queries, dim = q.shape
+    heads, page = k_pages.shape[1:3]
+    out, size = torch.zeros_like(q, dtype=torch.float64), torch.zeros_like(q, dtype=torch.float64)
+    received, biggest = [], 0.0
+    for b, n in enumerate(lengths.tolist()):
+        at = table[b, :-(-n // page)].long()
+        got = torch.zeros(heads, n, dtype=torch.float64, device=DEV)
+        seen = n - queries + 1 + torch.arange(queries, device=DEV) if causal else torch.full((queries,), n, device=DEV)
+        hidden = torch.arange(n, device=DEV)[None] >= seen[:, None]
+        for h in range(heads if n else 0):
+            k, v = ((c[at, h].double() * s[at, h].double()[:, None, None]).reshape(-1, dim)[:n]
+                    for c, s in ((k_pages, k_scale), (v_pages, v_scale)))
+            for g in range(heads_q // heads):
+                x = q[b, h * (heads_q // heads) + g].double() * dim ** -0.5
+                p = torch.softmax((x @ k.T).masked_fill(hidden, float("-inf")), -1).nan_to_num(0.0)
+                out[b, h * (heads_q // heads) + g] = p @ v
+                size[b, h * (heads_q // heads) + g] = p @ v.abs()
+                got[h] += p.sum(0)
+                biggest = max(biggest, float((x.abs() @ k.abs().T).max()))
+        received.append(got)
+    return out, received, size, biggest
+
+
+def check_attention(pk, q, cache, table, lengths, causal):
+    """Bounds: half a unit of the output type; 16-bit queries' weights have 11 bits, fp32 ones' 22; a score is off
+    by at most 16 * 2^-22 of the row's largest sum |q| |k| * scale, a weight by twice that; exponentials and
+    merges 2^-18. A mass is the sum of its rows' weights, one after the other in fp32."""
+    out, received, size, biggest = attention64(q, cache, table, lengths, causal)
+    score = 2 * 16 * 2.0 ** -22 * biggest + 2.0 ** -18
+    mass = torch.zeros(cache[1].shape + (cache[0].shape[2],), device=DEV)
+    got = pk.paged_kv_attention(q, *cache, table, lengths, causal=causal, mass=mass)
+    tol = UNIT[q.dtype] * out.abs() + (score + (2.0 ** -20 if q.dtype == torch.float32 else 2.0 ** -11)) * size + 1e-30
+    assert ((got.double() - out).abs() <= tol).all()
+    page, rows = cache[0].shape[2], q.shape[1] // cache[0].shape[1] * q.shape[2]
+    for b, n in enumerate(lengths.tolist()):
+        have = mass[table[b, :-(-n // page)].long()].transpose(0, 1).flatten(1)
+        want = torch.nn.functional.pad(received[b], (0, have.shape[1] - n))
+        assert ((have.double() - want).abs() <= want * (score + (rows + 2) * 2.0 ** -24 + 2.0 ** -20)).all()
+    return got
+
+
+def scratch(pk, q, cache, table, lengths, mass):
+    """Bytes that a call takes from the allocator beside its output."""
+    pk.paged_kv_attention(q, *cache, table, lengths, mass=mass)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    out = pk.paged_kv_attention(q, *cache, table, lengths, mass=mass)
+    return torch.cuda.max_memory_allocated() - before - out.numel() * out.element_size()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_prompt_with_mass(pk, dtype, causal):
+    """A prompt whose scores (0.35 GB a sequence) do not fit in what a call takes: its query tokens go in parts."""
+    cache = pool(145, 2, 64, 64, 3)
+    table = torch.randperm(145, generator=torch.Generator().manual_seed(1))[:144].to(torch.int32).to(DEV)
+    table = torch.cat([table[:141], table[141:].repeat(47)]).reshape(2, 141)
+    lengths = torch.tensor([9000, 150], dtype=torch.int32, device=DEV)
+    q = torch.randn(2, 16, 600, 64, device=DEV).to(dtype)
+    check_attention(pk, q, cache, table, lengths, causal)
+    mass = torch.zeros(145, 2, 64, device=DEV)
+    assert scratch(pk, q, cache, table, lengths, mass) <= 300 << 20
+
+
+def test_wide_page_table_with_mass(pk):
+    """Short sequences in a table with room for 524288 tokens each (64 MB of scores a sequence)."""
+    cache = pool(300, 8, 64, 64, 4)
+    lengths = torch.tensor([1 + 157 * b for b in range(10)], dtype=torch.int32, device=DEV)
+    table = torch.full((10, 8192), -1, dtype=torch.int32, device=DEV)
+    table[:, :30] = torch.randperm(300, generator=torch.Generator().manual_seed(2)).reshape(10, 30).to(torch.int32).to(DEV)
+    q = torch.randn(10, 32, 1, 64, device=DEV).to(torch.bfloat16)
+    wide = check_attention(pk, q, cache, table, lengths, True)
+    # the same weights and values, cut differently over the GPU: twice the bound of one of them at most
+    narrow = pk.paged_kv_attention(q, *cache, table[:, :30], lengths)
+    assert (wide - narrow).abs().max() <= 2.0 ** -6 * narrow.abs().max()
+    assert scratch(pk, q, cache, table, lengths, torch.zeros(300, 8, 64, device=DEV)) <= 300 << 20
