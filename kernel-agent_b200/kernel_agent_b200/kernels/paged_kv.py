@@ -287,6 +287,11 @@ class PagedFp8KVCache:
     def free_pages(self) -> int:
         return len(self._free)
 
+    def _table(self) -> torch.Tensor:
+        """The columns of the page table that any sequence has pages in: launches and scratch memory of the
+        functions follow its width."""
+        return self.page_table[:, :max(1, max(map(len, self._pages), default=1))]
+
     def _write_table(self) -> None:
         # -1 past a sequence's pages: a kernel that comes there skips it and reports it
         rows = [pages + [-1] * (self.max_pages - len(pages)) for pages in self._pages]
@@ -340,7 +345,8 @@ class PagedFp8KVCache:
 
     def attend(self, q: torch.Tensor, scale: float | None = None, causal: bool = True) -> torch.Tensor:
         """:func:`paged_kv_attention` of ``q`` over the cache; adds to :attr:`mass` where there is one."""
-        return paged_kv_attention(q, *self.pool, scale=scale, causal=causal, mass=self.mass)
+        return paged_kv_attention(q, self.k_pages, self.k_scale, self.v_pages, self.v_scale, self._table(),
+                                  self.lengths, scale=scale, causal=causal, mass=self.mass)
 
     def evict(self, budget: int, recent: int = 0, sinks: int = 0) -> tuple[list[int], torch.Tensor | None]:
         """Cut every sequence of more than ``budget`` tokens to ``budget``, as :func:`evict_kv_pages`
@@ -364,7 +370,7 @@ class PagedFp8KVCache:
         which = to_device(over, torch.int64, dev)
         target = to_device(to, torch.int32, dev)
         kept, lengths = evict_kv_pages(self.k_pages, self.k_scale, self.v_pages, self.v_scale, self.mass,
-                                       self.page_table[which], self.lengths[which], target, budget=budget,
+                                       self._table()[which], self.lengths[which], target, budget=budget,
                                        recent=recent, sinks=sinks)
         self.lengths[which] = lengths
         del self._free[len(self._free) - len(taken):]

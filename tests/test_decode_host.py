@@ -249,3 +249,25 @@ def test_linear_workspace_is_bounded(m, n, k, fmt):
     assert size(m) <= max(256 << 20, size(32))
     for rows in (1, 2, 5, 8, 9, 16, 17, 31):  # what is left for the last group needs no more
         assert size(m // 32 * 32 + rows) <= max(256 << 20, size(32), size(rows))
+
+
+def test_the_cache_hands_over_only_the_table_in_use(host_cache, monkeypatch):
+    """The launches and scratch memory of attention and eviction follow the table's width, by default that of
+    the whole pool: they get as much of it as a sequence holds pages."""
+    seen = []
+    monkeypatch.setattr(paged_kv, "paged_kv_attention", lambda q, k, ks, v, vs, table, lengths, **kw: seen.append(table.clone()))
+
+    def evict(k, ks, v, vs, mass, table, lengths, to, budget, **kw):
+        seen.append(table.clone())
+        return torch.zeros(len(lengths), 1, budget, dtype=torch.int32), torch.full_like(lengths, budget)
+
+    monkeypatch.setattr(paged_kv, "evict_kv_pages", evict)
+    cache = host_cache(3, 1, 64, num_pages=400, page_tokens=16)
+    q = torch.zeros(3, 1, 64)
+    cache.attend(q)
+    cache.reserve([5, 60, 17])
+    cache.attend(q)
+    cache.advance([5, 60, 17])
+    cache.evict(20)
+    assert [tuple(t.shape) for t in seen] == [(3, 1), (3, 4), (1, 4)]
+    assert seen[2][0].tolist() == seen[1][1].tolist()

@@ -304,3 +304,24 @@ def test_wide_page_table_with_mass(pk):
     narrow = pk.paged_kv_attention(q, *cache, table[:, :30], lengths)
     assert (wide - narrow).abs().max() <= 2.0 ** -6 * narrow.abs().max()
     assert scratch(pk, q, cache, table, lengths, torch.zeros(300, 8, 64, device=DEV)) <= 300 << 20
+
+
+def test_cache_of_a_large_pool(pk):
+    """The class's own table is as wide as the pool; attention and eviction see what is in use, and a prompt
+    attends over the paged cache with its mass."""
+    cache = pk.PagedFp8KVCache(3, 2, 64, num_pages=4000, page_tokens=64)
+    g = torch.Generator(device=DEV).manual_seed(9)
+    x = torch.randn(3, 2, 200, 64, generator=g, device=DEV).to(torch.float16)
+    cache.append(x, x * 0.5, counts=[200, 0, 130])
+    q = torch.randn(3, 4, 130, 64, generator=g, device=DEV).to(torch.float16)
+    out = cache.attend(q)
+    parts = cache.k_pages, cache.k_scale, cache.v_pages, cache.v_scale
+    assert torch.equal(out, check_attention(pk, q, parts, cache.page_table[:, :4], cache.lengths, True))
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    cache.attend(q)
+    assert torch.cuda.max_memory_allocated() - before <= 16 << 20
+    over, kept = cache.evict(96, recent=32, sinks=4)
+    assert over == [0, 2] and cache.lengths.tolist() == cache.tokens == [96, 0, 96]
