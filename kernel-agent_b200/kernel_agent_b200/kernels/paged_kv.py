@@ -292,10 +292,15 @@ class PagedFp8KVCache:
         functions follow its width."""
         return self.page_table[:, :max(1, max(map(len, self._pages), default=1))]
 
-    def _write_table(self) -> None:
+    def _write_table(self, changed: list[tuple[int, int, int]]) -> None:
+        """Writes the entries ``[first, last)`` of the sequences in ``changed`` (sequence, first, last)."""
+        at = [(b, i) for b, first, last in changed for i in range(first, last)]
+        if not at:
+            return
         # -1 past a sequence's pages: a kernel that comes there skips it and reports it
-        rows = [pages + [-1] * (self.max_pages - len(pages)) for pages in self._pages]
-        self.page_table.copy_(to_device(rows, torch.int32, self.page_table.device).reshape(self.page_table.shape))
+        pages = [self._pages[b][i] if i < len(self._pages[b]) else -1 for b, i in at]
+        sent = to_device([[b * self.max_pages + i for b, i in at], pages], torch.int64, self.page_table.device)
+        self.page_table.view(-1).index_copy_(0, sent[0], sent[1].to(torch.int32))
 
     def _not_captured(self) -> None:
         # neither the host's counts nor the host memory of a table's copy would be there for a replay
@@ -316,9 +321,10 @@ class PagedFp8KVCache:
             raise ValueError(f"a sequence would pass {self.max_pages} pages")
         if any(need):
             self._not_captured()
+            held = [len(p) for p in self._pages]
             for pages, n in zip(self._pages, need):
                 pages += [self._free.pop() for _ in range(n)]
-            self._write_table()
+            self._write_table([(b, held[b], held[b] + n) for b, n in enumerate(need)])
 
     def advance(self, counts: list[int]) -> None:
         """Count ``counts[b]`` tokens of each sequence that replays of a captured step have appended through
@@ -374,16 +380,20 @@ class PagedFp8KVCache:
                                        recent=recent, sinks=sinks)
         self.lengths[which] = lengths
         del self._free[len(self._free) - len(taken):]
+        changed = []
         for b, pages in zip(over, to):
+            changed.append((b, 0, max(len(pages), len(self._pages[b]))))
             self._free += self._pages[b]
             self._pages[b], self.tokens[b] = pages, budget
-        self._write_table()
+        self._write_table(changed)
         return over, kept
 
     def free(self, sequence: int) -> None:
         """End a sequence: its pages are free, its row of the batch is empty."""
         self._not_captured()
+        sequence = range(len(self.tokens))[sequence]
+        held = len(self._pages[sequence])
         self._free += self._pages[sequence]
         self._pages[sequence], self.tokens[sequence] = [], 0
         self.lengths[sequence] = 0
-        self._write_table()
+        self._write_table([(sequence, 0, held)])

@@ -271,3 +271,40 @@ def test_the_cache_hands_over_only_the_table_in_use(host_cache, monkeypatch):
     cache.evict(20)
     assert [tuple(t.shape) for t in seen] == [(3, 1), (3, 4), (1, 4)]
     assert seen[2][0].tolist() == seen[1][1].tolist()
+
+
+def test_a_page_taken_writes_its_table_entry_alone(host_cache, monkeypatch):
+    """A step that takes a page sends that entry, not the whole table; entries of freed and moved pages go."""
+    sent = []
+
+    def to_device(values, dtype, device):
+        t = torch.tensor(values, dtype=dtype)
+        sent.append(t.numel())
+        return t
+
+    monkeypatch.setattr(paged_kv, "to_device", to_device)
+    monkeypatch.setattr(paged_kv, "evict_kv_pages", lambda k, ks, v, vs, mass, table, lengths, to, budget, **kw: (
+        torch.zeros(len(lengths), 1, budget, dtype=torch.int32), torch.full_like(lengths, budget)))
+    cache = host_cache(8, 1, 64, num_pages=1000, page_tokens=16)
+
+    def check():
+        want = torch.full((8, 1000), -1, dtype=torch.int32)
+        for b, pages in enumerate(cache._pages):
+            want[b, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
+        assert torch.equal(cache.page_table, want)
+
+    for counts in ([100, 0, 16, 1, 30, 2, 2, 2], [0] * 7 + [20], [16] * 8):
+        sent.clear()
+        cache.reserve(counts)
+        cache.advance(counts)
+        check()
+        assert sum(sent) <= 100
+    sent.clear()
+    over, _ = cache.evict(20)
+    assert over == [0, 2, 4, 7]
+    check()
+    cache.free(1)
+    check()
+    cache.free(1)
+    check()
+    assert sum(sent) <= 100
