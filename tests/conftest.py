@@ -36,6 +36,8 @@ def _cuda() -> bool:
 
 
 def pytest_collection_modifyitems(config, items):
+    # looks at the library as it is loaded, before any test that makes it refuse a call
+    items.sort(key=lambda item: item.name != "test_no_gpu_calls_needed_for_metadata")
     if _cuda():
         return
     skip = pytest.mark.skip(reason="needs a CUDA device")
