@@ -22,9 +22,15 @@
 //  * Queries enter as f16, each row in units of a power of two that puts its largest value in
 //    [2^14, 2^15): bf16 and f16 values keep all their bits down to 2^-29 of the row's largest;
 //    fp32 ones are split into two f16 terms (22 bits) and the product is taken twice.
+//  * The weights enter the product with V in two f16 terms too (22 bits; with one, outputs were off by up
+//    to 2^-12 of sum p |v|, a tenth more than f16's own rounding in all). Up to four rows, as with four
+//    query heads per KV head, leave half of the MMA's columns: these hold the rows once more, take the second
+//    terms and are added at an item's end, at no product more (64 x 2048: 31.9 -> 32.2 us, 4 x 65536 of
+//    D = 64: 52.0 -> 52.4). More rows take the product twice (4 x 131072, 8 rows: 52.8 both ways; 16 x 4096
+//    of 16 rows: 20.8 -> 22.4).
 //  * The running maximum is that of t = s + log2(V scale), s the score in log2 units: the weight
 //    that multiplies the V codes is w = 2^(s - m) * V scale, with m = t - 10 at a slab's largest t,
-//    so w fits f16 with 11 bits down to 2^-24 of the largest at least and the page's scale costs
+//    so w fits f16, its two terms keep it to 2^-35 of the largest at least, and the page's scale costs
 //    one multiplication. Sums use 2^(s - m) itself, in fp32. (Adding every slab's product to the
 //    output with its own scale instead would cost 32 more multiply-adds per lane and slab.)
 //    log2(V scale) is cut at -80, which keeps the sums finite; pages whose scale is below about
@@ -130,10 +136,11 @@ __device__ __forceinline__ void copies_wait() {
 
 // ------------------------------------------------------------------ layout
 
-// NR: groups of 8 query rows that share one pass over the cache (the MMA's N). SL: tokens of a slab.
-template <int D, int NR, int SL, bool SPLIT>
+// ROWS: query rows that share one pass over the cache: 8 or 16, the MMA's columns, or 4, whose columns 4 .. 7
+// hold the same rows again and take the second terms of their weights. SL: tokens of a slab.
+template <int D, int ROWS, int SL, bool SPLIT>
 struct PagesLayout {
-  static constexpr int kWarps = 4, kThreads = kWarps * 32, kRows = 8 * NR;
+  static constexpr int kWarps = 4, kThreads = kWarps * 32, kRows = ROWS, NR = ROWS == 16 ? 2 : 1, kCols = 8 * NR;
   static constexpr bool kLight = NR == 1 && !SPLIT;
   static constexpr int kSlabBytes = SL * D;  // K or V of one slab
   static constexpr int kStageBytes = 2 * kSlabBytes;
@@ -146,7 +153,7 @@ struct PagesLayout {
   static constexpr int kMergeBytes = kWarps * kRows * (kPitch + 2) * 4;
   static constexpr int kRing = kWarps * kStages * kStageBytes > kMergeBytes ? kWarps * kStages * kStageBytes : kMergeBytes;
   static constexpr int kScales = kWarps * kStages * 2 * 4;
-  static constexpr int kSmem = kQBytes + kRing + kScales + kRows * 4 + 32;
+  static constexpr int kSmem = kQBytes + kRing + kScales + kCols * 4 + 32;
 };
 
 // Byte offset of 16-byte chunk `chunk` of token `row` in a slab: the chunks are permuted so that
@@ -205,21 +212,22 @@ __device__ __forceinline__ void pages_finish(const PagesAttnArgs& a, int b, int 
   }
 }
 
-template <int T, int D, int NR, int SL>
-__global__ void __launch_bounds__(PagesLayout<D, NR, SL, T == kF32>::kThreads, PagesLayout<D, NR, SL, T == kF32>::kBlocks)
+template <int T, int D, int ROWS, int SL>
+__global__ void __launch_bounds__(PagesLayout<D, ROWS, SL, T == kF32>::kThreads, PagesLayout<D, ROWS, SL, T == kF32>::kBlocks)
 pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
-  constexpr bool SPLIT = T == kF32, Q_HELD = NR == 1 && !SPLIT;
-  using L = PagesLayout<D, NR, SL, SPLIT>;
+  using L = PagesLayout<D, ROWS, SL, T == kF32>;
+  constexpr int NR = L::NR, COLS = L::kCols;
+  constexpr bool SPLIT = T == kF32, Q_HELD = NR == 1 && !SPLIT, TWICE = ROWS == 4;
   constexpr int U = SL / 16, SHIFT = SL == 16 ? 4 : 5;  // 16-token parts of a slab
   constexpr int COST = kItemCost * 16 / SL;
-  constexpr int ST = L::kStages, NW = L::kWarps, NT = L::kThreads, ROWS = L::kRows, PITCH = L::kPitch;
+  constexpr int ST = L::kStages, NW = L::kWarps, NT = L::kThreads, PITCH = L::kPitch;
   constexpr int STEPS = D / 16, MT = D / 16, CHUNKS = D / 16, COPIES = SL * D / 512;
   extern __shared__ __align__(128) uint8_t smem[];
   uint2* q_frag = reinterpret_cast<uint2*>(smem);                  // [hi, lo][NR][STEPS][32]
   uint8_t* ring = smem + L::kQBytes;
   float* sc_all = reinterpret_cast<float*>(ring + L::kRing);
-  float* q_unit = sc_all + NW * ST * 2;                            // [ROWS] units of the query rows
-  int* shared_i = reinterpret_cast<int*>(q_unit + ROWS);
+  float* q_unit = sc_all + NW * ST * 2;                            // [COLS] units of the query rows
+  int* shared_i = reinterpret_cast<int*>(q_unit + COLS);
   float* merge_o = reinterpret_cast<float*>(ring);                 // [NW][ROWS][PITCH]
   float* merge_ml = merge_o + NW * ROWS * PITCH;                   // [NW][ROWS][2]
 
@@ -313,9 +321,9 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
     const int rows = min(ROWS, a.rows - it.tile * ROWS);
     const int seen_by_all = a.causal ? max(0, n - a.q_len + 1) : n;
     if (s1 > 0) {
-      // tokens that row r of the tile sees
-      auto seen_of = [&](int r) -> int {
-        return a.causal ? max(0, n - a.q_len + 1 + (it.tile * ROWS + r) % a.q_len) : n;
+      // tokens that the row of column c sees
+      auto seen_of = [&](int c) -> int {
+        return a.causal ? max(0, n - a.q_len + 1 + (it.tile * ROWS + c % ROWS) % a.q_len) : n;
       };
 
       const uint8_t* kbase = p.codes[0] + it.h * p.sh[0];
@@ -371,11 +379,11 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
       // ---- the queries, as B fragments: b0 / b1 of step j are dims chunk * 16 + 4 i + {0, 1} / {2, 3}
       // of row g, where lane t reads K's chunks 2 t and 2 t + 1 (D = 128) or t (D = 64)
       {
-        constexpr int PARTS = NT / ROWS, E = D / PARTS;
-        const int r = tid / PARTS, part = tid % PARTS, rr = it.tile * ROWS + r;
+        constexpr int PARTS = NT / COLS, E = D / PARTS;
+        const int r = tid / PARTS, part = tid % PARTS, rr = it.tile * ROWS + r % ROWS;
         float v[E];
         uint32_t top = 0;
-        if (r < rows) {
+        if (r % ROWS < rows) {
           const int hq = it.h * group + rr / a.q_len, qi = rr % a.q_len;
           const int64_t base = it.b * a.qb + hq * a.qh + qi * a.qt + part * E;
 #pragma unroll
@@ -551,15 +559,50 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
               scale_pair(x[2], x[3], vsc, vsc);
               // the weights of 8 tokens x 8 rows, transposed into the B fragment of O^T = V^T P^T
               const uint32_t w0 = f16x2_of(x[0], x[1]), w1 = f16x2_of(x[2], x[3]);
-              pb[r][u][0] = transpose8(w0);
-              pb[r][u][1] = transpose8(w1);
-              if constexpr (SPLIT) {
-                const float2 h0 = f16x2_values(w0), h1 = f16x2_values(w1);
-                pl[r][u][0] = transpose8(f16x2_of(x[0] - h0.x, x[1] - h0.y));
-                pl[r][u][1] = transpose8(f16x2_of(x[2] - h1.x, x[3] - h1.y));
+              const float2 h0 = f16x2_values(w0), h1 = f16x2_values(w1);
+              const uint32_t l0 = f16x2_of(x[0] - h0.x, x[1] - h0.y), l1 = f16x2_of(x[2] - h1.x, x[3] - h1.y);
+              if constexpr (!TWICE) {
+                pb[r][u][0] = transpose8(w0);
+                pb[r][u][1] = transpose8(w1);
+                pl[r][u][0] = transpose8(l0);
+                pl[r][u][1] = transpose8(l1);
+              } else {
+                pb[r][u][0] = transpose8(t < 2 ? w0 : l0);
+                pb[r][u][1] = transpose8(t < 2 ? w1 : l1);
               }
             }
           }
+          // the tokens that only some rows see (fewer than q_len of them). With 16 rows before the
+          // product, so that the weights' registers are free in it (92 to 144 bytes spill otherwise)
+          auto some_see = [&] {
+            for (int x = max(seen_by_all, slab * SL); x < min(n, slab * SL + SL); ++x) {
+              const int k = x - slab * SL, from = ((k & 7) << 2) | t;
+              const int page = __ldg(table + (x >> p.page_shift));
+              const uint8_t* v = vbase + page * p.sp[1] + (x & (P - 1)) * p.st[1] + g * (D / 8);
+  #pragma unroll
+              for (int r = 0; r < NR; ++r) {
+                float w0 = 0.0f, w1 = 0.0f;
+  #pragma unroll
+                for (int i = 0; i < 2 * U; ++i) {
+                  const float e0 = __shfl_sync(0xffffffffu, s[r][i >> 1][(i & 1) * 2], from);
+                  const float e1 = __shfl_sync(0xffffffffu, s[r][i >> 1][(i & 1) * 2 + 1], from);
+                  if (k >> 3 == i) w0 = e0, w1 = e1;
+                }
+                bool sees0 = x < seen_of(r * 8 + 2 * t), sees1 = x < seen_of(r * 8 + 2 * t + 1);
+                if constexpr (TWICE) sees0 = sees0 && t < 2, sees1 = sees1 && t < 2;
+  #pragma unroll
+                for (int j = 0; j < MT; ++j) {
+  #pragma unroll
+                  for (int e = 0; e < 2; ++e) {
+                    const float value = e4m3_value_hw(__ldg(v + 2 * j + e));
+                    if (sees0) o[r][j][2 * e] = fmaf(w0, value, o[r][j][2 * e]);
+                    if (sees1) o[r][j][2 * e + 1] = fmaf(w1, value, o[r][j][2 * e + 1]);
+                  }
+                }
+              }
+            }
+          };
+          if constexpr (ROWS == 16) some_see();
           // ---- O^T: row g of MMA tile j is dim g * D / 8 + 2 j, row g + 8 the next one, so a lane's
           // bytes of a token are consecutive; tokens 2 t, 2 t + 1 and 2 t + 8, 2 t + 9 of each part
           constexpr int W = D / 32;  // 4-byte words per lane and token
@@ -589,39 +632,14 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
               for (int r = 0; r < NR; ++r) {
                 mma_f16(o[r][2 * w], va, pb[r][u][0], pb[r][u][1]);
                 mma_f16(o[r][2 * w + 1], vc, pb[r][u][0], pb[r][u][1]);
-                if constexpr (SPLIT) {
+                if constexpr (!TWICE) {
                   mma_f16(o[r][2 * w], va, pl[r][u][0], pl[r][u][1]);
                   mma_f16(o[r][2 * w + 1], vc, pl[r][u][0], pl[r][u][1]);
                 }
               }
             }
           }
-          // the tokens that only some rows see (fewer than q_len of them)
-          for (int x = max(seen_by_all, slab * SL); x < min(n, slab * SL + SL); ++x) {
-            const int k = x - slab * SL, from = ((k & 7) << 2) | t;
-            const int page = __ldg(table + (x >> p.page_shift));
-            const uint8_t* v = vbase + page * p.sp[1] + (x & (P - 1)) * p.st[1] + g * (D / 8);
-#pragma unroll
-            for (int r = 0; r < NR; ++r) {
-              float w0 = 0.0f, w1 = 0.0f;
-#pragma unroll
-              for (int i = 0; i < 2 * U; ++i) {
-                const float e0 = __shfl_sync(0xffffffffu, s[r][i >> 1][(i & 1) * 2], from);
-                const float e1 = __shfl_sync(0xffffffffu, s[r][i >> 1][(i & 1) * 2 + 1], from);
-                if (k >> 3 == i) w0 = e0, w1 = e1;
-              }
-              const bool sees0 = x < seen_of(r * 8 + 2 * t), sees1 = x < seen_of(r * 8 + 2 * t + 1);
-#pragma unroll
-              for (int j = 0; j < MT; ++j) {
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const float value = e4m3_value_hw(__ldg(v + 2 * j + e));
-                  if (sees0) o[r][j][2 * e] = fmaf(w0, value, o[r][j][2 * e]);
-                  if (sees1) o[r][j][2 * e + 1] = fmaf(w1, value, o[r][j][2 * e + 1]);
-                }
-              }
-            }
-          }
+          if constexpr (ROWS != 16) some_see();
         }
         stage = stage == ST - 1 ? 0 : stage + 1;
       }
@@ -632,6 +650,14 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
         for (int x = 4; x <= 16; x <<= 1) {
           l[r][0] += __shfl_xor_sync(0xffffffffu, l[r][0], x);
           l[r][1] += __shfl_xor_sync(0xffffffffu, l[r][1], x);
+        }
+      }
+
+      if constexpr (TWICE) {  // columns 4 .. 7 to 0 .. 3
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[0][j][e] += __shfl_xor_sync(0xffffffffu, o[0][j][e], 2);
         }
       }
 

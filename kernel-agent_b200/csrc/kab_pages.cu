@@ -95,8 +95,8 @@ void launch_append(const AppendArgs& a, dim3 grid, int ch, unsigned* status, cud
   else append_pages_kernel<T, 8><<<grid, 256, 0, s>>>(a, status);
 }
 
-// Query rows that share one pass over the cache: one group of 8 where that is all, else two.
-int tile_rows(int rows) { return rows <= 8 ? 8 : 16; }
+// Query rows that share one pass over the cache.
+int tile_rows(int rows) { return rows <= 4 ? 4 : rows <= 8 ? 8 : 16; }
 
 int attention_check(const KabKvPagesAttention* p, PagesAttnArgs* g) {
   KAB_REQUIRE(p != nullptr, "null parameters");
@@ -161,14 +161,14 @@ size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
 // Opts the kernel instance into its shared memory and returns the blocks of it that fit on the
 // GPU at once (asked once per device), or -1.
-template <int T, int D, int NR, int SL>
+template <int T, int D, int ROWS, int SL>
 int attention_blocks() {
-  using L = PagesLayout<D, NR, SL, T == kF32>;
+  using L = PagesLayout<D, ROWS, SL, T == kF32>;
   static int blocks[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
   if (blocks[dev] == 0) {
-    auto kern = pages_attention_kernel<T, D, NR, SL>;
+    auto kern = pages_attention_kernel<T, D, ROWS, SL>;
     int n = 0;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem) != cudaSuccess ||
         cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, L::kThreads, L::kSmem) != cudaSuccess || n < 1)
@@ -178,25 +178,31 @@ int attention_blocks() {
   return blocks[dev];
 }
 
-// The kernel instance of a call: f(type, head_dim, groups of rows, tokens of a slab).
+// The kernel instance of a call: f(type, head_dim, rows of a tile, tokens of a slab).
 template <int V>
 using Int = std::integral_constant<int, V>;
+template <int T, int D, int SL, typename F>
+auto with_rows(int rows, F&& f) {
+  const int tile = tile_rows(rows);
+  return tile == 4   ? f(Int<T>(), Int<D>(), Int<4>(), Int<SL>())
+         : tile == 8 ? f(Int<T>(), Int<D>(), Int<8>(), Int<SL>())
+                     : f(Int<T>(), Int<D>(), Int<16>(), Int<SL>());
+}
 template <int T, int D, typename F>
-auto with_groups(int rows, int64_t page, F&& f) {
-  if (page == 16) return tile_rows(rows) == 8 ? f(Int<T>(), Int<D>(), Int<1>(), Int<16>()) : f(Int<T>(), Int<D>(), Int<2>(), Int<16>());
-  return tile_rows(rows) == 8 ? f(Int<T>(), Int<D>(), Int<1>(), Int<32>()) : f(Int<T>(), Int<D>(), Int<2>(), Int<32>());
+auto with_slabs(int rows, int64_t page, F&& f) {
+  return page == 16 ? with_rows<T, D, 16>(rows, f) : with_rows<T, D, 32>(rows, f);
 }
 template <typename F>
 auto with_instance(const KabKvPagesAttention* p, int rows, F&& f) {
   const int64_t d = p->cache.head_dim, page = p->cache.page_tokens;
-  if (p->q_dtype == KAB_BF16) return d == 128 ? with_groups<kBF16, 128>(rows, page, f) : with_groups<kBF16, 64>(rows, page, f);
-  if (p->q_dtype == KAB_F16) return d == 128 ? with_groups<kF16, 128>(rows, page, f) : with_groups<kF16, 64>(rows, page, f);
-  return d == 128 ? with_groups<kF32, 128>(rows, page, f) : with_groups<kF32, 64>(rows, page, f);
+  if (p->q_dtype == KAB_BF16) return d == 128 ? with_slabs<kBF16, 128>(rows, page, f) : with_slabs<kBF16, 64>(rows, page, f);
+  if (p->q_dtype == KAB_F16) return d == 128 ? with_slabs<kF16, 128>(rows, page, f) : with_slabs<kF16, 64>(rows, page, f);
+  return d == 128 ? with_slabs<kF32, 128>(rows, page, f) : with_slabs<kF32, 64>(rows, page, f);
 }
 
 int attention_plan(const KabKvPagesAttention* p, const PagesAttnArgs& g, AttentionPlan* plan) {
-  plan->grid = with_instance(p, g.rows, [](auto T, auto D, auto NR, auto SL) {
-    return attention_blocks<decltype(T)::value, decltype(D)::value, decltype(NR)::value, decltype(SL)::value>();
+  plan->grid = with_instance(p, g.rows, [](auto T, auto D, auto ROWS, auto SL) {
+    return attention_blocks<decltype(T)::value, decltype(D)::value, decltype(ROWS)::value, decltype(SL)::value>();
   });
   if (plan->grid < 0) return fail(KAB_ECUDA, "cannot configure the paged attention kernel");
   const size_t items = static_cast<size_t>(g.pool.batch) * g.pool.heads;
@@ -227,10 +233,10 @@ cudaError_t launch_after(void (*kern)(Args...), dim3 grid, int threads, cudaStre
   return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
-template <int T, int D, int NR, int SL>
+template <int T, int D, int ROWS, int SL>
 int launch_attention(const PagesAttnArgs& g, const AttentionPlan& plan, unsigned* status, cudaStream_t s) {
-  using L = PagesLayout<D, NR, SL, T == kF32>;
-  pages_attention_kernel<T, D, NR, SL><<<plan.grid, L::kThreads, L::kSmem, s>>>(g, status);
+  using L = PagesLayout<D, ROWS, SL, T == kF32>;
+  pages_attention_kernel<T, D, ROWS, SL><<<plan.grid, L::kThreads, L::kSmem, s>>>(g, status);
   if (int e = check_launch("kab_kv_pages_attention")) return e;
   const int rows = std::min(g.rows, L::kRows);
   if (g.cuts_by_item)
@@ -342,8 +348,8 @@ int kab_kv_pages_attention(const KabKvPagesAttention* params, void* workspace, s
         g.ml = reinterpret_cast<float*>(w + plan.cuts + plan.partial);
         g.scores = reinterpret_cast<float*>(w + plan.cuts + plan.partial + plan.ml);
       }
-      const int e = with_instance(params, g.rows, [&](auto T, auto D, auto NR, auto SL) {
-        return launch_attention<decltype(T)::value, decltype(D)::value, decltype(NR)::value, decltype(SL)::value>(
+      const int e = with_instance(params, g.rows, [&](auto T, auto D, auto ROWS, auto SL) {
+        return launch_attention<decltype(T)::value, decltype(D)::value, decltype(ROWS)::value, decltype(SL)::value>(
             g, plan, status, s);
       });
       if (e != KAB_OK) return e;

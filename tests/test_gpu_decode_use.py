@@ -325,3 +325,24 @@ def test_cache_of_a_large_pool(pk):
     assert torch.cuda.max_memory_allocated() - before <= 16 << 20
     over, kept = cache.evict(96, recent=32, sinks=4)
     assert over == [0, 2] and cache.lengths.tolist() == cache.tokens == [96, 0, 96]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("heads_q,queries", [(1, 1), (4, 1), (2, 2), (5, 1), (8, 1), (3, 4), (16, 1), (11, 3)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_weights_keep_22_bits(pk, dtype, heads_q, queries, dim):
+    """Outputs near zero show what the weights lost: beside the output's own rounding (half a unit) only a score's
+    error (twice 16 * 2^-22 of sum |q| |k| * scale, small queries here), 2^-18 for exponentials and merges and
+    2^-20 for the weights, of sum p |v|. One, two, four, eight, 12, 16 and 33 rows per KV head."""
+    for page, n in ((16, 77), (64, 1500)):
+        cache = pool(-(-n // page), 1, page, dim, 11)
+        table = torch.arange(-(-n // page), dtype=torch.int32, device=DEV).reshape(1, -1)
+        lengths = torch.tensor([n], dtype=torch.int32, device=DEV)
+        g = torch.Generator(device=DEV).manual_seed(dim + heads_q)
+        q = (torch.randn(1, heads_q, queries, dim, generator=g, device=DEV) * 0.05).to(dtype)
+        out, _, size, biggest = attention64(q, cache, table, lengths, True)
+        tol = UNIT[dtype] * out.abs() + (2 * 16 * 2.0 ** -22 * biggest + 2.0 ** -18 + 2.0 ** -20) * size
+        if dtype == torch.float16:
+            tol += 2.0 ** -25  # half of its smallest step
+        got = pk.paged_kv_attention(q, *cache, table, lengths)
+        assert ((got.double() - out).abs() <= tol).all()
