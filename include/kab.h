@@ -490,8 +490,10 @@ int kab_kv_decode_fp8(const KabKvDecodeParams* params, void* workspace, size_t w
  * [n, k / 2] (low nibble = even k, 8-byte aligned rows), scales e4m3 per 16 (KAB_NVFP4) or e8m0
  * per 32 (KAB_MXFP4), 4-byte aligned, [n, k / block] row-major or, with `swizzle`, in the 128 x 4 blocked layout
  * the GEMMs read. x [m, k] of `dtype` (row stride ldx elements, 16-byte aligned rows), bias of
- * `bias_dtype` or NULL, out [m, ldo] of `dtype`. Products are exact, sums fp32. Rows of x past
- * 32 read the weight again. The workspace (kab_gemv_fp4_workspace; may be 0 bytes, 256-byte aligned)
+ * `bias_dtype` or NULL, out [m, ldo] of `dtype`. Sums are fp32, of exact products with x in f16 terms:
+ * bf16 and fp16 values keep all their bits down to 2^-28 of the row's largest finite value, fp32 ones are
+ * off by at most 2^-23 of themselves or 2^-39 of it; infinities and NaN stay. MXFP4 scales past 2^100 may overflow the sums. Rows
+ * of x past 32 read the weight again. The workspace (kab_gemv_fp4_workspace; may be 0 bytes, 256-byte aligned)
  * is scratch of one launch: it serves one stream at a time and need not be cleared. */
 int kab_gemv_fp4_workspace(int64_t m, int64_t n, int64_t k, int fmt, int dtype, size_t* bytes);
 int kab_gemv_fp4(const void* x, int dtype, int64_t ldx, const uint8_t* codes, const uint8_t* scales,

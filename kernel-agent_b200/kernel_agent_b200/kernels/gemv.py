@@ -37,9 +37,10 @@ def _plan(m: int, n: int, k: int, fmt: int, dtype: int, device: int) -> int:
 
 def fp4_w4a16_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, tensor_scale: torch.Tensor | float,
                      bias: torch.Tensor | None = None, *, fmt: str = "nvfp4") -> torch.Tensor:
-    """``x @ Wᵀ (+ bias)`` with ``W = e2m1(codes) * scales * tensor_scale``: exact products of
-    ``x`` (bf16, fp16 or fp32) and the weight's values, fp32 sums, ``acc * tensor_scale (+
-    bias)`` in fp32 and one rounding to ``x``'s dtype.
+    """``x @ Wᵀ (+ bias)`` with ``W = e2m1(codes) * scales * tensor_scale``: products of ``x`` and the
+    weight's values, fp32 sums, ``acc * tensor_scale (+ bias)`` and one rounding to ``x``'s dtype. The
+    products are exact for bf16 and fp16 ``x`` down to 2^-28 of a row's largest finite value; fp32 ``x``
+    enters with 22 bits (the result's error is up to 6e-7 of its size where fp32 products give 1e-7).
 
     ``x [..., K]``; ``codes [N, K / 2]`` (packed e2m1, low nibble first); ``scales [N, K /
     block]`` (e4m3 per 16 for ``fmt="nvfp4"``, e8m0 per 32 for ``"mxfp4"``) or the same already
