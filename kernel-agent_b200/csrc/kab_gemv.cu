@@ -30,8 +30,10 @@ struct GemvPlan {
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
 // Blocks apart (GROUPED) while its MMAs (8 per 128 codes and group) stay below the stream's time: one
-// or two tokens of NVFP4, up to four of MXFP4 (half of that in fp32, whose x has two terms). At eight
-// tokens of MXFP4 and 28672 x 14336 scaled codes took 98 us, blocks apart 125.
+// or two tokens of NVFP4, up to four of MXFP4 (half of that in fp32, whose x has two terms). Blocks apart
+// against scaled codes at 28672 x 8192 (4096 x 4096): two tokens of NVFP4 36.7 and 39.4 us (7.3 and 8.3),
+// three 62.9 and 39.9 (10.9 and 9.0); four of MXFP4 40.0 and 49.0 (8.4 and 9.7), five 70.1 and 52.3 (12.1 and
+// 9.8).
 GemvPlan gemv_plan(int64_t m, int64_t n, int64_t k, int fmt, int dtype) {
   GemvPlan p{};
   const bool mx = fmt == KAB_MXFP4, split = dtype == KAB_F32;

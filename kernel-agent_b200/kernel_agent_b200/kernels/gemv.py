@@ -46,7 +46,10 @@ def fp4_w4a16_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     block]`` (e4m3 per 16 for ``fmt="nvfp4"``, e8m0 per 32 for ``"mxfp4"``) or the same already
     swizzled (flat, 128 x 4 blocks); ``tensor_scale`` one value or one per row of the weight.
     Made for up to about 32 rows of ``x``, where the weight's bytes bound it; more rows work, the
-    weight being read again for every 32."""
+    weight being read again for every 32. Against :func:`~kernel_agent_b200.kernels.quant.fp4_w4a4_linear`
+    on the same codes and scales: 29.6 us and 103 for one row of 28672 x 8192 NVFP4, 94 and 99 for 32;
+    MXFP4 29.5 and 79 for one row, 74 and 77 for 16, 120 and 72 for 32. So from about 32 rows of NVFP4
+    and 20 of MXFP4 that one is the faster, where ``x`` may be rounded to FP4."""
     if fmt not in _FORMATS:
         raise ValueError(f"unknown FP4 format {fmt!r} (one of {', '.join(_FORMATS)})")
     code, block, kind = _FORMATS[fmt]
