@@ -8,7 +8,7 @@
 // accumulators): e4m3 -> f16 is one exact conversion per two codes, and the instruction's fragments
 // let the codes go from shared memory to the tensor core without leaving the warp. The cache is its
 // 16-row operand in both products, S^T = K Q^T and O^T = V^T P^T, and the query rows its 8 columns
-// (one group of 8, or two): no operand is padding where a KV head has 8 rows. (With the queries as the
+// (one group of 8, or two; four rows twice): no operand is padding where a KV head has 4 or 8 rows. (With the queries as the
 // 16-row operand the same kernel had twice the products and outputs: 66 us against 60 at 4 sequences
 // of 131072 tokens.) What has to be fast is the stream: every warp keeps its own ring of slabs of K
 // and V in flight with cp.async (32 tokens each, 16 where a page has no more: 54 us against 60) and
@@ -38,7 +38,7 @@
 //
 // 4 sequences of 131072 tokens, 16 / 2 heads, D = 128: 52 us = 5.2 TB/s = 0.79 of the measured copy,
 // of which about 8 us are fixed (two launches, the line's cut, the pipelines' fill, the merge): one
-// sequence of 4096 tokens, whose stream is 1.3 us, takes 10.4 us.
+// sequence of 4096 tokens, whose stream is 1.3 us, takes 10.8 us.
 #pragma once
 
 #include "kv_pages.cuh"
@@ -60,7 +60,7 @@ struct PagesAttnArgs {
   int heads_q, q_len, causal;  // q_len: query tokens of this launch, of those of the call
   int tail;                    // causal: newest tokens of every sequence that belong to later launches' queries
   int q_skip, out_rows;        // the call's query tokens less this launch's; rows of one KV head in `out`
-  int rows, row_tiles;   // rows of one KV head (query heads x query tokens), tiles of 8 or 16 of them
+  int rows, row_tiles;   // rows of one KV head (query heads x query tokens), tiles of 4, 8 or 16 of them
   float* partial;        // [grid, 2 slots, a tile's rows, D + 2]: output, maximum, sum
   PagesCut* cuts;        // [items or grid]: the shared items, by item or by the block that begins them
   int cuts_by_item;
