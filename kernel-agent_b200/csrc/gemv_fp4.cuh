@@ -26,7 +26,9 @@
 //    itself.
 //  * x enters as f16, each token (and K slice) in units of a power of two that puts its largest
 //    finite value in [2^14, 2^15): bf16 and f16 keep all their bits down to 2^-29 of it; fp32 is
-//    split into two f16 terms (22 bits) and multiplied twice. It stays in shared memory while a block
+//    split into two f16 terms (22 bits) and multiplied twice, the products of 128 codes added to the rest in
+//    fp32 (sums carried by the MMAs alone, which cut them, were off by 3e-6 at 8 x 8192 x 8192 and 7e-6 at K =
+//    28672; 3e-7 now, at the same time). It stays in shared memory while a block
 //    streams its rows, converted there for one token, by a launch before for more (5 x 1001 x 4080: 8.1 us,
 //    with every block converting for itself 13.3).
 //  * The (32-row tile, 256-code chunk) pairs of a K slice stand in one line, cut into equal parts for
@@ -471,7 +473,21 @@ __global__ void __launch_bounds__(kGemvThreads, gemv_columns(MX, NT, GROUPED) > 
           f[q][h][1] = __byte_perm(v, v, 0x3232);
         }
       }
-      products(w, half_chunk, f, acc);
+      if constexpr (SPLIT) {  // an MMA cuts its sum to 24 bits: fp32 results get a rounded addition per 128 codes
+        Sums c;
+        clear(c);
+        products(w, half_chunk, f, c);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[q][j][e] += c[q][j][e];
+          }
+        }
+      } else {
+        products(w, half_chunk, f, acc);
+      }
     } else {
       auto pow2 = [](int d) -> uint32_t {  // 2^d as an f16 pair, d in -24 .. 15
         const uint32_t h = d >= -14 ? static_cast<uint32_t>(d + 15) << 10 : 1u << (d + 24);

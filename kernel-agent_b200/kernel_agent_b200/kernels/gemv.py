@@ -40,7 +40,7 @@ def fp4_w4a16_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     """``x @ Wᵀ (+ bias)`` with ``W = e2m1(codes) * scales * tensor_scale``: products of ``x`` and the
     weight's values, fp32 sums, ``acc * tensor_scale (+ bias)`` and one rounding to ``x``'s dtype. The
     products are exact for bf16 and fp16 ``x`` down to 2^-28 of a row's largest finite value; fp32 ``x``
-    enters with 22 bits (the result's error is up to 6e-7 of its size where fp32 products give 1e-7).
+    enters with 22 bits (the result's error is about 3e-7 of its size).
 
     ``x [..., K]``; ``codes [N, K / 2]`` (packed e2m1, low nibble first); ``scales [N, K /
     block]`` (e4m3 per 16 for ``fmt="nvfp4"``, e8m0 per 32 for ``"mxfp4"``) or the same already

@@ -346,3 +346,27 @@ def test_weights_keep_22_bits(pk, dtype, heads_q, queries, dim):
             tol += 2.0 ** -25  # half of its smallest step
         got = pk.paged_kv_attention(q, *cache, table, lengths)
         assert ((got.double() - out).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("m", [1, 2, 3, 8, 16, 32])
+def test_linear_fp32_sums_do_not_drift(gv, m, fmt):
+    """Positive products, whose sum only grows: an MMA cuts what it adds to to 24 bits instead of rounding it
+    (up to 2^-23 of it, always downwards), so no more than 128 codes' worth, 16 MMAs with x's two terms, may
+    follow one another before a rounded addition. The mean over all outputs shows the cuts (up to 16 * 2^-23)
+    and leaves the roundings out (2^-24 for what remains of them)."""
+    n, k = 8192, 28672  # a warp's part has up to 112 chunks of 256 codes
+    g = torch.Generator().manual_seed(m)
+    codes = (torch.randint(0, 256, (n, k // 2), generator=g, dtype=torch.int32).to(torch.uint8) & 0x77).to(DEV)
+    level = torch.tensor([0.0, 0.5, 1, 1.5, 2, 3, 4, 6], dtype=torch.float64, device=DEV)
+    w = torch.stack([level[(codes & 15).long()], level[(codes >> 4).long()]], -1).reshape(n, k)
+    if fmt == "nvfp4":
+        scales = torch.rand(n, k // 16, generator=g).add(0.5).to(E4M3).to(DEV)
+        w = w * scales.double().repeat_interleave(16, 1)
+    else:
+        raw = torch.randint(124, 131, (n, k // 32), generator=g, dtype=torch.int32).to(torch.uint8).to(DEV)
+        scales, w = raw.view(torch.float8_e8m0fnu), w * torch.exp2(raw.double() - 127).repeat_interleave(32, 1)
+    x = torch.rand(m, k, generator=g).add(0.1).to(DEV)
+    want = x.double() @ w.T
+    y = gv.fp4_w4a16_linear(x, codes, scales, 1.0, fmt=fmt)
+    assert abs(float(((y.double() - want) / want).mean())) <= 16 * 2.0 ** -23 + 2.0 ** -24
