@@ -28,6 +28,11 @@
 //    terms and are added at an item's end, at no product more (64 x 2048: 31.9 -> 32.2 us, 4 x 65536 of
 //    D = 64: 52.0 -> 52.4). More rows take the product twice (4 x 131072, 8 rows: 52.8 both ways; 16 x 4096
 //    of 16 rows: 20.8 -> 22.4).
+//  * An MMA cuts the sum that it carries to 24 bits instead of rounding it. For fp32 queries the products of 16
+//    tokens start from zero and are added to the output by themselves (16 x 60000 tokens, 32 / 8 heads,
+//    positive values: off by 3e-7, carried 1.1e-5; 4 x 131072 52.4 -> 53.0 us, 16 x 4096 of 16 rows 24.2 ->
+//    27.1). 16-bit outputs, whose last bit is 2^-11 and 2^-8, take the carried sums (f16 with 16 rows: 22.3 us,
+//    25.7 otherwise).
 //  * The running maximum is that of t = s + log2(V scale), s the score in log2 units: the weight
 //    that multiplies the V codes is w = 2^(s - m) * V scale, with m = t - 10 at a slab's largest t,
 //    so w fits f16, its two terms keep it to 2^-35 of the largest at least, and the page's scale costs
@@ -111,6 +116,13 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // a *= c, b *= d in one instruction.
 __device__ __forceinline__ void scale_pair(float& a, float& b, float c, float d) {
   asm("{\n .reg .b64 x, y;\n mov.b64 x, {%0, %1};\n mov.b64 y, {%2, %3};\n mul.rn.f32x2 x, x, y;\n"
+      " mov.b64 {%0, %1}, x;\n}"
+      : "+f"(a), "+f"(b)
+      : "f"(c), "f"(d));
+}
+// a += c, b += d in one instruction.
+__device__ __forceinline__ void add_pair(float& a, float& b, float c, float d) {
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%0, %1};\n mov.b64 y, {%2, %3};\n add.rn.f32x2 x, x, y;\n"
       " mov.b64 {%0, %1}, x;\n}"
       : "+f"(a), "+f"(b)
       : "f"(c), "f"(d));
@@ -630,11 +642,21 @@ pages_attention_kernel(PagesAttnArgs a, unsigned* status) {
               const uint32_t vc[4] = {e4m3x2_f16(x1), e4m3x2_f16_high(x1), e4m3x2_f16(y1), e4m3x2_f16_high(y1)};
 #pragma unroll
               for (int r = 0; r < NR; ++r) {
-                mma_f16(o[r][2 * w], va, pb[r][u][0], pb[r][u][1]);
-                mma_f16(o[r][2 * w + 1], vc, pb[r][u][0], pb[r][u][1]);
+                float none[2][4] = {};
+                float(&to0)[4] = SPLIT ? none[0] : o[r][2 * w];
+                float(&to1)[4] = SPLIT ? none[1] : o[r][2 * w + 1];
+                mma_f16(to0, va, pb[r][u][0], pb[r][u][1]);
+                mma_f16(to1, vc, pb[r][u][0], pb[r][u][1]);
                 if constexpr (!TWICE) {
-                  mma_f16(o[r][2 * w], va, pl[r][u][0], pl[r][u][1]);
-                  mma_f16(o[r][2 * w + 1], vc, pl[r][u][0], pl[r][u][1]);
+                  mma_f16(to0, va, pl[r][u][0], pl[r][u][1]);
+                  mma_f16(to1, vc, pl[r][u][0], pl[r][u][1]);
+                }
+                if constexpr (SPLIT) {  // a rounded addition for every 16 tokens
+#pragma unroll
+                  for (int e = 0; e < 4; e += 2) {
+                    add_pair(o[r][2 * w][e], o[r][2 * w][e + 1], to0[e], to0[e + 1]);
+                    add_pair(o[r][2 * w + 1][e], o[r][2 * w + 1][e + 1], to1[e], to1[e + 1]);
+                  }
                 }
               }
             }

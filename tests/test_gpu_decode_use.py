@@ -370,3 +370,28 @@ def test_linear_fp32_sums_do_not_drift(gv, m, fmt):
     want = x.double() @ w.T
     y = gv.fp4_w4a16_linear(x, codes, scales, 1.0, fmt=fmt)
     assert abs(float(((y.double() - want) / want).mean())) <= 16 * 2.0 ** -23 + 2.0 ** -24
+
+
+@pytest.mark.parametrize("heads_q", [8, 64])
+def test_fp32_outputs_do_not_drift(pk, heads_q):
+    """Long contexts of positive values: an MMA cuts the sum that it carries (up to 2^-23 of it, always downwards),
+    so the products of 16 tokens, two MMAs, are added with a rounding. The mean over a head's outputs shows the
+    cuts (2 * 2^-23), exponentials and merges (2^-18) and leaves the roundings out."""
+    batch, heads, n, page, dim = 8, 8, 60000, 64, 64
+    pages = -(-n // page)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    codes = [torch.empty(batch * pages, heads, page, dim, dtype=E4M3, device=DEV) for _ in range(2)]
+    for c in codes:
+        for lo in range(0, batch * pages, 500):
+            x = torch.randn(c[lo:lo + 500].shape, generator=g, device=DEV)
+            c[lo:lo + 500] = ((x.abs() if c is codes[1] else x) * 64).clamp(-448, 448).to(E4M3)
+    scale = torch.full((batch * pages, heads), 2.0 ** -6, device=DEV)
+    table = torch.arange(batch * pages, dtype=torch.int32, device=DEV).reshape(batch, pages)
+    lengths = torch.full((batch,), n, dtype=torch.int32, device=DEV)
+    q = torch.randn(batch, heads_q, dim, generator=g, device=DEV)
+    got = pk.paged_kv_attention(q, codes[0], scale, codes[1], scale, table, lengths)
+    for b, h in ((0, 0), (3, 5), (7, 7)):
+        k, v = ((c[table[b].long(), h].double() * 2.0 ** -6).reshape(-1, dim)[:n] for c in codes)
+        rows = slice(h * heads_q // heads, (h + 1) * heads_q // heads)
+        want = torch.softmax(q[b, rows].double() @ k.T * dim ** -0.5, -1) @ v
+        assert abs(float(((got[b, rows].double() - want) / want).mean())) <= 2 * 2.0 ** -23 + 2.0 ** -18
