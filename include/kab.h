@@ -569,7 +569,8 @@ int kab_kv_pages_attention(const KabKvPagesAttention* params, void* workspace, s
  * the largest), in their order, and copies their codes, scales and masses into the pages
  * out_table[b * out_stride + i / page_tokens] of the same pool, which no sequence may use. Each
  * written page's scale is the smallest power of two that holds its values (as in the append).
- * kept [batch, heads_kv, budget]: the kept token numbers, -1 past the last; lengths_out [batch].
+ * kept [batch, heads_kv, budget]: the kept token numbers, -1 past the last; lengths_out [batch], not
+ * `lengths` itself.
  * sinks + recent <= budget. */
 int kab_kv_pages_evict(const KabKvPages* cache, const int32_t* out_table, int64_t out_stride, int64_t budget,
                        int64_t recent, int64_t sinks, int32_t* kept, int32_t* lengths_out, void* stream);

@@ -369,6 +369,7 @@ int kab_kv_pages_evict(const KabKvPages* cache, const int32_t* out_table, int64_
   if (cache->batch == 0) return KAB_OK;
   KAB_REQUIRE(out_table && kept && lengths_out, "null pointer");
   KAB_REQUIRE(cache->mass != nullptr || cache->num_pages == 0, "an eviction needs the tokens' mass");
+  KAB_REQUIRE(lengths_out != cache->lengths, "lengths_out must not be the lengths that the eviction reads");
   unsigned* status = status_word();
   KAB_REQUIRE(status != nullptr, "no device status word");
   a.out_table = out_table;

@@ -308,3 +308,15 @@ def test_a_page_taken_writes_its_table_entry_alone(host_cache, monkeypatch):
     cache.free(1)
     check()
     assert sum(sent) <= 100
+
+
+def test_eviction_refuses_to_overwrite_the_lengths_it_reads():
+    """Blocks read a sequence's length while the first one writes the new one."""
+    p = nat.KabKvPages()
+    p.k_pages = p.v_pages = p.k_scale = p.v_scale = p.mass = p.page_table = p.lengths = 256
+    p.num_pages, p.heads_kv, p.page_tokens, p.head_dim, p.max_pages, p.batch, p.table_stride = 8, 2, 64, 128, 4, 1, 4
+    p.k_stride_page = p.v_stride_page = 2 * 64 * 128
+    p.k_stride_head = p.v_stride_head = 64 * 128
+    p.k_stride_token = p.v_stride_token = 128
+    with pytest.raises(ValueError, match="lengths_out"):
+        nat.call("kab_kv_pages_evict", ctypes.byref(p), 512, 4, 8, 2, 2, 1024, 256, None)
