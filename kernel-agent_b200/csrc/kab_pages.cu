@@ -117,7 +117,7 @@ int attention_check(const KabKvPagesAttention* p, PagesAttnArgs* g) {
   return KAB_OK;
 }
 
-// What one round of launches takes of a call: sequences and query tokens.
+// What one set of launches takes of a call: sequences and query tokens.
 struct AttentionPart {
   int64_t batch, queries;
 };
